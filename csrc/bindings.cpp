@@ -274,6 +274,7 @@ void set_error_for_test(int64_t device, int64_t code) {
 void register_ops(pybind11::module& m);
 void register_comm(pybind11::module& m);
 void register_moe(pybind11::module& m);
+void register_objectives(pybind11::module& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "parallel_b200 sm_100a kernels";
@@ -305,4 +306,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_ops(m);
   register_comm(m);
   register_moe(m);
+  register_objectives(m);
 }

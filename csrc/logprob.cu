@@ -1,0 +1,641 @@
+// Log-probabilities of given tokens through a language-model head, without the
+// logits: logp[t] = l_id - log sum_v exp(l_v), l_v = (h_t . w_v) / temperature.
+//
+//   logprob_gemm    CTA-pair tcgen05 GEMM h w^T whose epilogue turns each row
+//                   of an output tile into (max, sum of 2^(x - max)) of
+//                   x = l * log2(e), the target column left out; under a
+//                   gradient it also stores E = bf16(2^(x - tile max)).
+//   logprob_finish  per row: the target logit as its own dot product, the
+//                   merge of the row's tile statistics, logp and the row's
+//                   base-2 log-sum-exp.
+//   logprob_pack    (under a gradient) brings the rows that have a token to the
+//                   front; logprob_unpack takes their gradients back.
+//   logprob_bwd     in place over E: the gradient of the logits,
+//                   dl_v = c ([v = id] - 2^(x_v - lse2)), c = dlogp / temperature.
+//
+// The target logit is kept out of the sums and summed on its own in 64 bits,
+// and logp = -log1p(sum of the others / target): the tensor core truncates as
+// it accumulates (measured on a target logit of 13: 1.6e-5 low at H = 1024,
+// 5e-5 at H = 4096), and where the target is nearly certain all of logp hangs
+// on that logit.  The other logits enter as a sum of many, where the error of
+// one does not show.
+//
+// E is relative to the tile's own maximum, which is known when the tile is
+// stored, while the row's log-sum-exp is not: an entry keeps 8 bits of its
+// probability whatever its size, and the backward is one multiplication per
+// entry (the factor 2^(tile max - lse2) is shared by a tile's row) in a pass
+// bound by memory.  bf16 logits would lose |l| / 256 of the exponent instead.
+#include <cuda_bf16.h>
+#include <math.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "host_util.h"
+#include "objectives.cuh"
+#include "ptx.cuh"
+
+namespace pb {
+namespace {
+
+constexpr int BM_CTA = 128;  // rows of h per CTA (a pair's tile has 256)
+constexpr int BK = 64;
+constexpr int BN_MAX = 256;
+constexpr int kThreads = 192;
+constexpr int A_BYTES = BM_CTA * BK * 2;
+constexpr int B_BYTES = (BN_MAX / 2) * BK * 2;
+constexpr int STAGES = 6;
+constexpr int kBox = 32;  // E is stored in 32 x 32 boxes of 64-byte rows (64-byte swizzle)
+constexpr int kBoxBytes = kBox * kBox * 2;
+constexpr int EPI_BYTES = 4 * 2 * kBoxBytes;  // two boxes for each of the 4 epilogue warps
+constexpr int SMEM_BYTES = STAGES * (A_BYTES + B_BYTES) + EPI_BYTES + 1024 + 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Wait for this thread's TMEM loads; the registers are operands, so no use of
+// them can move above the wait.
+__device__ __forceinline__ void wait_ld(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                 "+f"(v[30]), "+f"(v[31])::"memory");
+}
+
+// Accumulators of columns [n0, n0 + 32): -inf past the vocabulary and at the
+// row's target, so neither enters the maximum or the sum.
+__device__ __forceinline__ void mask_cols(float* v, int n0, int V, int64_t id) {
+  uint32_t out = 0;  // bit j: column n0 + j is masked
+  if (n0 + 32 > V) out = n0 >= V ? 0xffffffffu : 0xffffffffu << (V - n0);
+  const int64_t d = id - n0;
+  if (d >= 0 && d < 32) out |= 1u << (int)d;
+  if (out) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (out & (1u << j)) v[j] = -INFINITY;
+  }
+}
+
+__device__ __forceinline__ float max32(const float* v) {
+  float m = v[0];
+#pragma unroll
+  for (int j = 1; j < 32; ++j) m = fmaxf(m, v[j]);
+  return m;
+}
+
+// Statistics of one accumulator row (one thread) of `bn` columns from TMEM:
+// running maximum and sum over 32-column chunks.  `release` runs after the
+// last TMEM read.
+template <typename Release>
+__device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, int V, int64_t id, float scale,
+                                            Release release) {
+  float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < bn; c += 32) {
+    float v[32];
+    tmem_ld32(t_row + c, v);
+    wait_ld(v);
+    if (c + 32 >= bn) release();
+    mask_cols(v, n_base + c, V, id);
+    const float mn = fmaxf(m, max32(v) * scale);
+    const float ref = mn == -INFINITY ? 0.f : mn;  // nothing but masked columns so far
+    s *= ex2(m - ref);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s += ex2(fmaf(v[j], scale, -ref));
+    m = mn;
+  }
+  return make_float2(m, s);
+}
+
+// The same with E stored: the maximum first (E needs one reference for the
+// whole tile), then the exponentials, 32 x 32 boxes through TMA.
+template <typename Release>
+__device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_base, int V, int64_t id, float scale,
+                                                  const CUtensorMap* tmE, uint8_t* stage, int lane, int y0,
+                                                  Release release) {
+  float m = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < bn; c += 32) {
+    float v[32];
+    tmem_ld32(t_row + c, v);
+    wait_ld(v);
+    mask_cols(v, n_base + c, V, id);
+    m = fmaxf(m, max32(v));
+  }
+  m *= scale;
+  const float ref = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < bn; c += 32) {
+    float v[32];
+    tmem_ld32(t_row + c, v);
+    wait_ld(v);
+    if (c + 32 >= bn) release();
+    const int n0 = n_base + c;
+    mask_cols(v, n0, V, id);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      v[j] = ex2(fmaf(v[j], scale, -ref));
+      s += v[j];
+    }
+    // two boxes alternate: chunk c is staged while chunk c - 1 drains
+    uint8_t* box = stage + ((c >> 5) & 1) * kBoxBytes;
+    if (lane == 0) bulk_wait_group_read<1>();
+    __syncwarp();
+    uint8_t* row = box + lane * 64;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint4 u;
+      u.x = pack_bf16x2(v[q * 8 + 0], v[q * 8 + 1]);
+      u.y = pack_bf16x2(v[q * 8 + 2], v[q * 8 + 3]);
+      u.z = pack_bf16x2(v[q * 8 + 4], v[q * 8 + 5]);
+      u.w = pack_bf16x2(v[q * 8 + 6], v[q * 8 + 7]);
+      *reinterpret_cast<uint4*>(row + ((q ^ ((lane >> 1) & 3)) << 4)) = u;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (n0 < V) tma_store_2d(tmE, box, n0, y0);  // rows and columns past the extents are clipped
+      bulk_commit_group();
+    }
+  }
+  return make_float2(m, s);
+}
+
+// Roles per CTA: warp 0 TMA producer, warp 1 TMEM allocator and (even CTA) MMA
+// issuer, warps 2..5 epilogue, one output row per thread.  The accumulator is
+// double buffered in TMEM, so the epilogue of one tile runs under the MMAs of
+// the next.  Row tiles run innermost: every pair works on the same few column
+// tiles of w, which is read from memory once.
+template <bool STORE>
+__global__ void __launch_bounds__(kThreads, 1)
+    logprob_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                        const __grid_constant__ CUtensorMap tmE, const int64_t* __restrict__ ids,
+                        float2* __restrict__ stats, int T, int V, int H, int bn, float scale, int* err) {
+  pdl_prologue();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * A_BYTES;
+  uint8_t* sEpi = sB + STAGES * B_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sEpi + EPI_BYTES);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* tfull_bar = empty_bar + STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;  // used on the even CTA (256 arrivals: both epilogues)
+  uint64_t* drain_bar = tempty_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull_bar[i], 1);
+      mbar_init(&tempty_bar[i], 2 * 128);
+    }
+    mbar_init(drain_bar, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 2 * BN_MAX);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // barriers of both CTAs initialised before any cross-CTA use
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int tiles_m = (T + 2 * BM_CTA - 1) / (2 * BM_CTA);
+  const int tiles_n = (V + bn - 1) / bn;
+  const int64_t num_tiles = (int64_t)tiles_m * tiles_n;
+  const int num_kb = (H + BK - 1) / BK;
+  const int n_clusters = gridDim.x >> 1;
+  const int cid = blockIdx.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t stage_bytes = 2 * (A_BYTES + (uint32_t)(bn / 2) * BK * 2);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t w = cid; w < num_tiles && ok; w += n_clusters) {
+        const int tm = (int)(w % tiles_m), tn = (int)(w / tiles_m);
+        const int a_row = tm * 2 * BM_CTA + (int)rank * BM_CTA;
+        const int b_row = tn * bn + (int)rank * (bn / 2);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, err)) { ok = false; break; }
+          const uint32_t full_even = mapa_shared(smem_u32(&full_bar[stage]), 0);
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], stage_bytes);
+          tma_load_2d_pair(sA + stage * A_BYTES, &tmA, full_even, kb * BK, a_row);
+          tma_load_2d_pair(sB + stage * B_BYTES, &tmB, full_even, kb * BK, b_row);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (leader && lane == 0) {
+      const uint32_t idesc = idesc_bf16(2 * BM_CTA, bn, false, false);
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      for (int64_t w = cid; w < num_tiles && ok; w += n_clusters, ++local) {
+        const int acc = local & 1;
+        const uint32_t acc_phase = (local >> 1) & 1;
+        if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, err)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN_MAX;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, err)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_base = smem_u32(sA + stage * A_BYTES);
+          const uint32_t b_base = smem_u32(sB + stage * B_BYTES);
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk)
+            mma_bf16_ss_pair(d_tmem, smem_desc_sw128(a_base + kk * 32, 16, 1024),
+                             smem_desc_sw128(b_base + kk * 32, 16, 1024), idesc, (kb != 0 || kk != 0) ? 1u : 0u);
+          mma_commit_pair(&empty_bar[stage], 0x3);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (ok) mma_commit_pair(&tfull_bar[acc], 0x3);
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    uint8_t* stage = sEpi + quarter * 2 * kBoxBytes;
+    int local = 0;
+    for (int64_t w = cid; w < num_tiles; w += n_clusters, ++local) {
+      const int tm = (int)(w % tiles_m), tn = (int)(w / tiles_m);
+      const int acc = local & 1;
+      const uint32_t acc_phase = (local >> 1) & 1;
+      if (!mbar_wait(&tfull_bar[acc], acc_phase, err)) break;
+      tc_fence_after();
+      const int y0 = tm * 2 * BM_CTA + (int)rank * BM_CTA + quarter * 32;
+      const int t = y0 + lane;
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN_MAX;
+      const uint32_t tempty = mapa_shared(smem_u32(&tempty_bar[acc]), 0);
+      auto release = [&] {
+        tc_fence_before();
+        mbar_arrive_cluster(tempty);
+      };
+      if (y0 >= T) {  // no row of this warp is in range
+        release();
+        continue;
+      }
+      const int64_t id = t < T ? ids[t] : -1;
+      float2 st;
+      if constexpr (STORE)
+        st = row_stats_store(t_row, bn, tn * bn, V, id, scale, &tmE, stage, lane, y0, release);
+      else
+        st = row_stats(t_row, bn, tn * bn, V, id, scale, release);
+      if (t < T) stats[(int64_t)t * tiles_n + tn] = st;
+    }
+    // the box stores must have finished before the kernel's shared memory goes
+    if (STORE && lane == 0) bulk_wait_group<0>();
+  }
+
+  // On an error path the MMA issuer may have left MMAs in flight: drain them
+  // (bounded) before the accumulator columns are released.
+  if (warp == 1 && lane == 0 && leader && *((volatile int*)err) != 0) {
+    mma_commit_pair(drain_bar, 0x1);
+    const uint64_t t0 = globaltimer();
+    while (!mbar_try_wait(smem_u32(drain_bar), 0) && globaltimer() - t0 < 100000000ull) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the pair MMA may still read its shared memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * BN_MAX);
+  }
+}
+
+// ---------------------------------------------------------------- finish
+constexpr int kFinThreads = 128;
+
+// One block per row of h; its log-probability goes to row perm[t] (t without
+// perm).  dot in 64 bits (bf16 products are exact in fp32; eight
+// of them are added in fp32, the rest in double), then the tile statistics:
+// with d = m - x_id (base 2), logp = -log(1 + s 2^d), written so that neither
+// a large nor a small d loses digits.
+__global__ void __launch_bounds__(kFinThreads)
+    logprob_finish_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const __nv_bfloat16* __restrict__ w,
+                          int64_t ldw, const int64_t* __restrict__ ids, const int* __restrict__ perm,
+                          const float2* __restrict__ stats, int tiles, int V, int H, float scale,
+                          float* __restrict__ logp, float* __restrict__ lse2) {
+  pdl_prologue();
+  const int64_t t = blockIdx.x;
+  const int64_t out = perm ? perm[t] : t;
+  const int64_t id = ids[t];
+  if (id < 0 || id >= V) {
+    // no token: 0.  An id past the vocabulary has no log-probability: NaN.
+    if (threadIdx.x == 0) {
+      logp[out] = id < 0 ? 0.f : NAN;
+      lse2[t] = id < 0 ? 0.f : NAN;
+    }
+    return;
+  }
+  double dot = 0.0;
+  const uint4* hr = reinterpret_cast<const uint4*>(h + t * ldh);
+  const uint4* wr = reinterpret_cast<const uint4*>(w + id * ldw);
+  for (int i = threadIdx.x; i < H / 8; i += kFinThreads) {
+    const uint4 a = hr[i], b = wr[i];
+    const uint32_t* ap = &a.x;
+    const uint32_t* bp = &b.x;
+    float p = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 x = unpack_bf16x2(ap[q]), y = unpack_bf16x2(bp[q]);
+      p = fmaf(x.x, y.x, p);
+      p = fmaf(x.y, y.y, p);
+    }
+    dot += (double)p;
+  }
+  float m = -INFINITY, s = 0.f;
+  const float2* sr = stats + t * tiles;
+  for (int i = threadIdx.x; i < tiles; i += kFinThreads) {
+    const float2 v = sr[i];
+    const float mn = fmaxf(m, v.x);
+    if (mn == -INFINITY) {
+      s += v.y;  // 0, or the NaN of a NaN logit
+      continue;
+    }
+    s = s * ex2(m - mn) + v.y * ex2(v.x - mn);
+    m = mn;
+  }
+  __shared__ double sd[kFinThreads / 32];
+  __shared__ float sm[kFinThreads / 32], ss[kFinThreads / 32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    const float mn = fmaxf(m, m2);
+    s = mn == -INFINITY ? s + s2 : s * ex2(m - mn) + s2 * ex2(m2 - mn);
+    m = mn;
+  }
+  const int wp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+    sd[wp] = dot;
+    sm[wp] = m;
+    ss[wp] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+#pragma unroll
+  for (int i = 1; i < kFinThreads / 32; ++i) {
+    dot += sd[i];
+    const float mn = fmaxf(m, sm[i]);
+    s = mn == -INFINITY ? s + ss[i] : s * ex2(m - mn) + ss[i] * ex2(sm[i] - mn);
+    m = mn;
+  }
+  const double x_id = dot * (double)scale;
+  const float d = (float)((double)m - x_id);
+  float lp;
+  if (d <= 0.f)
+    lp = -log1pf(s * exp2f(d));
+  else
+    lp = -(d * kLn2 + logf(s + exp2f(-d)));
+  logp[out] = lp;
+  lse2[t] = (float)(x_id - (double)lp * (double)kLog2e);
+}
+
+// ---------------------------------------------------------------- backward
+constexpr int kBwdThreads = 256;
+
+// A warp takes a tile of a row at a time: one factor for bn consecutive
+// entries, 8 of them per lane and step.  The target's own entry is
+// c (1 - p) = -c expm1(logp), which bf16 E could not give where p is near 1.
+__global__ void __launch_bounds__(kBwdThreads)
+    logprob_bwd_kernel(__nv_bfloat16* __restrict__ e, int64_t lde, const float2* __restrict__ stats, int tiles,
+                       const float* __restrict__ lse2, const float* __restrict__ logp,
+                       const int64_t* __restrict__ ids, const int* __restrict__ perm, const float* __restrict__ g,
+                       float inv_tau, int V, int bn) {
+  pdl_prologue();
+  const int64_t t = blockIdx.x;
+  const int64_t id = ids[t];
+  const int src = perm[t];  // logp and g are in the caller's row order
+  const float c = id < 0 ? 0.f : g[src] * inv_tau;
+  const float l2 = lse2[t];
+  __nv_bfloat16* row = e + t * lde;
+  const int lane = threadIdx.x & 31;
+  const int warps = (int)gridDim.y * (kBwdThreads / 32);
+  for (int tile = blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += warps) {
+    const float f = id < 0 ? 0.f : -c * ex2(stats[t * tiles + tile].x - l2);
+    const int end = min(V, (tile + 1) * bn);
+    for (int col = tile * bn + lane * 8; col < end; col += 256) {
+      uint4* p4 = reinterpret_cast<uint4*>(row + col);
+      uint4 u = make_uint4(0u, 0u, 0u, 0u);
+      if (id >= 0) {
+        u = *p4;
+        uint32_t* p = &u.x;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 x = unpack_bf16x2(p[q]);
+          float a = x.x * f, b = x.y * f;
+          if (col + 2 * q == id) a = -c * expm1f(logp[src]);
+          if (col + 2 * q + 1 == id) b = -c * expm1f(logp[src]);
+          p[q] = pack_bf16x2(a, b);
+        }
+      }
+      *p4 = u;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- packing
+// Rows with a token first, in order, then the others: pos[t] is row t's place,
+// perm its inverse.  The packed rows without a token are zeros, so what stands
+// in them (padding, even NaN) cannot reach the head's gradient, a sum over
+// rows in which their coefficient is 0.
+// A block takes kPackRows rows and counts the ids before them itself (T ids
+// from L2; at T = 8192 a block reads 64 KB), so one launch does it all.
+constexpr int kPackThreads = 256;
+constexpr int kPackRows = 64;
+
+__global__ void __launch_bounds__(kPackThreads)
+    logprob_pack_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const int64_t* __restrict__ ids, int T,
+                        int H, __nv_bfloat16* __restrict__ hp, int64_t* __restrict__ idp, int* __restrict__ perm,
+                        int* __restrict__ pos, int* __restrict__ count) {
+  pdl_prologue();
+  __shared__ int s_before[kPackThreads / 32], s_total[kPackThreads / 32];
+  __shared__ int s_pos[kPackRows];
+  const int r0 = blockIdx.x * kPackRows;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int before = 0, total = 0;
+  for (int t = threadIdx.x; t < T; t += kPackThreads) {
+    const int v = ids[t] >= 0 ? 1 : 0;
+    total += v;
+    if (t < r0) before += v;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  if (lane == 0) {
+    s_before[warp] = before;
+    s_total[warp] = total;
+  }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int i = 0; i < kPackThreads / 32; ++i) {
+    before += s_before[i];
+    total += s_total[i];
+  }
+  if (warp == 0) {
+    for (int i = 0; i < kPackRows; i += 32) {
+      const int t = r0 + i + lane;
+      const int64_t id = t < T ? ids[t] : -1;
+      const uint32_t live = __ballot_sync(0xffffffffu, id >= 0);
+      const int mine = before + __popc(live & ((1u << lane) - 1u));
+      if (t < T) {
+        const int p = id >= 0 ? mine : total + (t - mine);
+        s_pos[i + lane] = p;
+        pos[t] = p;
+        perm[p] = t;
+        idp[p] = id;
+      }
+      before += __popc(live);
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) count[0] = total;
+  __syncthreads();
+  for (int i = warp; i < kPackRows && r0 + i < T; i += kPackThreads / 32) {
+    const int p = s_pos[i];
+    const uint4* src = reinterpret_cast<const uint4*>(h + (int64_t)(r0 + i) * ldh);
+    uint4* dst = reinterpret_cast<uint4*>(hp + (int64_t)p * H);
+    for (int k = lane; k < H / 8; k += 32) dst[k] = p < total ? src[k] : make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// dst[t] = src[pos[t]] for rows with a token, 0 for the others; a warp a row.
+__global__ void __launch_bounds__(256)
+    logprob_unpack_kernel(const __nv_bfloat16* __restrict__ src, const int* __restrict__ pos,
+                          const int* __restrict__ count, int T, int H, __nv_bfloat16* __restrict__ dst) {
+  pdl_prologue();
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (t >= T) return;
+  const int p = pos[t];
+  const bool live = p < count[0];
+  const uint4* s = reinterpret_cast<const uint4*>(src + (int64_t)p * H);
+  uint4* d = reinterpret_cast<uint4*>(dst + (int64_t)t * H);
+  for (int k = threadIdx.x & 31; k < H / 8; k += 32) d[k] = live ? s[k] : make_uint4(0u, 0u, 0u, 0u);
+}
+
+template <bool STORE>
+void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& te, const LogprobParams& p, int bn,
+                 float scale, cudaStream_t stream) {
+  auto kern = logprob_gemm_kernel<STORE>;
+  static std::mutex mu;
+  static int max_clusters[64] = {0};
+  int dev = 0;
+  PB_CUDA_CHECK(cudaGetDevice(&dev));
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  int clusters = 0;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (max_clusters[dev & 63] == 0) {
+      PB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+      cfg.gridDim = dim3(2 * num_sms(dev) / 2, 1, 1);
+      int n = 0;
+      PB_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+      PB_CHECK(n > 0, "logprob: no cluster of two CTAs fits on this GPU");
+      max_clusters[dev & 63] = n;
+    }
+    clusters = max_clusters[dev & 63];
+  }
+  const int64_t tiles = (int64_t)((p.T + 2 * BM_CTA - 1) / (2 * BM_CTA)) * ((p.V + bn - 1) / bn);
+  clusters = (int)std::max<int64_t>(1, std::min<int64_t>(clusters, tiles));
+  cfg.gridDim = dim3(2 * clusters, 1, 1);
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, te, p.ids, reinterpret_cast<float2*>(p.stats), p.T, p.V, p.H,
+                                   bn, scale, error_word(dev)));
+}
+
+}  // namespace
+
+int logprob_tile_n(int T, int V) {
+  (void)T;
+  (void)V;
+  return BN_MAX;
+}
+
+void logprob_fwd(const LogprobParams& p, cudaStream_t stream) {
+  PB_CHECK(p.T > 0 && p.V > 0 && p.H > 0, "logprob: empty problem");
+  PB_CHECK(p.H % 8 == 0 && p.ldh % 8 == 0 && p.ldw % 8 == 0,
+           "logprob: hidden size and row strides must be multiples of 8 elements");
+  PB_CHECK((reinterpret_cast<uintptr_t>(p.h) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.w) & 15) == 0,
+           "logprob: h and w must be 16-byte aligned");
+  const int bn = p.bn;
+  PB_CHECK(bn >= 32 && bn <= BN_MAX && bn % 32 == 0, "logprob: tile width must be a multiple of 32, at most 256");
+  const float scale = kLog2e * p.inv_tau;
+  const CUtensorMap ta = make_tmap_2d_bf16(p.h, p.H, p.T, p.ldh, BK, BM_CTA);
+  const CUtensorMap tb = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, bn / 2);
+  CUtensorMap te{};
+  if (p.e) {
+    PB_CHECK(p.lde % 8 == 0 && (reinterpret_cast<uintptr_t>(p.e) & 15) == 0, "logprob: E must have 16-byte rows");
+    te = make_tmap_2d_bf16_swz(p.e, p.V, p.T, p.lde, kBox, kBox, 64);
+    launch_gemm<true>(ta, tb, te, p, bn, scale, stream);
+  } else {
+    launch_gemm<false>(ta, tb, te, p, bn, scale, stream);
+  }
+  const int tiles = (p.V + bn - 1) / bn;
+  launch_k(logprob_finish_kernel, p.T, kFinThreads, 0, stream, (const __nv_bfloat16*)p.h, p.ldh,
+           (const __nv_bfloat16*)p.w, p.ldw, p.ids, p.perm, (const float2*)p.stats, tiles, p.V, p.H, scale, p.logp, p.lse2);
+}
+
+void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse2, const float* logp, const int64_t* ids,
+                 const int* perm, const float* g, float inv_tau, int T, int V, int bn, cudaStream_t stream) {
+  if (T == 0) return;
+  const int tiles = (V + bn - 1) / bn;
+  // enough blocks for every SM when there are few rows
+  const int segs = std::max(1, std::min((tiles + 7) / 8, (8 * num_sms() + T - 1) / T));
+  launch_k(logprob_bwd_kernel, dim3(T, segs), kBwdThreads, 0, stream, (__nv_bfloat16*)e, lde, (const float2*)stats,
+           tiles, lse2, logp, ids, perm, g, inv_tau, V, bn);
+}
+
+void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, void* hp, int64_t* idp, int* perm,
+                  int* pos, int* count, cudaStream_t stream) {
+  PB_CHECK(H % 8 == 0 && ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0 &&
+               (reinterpret_cast<uintptr_t>(hp) & 15) == 0,
+           "logprob: h must have 16-byte rows");
+  launch_k(logprob_pack_kernel, (T + kPackRows - 1) / kPackRows, kPackThreads, 0, stream, (const __nv_bfloat16*)h, ldh,
+           ids, T, H, (__nv_bfloat16*)hp, idp, perm, pos, count);
+}
+
+void logprob_unpack(const void* src, const int* pos, const int* count, int T, int H, void* dst, cudaStream_t stream) {
+  launch_k(logprob_unpack_kernel, (T + 7) / 8, 256, 0, stream, (const __nv_bfloat16*)src, pos, count, T, H,
+           (__nv_bfloat16*)dst);
+}
+
+}  // namespace pb

@@ -1,0 +1,157 @@
+"""Differentiable post-training objectives: what a trained language model is tuned with after pre-training.
+
+* ``lm_head_log_probs``  log-probabilities of given tokens through the LM head,
+  for scoring (no gradient: the logits are never stored) and for training.
+
+As in ``functional``, CUDA tensors run the sm_100a kernels and CPU tensors run
+the plain PyTorch statement of the same formula.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import gemm as G
+from ._ext import ext
+
+
+def _one_backward(ctx, what: str) -> None:
+    if getattr(ctx, "consumed", False):
+        raise RuntimeError(f"{what} supports one backward pass per forward")
+    ctx.consumed = True
+
+
+def _rows_bf16(t: torch.Tensor, what: str) -> torch.Tensor:
+    """``t`` as bf16 rows that TMA can read: unit inner stride, 16-byte row
+    stride and base (a copy if it has another layout)."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{what} must be bfloat16 on CUDA, got {t.dtype}")
+    if t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+# ----------------------------------------------------------------- log-probabilities through the LM head
+class _LMHeadLogProbsFn(torch.autograd.Function):
+    """The forward keeps bf16 exponentials of the logits (not the logits) for
+    at most ``max_block_bytes``; the backward scales them in place into the
+    logits' gradient and multiplies it with the head and the hidden states.
+    Rows beyond that are scored without storing and run through the forward
+    kernel again in the backward, block by block.  All of it works on the
+    packed rows: those with a token in front, zeros behind."""
+
+    @staticmethod
+    def forward(ctx, h, w, ids, inv_tau, max_block_bytes):
+        T, V = h.shape[0], w.shape[0]
+        hp, idp, perm, pos, count = ext().logprob_pack(h, ids)
+        logp = torch.empty(T, device=h.device, dtype=torch.float32)
+        block = _block_rows(T, V, max_block_bytes)
+        e = _exp_buffer(block, V, h.device)
+        lse2, stats, bn = ext().logprob_fwd(hp[:block], w, idp[:block], inv_tau, logp, e, perm[:block])
+        lses = [lse2]
+        for r0 in range(block, T, block):
+            rows = slice(r0, min(T, r0 + block))
+            lses.append(ext().logprob_fwd(hp[rows], w, idp[rows], inv_tau, logp, None, perm[rows])[0])
+        # kept outside save_for_backward: e is overwritten by the backward
+        ctx.kept = (e, stats, bn, lses)
+        ctx.save_for_backward(hp, w, idp, perm, pos, count, logp)
+        ctx.inv_tau, ctx.block = inv_tau, block
+        return logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        _one_backward(ctx, "lm_head_log_probs")
+        hp, w, idp, perm, pos, count, logp = ctx.saved_tensors
+        (e, stats, bn, lses), ctx.kept = ctx.kept, None
+        need_h, need_w = ctx.needs_input_grad[:2]
+        T, (V, H) = hp.shape[0], w.shape
+        g = g.contiguous()
+        dhp = torch.empty_like(hp) if need_h else None
+        single = ctx.block >= T
+        # one row block: the head's gradient is rounded once by its product; several
+        # blocks add up in fp32 first
+        dw = torch.empty(V, H, device=hp.device, dtype=w.dtype if single else torch.float32) if need_w else None
+        for i, r0 in enumerate(range(0, T, ctx.block)):
+            rows = slice(r0, min(T, r0 + ctx.block))
+            if r0:
+                e = e[:rows.stop - r0]
+                again = torch.empty_like(logp)  # the forward's logp stands
+                _, stats, bn = ext().logprob_fwd(hp[rows], w, idp[rows], ctx.inv_tau, again, e, perm[rows])
+            ext().logprob_bwd(e, stats, lses[i], idp[rows], perm[rows], logp, g, ctx.inv_tau, bn)
+            if need_h:
+                _grad_rows(e, w, dhp[rows])
+            if need_w:
+                _grad_head(e, hp[rows], dw, accumulate=r0 > 0)
+        dh = ext().logprob_unpack(dhp, pos, count) if need_h else None
+        if need_w and not single:
+            out = torch.empty(V, H, device=hp.device, dtype=w.dtype)
+            ext().cast_f32_to_bf16(dw, out)
+            dw = out
+        return dh, dw, None, None, None
+
+
+def _grad_rows(dl: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> None:
+    """``out = dl @ w`` over the vocabulary."""
+    ext().gemm(dl, w, out, False, True, G.EPI_STORE_BF16, 1.0)
+
+
+def _grad_head(dl: torch.Tensor, h: torch.Tensor, out: torch.Tensor, accumulate: bool) -> None:
+    """``out (+)= dl.T @ h``, out bf16 or (over several row blocks) fp32."""
+    if out.dtype == torch.bfloat16:
+        epi = G.EPI_STORE_BF16
+    else:
+        epi = G.EPI_ACCUM_F32 if accumulate else G.EPI_STORE_F32
+    ext().gemm(dl, h, out, True, True, epi, 1.0)
+
+
+def _block_rows(T: int, V: int, max_block_bytes: int) -> int:
+    """Rows of a [rows, V] bf16 block of at most ``max_block_bytes`` (whole
+    256-row tiles, one at least)."""
+    return max(1, min(T, max(256, int(max_block_bytes // (V * 2)) // 256 * 256)))
+
+
+def _exp_buffer(rows: int, V: int, device) -> torch.Tensor:
+    """bf16 [rows, V] with 128-byte aligned rows."""
+    return torch.empty(rows, (V + 63) // 64 * 64, device=device, dtype=torch.bfloat16)[:, :V]
+
+
+def lm_head_log_probs(h: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, temperature: float = 1.0,
+                      max_block_bytes: int = 6 << 30) -> torch.Tensor:
+    """fp32 ``log_softmax(h @ w.T / temperature)[..., ids]``, shaped as ``ids``.
+
+    h [..., H] hidden states, w [V, H] the LM head, ids int64 with one entry
+    per row of h.  A negative id (``IGNORE_INDEX``) marks a row without a
+    token: its log-probability is 0 and it sends back no gradient.  An id >= V
+    gives NaN (an ``IndexError`` on CPU).  The gradient goes to h and w; one
+    backward pass per forward.  ``max_block_bytes`` bounds the [rows, V] block
+    held between forward and backward; rows beyond it are computed twice."""
+    if not temperature > 0.0:
+        raise ValueError(f"temperature has to be positive, got {temperature}")
+    if w.dim() != 2 or h.shape[-1] != w.shape[1]:
+        raise ValueError(f"h {tuple(h.shape)} and w {tuple(w.shape)} must share their last dimension")
+    if ids.dtype != torch.int64 or ids.numel() * h.shape[-1] != h.numel():
+        raise ValueError(f"ids must be int64 with one entry per row of h, got {ids.dtype} {tuple(ids.shape)} for "
+                         f"{tuple(h.shape)}")
+    h2, flat = h.reshape(-1, h.shape[-1]), ids.reshape(-1).contiguous()
+    if not h2.is_cuda:
+        return _log_probs_plain(h2, w, flat, temperature).view(ids.shape)
+    if flat.numel() == 0:
+        return (h2.float().sum(-1) + w[:0].float().sum()).view(ids.shape)
+    h2, w = _rows_bf16(h2, "h"), _rows_bf16(w, "w")
+    inv_tau = 1.0 / float(temperature)
+    if torch.is_grad_enabled() and (h2.requires_grad or w.requires_grad):
+        return _LMHeadLogProbsFn.apply(h2, w, flat, inv_tau, max_block_bytes).view(ids.shape)
+    logp = torch.empty(flat.shape, device=h.device, dtype=torch.float32)
+    ext().logprob_fwd(h2, w, flat, inv_tau, logp)
+    return logp.view(ids.shape)
+
+
+def _log_probs_plain(h, w, ids, temperature):
+    if ids.numel() and int(ids.max()) >= w.shape[0]:
+        raise IndexError(f"token id {int(ids.max())} is outside the vocabulary of {w.shape[0]}")
+    rows = (ids >= 0).nonzero()[:, 0]
+    logp = torch.log_softmax(F.linear(h[rows], w).float() / temperature, dim=-1)
+    picked = logp.gather(1, ids[rows][:, None])[:, 0]
+    return torch.zeros(ids.shape, dtype=torch.float32, device=h.device).index_put((rows,), picked)

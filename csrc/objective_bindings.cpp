@@ -3,7 +3,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <limits>
+#include <string>
 #include <vector>
 
 #include "objectives.cuh"
@@ -14,8 +16,13 @@ cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 constexpr int64_t kIntMax = std::numeric_limits<int>::max();
 
+// Numbers enter error messages as strings: where the extension carries its own
+// copy of the C++ runtime, streaming an integer into a message would use a
+// locale of the other copy and crash instead of raising.
+std::string num(int64_t n) { return std::to_string(n); }
+
 #define CHECK_SAME_DEVICE(a, b) \
-  TORCH_CHECK((a).device() == (b).device(), #a " and " #b " must be on one device, got ", (a).device(), " and ", (b).device())
+  TORCH_CHECK((a).device() == (b).device(), #a " and " #b " must be on one device, got ", (a).device().str(), " and ", (b).device().str())
 
 void check_rows_bf16(const at::Tensor& t, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.stride(1) == 1, what,
@@ -29,13 +36,13 @@ void check_ids(const at::Tensor& ids, int64_t T, const char* what) {
 
 int* check_rows_i32(const at::Tensor& t, int64_t n, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() == n, what,
-              " must be contiguous CUDA int32 of ", n, " entries");
+              " must be contiguous CUDA int32 of ", num(n), " entries");
   return t.data_ptr<int>();
 }
 
 float* check_rows_f32(const at::Tensor& t, int64_t n, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == n, what,
-              " must be contiguous CUDA fp32 of ", n, " entries");
+              " must be contiguous CUDA fp32 of ", num(n), " entries");
   return t.data_ptr<float>();
 }
 
@@ -80,7 +87,7 @@ std::tuple<at::Tensor, at::Tensor, int64_t> logprob_fwd(const at::Tensor& h, con
   check_rows_bf16(h, "logprob: h");
   check_rows_bf16(w, "logprob: w");
   const int64_t T = h.size(0), H = h.size(1), V = w.size(0);
-  TORCH_CHECK(w.size(1) == H, "logprob: h has ", H, " columns, w has ", w.size(1));
+  TORCH_CHECK(w.size(1) == H, "logprob: h has ", num(H), " columns, w has ", num(w.size(1)));
   TORCH_CHECK(T >= 1 && V >= 1 && T <= kIntMax / 2 && V <= kIntMax / 2, "logprob: row and vocabulary counts");
   check_ids(ids, T, "logprob: ids");
   TORCH_CHECK(logp.is_cuda() && logp.scalar_type() == at::kFloat && logp.is_contiguous() && logp.numel() >= T,
@@ -144,6 +151,171 @@ void logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor& lse2,
                   (float)inv_tau, (int)T, (int)V, (int)bn, cur_stream());
 }
 
+// ---------------------------------------------------------------- policy and preference losses
+const float* check_tokens(const at::Tensor& t, int64_t B, int64_t S, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(0) == B && t.size(1) == S &&
+                  (t.stride(1) == 1 || S <= 1),
+              what, " must be CUDA fp32 [", num(B), ", ", num(S), "] with unit inner stride");
+  return t.data_ptr<float>();
+}
+
+const uint8_t* check_mask(const at::Tensor& t, int64_t B, int64_t S) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBool && t.dim() == 2 && t.size(0) == B && t.size(1) == S &&
+                  (t.stride(1) == 1 || S <= 1),
+              "mask must be CUDA bool [", num(B), ", ", num(S), "] with unit inner stride");
+  return reinterpret_cast<const uint8_t*>(t.data_ptr<bool>());
+}
+
+bool given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+
+struct Chunks {
+  int chunk, n;
+};
+Chunks chunks_of(int64_t rows, int64_t S) {
+  TORCH_CHECK(rows <= kIntMax && S <= kIntMax, "token log-probabilities: at most 2^31 - 1 rows and columns");
+  const int chunk = pb::objective_chunk(rows, S);
+  const int64_t n = std::max<int64_t>(1, (S + chunk - 1) / chunk);
+  TORCH_CHECK(rows * n <= kIntMax, "token log-probabilities: too many tokens for one call");
+  return {chunk, (int)n};
+}
+
+// policy_fwd(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence, want_grad) ->
+// (loss, clip fraction, kl, coef or None, inv, inv_row or None)
+std::vector<c10::optional<at::Tensor>> policy_fwd(const at::Tensor& logp, const at::Tensor& old, const at::Tensor& adv,
+                                                  const c10::optional<at::Tensor>& mask,
+                                                  const c10::optional<at::Tensor>& ref, double low, double high,
+                                                  double kl_coef, bool per_sequence, bool want_grad) {
+  TORCH_CHECK(logp.dim() == 2, "policy_fwd: logp [B, S]");
+  const int64_t B = logp.size(0), S = logp.size(1);
+  pb::PolicyParams p{};
+  p.logp = check_tokens(logp, B, S, "policy_fwd: logp");
+  p.old = check_tokens(old, B, S, "policy_fwd: old log-probabilities");
+  TORCH_CHECK(adv.is_cuda() && adv.scalar_type() == at::kFloat && adv.dim() == 2 && adv.size(0) == B && adv.size(1) == S,
+              "policy_fwd: advantages must be CUDA fp32 [B, S] (any strides)");
+  CHECK_SAME_DEVICE(logp, old);
+  CHECK_SAME_DEVICE(logp, adv);
+  p.adv = adv.data_ptr<float>();
+  p.ld_logp = logp.stride(0);
+  p.ld_old = old.stride(0);
+  p.adv_sb = adv.stride(0);
+  p.adv_ss = adv.stride(1);
+  if (given(mask)) {
+    CHECK_SAME_DEVICE(logp, *mask);
+    p.mask = check_mask(*mask, B, S);
+    p.ld_mask = mask->stride(0);
+  }
+  if (given(ref)) {
+    CHECK_SAME_DEVICE(logp, *ref);
+    p.ref = check_tokens(*ref, B, S, "policy_fwd: reference log-probabilities");
+    p.ld_ref = ref->stride(0);
+  }
+  const c10::cuda::CUDAGuard g(logp.device());
+  const Chunks c = chunks_of(B, S);
+  p.B = (int)B;
+  p.S = (int)S;
+  p.chunk = c.chunk;
+  p.nchunk = c.n;
+  p.low = (float)low;
+  p.high = (float)high;
+  p.kl_coef = (float)kl_coef;
+  p.per_sequence = per_sequence;
+  const auto f32 = logp.options();
+  at::Tensor loss = at::empty({}, f32), clip = at::empty({}, f32), kl = at::empty({}, f32);
+  // scratch: 4 floats per chunk, then the ticket
+  at::Tensor scratch = at::empty({B * c.n * 4 + 1}, f32);
+  at::Tensor inv = at::empty({1}, f32);
+  c10::optional<at::Tensor> coef, inv_row;
+  if (want_grad) coef = at::empty({B, S}, f32);
+  if (per_sequence) inv_row = at::empty({B}, f32);
+  p.coef = want_grad ? coef->data_ptr<float>() : nullptr;
+  p.inv_row = per_sequence ? inv_row->data_ptr<float>() : nullptr;
+  p.inv = inv.data_ptr<float>();
+  p.loss = loss.data_ptr<float>();
+  p.clip = clip.data_ptr<float>();
+  p.kl = kl.data_ptr<float>();
+  p.parts = reinterpret_cast<float4*>(scratch.data_ptr<float>());
+  p.ticket = reinterpret_cast<int*>(scratch.data_ptr<float>() + B * c.n * 4);
+  pb::policy_fwd(p, cur_stream());
+  return {loss, clip, kl, coef, inv, inv_row};
+}
+
+// policy_bwd(coef [B, S], g scalar, inv, inv_row or None) -> d loss / d logp [B, S]
+at::Tensor policy_bwd(const at::Tensor& coef, const at::Tensor& g, const at::Tensor& inv,
+                      const c10::optional<at::Tensor>& inv_row) {
+  TORCH_CHECK(coef.dim() == 2, "policy_bwd: coef [B, S]");
+  const int64_t B = coef.size(0), S = coef.size(1);
+  const float* cp = check_rows_f32(coef, B * S, "policy_bwd: coef");
+  const float* rp = given(inv_row) ? check_rows_f32(*inv_row, B, "policy_bwd: inv_row") : nullptr;
+  CHECK_SAME_DEVICE(coef, g);
+  const c10::cuda::CUDAGuard guard(coef.device());
+  at::Tensor out = at::empty_like(coef);
+  const Chunks c = chunks_of(B, S);
+  pb::policy_bwd(cp, check_rows_f32(g, 1, "policy_bwd: g"), check_rows_f32(inv, 1, "policy_bwd: inv"), rp,
+                 out.data_ptr<float>(), (int)B, (int)S, c.chunk, c.n, cur_stream());
+  return out;
+}
+
+// preference_fwd(logp [2P, S], ref, mask, beta, smoothing, average) -> (loss, rewards [2P], coef [2P])
+std::vector<at::Tensor> preference_fwd(const at::Tensor& logp, const c10::optional<at::Tensor>& ref,
+                                       const c10::optional<at::Tensor>& mask, double beta, double smoothing,
+                                       bool average) {
+  TORCH_CHECK(logp.dim() == 2 && logp.size(0) >= 2 && logp.size(0) % 2 == 0, "preference_fwd: logp [2P, S], P >= 1");
+  const int64_t B = logp.size(0), S = logp.size(1);
+  pb::PreferenceParams p{};
+  p.logp = check_tokens(logp, B, S, "preference_fwd: logp");
+  p.ld_logp = logp.stride(0);
+  if (given(ref)) {
+    CHECK_SAME_DEVICE(logp, *ref);
+    p.ref = check_tokens(*ref, B, S, "preference_fwd: reference log-probabilities");
+    p.ld_ref = ref->stride(0);
+  }
+  if (given(mask)) {
+    CHECK_SAME_DEVICE(logp, *mask);
+    p.mask = check_mask(*mask, B, S);
+    p.ld_mask = mask->stride(0);
+  }
+  const c10::cuda::CUDAGuard g(logp.device());
+  const Chunks c = chunks_of(B, S);
+  p.P = (int)(B / 2);
+  p.S = (int)S;
+  p.chunk = c.chunk;
+  p.nchunk = c.n;
+  p.beta = (float)beta;
+  p.smoothing = (float)smoothing;
+  p.average = average;
+  const auto f32 = logp.options();
+  at::Tensor loss = at::empty({}, f32), rewards = at::empty({B}, f32), coef = at::empty({B}, f32);
+  at::Tensor scratch = at::empty({B * c.n * 2 + 1}, f32);
+  p.parts = reinterpret_cast<float2*>(scratch.data_ptr<float>());
+  p.ticket = reinterpret_cast<int*>(scratch.data_ptr<float>() + B * c.n * 2);
+  p.loss = loss.data_ptr<float>();
+  p.rewards = rewards.data_ptr<float>();
+  p.coef = coef.data_ptr<float>();
+  pb::preference_fwd(p, cur_stream());
+  return {loss, rewards, coef};
+}
+
+// preference_bwd(coef [2P], g scalar, mask or None, S) -> d loss / d logp [2P, S]
+at::Tensor preference_bwd(const at::Tensor& coef, const at::Tensor& g, const c10::optional<at::Tensor>& mask,
+                          int64_t S) {
+  const int64_t B = coef.numel();
+  const float* cp = check_rows_f32(coef, B, "preference_bwd: coef");
+  const uint8_t* mp = nullptr;
+  int64_t ldm = 0;
+  if (given(mask)) {
+    CHECK_SAME_DEVICE(coef, *mask);
+    mp = check_mask(*mask, B, S);
+    ldm = mask->stride(0);
+  }
+  CHECK_SAME_DEVICE(coef, g);
+  const c10::cuda::CUDAGuard guard(coef.device());
+  at::Tensor out = at::empty({B, S}, coef.options());
+  const Chunks c = chunks_of(B, S);
+  pb::preference_bwd(cp, check_rows_f32(g, 1, "preference_bwd: g"), mp, ldm, out.data_ptr<float>(), (int)B, (int)S,
+                     c.chunk, c.n, cur_stream());
+  return out;
+}
+
 }  // namespace
 
 void register_objectives(pybind11::module& m) {
@@ -154,4 +326,10 @@ void register_objectives(pybind11::module& m) {
         py::arg("e") = py::none(), py::arg("perm") = py::none());
   m.def("logprob_bwd", &logprob_bwd, py::arg("e"), py::arg("stats"), py::arg("lse2"), py::arg("ids"), py::arg("perm"),
         py::arg("logp"), py::arg("g"), py::arg("inv_tau"), py::arg("bn"));
+  m.def("policy_fwd", &policy_fwd, py::arg("logp"), py::arg("old"), py::arg("adv"), py::arg("mask"), py::arg("ref"),
+        py::arg("low"), py::arg("high"), py::arg("kl_coef"), py::arg("per_sequence"), py::arg("want_grad"));
+  m.def("policy_bwd", &policy_bwd, py::arg("coef"), py::arg("g"), py::arg("inv"), py::arg("inv_row"));
+  m.def("preference_fwd", &preference_fwd, py::arg("logp"), py::arg("ref"), py::arg("mask"), py::arg("beta"),
+        py::arg("smoothing"), py::arg("average"));
+  m.def("preference_bwd", &preference_bwd, py::arg("coef"), py::arg("g"), py::arg("mask"), py::arg("S"));
 }

@@ -1,0 +1,290 @@
+// Losses over token log-probabilities [B, S] (fp32): the clipped policy loss
+// with a KL term and the preference loss over pairs of sequences.
+//
+// Both are bound by launch latency up to some 100k tokens and by memory above
+// (17 / 9 bytes read per token).  One launch forward, one backward: a warp
+// sums a chunk of one row, writes the chunk's partial sums, and the last
+// block to finish adds the partials in chunk order (fp64), so the results
+// have the same bits on every run.  Positions outside the mask are never
+// part of an operation: they may hold anything.
+#include <math.h>
+
+#include <algorithm>
+
+#include "host_util.h"
+#include "objectives.cuh"
+#include "ptx.cuh"
+
+namespace pb {
+namespace {
+
+constexpr int kWarps = 8;          // per block when there are many units
+constexpr int kOneBlockUnits = 32;  // up to this many units one block does it all, without a ticket
+
+__device__ __forceinline__ float warp_add(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sum of one double per thread over the block; the same order on every run.
+// Every thread gets the sum; `sh` holds 32 doubles.
+__device__ __forceinline__ double block_add(double v, double* sh) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) v += sh[i];
+  return v;
+}
+
+// True in every thread of the last block to arrive (ticket zeroed before the
+// launch); the partials of all blocks are then visible.
+__device__ __forceinline__ bool last_block(int* ticket) {
+  if (gridDim.x == 1) {
+    __syncthreads();
+    return true;
+  }
+  __shared__ bool last;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(ticket, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (last) __threadfence();
+  return last;
+}
+
+__global__ void __launch_bounds__(1024) policy_fwd_kernel(const PolicyParams p) {
+  pdl_prologue();
+  const int lane = threadIdx.x & 31;
+  const int64_t units = (int64_t)p.B * p.nchunk;
+  const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (unit < units) {
+    const int64_t b = unit / p.nchunk;
+    const int64_t s0 = (unit % p.nchunk) * p.chunk;
+    const int64_t s1 = min((int64_t)p.S, s0 + p.chunk);
+    const float* lp = p.logp + b * p.ld_logp;
+    const float* old = p.old + b * p.ld_old;
+    const float* ref = p.ref ? p.ref + b * p.ld_ref : nullptr;
+    const float* adv = p.adv + b * p.adv_sb;
+    const uint8_t* mask = p.mask ? p.mask + b * p.ld_mask : nullptr;
+    float loss = 0.f, n = 0.f, clip = 0.f, kl = 0.f;
+#pragma unroll 4
+    for (int64_t s = s0 + lane; s < s1; s += 32) {
+      float coef = 0.f;
+      if (!mask || mask[s]) {
+        const float l = lp[s], a = adv[s * p.adv_ss];
+        const float r = expf(l - old[s]);
+        const float u = r * a;
+        const float c = fminf(fmaxf(r, p.low), p.high) * a;
+        const bool clipped = u > c;  // false for NaN: u carries it on
+        float per = clipped ? -c : -u;
+        coef = clipped ? 0.f : -u;
+        if (ref) {
+          const float x = ref[s] - l;
+          const float e = expm1f(x);  // exp(x) - 1 - x without the cancellation at small x
+          kl += e - x;
+          per += p.kl_coef * (e - x);
+          coef -= p.kl_coef * e;
+        }
+        loss += per;
+        n += 1.f;
+        clip += clipped ? 1.f : 0.f;
+      }
+      if (p.coef) p.coef[b * p.S + s] = coef;
+    }
+    loss = warp_add(loss);
+    n = warp_add(n);
+    clip = warp_add(clip);
+    kl = warp_add(kl);
+    if (lane == 0) p.parts[unit] = make_float4(loss, n, clip, kl);
+  }
+  if (!last_block(p.ticket)) return;
+  __shared__ double sh[32];
+  double loss = 0.0, n = 0.0, clip = 0.0, kl = 0.0;
+  if (!p.per_sequence) {
+    for (int64_t i = threadIdx.x; i < units; i += blockDim.x) {
+      const float4 v = __ldcg(p.parts + i);
+      loss += v.x;
+      n += v.y;
+      clip += v.z;
+      kl += v.w;
+    }
+  } else {
+    double live = 0.0;
+    for (int64_t b = threadIdx.x; b < p.B; b += blockDim.x) {
+      double row = 0.0, rn = 0.0;
+      for (int c = 0; c < p.nchunk; ++c) {
+        const float4 v = __ldcg(p.parts + b * p.nchunk + c);
+        row += v.x;
+        rn += v.y;
+        clip += v.z;
+        kl += v.w;
+      }
+      if (rn > 0.0) {
+        loss += row / rn;
+        live += 1.0;
+      }
+      n += rn;
+      p.inv_row[b] = rn > 0.0 ? (float)(1.0 / rn) : 0.f;
+    }
+    live = block_add(live, sh);
+    if (threadIdx.x == 0) p.inv[0] = (float)(1.0 / fmax(live, 1.0));
+    loss /= fmax(live, 1.0);
+  }
+  loss = block_add(loss, sh);
+  n = block_add(n, sh);
+  clip = block_add(clip, sh);
+  kl = block_add(kl, sh);
+  if (threadIdx.x == 0) {
+    const double inv = 1.0 / fmax(n, 1.0);
+    if (!p.per_sequence) p.inv[0] = (float)inv;
+    p.loss[0] = (float)(p.per_sequence ? loss : loss * inv);
+    p.clip[0] = (float)(clip * inv);
+    p.kl[0] = (float)(kl * inv);
+  }
+}
+
+// out = coef * g * inv (* inv_row of its row)
+__global__ void __launch_bounds__(kWarps * 32)
+    policy_bwd_kernel(const float* __restrict__ coef, const float* __restrict__ g, const float* __restrict__ inv,
+                      const float* __restrict__ inv_row, float* __restrict__ out, int B, int S, int chunk,
+                      int nchunk) {
+  pdl_prologue();
+  const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (unit >= (int64_t)B * nchunk) return;
+  const int64_t b = unit / nchunk;
+  const int64_t s0 = (unit % nchunk) * chunk, s1 = min((int64_t)S, s0 + chunk);
+  const float w = g[0] * inv[0] * (inv_row ? inv_row[b] : 1.f);
+#pragma unroll 4
+  for (int64_t s = s0 + (threadIdx.x & 31); s < s1; s += 32) {
+    const float c = coef[b * S + s];
+    out[b * S + s] = c == 0.f ? 0.f : c * w;  // exactly 0 outside the mask, whatever g is
+  }
+}
+
+__global__ void __launch_bounds__(1024) preference_fwd_kernel(const PreferenceParams p) {
+  pdl_prologue();
+  const int lane = threadIdx.x & 31;
+  const int rows = 2 * p.P;
+  const int64_t units = (int64_t)rows * p.nchunk;
+  const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (unit < units) {
+    const int64_t b = unit / p.nchunk;
+    const int64_t s0 = (unit % p.nchunk) * p.chunk;
+    const int64_t s1 = min((int64_t)p.S, s0 + p.chunk);
+    const float* lp = p.logp + b * p.ld_logp;
+    const float* ref = p.ref ? p.ref + b * p.ld_ref : nullptr;
+    const uint8_t* mask = p.mask ? p.mask + b * p.ld_mask : nullptr;
+    float d = 0.f, n = 0.f;
+#pragma unroll 4
+    for (int64_t s = s0 + lane; s < s1; s += 32) {
+      if (!mask || mask[s]) {
+        d += lp[s] - (ref ? ref[s] : 0.f);
+        n += 1.f;
+      }
+    }
+    d = warp_add(d);
+    n = warp_add(n);
+    if (lane == 0) p.parts[unit] = make_float2(d, n);
+  }
+  if (!last_block(p.ticket)) return;
+  __shared__ double sh[32];
+  double loss = 0.0;
+  for (int i = threadIdx.x; i < p.P; i += blockDim.x) {
+    double r[2], w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {  // the chosen row, the rejected row
+      const int64_t b = i + (int64_t)k * p.P;
+      double d = 0.0, n = 0.0;
+      for (int c = 0; c < p.nchunk; ++c) {
+        const float2 v = __ldcg(p.parts + b * p.nchunk + c);
+        d += v.x;
+        n += v.y;
+      }
+      w[k] = (double)p.beta / (p.average ? fmax(n, 1.0) : 1.0);
+      r[k] = w[k] * d;
+      p.rewards[b] = (float)r[k];
+    }
+    const float gap = (float)(r[0] - r[1]);
+    const float soft = log1pf(expf(-fabsf(gap)));  // -log sigmoid(x) = soft + max(-x, 0)
+    const float neg = gap < 0.f ? -gap : 0.f, pos = gap > 0.f ? gap : 0.f;
+    const float e = p.smoothing;
+    loss += (double)((1.f - e) * (soft + neg) + e * (soft + pos));
+    // sigmoid(-gap) and sigmoid(gap), each without cancellation
+    const float t = expf(-fabsf(gap));
+    const float small = t / (1.f + t), big = 1.f / (1.f + t);
+    const float s_neg = gap >= 0.f ? small : big, s_pos = gap >= 0.f ? big : small;
+    const float dgap = (e * s_pos - (1.f - e) * s_neg) / (float)p.P;
+    p.coef[i] = (float)(w[0] * (double)dgap);
+    p.coef[i + p.P] = (float)(-w[1] * (double)dgap);
+  }
+  loss = block_add(loss, sh);
+  if (threadIdx.x == 0) p.loss[0] = (float)(loss / (double)p.P);
+}
+
+// out = g * coef[row] inside the mask, 0 outside
+__global__ void __launch_bounds__(kWarps * 32)
+    preference_bwd_kernel(const float* __restrict__ coef, const float* __restrict__ g,
+                          const uint8_t* __restrict__ mask, int64_t ld_mask, float* __restrict__ out, int rows, int S,
+                          int chunk, int nchunk) {
+  pdl_prologue();
+  const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (unit >= (int64_t)rows * nchunk) return;
+  const int64_t b = unit / nchunk;
+  const int64_t s0 = (unit % nchunk) * chunk, s1 = min((int64_t)S, s0 + chunk);
+  const float w = g[0] * coef[b];
+#pragma unroll 4
+  for (int64_t s = s0 + (threadIdx.x & 31); s < s1; s += 32)
+    out[b * S + s] = (!mask || mask[b * ld_mask + s]) ? w : 0.f;
+}
+
+int unit_blocks(int64_t units) { return (int)((units + kWarps - 1) / kWarps); }
+
+}  // namespace
+
+// Tokens of a row that one warp sums: long enough to amortise its reduction,
+// short enough that a small batch still covers the SMs (8 warps on each).
+int objective_chunk(int64_t rows, int64_t S) {
+  int chunk = 1024;
+  while (chunk > 128 && rows * ((S + chunk - 1) / chunk) < (int64_t)8 * num_sms()) chunk /= 2;
+  return chunk;
+}
+
+void policy_fwd(const PolicyParams& p, cudaStream_t stream) {
+  const int64_t units = (int64_t)p.B * p.nchunk;
+  if (units <= kOneBlockUnits) {
+    launch_k(policy_fwd_kernel, 1, 32 * std::max<int>(1, (int)units), 0, stream, p);
+    return;
+  }
+  PB_CUDA_CHECK(cudaMemsetAsync(p.ticket, 0, sizeof(int), stream));
+  launch_k(policy_fwd_kernel, unit_blocks(units), 32 * kWarps, 0, stream, p);
+}
+
+void policy_bwd(const float* coef, const float* g, const float* inv, const float* inv_row, float* out, int B, int S,
+                int chunk, int nchunk, cudaStream_t stream) {
+  if (B == 0 || S == 0) return;
+  launch_k(policy_bwd_kernel, unit_blocks((int64_t)B * nchunk), 32 * kWarps, 0, stream, coef, g, inv, inv_row, out, B,
+           S, chunk, nchunk);
+}
+
+void preference_fwd(const PreferenceParams& p, cudaStream_t stream) {
+  const int64_t units = (int64_t)2 * p.P * p.nchunk;
+  if (units <= kOneBlockUnits) {
+    launch_k(preference_fwd_kernel, 1, 32 * std::max<int>(1, (int)units), 0, stream, p);
+    return;
+  }
+  PB_CUDA_CHECK(cudaMemsetAsync(p.ticket, 0, sizeof(int), stream));
+  launch_k(preference_fwd_kernel, unit_blocks(units), 32 * kWarps, 0, stream, p);
+}
+
+void preference_bwd(const float* coef, const float* g, const uint8_t* mask, int64_t ld_mask, float* out, int rows,
+                    int S, int chunk, int nchunk, cudaStream_t stream) {
+  if (rows == 0 || S == 0) return;
+  launch_k(preference_bwd_kernel, unit_blocks((int64_t)rows * nchunk), 32 * kWarps, 0, stream, coef, g, mask, ld_mask,
+           out, rows, S, chunk, nchunk);
+}
+
+}  // namespace pb

@@ -40,4 +40,41 @@ void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, 
 // dst[t] = src[pos[t]] where row t has a token, else 0
 void logprob_unpack(const void* src, const int* pos, const int* count, int T, int H, void* dst, cudaStream_t stream);
 
+// ---- losses over token log-probabilities (objectives.cu); rows b have their
+// own strides, mask is bool bytes (optional).  chunk: objective_chunk(rows, S),
+// nchunk = max(1, ceil(S / chunk)); parts and ticket are scratch.
+int objective_chunk(int64_t rows, int64_t S);
+struct PolicyParams {
+  const float *logp, *old, *adv, *ref;  // ref optional
+  const uint8_t* mask;
+  int64_t ld_logp, ld_old, adv_sb, adv_ss, ld_ref, ld_mask;
+  int B, S, chunk, nchunk;
+  float low, high, kl_coef;  // the clip range [low, high] of the ratio
+  bool per_sequence;         // mean over rows of the row means, else mean over tokens
+  float* coef;               // optional [B, S]: d (token loss) / d logp, 0 outside the mask
+  float4* parts;             // [B * nchunk]
+  int* ticket;
+  float *loss, *clip, *kl;  // scalars
+  float *inv, *inv_row;     // gradient = coef * inv (* inv_row [B] when per_sequence)
+};
+void policy_fwd(const PolicyParams& p, cudaStream_t stream);
+void policy_bwd(const float* coef, const float* g, const float* inv, const float* inv_row, float* out, int B, int S,
+                int chunk, int nchunk, cudaStream_t stream);
+
+// rows [0, P) are the chosen sequences, rows [P, 2P) the rejected ones
+struct PreferenceParams {
+  const float *logp, *ref;  // ref optional
+  const uint8_t* mask;
+  int64_t ld_logp, ld_ref, ld_mask;
+  int P, S, chunk, nchunk;
+  float beta, smoothing;
+  bool average;
+  float2* parts;  // [2P * nchunk]
+  int* ticket;
+  float *loss, *rewards, *coef;  // scalar, [2P], [2P]: d loss / d (logp of a token of the row)
+};
+void preference_fwd(const PreferenceParams& p, cudaStream_t stream);
+void preference_bwd(const float* coef, const float* g, const uint8_t* mask, int64_t ld_mask, float* out, int rows,
+                    int S, int chunk, int nchunk, cudaStream_t stream);
+
 }  // namespace pb

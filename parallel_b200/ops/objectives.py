@@ -1,12 +1,19 @@
 """Differentiable post-training objectives: what a trained language model is tuned with after pre-training.
 
 * ``lm_head_log_probs``  log-probabilities of given tokens through the LM head,
-  for scoring (no gradient: the logits are never stored) and for training.
+  for scoring (no gradient: the logits are never stored) and for training;
+* ``policy_loss``        clipped policy-gradient loss with a KL term over token
+  log-probabilities;
+* ``preference_loss``    loss on paired sequences (log-ratio of the chosen and
+  the rejected one against a reference).
 
 As in ``functional``, CUDA tensors run the sm_100a kernels and CPU tensors run
 the plain PyTorch statement of the same formula.
 """
 from __future__ import annotations
+
+import math
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
@@ -155,3 +162,167 @@ def _log_probs_plain(h, w, ids, temperature):
     logp = torch.log_softmax(F.linear(h[rows], w).float() / temperature, dim=-1)
     picked = logp.gather(1, ids[rows][:, None])[:, 0]
     return torch.zeros(ids.shape, dtype=torch.float32, device=h.device).index_put((rows,), picked)
+
+
+# ----------------------------------------------------------------- losses over token log-probabilities
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor           # scalar, differentiable in logp
+    clip_fraction: torch.Tensor  # share of the tokens whose ratio was clipped
+    kl: torch.Tensor             # mean over the tokens of the KL estimate (0 without a reference)
+
+
+class PreferenceLoss(NamedTuple):
+    loss: torch.Tensor     # scalar, differentiable in logp
+    rewards: torch.Tensor  # [2P] beta x log ratio of each sequence (chosen rows, then rejected rows)
+
+
+def _tokens(t: torch.Tensor | None, like: torch.Tensor, what: str) -> torch.Tensor | None:
+    """fp32 [B, S] without gradient, rows of unit inner stride."""
+    if t is None:
+        return None
+    if t.dtype != like.dtype:
+        raise TypeError(f"{what} must be {like.dtype}, got {t.dtype}")
+    if t.shape != like.shape:
+        raise ValueError(f"{what} {tuple(t.shape)} must have logp's shape {tuple(like.shape)}")
+    t = t.detach()
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _check_logp(logp: torch.Tensor, mask: torch.Tensor | None) -> None:
+    if logp.dim() != 2 or (logp.is_cuda and logp.dtype != torch.float32) or not logp.is_floating_point():
+        raise ValueError(f"logp must be fp32 [sequences, tokens], got {logp.dtype} {tuple(logp.shape)}")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != logp.shape):
+        raise ValueError(f"mask must be bool {tuple(logp.shape)}, got {mask.dtype} {tuple(mask.shape)}")
+
+
+def _unit_inner(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
+class _PolicyLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logp, old, adv, mask, ref, low, high, kl_coef, per_sequence):
+        loss, clip, kl, coef, inv, inv_row = ext().policy_fwd(logp, old, adv, mask, ref, low, high, kl_coef,
+                                                              per_sequence, True)
+        ctx.save_for_backward(coef, inv, inv_row)
+        ctx.mark_non_differentiable(clip, kl)
+        return loss, clip, kl
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _clip, _kl):
+        coef, inv, inv_row = ctx.saved_tensors
+        return (ext().policy_bwd(coef, g, inv, inv_row),) + (None,) * 8
+
+
+def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
+                mask: torch.Tensor | None = None, ref_logp: torch.Tensor | None = None, clip_low: float = 0.2,
+                clip_high: float = 0.2, kl_coef: float = 0.0, reduction: str = "token") -> PolicyLoss:
+    """Clipped policy loss of token log-probabilities, logp fp32 [B, S].
+
+    With r = exp(logp - old_logp) and advantage A, a token's loss is
+    ``-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef k`` with
+    ``k = exp(ref_logp - logp) - (ref_logp - logp) - 1``.  advantages: [B, S],
+    or [B] / [B, 1] for one value per sequence.  mask (bool [B, S]) selects the
+    tokens that count; the others may hold anything.  ``reduction``: "token" is
+    the mean over all tokens that count, "sequence" the mean over sequences
+    (those with a token that counts) of their token means; without any token
+    the loss is 0.  The gradient goes to logp alone; where the ratio stands
+    exactly on the edge of the clip range it is that of the unclipped side."""
+    _check_logp(logp, mask)
+    if reduction not in ("token", "sequence"):
+        raise ValueError(f"reduction has to be 'token' or 'sequence', got {reduction!r}")
+    if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0):
+        raise ValueError(f"clip range: 0 <= clip_low <= 1 and clip_high >= 0, got {clip_low} and {clip_high}")
+    B, S = logp.shape
+    adv = advantages.detach()
+    if adv.dim() == 1:
+        adv = adv[:, None]
+    if adv.dtype != logp.dtype:
+        raise TypeError(f"advantages must be {logp.dtype}, got {adv.dtype}")
+    if tuple(adv.shape) not in ((B, S), (B, 1)):
+        raise ValueError(f"advantages {tuple(advantages.shape)}: [{B}, {S}], [{B}, 1] or [{B}] expected")
+    adv = adv.expand(B, S)
+    old, ref = _tokens(old_logp, logp, "old_logp"), _tokens(ref_logp, logp, "ref_logp")
+    low, high, per_sequence = 1.0 - clip_low, 1.0 + clip_high, reduction == "sequence"
+    if not logp.is_cuda:
+        return _policy_plain(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence)
+    lp, m = _unit_inner(logp), _unit_inner(mask)
+    if torch.is_grad_enabled() and lp.requires_grad:
+        return PolicyLoss(*_PolicyLossFn.apply(lp, old, adv, m, ref, low, high, float(kl_coef), per_sequence))
+    return PolicyLoss(*ext().policy_fwd(lp, old, adv, m, ref, low, high, float(kl_coef), per_sequence, False)[:3])
+
+
+def _policy_plain(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence):
+    m = torch.ones_like(logp, dtype=torch.bool) if mask is None else mask
+    at = m.nonzero(as_tuple=True)  # the tokens that count; the others never enter
+    x = logp[at]
+    ratio = torch.exp(x - old[at])
+    u, c = ratio * adv[at], ratio.detach().clamp(low, high) * adv[at]
+    clipped = u.detach() > c
+    per = -torch.where(clipped, c, u)
+    kl = torch.zeros_like(x)
+    if ref is not None:
+        d = ref[at] - x
+        kl = torch.expm1(d) - d
+        per = per + kl_coef * kl
+    n = max(1, x.numel())
+    if per_sequence:
+        rows = m.sum(1)
+        weight = (1.0 / rows.clamp_min(1).to(x.dtype) / max(1, int((rows > 0).sum())))[at[0]]
+    else:
+        weight = 1.0 / n
+    return PolicyLoss((per * weight).sum(), clipped.to(x.dtype).sum() / n, kl.detach().sum() / n)
+
+
+class _PreferenceLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logp, ref, mask, beta, smoothing, average):
+        loss, rewards, coef = ext().preference_fwd(logp, ref, mask, beta, smoothing, average)
+        ctx.save_for_backward(coef, mask)
+        ctx.S = logp.shape[1]
+        ctx.mark_non_differentiable(rewards)
+        return loss, rewards
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _rewards):
+        coef, mask = ctx.saved_tensors
+        return (ext().preference_bwd(coef, g, mask, ctx.S),) + (None,) * 5
+
+
+def preference_loss(logp: torch.Tensor, ref_logp: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                    beta: float = 0.1, label_smoothing: float = 0.0, average: bool = False) -> PreferenceLoss:
+    """Loss on pairs of sequences from token log-probabilities, logp fp32 [2P, S].
+
+    Row p is the chosen sequence of pair p and row P + p the rejected one.  A
+    sequence's reward is ``beta`` times the sum (``average``: the mean) over
+    its tokens in ``mask`` of logp - ref_logp (ref_logp None: logp alone), the
+    gap d of a pair is the difference of its rewards, and the loss the mean
+    over pairs of ``-(1 - label_smoothing) log sigmoid(d) - label_smoothing
+    log sigmoid(-d)``.  Positions outside the mask may hold anything; a row
+    without a token has reward 0.  The gradient goes to logp alone."""
+    _check_logp(logp, mask)
+    if logp.shape[0] < 2 or logp.shape[0] % 2:
+        raise ValueError(f"logp holds P chosen rows and P rejected rows, got {logp.shape[0]} rows")
+    if not 0.0 <= label_smoothing <= 1.0 or not math.isfinite(beta):
+        raise ValueError(f"0 <= label_smoothing <= 1 and a finite beta, got {label_smoothing} and {beta}")
+    ref = _tokens(ref_logp, logp, "ref_logp")
+    if not logp.is_cuda:
+        return _preference_plain(logp, ref, mask, beta, label_smoothing, average)
+    lp, m = _unit_inner(logp), _unit_inner(mask)
+    if torch.is_grad_enabled() and lp.requires_grad:
+        return PreferenceLoss(*_PreferenceLossFn.apply(lp, ref, m, float(beta), float(label_smoothing), bool(average)))
+    return PreferenceLoss(*ext().preference_fwd(lp, ref, m, float(beta), float(label_smoothing), bool(average))[:2])
+
+
+def _preference_plain(logp, ref, mask, beta, smoothing, average):
+    m = torch.ones_like(logp, dtype=torch.bool) if mask is None else mask
+    at = m.nonzero(as_tuple=True)
+    diff = logp[at] - (0.0 if ref is None else ref[at])
+    sums = torch.zeros(logp.shape[0], dtype=logp.dtype, device=logp.device).index_add(0, at[0], diff)
+    rewards = beta * (sums / m.sum(1).clamp_min(1).to(logp.dtype) if average else sums)
+    P = logp.shape[0] // 2
+    gap = rewards[:P] - rewards[P:]
+    loss = -((1.0 - smoothing) * F.logsigmoid(gap) + smoothing * F.logsigmoid(-gap)).mean()
+    return PreferenceLoss(loss, rewards.detach())

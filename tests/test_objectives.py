@@ -34,3 +34,72 @@ def test_log_probs_refusals():
     with pytest.raises(IndexError):
         O.lm_head_log_probs(h, w, ids + 9)
     assert O.lm_head_log_probs(h[:0], w, ids[:0]).shape == (0,)
+
+
+def _differences(fn, x):
+    """Autograd against central differences in 64 bits along a random direction."""
+    x = x.detach().double().requires_grad_(True)
+    (grad,) = torch.autograd.grad(fn(x), x)
+    d = torch.randn_like(x)
+    with torch.no_grad():
+        fd = (fn(x + 1e-6 * d) - fn(x - 1e-6 * d)) / 2e-6
+    assert abs((fd - (grad * d).sum()).item()) < 1e-6
+
+
+def test_policy_loss_formula_and_gradient():
+    torch.manual_seed(1)
+    B, S = 5, 9
+    logp = -torch.rand(B, S).double() * 3
+    old, ref, adv = logp - 0.3 * torch.randn(B, S), logp + 0.2 * torch.randn(B, S), torch.randn(B).double()
+    mask = torch.rand(B, S) < 0.7
+    mask[2] = False
+    for t in (old, ref):
+        t[~mask] = float("nan")
+    for reduction in ("token", "sequence"):
+        def fn(x):
+            return O.policy_loss(x, old, adv, mask=mask, ref_logp=ref, clip_low=0.1, clip_high=0.3, kl_coef=0.2,
+                                 reduction=reduction).loss
+        r = (logp - old).exp()
+        a = adv[:, None]
+        k = (ref - logp).exp() - (ref - logp) - 1
+        per = torch.where(mask, -torch.minimum(r * a, r.clamp(0.9, 1.3) * a) + 0.2 * k, torch.zeros_like(r))
+        rows = mask.sum(1)
+        ref_loss = per.sum() / mask.sum() if reduction == "token" else \
+            (per.sum(1) / rows.clamp_min(1)).sum() / (rows > 0).sum()
+        assert torch.allclose(fn(logp), ref_loss)
+        _differences(fn, logp)
+
+
+def test_preference_loss_formula_and_gradient():
+    torch.manual_seed(2)
+    P, S = 3, 8
+    logp = -torch.rand(2 * P, S).double()
+    ref = logp + torch.randn(2 * P, S)
+    mask = torch.rand(2 * P, S) < 0.6
+    mask[4] = False
+    ref[~mask] = float("inf")
+    for average in (False, True):
+        def fn(x):
+            return O.preference_loss(x, ref_logp=ref, mask=mask, beta=0.7, label_smoothing=0.2, average=average).loss
+        r = torch.where(mask, logp - ref, torch.zeros_like(logp)).sum(1)
+        r = 0.7 * (r / mask.sum(1).clamp_min(1) if average else r)
+        gap = r[:P] - r[P:]
+        want = -(0.8 * torch.sigmoid(gap).log() + 0.2 * torch.sigmoid(-gap).log()).mean()
+        assert torch.allclose(fn(logp), want)
+        _differences(fn, logp)
+
+
+def test_policy_and_preference_refusals():
+    x = torch.zeros(4, 5)
+    with pytest.raises(ValueError):
+        O.policy_loss(x, x, x, reduction="sum")
+    with pytest.raises(ValueError):
+        O.policy_loss(x[0], x[0], x[0])
+    with pytest.raises(ValueError):
+        O.policy_loss(x, x, x[:, :3])
+    with pytest.raises(TypeError):
+        O.policy_loss(x, x.double(), x)
+    with pytest.raises(ValueError):
+        O.preference_loss(x[:3])
+    with pytest.raises(ValueError):
+        O.preference_loss(x, mask=x)

@@ -212,3 +212,237 @@ def test_lm_head_log_probs_special_values_and_refusals():
     with pytest.raises(RuntimeError, match="one backward"):
         out.backward()
     _synced()
+
+
+# ----------------------------------------------------------------- policy loss
+LOW, HIGH, KL = 0.2, 0.28, 0.05
+F32 = 2.0 ** -24
+
+
+def _token_inputs(B, S, seed, masked=True):
+    """Log-probabilities with garbage outside the mask: a prompt, a padded tail and whole empty rows."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def randn(*shape):
+        return torch.randn(*shape, device="cuda", generator=g)
+
+    logp = -randn(B, S).abs() * 1.5
+    d = 0.2 * randn(B, S)
+    for edge in (math.log(1 - LOW), math.log(1 + HIGH)):  # a ratio on the clip's edge is decided by rounding
+        d = torch.where((d - edge).abs() < 1e-3, torch.full_like(d, edge + 2e-3), d)
+    old, ref, adv = logp - d, logp + 0.3 * randn(B, S), randn(B, S)
+    mask = None
+    if masked:
+        pos = torch.arange(S, device="cuda")[None]
+        start = (torch.rand(B, 1, device="cuda", generator=g) * S * 0.4).long()
+        mask = (pos >= start) & (pos < start + 1 + (torch.rand(B, 1, device="cuda", generator=g) * S).long())
+        mask &= torch.rand(B, 1, device="cuda", generator=g) >= 0.2
+        junk = torch.tensor([float("nan"), float("inf"), -float("inf"), 3e38], device="cuda")
+        out = junk[torch.randint(0, 4, (B, S), device="cuda", generator=g)]
+        logp, old, ref, adv = (torch.where(mask, t, out) for t in (logp, old, ref, adv))
+    return logp, old, ref, adv, mask
+
+
+def _policy_reference(logp, old, ref, adv, mask, per_sequence):
+    m = torch.ones_like(logp, dtype=torch.bool) if mask is None else mask
+
+    def clean(t):
+        return torch.where(m, t, torch.zeros_like(t)).double()
+
+    lp, o, a = clean(logp), clean(old), clean(adv.expand_as(logp))
+    r = (lp - o).exp()
+    past = ((a > 0) & (r > 1 + HIGH)) | ((a < 0) & (r < 1 - LOW))
+    per = -torch.where(past, torch.where(a > 0, 1 + HIGH, 1 - LOW) * a, r * a)
+    grad, scale, kl = torch.where(past, 0.0, -r * a), (r * a).abs(), torch.zeros_like(lp)
+    if ref is not None:
+        x = clean(ref) - lp
+        kl = torch.expm1(x) - x
+        per, grad, scale = per + KL * kl, grad - KL * torch.expm1(x), scale + KL * torch.expm1(x).abs()
+    n, rows = max(1, int(m.sum())), m.sum(1)
+    w = m.double() / n
+    if per_sequence:
+        w = m.double() / rows.clamp(min=1)[:, None] / max(1, int((rows > 0).sum()))
+    return ((per * w).sum(), (past & m).sum().double() / n, (kl * m).sum() / n, grad * w, scale * w,
+            ((per.abs() + 1) * w).sum())
+
+
+@pytest.mark.parametrize("B,S", [(1, 1), (3, 1), (1, 33), (8, 509), (5, 1000), (64, 300), (600, 7), (40, 5003)])
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_policy_loss(B, S, reduction):
+    from parallel_b200.ops import objectives as O
+
+    for masked, with_ref, per_row_adv in ((True, True, False), (False, False, True), (True, False, True)):
+        logp, old, ref, adv, mask = _token_inputs(B, S, seed=B + S, masked=masked)
+        if per_row_adv:
+            adv = torch.randn(B, device="cuda")
+        logp.requires_grad_(True)
+        args = dict(mask=mask, ref_logp=ref if with_ref else None, clip_low=LOW, clip_high=HIGH, kl_coef=KL,
+                    reduction=reduction)
+        out = O.policy_loss(logp, old, adv, **args)
+        (grad,) = torch.autograd.grad(3.0 * out.loss, logp)
+        with torch.no_grad():
+            scored = O.policy_loss(logp, old, adv, **args)
+        _synced()
+        wide = adv[:, None] if per_row_adv else adv
+        loss, clip, kl, rgrad, scale, size = _policy_reference(logp.detach(), old, ref if with_ref else None, wide,
+                                                               mask, reduction == "sequence")
+        # exp of a log ratio of a few units: an argument off by 2^-24 of |logp| <= 8, and 2 ulp of exp itself
+        tol = 40 * F32
+        assert abs(out.loss.item() - loss.item()) <= tol * size.item()
+        assert abs(out.clip_fraction.item() - clip.item()) <= 2 * F32
+        assert abs(out.kl.item() - kl.item()) <= tol * (kl.item() + 1)
+        assert ((grad.double() - 3 * rgrad).abs() <= 3 * tol * scale).all()
+        if mask is not None:
+            assert torch.equal(grad[~mask], torch.zeros_like(grad[~mask]))
+        assert all(torch.equal(a.detach(), b) for a, b in zip(out, scored))
+
+
+def test_policy_loss_strided_inputs_streams_and_same_bits():
+    from parallel_b200.ops import objectives as O
+
+    B, S = 70, 777
+    logp, old, ref, adv, mask = _token_inputs(B, S, seed=1)
+    want = O.policy_loss(logp, old, adv, mask=mask, ref_logp=ref, clip_low=LOW, clip_high=HIGH, kl_coef=KL,
+                         reduction="sequence")
+
+    def shifted(t):
+        wide = torch.zeros(B, S + 5, device="cuda", dtype=t.dtype)
+        wide[:, 2:S + 2] = t
+        return wide[:, 2:S + 2]
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        lp = shifted(logp).requires_grad_(True)
+        got = O.policy_loss(lp, shifted(old), adv.t().contiguous().t(), mask=shifted(mask),
+                            ref_logp=ref.t().contiguous().t(), clip_low=LOW, clip_high=HIGH, kl_coef=KL,
+                            reduction="sequence")
+        g1 = torch.autograd.grad(got.loss, lp)[0]
+    torch.cuda.current_stream().wait_stream(stream)
+    g2 = torch.autograd.grad(
+        O.policy_loss(lp, old, adv, mask=mask, ref_logp=ref, clip_low=LOW, clip_high=HIGH, kl_coef=KL,
+                      reduction="sequence").loss, lp)[0]
+    _synced()
+    assert all(torch.equal(a.detach(), b) for a, b in zip(got, want)) and torch.equal(g1, g2)
+
+
+def test_policy_loss_without_tokens_and_refusals():
+    from parallel_b200.ops import objectives as O
+
+    lp = torch.full((3, 5), float("nan"), device="cuda", requires_grad=True)
+    none = torch.zeros(3, 5, device="cuda", dtype=torch.bool)
+    for reduction in ("token", "sequence"):
+        out = O.policy_loss(lp, lp, lp, mask=none, ref_logp=lp, kl_coef=1.0, reduction=reduction)
+        (g,) = torch.autograd.grad(out.loss, lp)
+        assert out.loss.item() == 0 and out.kl.item() == 0 and torch.equal(g, torch.zeros_like(g))
+    empty = torch.zeros(4, 0, device="cuda")
+    assert O.policy_loss(empty, empty, torch.zeros(4, device="cuda")).loss.item() == 0
+    x = torch.zeros(3, 5, device="cuda")
+    for bad in (dict(logp=x[0]), dict(logp=x.bfloat16()), dict(mask=none.int()), dict(mask=none[:2]),
+                dict(reduction="mean"), dict(clip_low=1.5), dict(clip_high=-0.1), dict(advantages=x[:, :2]),
+                dict(old_logp=x[:2])):
+        with pytest.raises(ValueError):
+            O.policy_loss(**{**dict(logp=x, old_logp=x, advantages=x), **bad})
+    for bad in (dict(advantages=x.double()), dict(ref_logp=x.half())):
+        with pytest.raises(TypeError):
+            O.policy_loss(**{**dict(logp=x, old_logp=x, advantages=x), **bad})
+    with pytest.raises(RuntimeError):
+        O.policy_loss(x, x.cpu(), x)
+    _synced()
+
+
+# ----------------------------------------------------------------- preference loss
+def _preference_reference(logp, ref, mask, beta, e, average):
+    m = torch.ones_like(logp, dtype=torch.bool) if mask is None else mask
+    zero = torch.zeros_like(logp)
+    diff = torch.where(m, logp, zero).double() - (0 if ref is None else torch.where(m, ref, zero).double())
+    w = beta / (m.sum(1).clamp(min=1).double() if average else 1.0)
+    rewards = w * diff.sum(1)
+    P = logp.shape[0] // 2
+    gap = rewards[:P] - rewards[P:]
+    ls = torch.nn.functional.logsigmoid
+    loss = -((1 - e) * ls(gap) + e * ls(-gap)).mean()
+    d = (e * torch.sigmoid(gap) - (1 - e) * torch.sigmoid(-gap)) / P
+    grad = m * (w * torch.cat([d, -d]))[:, None]
+    return loss, rewards, grad, (w * diff.abs().sum(1))
+
+
+@pytest.mark.parametrize("P,S", [(1, 1), (1, 300), (4, 300), (3, 2000), (100, 65), (700, 3), (20, 5003)])
+@pytest.mark.parametrize("average", [False, True])
+def test_preference_loss(P, S, average):
+    from parallel_b200.ops import objectives as O
+
+    for masked, with_ref, e in ((True, True, 0.0), (False, True, 0.1), (True, False, 0.1)):
+        logp, ref, _, _, mask = _token_inputs(2 * P, S, seed=P + S, masked=masked)
+        logp.requires_grad_(True)
+        args = dict(ref_logp=ref if with_ref else None, mask=mask, beta=0.1, label_smoothing=e, average=average)
+        out = O.preference_loss(logp, **args)
+        (grad,) = torch.autograd.grad(-2.0 * out.loss, logp)
+        with torch.no_grad():
+            scored = O.preference_loss(logp, **args)
+        _synced()
+        loss, rewards, rgrad, size = _preference_reference(logp.detach(), ref if with_ref else None, mask, 0.1, e,
+                                                           average)
+        # a lane adds up to 32 differences, a warp's tree 5 levels, the rest in 64 bits
+        tol = 40 * F32 * size + 2 * F32
+        assert ((out.rewards.double() - rewards).abs() <= tol).all()
+        gap_tol = (tol[:P] + tol[P:]).max().item()
+        assert abs(out.loss.item() - loss.item()) <= gap_tol + 8 * F32 * (1 + loss.item())
+        # the gradient of a row moves with the gap by at most a quarter of it, relative to the smaller sigmoid at most once
+        assert ((grad.double() + 2 * rgrad).abs() <= 2 * (gap_tol + 16 * F32) * rgrad.abs() + 1e-30).all()
+        assert torch.equal(out.loss.detach(), scored.loss) and torch.equal(out.rewards, scored.rewards)
+
+
+def test_preference_loss_extreme_gaps_empty_rows_and_refusals():
+    from parallel_b200.ops import objectives as O
+
+    # gaps of +-2000 with beta 1: the loss is 0 on one side and the gap on the other, nothing overflows
+    lp = torch.zeros(4, 10, device="cuda")
+    lp[0], lp[3] = -200.0, -200.0
+    lp.requires_grad_(True)
+    out = O.preference_loss(lp, beta=1.0)
+    (g,) = torch.autograd.grad(out.loss, lp)
+    _synced()
+    assert out.rewards.tolist() == [-2000.0, 0.0, 0.0, -2000.0] and out.loss.item() == 1000.0
+    assert g[:, 0].tolist() == [-0.5, 0.0, 0.5, 0.0]
+    mask = torch.zeros(4, 10, device="cuda", dtype=torch.bool)
+    nan = torch.full((4, 10), float("nan"), device="cuda", requires_grad=True)
+    for average in (False, True):
+        out = O.preference_loss(nan, ref_logp=nan, mask=mask, average=average)
+        (g,) = torch.autograd.grad(out.loss, nan)
+        assert abs(out.loss.item() - math.log(2)) < 1e-6 and torch.equal(g, torch.zeros_like(g))
+    x = torch.zeros(4, 5, device="cuda")
+    for bad in (dict(logp=x[:3]), dict(logp=x[:0]), dict(label_smoothing=1.5), dict(beta=float("nan")),
+                dict(mask=x), dict(ref_logp=x[:2])):
+        with pytest.raises(ValueError):
+            O.preference_loss(**{**dict(logp=x), **bad})
+    with pytest.raises(TypeError):
+        O.preference_loss(x, ref_logp=x.double())
+    _synced()
+
+
+def test_policy_and_preference_gradients_against_differences():
+    """Central differences on the kernels' own losses, summed over a batch small enough for fp32 to resolve them."""
+    from parallel_b200.ops import objectives as O
+
+    B, S = 4, 6
+    logp, old, ref, adv, mask = _token_inputs(B, S, seed=9, masked=False)
+    fns = {"policy": lambda t: O.policy_loss(t, old, adv, ref_logp=ref, clip_low=LOW, clip_high=HIGH, kl_coef=KL).loss,
+           "preference": lambda t: O.preference_loss(t, ref_logp=ref, beta=0.5, label_smoothing=0.1).loss}
+    # within +-eps of the edges the policy loss has a corner: those positions are left out
+    r = (logp - old).exp()
+    eps = 2.0 ** -7
+    away = ((r.log() - math.log(1 - LOW)).abs() > 2 * eps) & ((r.log() - math.log(1 + HIGH)).abs() > 2 * eps)
+    for fn in fns.values():
+        x = logp.clone().requires_grad_(True)
+        (grad,) = torch.autograd.grad(fn(x), x)
+        for b in range(B):
+            for s in range(S):
+                if not away[b, s]:
+                    continue
+                d = torch.zeros_like(logp)
+                d[b, s] = eps
+                with torch.no_grad():
+                    fd = (fn(logp + d).double() - fn(logp - d).double()).item() / (2 * eps)
+                # loss of order 1 in fp32 over 2 eps, and eps^2 / 6 times a third derivative of order 1
+                assert abs(fd - grad[b, s].item()) <= 8 * F32 / (2 * eps) * 8 + eps ** 2

@@ -316,6 +316,122 @@ at::Tensor preference_bwd(const at::Tensor& coef, const at::Tensor& g, const c10
   return out;
 }
 
+// ---------------------------------------------------------------- distillation
+// distill_prep(top [T, K], ids [T, K], mask [T] or None, V, inv_tau) ->
+// [q [T, K], id [T, K], live [T], row_loss [T], counters [2], loss]
+std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& ids,
+                                     const c10::optional<at::Tensor>& mask, int64_t V, double inv_tau) {
+  TORCH_CHECK(top.is_cuda() && (top.scalar_type() == at::kBFloat16 || top.scalar_type() == at::kFloat) &&
+                  top.dim() == 2 && (top.stride(1) == 1 || top.size(1) <= 1),
+              "distill: teacher logits must be CUDA bf16 or fp32 [T, K] with unit inner stride");
+  const int64_t T = top.size(0), K = top.size(1);
+  TORCH_CHECK(ids.is_cuda() && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.dim() == 2 &&
+                  ids.size(0) == T && ids.size(1) == K && (ids.stride(1) == 1 || K <= 1),
+              "distill: teacher ids must be CUDA int32 or int64, shaped as the teacher's logits, unit inner stride");
+  TORCH_CHECK(K >= 1 && K <= pb::kDistillMaxK, "distill: 1 to ", num(pb::kDistillMaxK), " teacher entries a row");
+  TORCH_CHECK(T <= kIntMax / 16 && V >= 1 && V <= kIntMax, "distill: row and vocabulary counts");
+  CHECK_SAME_DEVICE(top, ids);
+  pb::DistillParams p{};
+  if (given(mask)) {
+    TORCH_CHECK(mask->is_cuda() && mask->scalar_type() == at::kBool && mask->dim() == 1 && mask->numel() == T,
+                "distill: mask must be CUDA bool [T]");
+    CHECK_SAME_DEVICE(top, *mask);
+    p.mask = reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>());
+    p.ld_mask = mask->stride(0);
+  }
+  const c10::cuda::CUDAGuard g(top.device());
+  const auto f32 = top.options().dtype(at::kFloat), i32 = top.options().dtype(at::kInt);
+  at::Tensor q = at::empty({T, K}, f32), id = at::empty({T, K}, i32);
+  at::Tensor live = at::empty({T}, top.options().dtype(at::kByte)), row_loss = at::empty({T}, f32);
+  at::Tensor counters = at::empty({2}, i32), loss = T ? at::empty({}, f32) : at::zeros({}, f32);
+  p.top = top.data_ptr();
+  p.ids = ids.data_ptr();
+  p.ld_top = top.stride(0);
+  p.ld_ids = ids.stride(0);
+  p.top_bf16 = top.scalar_type() == at::kBFloat16;
+  p.ids32 = ids.scalar_type() == at::kInt;
+  p.T = p.T_all = (int)T;
+  p.V = (int)V;
+  p.K = (int)K;
+  p.inv_tau = (float)inv_tau;
+  p.q = q.data_ptr<float>();
+  p.id = id.data_ptr<int>();
+  p.live = live.data_ptr<uint8_t>();
+  p.counters = counters.data_ptr<int>();
+  pb::distill_prep(p, cur_stream());
+  return {q, id, live, row_loss, counters, loss};
+}
+
+// distill_rows(logits [T, V], prep (of all rows), row0, tau, grad [T, V] or None): the losses of rows
+// [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss
+void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep, int64_t row0, double tau,
+                  const c10::optional<at::Tensor>& grad) {
+  TORCH_CHECK(logits.is_cuda() && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat) &&
+                  logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) <= 1),
+              "distill: logits must be CUDA bf16 or fp32 [T, V] with unit inner stride");
+  TORCH_CHECK(prep.size() == 6, "distill: what distill_prep returned");
+  const bool bf16 = logits.scalar_type() == at::kBFloat16;
+  const int64_t T = logits.size(0), V = logits.size(1), T_all = prep[0].size(0), K = prep[0].size(1);
+  TORCH_CHECK(V >= 1 && V <= pb::distill_max_vocab(bf16), "distill: vocabularies of 1 to ",
+              num(pb::distill_max_vocab(bf16)), " entries, got ", num(V));
+  TORCH_CHECK(row0 >= 0 && row0 + T <= T_all, "distill: rows outside the teacher's");
+  for (const at::Tensor& t : prep) CHECK_SAME_DEVICE(logits, t);
+  if (T == 0) return;
+  pb::DistillParams p{};
+  const int64_t es = logits.element_size();
+  p.logits = logits.data_ptr();
+  p.ld = logits.stride(0);
+  if (given(grad)) {
+    TORCH_CHECK(grad->scalar_type() == logits.scalar_type() && grad->dim() == 2 && grad->size(0) == T &&
+                    grad->size(1) == V && (grad->stride(1) == 1 || V <= 1) &&
+                    (reinterpret_cast<uintptr_t>(grad->data_ptr()) & 15) ==
+                        (reinterpret_cast<uintptr_t>(logits.data_ptr()) & 15) &&
+                    (T <= 1 || (grad->stride(0) - logits.stride(0)) * es % 16 == 0),
+                "distill: grad must have logits' type, shape and alignment");
+    CHECK_SAME_DEVICE(logits, *grad);
+    p.grad = grad->data_ptr();
+    p.ld_grad = grad->stride(0);
+  }
+  const c10::cuda::CUDAGuard g(logits.device());
+  p.T = (int)T;
+  p.T_all = (int)T_all;
+  p.V = (int)V;
+  p.K = (int)K;
+  p.row0 = row0;
+  p.tau = (float)tau;
+  p.inv_tau = (float)(1.0 / tau);
+  p.q = check_rows_f32(prep[0], T_all * K, "distill: q");
+  p.id = check_rows_i32(prep[1], T_all * K, "distill: id");
+  TORCH_CHECK(prep[2].scalar_type() == at::kByte && prep[2].numel() == T_all, "distill: live");
+  p.live = prep[2].data_ptr<uint8_t>();
+  p.row_loss = check_rows_f32(prep[3], T_all, "distill: row_loss");
+  p.counters = check_rows_i32(prep[4], 2, "distill: counters");
+  p.loss = check_rows_f32(prep[5], 1, "distill: loss");
+  pb::distill_rows(p, bf16, cur_stream());
+}
+
+// grad_like(logits [T, V]) -> (grad [T, V], its flat storage): a tensor that is misaligned as logits is in every
+// row, so that both are read and written in the same 16-byte vectors
+std::vector<at::Tensor> grad_like(const at::Tensor& logits) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "grad_like: CUDA [T, V]");
+  const c10::cuda::CUDAGuard g(logits.device());
+  const int64_t T = logits.size(0), V = logits.size(1), unit = 16 / logits.element_size();
+  const int64_t shift = (int64_t)(reinterpret_cast<uintptr_t>(logits.data_ptr()) & 15) / logits.element_size();
+  const int64_t ld = V + ((logits.stride(0) - V) % unit + unit) % unit;
+  at::Tensor flat = at::empty({shift + T * ld}, logits.options());
+  return {flat.as_strided({T, V}, {ld, 1}, shift), flat};
+}
+
+// objective_scale(x flat, g scalar): x *= g unless g is 1
+void objective_scale(at::Tensor& x, const at::Tensor& g) {
+  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat),
+              "objective_scale: contiguous CUDA bf16 or fp32");
+  CHECK_SAME_DEVICE(x, g);
+  const c10::cuda::CUDAGuard guard(x.device());
+  pb::objective_scale(x.data_ptr(), x.numel(), x.scalar_type() == at::kBFloat16,
+                      check_rows_f32(g, 1, "objective_scale: g"), cur_stream());
+}
+
 }  // namespace
 
 void register_objectives(pybind11::module& m) {
@@ -332,4 +448,10 @@ void register_objectives(pybind11::module& m) {
   m.def("preference_fwd", &preference_fwd, py::arg("logp"), py::arg("ref"), py::arg("mask"), py::arg("beta"),
         py::arg("smoothing"), py::arg("average"));
   m.def("preference_bwd", &preference_bwd, py::arg("coef"), py::arg("g"), py::arg("mask"), py::arg("S"));
+  m.def("distill_prep", &distill_prep, py::arg("top"), py::arg("ids"), py::arg("mask"), py::arg("V"),
+        py::arg("inv_tau"));
+  m.def("distill_rows", &distill_rows, py::arg("logits"), py::arg("prep"), py::arg("row0"), py::arg("tau"),
+        py::arg("grad"));
+  m.def("grad_like", &grad_like, py::arg("logits"));
+  m.def("objective_scale", &objective_scale, py::arg("x"), py::arg("g"));
 }

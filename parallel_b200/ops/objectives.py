@@ -5,7 +5,9 @@
 * ``policy_loss``        clipped policy-gradient loss with a KL term over token
   log-probabilities;
 * ``preference_loss``    loss on paired sequences (log-ratio of the chosen and
-  the rejected one against a reference).
+  the rejected one against a reference);
+* ``distillation_loss``  distillation of given logits from a teacher's top
+  logits, and ``lm_head_distillation``, the same through the LM head.
 
 As in ``functional``, CUDA tensors run the sm_100a kernels and CPU tensors run
 the plain PyTorch statement of the same formula.
@@ -326,3 +328,146 @@ def _preference_plain(logp, ref, mask, beta, smoothing, average):
     gap = rewards[:P] - rewards[P:]
     loss = -((1.0 - smoothing) * F.logsigmoid(gap) + smoothing * F.logsigmoid(-gap)).mean()
     return PreferenceLoss(loss, rewards.detach())
+
+
+# ----------------------------------------------------------------- distillation from a teacher's top logits
+class _DistillationFn(torch.autograd.Function):
+    """The gradient is written in the forward pass, from the one read of the
+    logits, and scaled by the incoming gradient in the backward."""
+
+    @staticmethod
+    def forward(ctx, logits, top, ids, mask, tau):
+        prep = ext().distill_prep(top, ids, mask, logits.shape[1], 1.0 / tau)
+        grad, flat = ext().grad_like(logits)
+        ext().distill_rows(logits, prep, 0, tau, grad)
+        ctx.grads = (grad, flat)
+        return prep[-1]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        _one_backward(ctx, "distillation_loss")
+        (grad, flat), ctx.grads = ctx.grads, None
+        ext().objective_scale(flat, g)
+        return grad, None, None, None, None
+
+
+class _LMHeadDistillationFn(torch.autograd.Function):
+    """Blocks of logits, overwritten by their gradient, as in ``lm_head_cross_entropy``."""
+
+    @staticmethod
+    def forward(ctx, h, w, top, ids, mask, tau, max_block_bytes):
+        (T, H), V = h.shape, w.shape[0]
+        need_h, need_w = ctx.needs_input_grad[:2]
+        prep = ext().distill_prep(top, ids, mask, V, 1.0 / tau)
+        block = _block_rows(T, V, max_block_bytes)
+        buf = _exp_buffer(block, V, h.device)
+        dh = torch.empty(T, H, device=h.device, dtype=h.dtype) if need_h else None
+        dw = torch.empty(V, H, device=h.device, dtype=w.dtype if block >= T else torch.float32) if need_w else None
+        for r0 in range(0, T, block):
+            rows = slice(r0, min(T, r0 + block))
+            logits = buf[:rows.stop - r0]
+            ext().gemm(h[rows], w, logits, False, False, G.EPI_STORE_BF16, 1.0)
+            ext().distill_rows(logits, prep, r0, tau, logits if need_h or need_w else None)
+            if need_h:
+                _grad_rows(logits, w, dh[rows])
+            if need_w:
+                _grad_head(logits, h[rows], dw, accumulate=r0 > 0)
+        if need_w and block < T:
+            out = torch.empty(V, H, device=h.device, dtype=w.dtype)
+            ext().cast_f32_to_bf16(dw, out)
+            dw = out
+        ctx.grads = (dh, dw)
+        return prep[-1]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        _one_backward(ctx, "lm_head_distillation")
+        (dh, dw), ctx.grads = ctx.grads, None
+        for t in (dh, dw):
+            if t is not None:
+                ext().objective_scale(t, g)
+        return dh, dw, None, None, None, None, None
+
+
+def _check_teacher(rows, top_logits, top_ids, mask, temperature):
+    """Teacher entries as [T, K] and the mask as [T] for `rows` (the leading shape of the student's rows)."""
+    if not temperature > 0.0:
+        raise ValueError(f"temperature has to be positive, got {temperature}")
+    if top_logits.shape[:-1] != rows or top_ids.shape != top_logits.shape or top_logits.dim() < 1:
+        raise ValueError(f"teacher logits {tuple(top_logits.shape)} and ids {tuple(top_ids.shape)}: "
+                         f"[{', '.join(str(r) for r in rows)}, K] expected")
+    if top_logits.shape[-1] < 1:
+        raise ValueError("at least one teacher entry per row")
+    if top_ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"teacher ids must be int64 or int32, got {top_ids.dtype}")
+    if not top_logits.is_floating_point() or (top_logits.is_cuda and top_logits.dtype not in (torch.bfloat16,
+                                                                                              torch.float32)):
+        raise TypeError(f"teacher logits must be bf16 or fp32, got {top_logits.dtype}")
+    if mask is not None and (mask.dtype != torch.bool or mask.shape != rows):
+        raise ValueError(f"mask must be bool {tuple(rows)}, got {mask.dtype} {tuple(mask.shape)}")
+    K = top_logits.shape[-1]
+    top, ids = _unit_inner(top_logits.detach().reshape(-1, K)), _unit_inner(top_ids.reshape(-1, K))
+    return top, ids, None if mask is None else mask.reshape(-1)
+
+
+def distillation_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_ids: torch.Tensor,
+                      mask: torch.Tensor | None = None, temperature: float = 1.0) -> torch.Tensor:
+    """Mean over rows of the KL divergence from a teacher's top tokens to the student, a scalar in fp32.
+
+    logits [..., V] (bf16 or fp32) are the student's; top_logits [..., K]
+    (bf16 or fp32) and top_ids [..., K] (int64 or int32) the teacher's highest
+    logits and their tokens, an id < 0 marking an absent entry.  With
+    q = softmax(top_logits / temperature) over the entries present and
+    p = softmax(logits / temperature) over the vocabulary, a row's loss is
+    ``temperature^2 sum_k q_k (log q_k - log p[id_k])``; an id that comes
+    twice counts twice.  Rows outside mask (bool [...]) and rows without an
+    entry do not count, and may hold anything; without any row the loss is 0.
+    An id >= V makes the loss NaN (an ``IndexError`` on CPU).  The gradient
+    goes to logits alone; one backward pass per forward."""
+    top, ids, m = _check_teacher(logits.shape[:-1], top_logits, top_ids, mask, temperature)
+    x = logits.reshape(-1, logits.shape[-1])
+    tau = float(temperature)
+    if not x.is_cuda:
+        return _distillation_plain(x, top, ids, m, tau)
+    x = _unit_inner(x)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _DistillationFn.apply(x, top, ids, m, tau)
+    prep = ext().distill_prep(top, ids, m, x.shape[1], 1.0 / tau)
+    ext().distill_rows(x, prep, 0, tau, None)
+    return prep[-1]
+
+
+def lm_head_distillation(h: torch.Tensor, w: torch.Tensor, top_logits: torch.Tensor, top_ids: torch.Tensor,
+                         mask: torch.Tensor | None = None, temperature: float = 1.0,
+                         max_block_bytes: int = 6 << 30) -> torch.Tensor:
+    """``distillation_loss(h @ w.T, ...)`` for hidden states h [..., H] and the LM head w [V, H], with at most
+    ``max_block_bytes`` of bf16 logits held at a time; the gradient goes to h and w."""
+    if w.dim() != 2 or h.shape[-1] != w.shape[1]:
+        raise ValueError(f"h {tuple(h.shape)} and w {tuple(w.shape)} must share their last dimension")
+    top, ids, m = _check_teacher(h.shape[:-1], top_logits, top_ids, mask, temperature)
+    h2, tau = h.reshape(-1, h.shape[-1]), float(temperature)
+    if not h2.is_cuda:
+        return _distillation_plain(F.linear(h2, w), top, ids, m, tau)
+    if h2.shape[0] == 0:
+        return h2.float().sum() + w[:0].float().sum()
+    h2, w = _rows_bf16(h2, "h"), _rows_bf16(w, "w")
+    if not torch.is_grad_enabled():
+        h2, w = h2.detach(), w.detach()
+    return _LMHeadDistillationFn.apply(h2, w, top, ids, m, tau, max_block_bytes)
+
+
+def _distillation_plain(x, top, ids, mask, tau):
+    if ids.numel() and int(ids.max()) >= x.shape[1]:
+        raise IndexError(f"teacher id {int(ids.max())} is outside the vocabulary of {x.shape[1]}")
+    dt = torch.promote_types(x.dtype, torch.float32)
+    have = (ids >= 0) & (top != -math.inf)
+    counts = have.any(1) if mask is None else have.any(1) & mask
+    rows = counts.nonzero()[:, 0]
+    have, ids = have[rows], ids[rows].clamp_min(0).long()
+    log_q = torch.log_softmax(top[rows].to(dt).div(tau).masked_fill(~have, -math.inf), dim=1)
+    log_p = torch.log_softmax(x[rows].to(dt) / tau, dim=1).gather(1, ids)
+    zero = torch.zeros((), dtype=dt, device=x.device)
+    terms = torch.where(have, log_q.exp() * (torch.where(have, log_q, zero) - torch.where(have, log_p, zero)), zero)
+    return tau * tau * terms.sum() / max(1, rows.numel())

@@ -103,3 +103,50 @@ def test_policy_and_preference_refusals():
         O.preference_loss(x[:3])
     with pytest.raises(ValueError):
         O.preference_loss(x, mask=x)
+
+
+def test_distillation_loss_formula_and_gradient():
+    torch.manual_seed(3)
+    T, V, K, tau = 6, 11, 4, 1.7
+    logits, top = torch.randn(T, V).double(), torch.randn(T, K).double()
+    ids = torch.randint(0, V, (T, K))
+    ids[0], top[0] = torch.tensor([2, 2, 5, -1]), torch.tensor([1.0, 0.5, 2.0, float("nan")])
+    ids[1] = -100
+    mask = torch.tensor([True, True, False, True, True, True])
+    logits[2] = float("nan")
+
+    def fn(x):
+        return O.distillation_loss(torch.where(mask[:, None], x, logits), top, ids, mask=mask, temperature=tau)
+
+    want = 0.0
+    for t in (0, 3, 4, 5):
+        k = [i for i in range(K) if ids[t, i] >= 0]
+        q = torch.softmax(top[t, k] / tau, 0)
+        p = torch.softmax(logits[t] / tau, 0)
+        want += tau ** 2 * sum(q[j] * (q[j].log() - p[ids[t, i]].log()) for j, i in enumerate(k)) / 4
+    x = torch.where(torch.isnan(logits), torch.zeros_like(logits), logits)
+    assert torch.allclose(fn(x), want)
+    _differences(fn, x)
+
+
+def test_lm_head_distillation_plain_and_refusals():
+    torch.manual_seed(4)
+    h, w = torch.randn(2, 3, 8, requires_grad=True), torch.randn(9, 8, requires_grad=True)
+    top, ids = torch.randn(2, 3, 2), torch.randint(0, 9, (2, 3, 2))
+    a = O.lm_head_distillation(h, w, top, ids, temperature=1.3)
+    b = O.distillation_loss(h @ w.t(), top, ids.int(), temperature=1.3)
+    assert torch.allclose(a, b)
+    a.backward()
+    assert torch.isfinite(h.grad).all() and torch.isfinite(w.grad).all()
+    x = (h @ w.t()).detach()
+    assert O.distillation_loss(x, top, ids, mask=torch.zeros(2, 3, dtype=torch.bool)).item() == 0
+    with pytest.raises(IndexError):
+        O.distillation_loss(x, top, ids + 9)
+    with pytest.raises(ValueError):
+        O.distillation_loss(x, top[:1], ids[:1])
+    with pytest.raises(ValueError):
+        O.distillation_loss(x, top, ids, temperature=0)
+    with pytest.raises(TypeError):
+        O.distillation_loss(x, top, ids.float())
+    with pytest.raises(ValueError):
+        O.lm_head_distillation(h, w[:, :4], top, ids)

@@ -446,3 +446,191 @@ def test_policy_and_preference_gradients_against_differences():
                     fd = (fn(logp + d).double() - fn(logp - d).double()).item() / (2 * eps)
                 # loss of order 1 in fp32 over 2 eps, and eps^2 / 6 times a third derivative of order 1
                 assert abs(fd - grad[b, s].item()) <= 8 * F32 / (2 * eps) * 8 + eps ** 2
+
+
+# ----------------------------------------------------------------- distillation
+def _teacher_inputs(T, V, K, dtype, seed):
+    """Logits with junk in rows outside the mask and teacher entries with absent ids (junk values) among them."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    logits = torch.randn(T, V, device="cuda", generator=g) * 2.5
+    top = 4 + 5 * torch.rand(T, K, device="cuda", generator=g)
+    ids = torch.randint(0, V, (T, K), device="cuda", generator=g)  # some twice
+    logits.scatter_add_(1, ids, 0.8 * top)
+    absent = torch.rand(T, K, device="cuda", generator=g) < 0.2
+    ids, top = ids.masked_fill(absent, -1), top.masked_fill(absent, float("nan"))
+    mask = torch.rand(T, device="cuda", generator=g) >= 0.2
+    logits[~mask] = float("inf")
+    if T > 3:
+        ids[1] = -1  # a row without any entry
+        ids[2], top[2] = 0, 1.0  # one id for all,
+        top[2, : K // 2] = -float("inf")  # some of probability zero
+    return logits.to(dtype), top, ids, mask
+
+
+def _distill_reference(logits, top, ids, mask, tau):
+    have = (ids >= 0) & (top != -float("inf"))
+    rows = (mask & have.any(1)).nonzero()[:, 0]
+    n = max(1, rows.numel())
+    h, at = have[rows], ids[rows].clamp_min(0).long()
+    lp = torch.log_softmax(logits[rows].double() / tau, 1)
+    lq = torch.log_softmax((top[rows].double() / tau).masked_fill(~h, -float("inf")), 1)
+    q = torch.where(h, lq.exp(), 0.0)
+    loss = tau ** 2 * torch.where(h, q * (lq - lp.gather(1, at)), 0.0).sum() / n
+    grad = torch.zeros(logits.shape, dtype=torch.float64, device="cuda")
+    g = lp.exp()
+    g.scatter_add_(1, at, -q)
+    grad[rows] = g * (tau / n)
+    return loss, grad
+
+
+@pytest.mark.parametrize("T,V,K", [(1, 1, 1), (4, 3, 2), (5, 7, 9), (3, 64, 5), (33, 1000, 20), (130, 4099, 33),
+                                   (17, 32003, 64), (9, 151936, 128), (2, 262144, 7), (3, 50257, 1024)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_loss(T, V, K, dtype):
+    from parallel_b200.ops import objectives as O
+
+    logits, top, ids, mask = _teacher_inputs(T, V, K, dtype, seed=T + V + K)
+    for tau, t, i in ((1.0, top, ids), (2.0, top.bfloat16(), ids.int())):
+        x = logits.clone().requires_grad_(True)
+        loss = O.distillation_loss(x, t, i, mask=mask, temperature=tau)
+        (grad,) = torch.autograd.grad(0.5 * loss, x)
+        with torch.no_grad():
+            scored = O.distillation_loss(x, t, i, mask=mask, temperature=tau)
+        _synced()
+        ref, rgrad = _distill_reference(logits, t, i, mask, tau)
+        # a softmax over V terms: exponents of up to 40 units off by 2^-24 of themselves, trees of depth <= 40
+        tol = 100 * F32
+        assert abs(loss.item() - ref.item()) <= tol * tau ** 2 * (abs(ref.item()) + 40)
+        assert torch.equal(loss.detach(), scored)
+        assert grad.dtype == dtype and grad.shape == x.shape
+        # scaling by the incoming 0.5 is exact; bf16 rounds once
+        rounding = 2.0 ** -8 if dtype == torch.bfloat16 else tol
+        n = max(1, int((mask & (i >= 0).any(1)).sum()))
+        assert ((grad.double() - 0.5 * rgrad).abs() <= rounding * (0.5 * rgrad).abs() + tol * tau / n).all()
+        assert torch.equal(grad[~mask], torch.zeros_like(grad[~mask]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_loss_row_strides_and_alignments(dtype):
+    """Rows that start at every 2- or 4-byte offset, padded rows, column slices, another stream, the same bits."""
+    from parallel_b200.ops import objectives as O
+
+    T, V, K = 21, 1003, 6
+    logits, top, ids, mask = _teacher_inputs(T, V, K, dtype, seed=2)
+    ref, rgrad = _distill_reference(logits, top, ids, mask, 1.0)
+    first = None
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for shift in range(0, 9):
+            for pad in (0, 1, 5):
+                wide = torch.zeros(T, V + shift + pad, device="cuda", dtype=dtype)
+                wide[:, shift:shift + V] = logits
+                x = wide[:, shift:shift + V].requires_grad_(True)
+                loss = O.distillation_loss(x, top, ids, mask=mask)
+                (grad,) = torch.autograd.grad(loss, x)
+                rounding = 2.0 ** -8 if dtype == torch.bfloat16 else 100 * F32
+                assert abs(loss.item() - ref.item()) <= 100 * F32 * (ref.item() + 40)
+                assert ((grad.double() - rgrad).abs() <= rounding * rgrad.abs() + 100 * F32).all()
+                again = O.distillation_loss(x, top, ids, mask=mask)
+                assert torch.equal(again, loss)
+                if shift == 0 and pad == 0:
+                    first = loss.detach()
+        turned = O.distillation_loss(logits.t().contiguous().t(), top.t().contiguous().t(), ids.t().contiguous().t(),
+                                     mask=torch.stack([mask, ~mask], 1)[:, 0])
+    torch.cuda.current_stream().wait_stream(stream)
+    _synced()
+    assert torch.equal(turned, first)
+
+
+def test_distillation_loss_against_differences():
+    from parallel_b200.ops import objectives as O
+
+    T, V, K = 3, 13, 4
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(T, V, device="cuda", generator=g)
+    top = torch.randn(T, K, device="cuda", generator=g)
+    ids = torch.randint(0, V, (T, K), device="cuda", generator=g)
+    leaf = x.clone().requires_grad_(True)
+    (grad,) = torch.autograd.grad(O.distillation_loss(leaf, top, ids, temperature=1.5), leaf)
+    eps = 2.0 ** -6
+    for t in range(T):
+        for v in range(V):
+            d = torch.zeros_like(x)
+            d[t, v] = eps
+            up = O.distillation_loss(x + d, top, ids, temperature=1.5).item()
+            down = O.distillation_loss(x - d, top, ids, temperature=1.5).item()
+            # fp32 losses of order 1 over 2 eps; eps^2 / 6 times a third derivative below 1
+            assert abs((up - down) / (2 * eps) - grad[t, v].item()) <= 16 * F32 / (2 * eps) + eps ** 2 / 6
+
+
+def test_distillation_loss_special_rows_and_refusals():
+    from parallel_b200.ops import objectives as O
+
+    x = torch.zeros(4, 10, device="cuda", requires_grad=True)
+    top, ids = torch.zeros(4, 3, device="cuda"), torch.tensor([[1, 2, 3]] * 4, device="cuda")
+    none = torch.zeros(4, device="cuda", dtype=torch.bool)
+    loss = O.distillation_loss(x, top, ids, mask=none)
+    (grad,) = torch.autograd.grad(loss, x)
+    assert loss.item() == 0 and torch.equal(grad, torch.zeros_like(grad))
+    assert O.distillation_loss(x[:0], top[:0], ids[:0]).item() == 0
+    # a teacher token that the student forbids: an infinite loss with a finite gradient
+    y = torch.zeros(4, 10, device="cuda")
+    y[0, 2] = -float("inf")
+    y.requires_grad_(True)
+    loss = O.distillation_loss(y, top, ids)
+    (grad,) = torch.autograd.grad(loss, y)
+    assert loss.item() == float("inf") and torch.isfinite(grad).all()
+    # an id outside the vocabulary, a NaN among the teacher's values, a NaN among the logits
+    assert math.isnan(O.distillation_loss(x, top, ids + 8).item())
+    assert math.isnan(O.distillation_loss(x, top.masked_fill(ids == 2, float("nan")), ids).item())
+    z = torch.zeros(4, 10, device="cuda").index_fill(1, torch.tensor([5], device="cuda"), float("nan"))
+    assert math.isnan(O.distillation_loss(z, top, ids).item())
+    _synced()
+    for bad in (dict(temperature=0.0), dict(top_logits=top[:3]), dict(top_ids=ids[:, :2]), dict(mask=none.int()),
+                dict(mask=none[:2]), dict(top_logits=top[:, :0], top_ids=ids[:, :0])):
+        with pytest.raises(ValueError):
+            O.distillation_loss(**{**dict(logits=x, top_logits=top, top_ids=ids), **bad})
+    for bad in (dict(top_ids=ids.float()), dict(top_logits=top.half()), dict(top_logits=ids)):
+        with pytest.raises(TypeError):
+            O.distillation_loss(**{**dict(logits=x, top_logits=top, top_ids=ids), **bad})
+    big = torch.zeros(4, 1025, device="cuda")
+    for bad in (dict(logits=x.half()), dict(top_logits=top.cpu()), dict(top_logits=big, top_ids=big.long())):
+        with pytest.raises(RuntimeError):
+            O.distillation_loss(**{**dict(logits=x, top_logits=top, top_ids=ids), **bad})
+    with pytest.raises(RuntimeError, match="vocabularies"):
+        O.distillation_loss(torch.zeros(1, 262145, device="cuda"), top[:1], ids[:1])
+    loss = O.distillation_loss(x, top, ids)
+    loss.backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="one backward"):
+        loss.backward()
+    _synced()
+
+
+@pytest.mark.parametrize("blocks", [1, 3])
+def test_lm_head_distillation(blocks):
+    from parallel_b200.ops import objectives as O
+
+    T, H, V, K, tau = 700, 192, 5003, 12, 2.0
+    h, w, _, _ = _head_inputs(T, H, V, ignored=0.0, seed=21)
+    g = torch.Generator(device="cuda").manual_seed(22)
+    ids = torch.randint(0, V, (T, K), device="cuda", generator=g)
+    top = 6 * torch.rand(T, K, device="cuda", generator=g)
+    mask = torch.rand(T, device="cuda", generator=g) >= 0.3
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = O.lm_head_distillation(h, w, top, ids, mask=mask, temperature=tau,
+                                  max_block_bytes=(6 << 30) if blocks == 1 else 2 * V * 256)
+    dh, dw = torch.autograd.grad(2 * loss, (h, w))
+    with torch.no_grad():
+        scored = O.lm_head_distillation(h, w, top, ids, mask=mask, temperature=tau)
+    _synced()
+    logits = h.detach().double() @ w.detach().double().t()
+    ref, dl = _distill_reference(logits, top, ids, mask, tau)
+    # bf16 logits: each off by up to 2^-8 of itself, which moves log p by as much
+    tol = 2.0 ** -8 * logits.abs().max().item() * tau
+    assert abs(loss.item() - ref.item()) <= tol and abs(scored.item() - ref.item()) <= tol
+    # the softmax of rounded logits is off by up to 2^-8 x 10 (logits that carry probability) of its entries
+    assert _err(dh, 2 * dl @ w.detach().double()) <= 10 * 2.0 ** -8
+    assert _err(dw, 2 * dl.t() @ h.detach().double()) <= 10 * 2.0 ** -8
+    assert torch.equal(dh[~mask], torch.zeros_like(dh[~mask]))

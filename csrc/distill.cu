@@ -4,15 +4,21 @@
 //   loss_t = tau^2 sum_k q_k (log q_k - log p_{id_k}),  mean over the N rows that count
 //   d logits_v = tau (p_v - sum_k q_k [id_k = v]) / N.
 //
-//   distill_prep  a warp per row: q and the ids as int32, and N.
-//   distill_rows  a cluster of CTAs per row; every thread holds its share of
-//                 the row in registers, so that each logit is read once and
-//                 its gradient written once: the kernel is bound by memory.
+//   distill_prep  a warp per row: q, the ids as int32, and N.
+//   distill_rows  a CTA per row (a cluster per row when there are few rows),
+//                 two passes: running maximum and sum, then the gradient.
+//   distill_loss  the row losses, added in a fixed order.
 //
-// A row of 151,936 bf16 logits is 304 KB, more than one SM's shared memory and
-// too much to leave to L2 with a row per SM in flight; split over a cluster of
-// 8 CTAs it is 10 16-byte vectors a thread, and three or four such CTAs fit
-// an SM, so some load while others reduce and store.
+// What bounds it: one read and one write of each logit in HBM.  A row of
+// 151,936 bf16 logits is 304 KB, more than an SM's shared memory, so the second
+// pass reads it again, from L2: 2 CTAs on each of 148 SMs hold at most 90 MB of
+// rows there, of which a CTA in its first pass has not read all and one in its
+// second does not need all (it reads and writes with evict-first).
+// Sharing a row between the 8 CTAs of a cluster, which keeps it in registers
+// and needs no second read, was slower in every form that was tried (8192 x
+// 151936 bf16: 1211 us as short-lived CTAs, 1229 us persistent with bulk-copy
+// prefetch and the exponentials kept): each row then waits for an exchange
+// between 8 SMs, with too few warps beside it to fill the time.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -26,8 +32,7 @@ namespace pb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxCluster = 8;
-constexpr int kMaxWarps = 16;
+constexpr int kMaxCluster = kDistillMaxCluster;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -94,210 +99,286 @@ __global__ void __launch_bounds__(32 * kPrepWarps) distill_prep_kernel(const Dis
   const float inv = 1.f / s;
   for (int k = lane; k < p.K; k += 32) {
     const int64_t id = teacher_id(p, t, k);
-    p.q[t * p.K + k] = id >= 0 ? expf(teacher_value(p, t, k, id) - m) * inv : 0.f;
-    p.id[t * p.K + k] = id >= 0 && id < p.V ? (int)id : -1;
+    p.q[t * p.Kp + k] = id >= 0 ? expf(teacher_value(p, t, k, id) - m) * inv : 0.f;
+    p.id[t * p.Kp + k] = id >= 0 && id < p.V ? (int)id : -1;
+  }
+  for (int k = p.K + lane; k < p.Kp; k += 32) {
+    p.q[t * p.Kp + k] = 0.f;
+    p.id[t * p.Kp + k] = -1;
   }
 }
 
 // ---------------------------------------------------------------- student side
-__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float k2) {
-  const float mn = fmaxf(m, m2);
-  const float ref = mn == -INFINITY ? 0.f : mn;
-  s = s * ex2((m - ref) * k2) + s2 * ex2((m2 - ref) * k2);
-  m = mn;
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-__device__ __forceinline__ float2 ld_cluster_f2(const float2* p, uint32_t rank) {
-  float2 v;
-  const uint32_t a = mapa_shared(smem_u32(p), rank);
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
+// Store v at this shared-memory location of CTA `rank` of the cluster.
+__device__ __forceinline__ void st_cluster_f2(float2* p, uint32_t rank, float2 v) {
+  const uint32_t a = mapa_shared(smem_u32(p), rank);
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(v.x), "f"(v.y) : "memory");
+}
+
+// A 16-byte vector of a row: its maximum, its sum of exponentials, its
+// gradient.  ref: the reference maximum; k2 = log2(e) / tau.
 template <typename E>
 struct Vec;
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ float get(const uint4& u, int j) {
-    const uint32_t w = (&u.x)[j >> 1];
-    return __uint_as_float((j & 1) ? (w & 0xffff0000u) : (w << 16));
+  static __device__ __forceinline__ uint4 lowest() {
+    return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
   }
-  static __device__ __forceinline__ uint4 pack(const float* v) {
-    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                      pack_bf16x2(v[6], v[7]));
+  static __device__ __forceinline__ float max(const uint4& u) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const float2 t = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(t.x, t.y);
+  }
+  // exponents as one multiply-add, its addend rounded to 2^-24 of some 40 units: 2e-6 of a value of 2^-8
+  static __device__ __forceinline__ void sum(const uint4& u, float ref, float k2, float* s) {
+    const uint32_t* w = &u.x;
+    const float c = -ref * k2;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      s[q] += ex2(fmaf(__uint_as_float(w[q] << 16), k2, c));
+      s[q] += ex2(fmaf(__uint_as_float(w[q] & 0xffff0000u), k2, c));
+    }
+  }
+  // f exp((l - ref) / tau), lf = log2(f) inside the exponent
+  static __device__ __forceinline__ uint4 grad(const uint4& u, float ref, float k2, float, float lf) {
+    const float c = fmaf(-ref, k2, lf);
+    const uint32_t* w = &u.x;
+    uint4 g;
+    uint32_t* o = &g.x;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      o[q] = pack_bf16x2(ex2(fmaf(__uint_as_float(w[q] << 16), k2, c)),
+                         ex2(fmaf(__uint_as_float(w[q] & 0xffff0000u), k2, c)));
+    return g;
   }
 };
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ float get(const uint4& u, int j) { return __uint_as_float((&u.x)[j]); }
-  static __device__ __forceinline__ uint4 pack(const float* v) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  static __device__ __forceinline__ uint4 lowest() {
+    return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+  }
+  static __device__ __forceinline__ float max(const uint4& u) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
+                 fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  // the difference first: exact near the reference
+  static __device__ __forceinline__ void sum(const uint4& u, float ref, float k2, float* s) {
+    const uint32_t* w = &u.x;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s[q] += ex2((__uint_as_float(w[q]) - ref) * k2);
+  }
+  static __device__ __forceinline__ uint4 grad(const uint4& u, float ref, float k2, float f, float) {
+    const uint32_t* w = &u.x;
+    uint4 g;
+    uint32_t* o = &g.x;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = __float_as_uint(f * ex2((__uint_as_float(w[q]) - ref) * k2));
+    return g;
   }
 };
 
-// Grid: T clusters.  NV: 16-byte vectors of the row per thread.  A row may
-// start at any element: up to 16 bytes in front of and behind the aligned
-// vectors are taken one by one by the first CTA.
-template <typename E, int NV>
-__global__ void __launch_bounds__(32 * kMaxWarps) distill_rows_kernel(const DistillParams p) {
+constexpr int kRowThreads = 512;
+constexpr int kUnroll = 4;  // vectors a thread has in flight
+
+// Grid: a cluster of p.cluster CTAs per row.  A row may start at any element:
+// up to 16 bytes in front of and behind its aligned vectors are taken one by
+// one by the first CTA.
+template <typename E>
+__global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const DistillParams p) {
   pdl_prologue();
   using VE = Vec<E>;
+  constexpr int WARPS = kRowThreads / 32;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* sq = reinterpret_cast<float*>(smem);  // [K] teacher probabilities
-  float* sl = sq + p.K;                        // [K] student logits at the teacher's ids
-  int* sid = reinterpret_cast<int*>(sl + p.K);  // [K]
-  __shared__ float2 warp_stat[kMaxWarps];
-  __shared__ float2 cta_stat;
-  __shared__ float red[kMaxWarps];
-  __shared__ bool s_last;
+  int* sid = reinterpret_cast<int*>(smem);             // [Kp] the row's teacher entries
+  float* sq = reinterpret_cast<float*>(sid + p.Kp);    // [Kp]
+  float* sl = sq + p.Kp;                               // [Kp] student logits at the ids in this CTA's columns
+  __shared__ float2 stat[kMaxCluster * WARPS];
+  __shared__ float red[WARPS];
 
   const int C = p.cluster;
-  const uint32_t rank = cluster_ctarank();
+  const int rank = C == 1 ? 0 : (int)cluster_ctarank();
   const int64_t t = blockIdx.x / C;  // row of this block of logits
   const int64_t tg = p.row0 + t;     // row of the teacher's entries and of the loss
-  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const E* row = reinterpret_cast<const E*>(p.logits) + t * p.ld;
   E* out = p.grad ? reinterpret_cast<E*>(p.grad) + t * p.ld_grad : nullptr;
   const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(E));
   const int head = min(p.V, mis ? VE::N - mis : 0);
-  const int nvec = (p.V - head) / VE::N;
-  const int tail0 = head + nvec * VE::N;  // first column behind the vectors
-  const int per = (nvec + C - 1) / C;
-  const int v0 = (int)rank * per, v1 = min(nvec, v0 + per);
-  const uint4* vin = reinterpret_cast<const uint4*>(row + head);
-  uint4* vout = reinterpret_cast<uint4*>(out + head);
-  // the first CTA's single columns: [0, head) by threads 0.., [tail0, V) by threads 16..
+  const int nvec = (p.V - head) / VE::N, per = (nvec + C - 1) / C;
+  const int tail0 = head + nvec * VE::N;  // columns [0, head) and [tail0, V) stand outside the vectors
+  const int v0 = min(nvec, rank * per), nv = min(nvec, v0 + per) - v0;
+  const uint4* vin = reinterpret_cast<const uint4*>(row + head) + v0;
+  uint4* vout = reinterpret_cast<uint4*>(out + head) + v0;
+  const int c0 = head + v0 * VE::N, c1 = c0 + nv * VE::N;
   int xcol = -1;
   if (rank == 0) {
     if (tid < head) xcol = tid;
     else if (tid >= 16 && tid < 16 + p.V - tail0) xcol = tail0 + tid - 16;
   }
-  const bool live = p.live[tg] != 0;
 
-  if (!live) {  // a row that does not count: its logits are not read, its gradient is 0
+  if (!p.live[tg]) {  // a row that does not count: its logits are not read, its gradient is 0
     if (out) {
-      for (int i = v0 + tid; i < v1; i += nt) vout[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = tid; i < nv; i += kRowThreads) __stcs(vout + i, make_uint4(0u, 0u, 0u, 0u));
       if (xcol >= 0) store1(out + xcol, 0.f);
     }
-    if (rank == 0 && tid == 0) p.row_loss[tg] = 0.f;
-  } else {
-    uint4 raw[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = v0 + i * nt + tid;
-      if (v < v1) raw[i] = vin[v];
-    }
-    const float x = xcol >= 0 ? load1(row + xcol) : -INFINITY;
-    // the teacher's entries; the first CTA needs every one (loss), the others those in their columns
-    const int c0 = head + v0 * VE::N, c1 = head + v1 * VE::N;
-    for (int k = tid; k < p.K; k += nt) {
-      const int id = p.id[tg * p.K + k];
-      sid[k] = id;
-      sq[k] = p.q[tg * p.K + k];
-      if (id >= 0 && (rank == 0 || (id >= c0 && id < c1))) sl[k] = load1(row + id);
-    }
-    const float k2 = kLog2e * p.inv_tau;
-    float m = x;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (v0 + i * nt + tid < v1) {
-#pragma unroll
-        for (int j = 0; j < VE::N; ++j) m = fmaxf(m, VE::get(raw[i], j));
-      }
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s = xcol >= 0 ? ex2((x - ref) * k2) : 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (v0 + i * nt + tid < v1) {
-#pragma unroll
-        for (int j = 0; j < VE::N; ++j) s += ex2((VE::get(raw[i], j) - ref) * k2);
-      }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      merge(m, s, m2, s2, k2);
-    }
-    if (lane == 0) warp_stat[warp] = make_float2(m, s);
-    __syncthreads();
-    m = warp_stat[0].x;
-    s = warp_stat[0].y;
-    for (int i = 1; i < warps; ++i) merge(m, s, warp_stat[i].x, warp_stat[i].y, k2);
-    if (tid == 0) cta_stat = make_float2(m, s);
-    cluster_sync();
-    // every CTA merges the cluster's statistics in rank order: the same bits in all of them
-    float2 st = ld_cluster_f2(&cta_stat, 0);
-    m = st.x;
-    s = st.y;
-    for (int i = 1; i < C; ++i) {
-      st = ld_cluster_f2(&cta_stat, i);
-      merge(m, s, st.x, st.y, k2);
-    }
-    if (rank == 0) {
-      const float ls = logf(s);
-      float acc = 0.f;
-      for (int k = tid; k < p.K; k += nt) {
-        const float q = sq[k];
-        // log p = (l - m) / tau - log s
-        if (sid[k] >= 0 && q != 0.f) acc += q * (logf(q) - ((sl[k] - m) * p.inv_tau - ls));
-        else if (isnan(q)) acc = q;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-      if (lane == 0) red[warp] = acc;
-      __syncthreads();
-      if (tid == 0) {
-        for (int i = 1; i < warps; ++i) acc += red[i];
-        p.row_loss[tg] = p.tau * p.tau * acc;
-      }
-    }
-    if (out) {
-      const float sc = p.tau / (float)max(1, p.counters[0]);
-      const float f = sc / s;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int v = v0 + i * nt + tid;
-        if (v < v1) {
-          float g[VE::N];
-#pragma unroll
-          for (int j = 0; j < VE::N; ++j) g[j] = f * ex2((VE::get(raw[i], j) - m) * k2);
-          vout[v] = VE::pack(g);
-        }
-      }
-      if (xcol >= 0) store1(out + xcol, f * ex2((x - m) * k2));
-      __syncthreads();  // the plain gradients are written before the teacher's columns are corrected
-      for (int k = tid; k < p.K; k += nt) {
-        const int id = sid[k];
-        const bool mine = id >= c0 && id < c1, single = rank == 0 && id >= 0 && (id < head || id >= tail0);
-        if (mine || single) {
-          float q = 0.f;  // an id that comes twice has the sum of its entries; each writes the same value
-          for (int i = 0; i < p.K; ++i) q += sid[i] == id ? sq[i] : 0.f;
-          store1(out + id, f * ex2((sl[k] - m) * k2) - sc * q);
-        }
-      }
-    }
-    cluster_sync();  // no CTA leaves while another may read its statistics
+    if (tid == 0) p.row_loss[tg * C + rank] = 0.f;
+    return;
   }
-  // the last row to finish (over all blocks of rows) adds the row losses in a fixed order
-  if (rank != 0) return;
+
+  // first pass: this thread's maximum and sum, rescaled once per kUnroll vectors
+  const float k2 = kLog2e * p.inv_tau;
+  const float x = xcol >= 0 ? load1(row + xcol) : -INFINITY;
+  float m = x, s[4] = {x == -INFINITY ? 0.f : 1.f + (x - x), 0.f, 0.f, 0.f};  // x - x: 0, or NaN if x is not finite
+  // two groups of vectors in turn: one on its way while the other is summed
+  uint4 ua[kUnroll], ub[kUnroll];
+  auto load = [&](uint4* u, int i0) {
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) {
+      u[j] = VE::lowest();
+      if (i0 + j * kRowThreads < nv) u[j] = __ldcg(vin + i0 + j * kRowThreads);
+    }
+  };
+  auto add = [&](const uint4* u) {
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) mn = fmaxf(mn, VE::max(u[j]));
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    const float r = ex2((m - ref) * k2);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) s[q] *= r;
+    m = mn;
+#pragma unroll
+    for (int j = 0; j < kUnroll; ++j) VE::sum(u[j], ref, k2, s);
+  };
+  constexpr int kStep = kUnroll * kRowThreads;
+  load(ua, tid);
+  for (int i0 = tid; i0 < nv; i0 += 2 * kStep) {
+    load(ub, i0 + kStep);
+    add(ua);
+    load(ua, i0 + 2 * kStep);
+    if (i0 + kStep < nv) add(ub);
+  }
+  // the logits at the teacher's ids, before any gradient is written (which may be in their place)
+  for (int k = tid; k < p.Kp; k += kRowThreads) {
+    const int id = p.id[tg * p.Kp + k];
+    sid[k] = id;
+    sq[k] = p.q[tg * p.Kp + k];
+    const bool single = id >= 0 && (id < head || id >= tail0);
+    if (single ? rank == 0 : (id >= c0 && id < c1)) sl[k] = load1(row + id);
+  }
+  {
+    const float mw = warp_max(m);
+    const float ref = mw == -INFINITY ? 0.f : mw;
+    const float sw = warp_sum(((s[0] + s[1]) + (s[2] + s[3])) * ex2((m - ref) * k2));
+    // every CTA of the cluster gets every warp's pair
+    if (C == 1) {
+      if (lane == 0) stat[warp] = make_float2(mw, sw);
+      __syncthreads();
+    } else {
+      if (lane < C) st_cluster_f2(&stat[rank * WARPS + warp], lane, make_float2(mw, sw));
+      cluster_sync();
+    }
+  }
+  // all warps of all CTAs add the pairs in the same order: the same bits everywhere
+  float total;
+  {
+    m = -INFINITY;
+    for (int i = lane; i < C * WARPS; i += 32) m = fmaxf(m, stat[i].x);
+    m = warp_max(m);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float a = 0.f;
+    for (int i = lane; i < C * WARPS; i += 32) a += stat[i].y * ex2((stat[i].x - ref) * k2);
+    total = warp_sum(a);
+    if (m == -INFINITY) total = NAN;  // no finite logit
+  }
+  const float sc = p.tau / (float)max(1, p.counters[0]);
+  const float f = sc / total;
+
+  if (out) {  // second pass: the gradient of the softmax
+    const float lf = log2f(f);
+    auto again = [&](uint4* u, int i0) {
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j)
+        if (i0 + j * kRowThreads < nv) u[j] = __ldcs(vin + i0 + j * kRowThreads);
+    };
+    auto store = [&](const uint4* u, int i0) {
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j)
+        if (i0 + j * kRowThreads < nv) __stcs(vout + i0 + j * kRowThreads, VE::grad(u[j], m, k2, f, lf));
+    };
+    again(ua, tid);
+    for (int i0 = tid; i0 < nv; i0 += 2 * kStep) {
+      again(ub, i0 + kStep);
+      store(ua, i0);
+      again(ua, i0 + 2 * kStep);
+      store(ub, i0 + kStep);
+    }
+    if (xcol >= 0) store1(out + xcol, f * ex2((x - m) * k2));
+    __syncthreads();  // the plain gradients stand before the teacher's columns are corrected
+  }
+  // the teacher's entries in this CTA's columns: their share of the loss, and their gradient
+  const float ls = logf(total);
+  float acc = 0.f;
+  for (int k = tid; k < p.K; k += kRowThreads) {
+    const int id = sid[k];
+    const float q = sq[k];
+    if (id < 0) {
+      if (isnan(q)) acc = q;
+      continue;
+    }
+    const bool single = id < head || id >= tail0;
+    if (!(single ? rank == 0 : (id >= c0 && id < c1))) continue;
+    const float l = sl[k];
+    // log p = (l - m) / tau - log s
+    if (q != 0.f) acc += q * (logf(q) - ((l - m) * p.inv_tau - ls));
+    if (out) {
+      // entries of one id: each writes the gradient with the sum of their q
+      float together = 0.f;
+      for (int i = 0; i < p.Kp; i += 4) {
+        const int4 ids = *reinterpret_cast<const int4*>(sid + i);
+        const float4 qs = *reinterpret_cast<const float4*>(sq + i);
+        together += (ids.x == id ? qs.x : 0.f) + (ids.y == id ? qs.y : 0.f) + (ids.z == id ? qs.z : 0.f) +
+                    (ids.w == id ? qs.w : 0.f);
+      }
+      store1(out + id, f * ex2((l - m) * k2) - sc * together);
+    }
+  }
+  acc = warp_sum(acc);
+  if (lane == 0) red[warp] = acc;
   __syncthreads();
   if (tid == 0) {
-    __threadfence();
-    s_last = atomicAdd(p.counters + 1, 1) == p.T_all - 1;
+    for (int i = 1; i < WARPS; ++i) acc += red[i];
+    p.row_loss[tg * C + rank] = p.tau * p.tau * acc;
   }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  __shared__ double dred[kMaxWarps];
+}
+
+// The mean of the row losses, added in a fixed order by one block.
+constexpr int kLossThreads = 1024;
+__global__ void __launch_bounds__(kLossThreads) distill_loss_kernel(const DistillParams p) {
+  pdl_prologue();
+  __shared__ double part[kLossThreads / 32];
   double a = 0.0;
-  for (int i = tid; i < p.T_all; i += nt) a += (double)__ldcg(p.row_loss + i);
+  for (int64_t i = threadIdx.x; i < (int64_t)p.T_all * p.cluster; i += kLossThreads) a += (double)p.row_loss[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-  if (lane == 0) dred[warp] = a;
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
   __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < warps; ++i) a += dred[i];
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kLossThreads / 32; ++i) a += part[i];
     p.loss[0] = (float)(a / (double)max(1, p.counters[0]));
   }
 }
@@ -312,72 +393,48 @@ __global__ void __launch_bounds__(256) scale_kernel(E* __restrict__ x, int64_t n
     store1(x + i, load1(x + i) * s);
 }
 
-// Cluster size, threads and vectors per thread of a row of nvec vectors: the
-// smallest cluster whose threads hold at most 10 vectors each.
-struct Shape {
-  int cluster, threads, nv;
-};
-Shape shape_of(int nvec) {
-  for (int threads : {256, 512})
-    for (int c = 1; c <= kMaxCluster; c *= 2)
-      for (int nv : {1, 2, 4, 6, 8, 10, 16})
-        if ((nv <= 10 || (threads == 512 && c == kMaxCluster)) && (int64_t)threads * c * nv >= nvec)
-          if ((int64_t)((nvec + c - 1) / c) <= (int64_t)threads * nv) return {c, threads, nv};
-  return {0, 0, 0};
-}
-
-template <typename E, int NV>
-void launch_rows(const DistillParams& p, const Shape& sh, cudaStream_t stream) {
+template <typename E>
+void launch_rows(const DistillParams& p, cudaStream_t stream) {
+  auto kern = distill_rows_kernel<E>;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = sh.cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  cfg.gridDim = dim3((unsigned)p.T * sh.cluster, 1, 1);
-  cfg.blockDim = dim3(sh.threads, 1, 1);
-  cfg.dynamicSmemBytes = (size_t)p.K * 12;
+  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
+  cfg.blockDim = dim3(kRowThreads, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)p.Kp * 12;
   cfg.stream = stream;
-  PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, distill_rows_kernel<E, NV>, p));
-}
-
-template <typename E>
-void launch_rows_nv(const DistillParams& p, const Shape& sh, cudaStream_t stream) {
-  switch (sh.nv) {
-    case 1: return launch_rows<E, 1>(p, sh, stream);
-    case 2: return launch_rows<E, 2>(p, sh, stream);
-    case 4: return launch_rows<E, 4>(p, sh, stream);
-    case 6: return launch_rows<E, 6>(p, sh, stream);
-    case 8: return launch_rows<E, 8>(p, sh, stream);
-    case 10: return launch_rows<E, 10>(p, sh, stream);
-    default: return launch_rows<E, 16>(p, sh, stream);
-  }
+  cfg.gridDim = dim3((unsigned)p.T * p.cluster, 1, 1);
+  PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
 }  // namespace
 
-int64_t distill_max_vocab(bool bf16) { return (int64_t)kMaxCluster * 512 * 16 * (bf16 ? 8 : 4); }
-
 void distill_prep(const DistillParams& p, cudaStream_t stream) {
-  PB_CUDA_CHECK(cudaMemsetAsync(p.counters, 0, 2 * sizeof(int), stream));
+  PB_CUDA_CHECK(cudaMemsetAsync(p.counters, 0, sizeof(int), stream));
   if (p.T == 0) return;
   launch_k(distill_prep_kernel, (p.T + kPrepWarps - 1) / kPrepWarps, 32 * kPrepWarps, 0, stream, p);
 }
 
 void distill_rows(const DistillParams& p0, bool bf16, cudaStream_t stream) {
-  const Shape sh = shape_of(p0.V / (bf16 ? 8 : 4));
-  PB_CHECK(sh.cluster > 0 && p0.K <= kDistillMaxK, "distill: vocabulary or teacher entries out of range");
-  PB_CHECK((int64_t)p0.T * sh.cluster < ((int64_t)1 << 31), "distill: too many rows for one call");
+  PB_CHECK(p0.K <= kDistillMaxK && (int64_t)p0.T * kMaxCluster < ((int64_t)1 << 31), "distill: too many rows or entries");
   DistillParams p = p0;
-  p.cluster = sh.cluster;
+  // a CTA per row, or a cluster while that leaves SMs idle and each CTA still has 2 vectors a thread
+  const int nvec = p.V / (bf16 ? 8 : 4);
+  p.cluster = 1;
+  while (p.cluster < kMaxCluster && 2 * p.cluster * (int64_t)p.T <= 2 * num_sms() &&
+         nvec / p.cluster >= 4 * kRowThreads)
+    p.cluster *= 2;
   if (bf16)
-    launch_rows_nv<__nv_bfloat16>(p, sh, stream);
+    launch_rows<__nv_bfloat16>(p, stream);
   else
-    launch_rows_nv<float>(p, sh, stream);
+    launch_rows<float>(p, stream);
+  if (p.row0 + p.T == p.T_all) launch_k(distill_loss_kernel, 1, kLossThreads, 0, stream, p);
 }
 
 void objective_scale(void* x, int64_t n, bool bf16, const float* g, cudaStream_t stream) {

@@ -318,7 +318,7 @@ at::Tensor preference_bwd(const at::Tensor& coef, const at::Tensor& g, const c10
 
 // ---------------------------------------------------------------- distillation
 // distill_prep(top [T, K], ids [T, K], mask [T] or None, V, inv_tau) ->
-// [q [T, K], id [T, K], live [T], row_loss [T], counters [2], loss]
+// [q, id [T, K rounded up to 4], live [T], row_loss, counters [1], loss]
 std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& ids,
                                      const c10::optional<at::Tensor>& mask, int64_t V, double inv_tau) {
   TORCH_CHECK(top.is_cuda() && (top.scalar_type() == at::kBFloat16 || top.scalar_type() == at::kFloat) &&
@@ -341,9 +341,11 @@ std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& id
   }
   const c10::cuda::CUDAGuard g(top.device());
   const auto f32 = top.options().dtype(at::kFloat), i32 = top.options().dtype(at::kInt);
-  at::Tensor q = at::empty({T, K}, f32), id = at::empty({T, K}, i32);
-  at::Tensor live = at::empty({T}, top.options().dtype(at::kByte)), row_loss = at::empty({T}, f32);
-  at::Tensor counters = at::empty({2}, i32), loss = T ? at::empty({}, f32) : at::zeros({}, f32);
+  const int64_t Kp = (K + 3) / 4 * 4;
+  at::Tensor q = at::empty({T, Kp}, f32), id = at::empty({T, Kp}, i32);
+  at::Tensor live = at::empty({T}, top.options().dtype(at::kByte));
+  at::Tensor row_loss = at::empty({T * pb::kDistillMaxCluster}, f32);
+  at::Tensor counters = at::empty({1}, i32), loss = T ? at::empty({}, f32) : at::zeros({}, f32);
   p.top = top.data_ptr();
   p.ids = ids.data_ptr();
   p.ld_top = top.stride(0);
@@ -353,6 +355,7 @@ std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& id
   p.T = p.T_all = (int)T;
   p.V = (int)V;
   p.K = (int)K;
+  p.Kp = (int)Kp;
   p.inv_tau = (float)inv_tau;
   p.q = q.data_ptr<float>();
   p.id = id.data_ptr<int>();
@@ -362,19 +365,19 @@ std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& id
   return {q, id, live, row_loss, counters, loss};
 }
 
-// distill_rows(logits [T, V], prep (of all rows), row0, tau, grad [T, V] or None): the losses of rows
+// distill_rows(logits [T, V], prep (of all rows), K, row0, tau, grad [T, V] or None): the losses of rows
 // [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss
-void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep, int64_t row0, double tau,
+void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep, int64_t K, int64_t row0, double tau,
                   const c10::optional<at::Tensor>& grad) {
   TORCH_CHECK(logits.is_cuda() && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat) &&
                   logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) <= 1),
               "distill: logits must be CUDA bf16 or fp32 [T, V] with unit inner stride");
   TORCH_CHECK(prep.size() == 6, "distill: what distill_prep returned");
   const bool bf16 = logits.scalar_type() == at::kBFloat16;
-  const int64_t T = logits.size(0), V = logits.size(1), T_all = prep[0].size(0), K = prep[0].size(1);
-  TORCH_CHECK(V >= 1 && V <= pb::distill_max_vocab(bf16), "distill: vocabularies of 1 to ",
-              num(pb::distill_max_vocab(bf16)), " entries, got ", num(V));
-  TORCH_CHECK(row0 >= 0 && row0 + T <= T_all, "distill: rows outside the teacher's");
+  const int64_t T = logits.size(0), V = logits.size(1), T_all = prep[0].size(0), Kp = prep[0].size(1);
+  TORCH_CHECK(V >= 1 && V <= kIntMax, "distill: vocabulary");
+  TORCH_CHECK(row0 >= 0 && row0 + T <= T_all && K >= 1 && (K + 3) / 4 * 4 == Kp,
+              "distill: rows or entries other than the teacher's");
   for (const at::Tensor& t : prep) CHECK_SAME_DEVICE(logits, t);
   if (T == 0) return;
   pb::DistillParams p{};
@@ -400,12 +403,13 @@ void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep,
   p.row0 = row0;
   p.tau = (float)tau;
   p.inv_tau = (float)(1.0 / tau);
-  p.q = check_rows_f32(prep[0], T_all * K, "distill: q");
-  p.id = check_rows_i32(prep[1], T_all * K, "distill: id");
+  p.Kp = (int)Kp;
+  p.q = check_rows_f32(prep[0], T_all * Kp, "distill: q");
+  p.id = check_rows_i32(prep[1], T_all * Kp, "distill: id");
   TORCH_CHECK(prep[2].scalar_type() == at::kByte && prep[2].numel() == T_all, "distill: live");
   p.live = prep[2].data_ptr<uint8_t>();
-  p.row_loss = check_rows_f32(prep[3], T_all, "distill: row_loss");
-  p.counters = check_rows_i32(prep[4], 2, "distill: counters");
+  p.row_loss = check_rows_f32(prep[3], T_all * pb::kDistillMaxCluster, "distill: row_loss");
+  p.counters = check_rows_i32(prep[4], 1, "distill: counters");
   p.loss = check_rows_f32(prep[5], 1, "distill: loss");
   pb::distill_rows(p, bf16, cur_stream());
 }
@@ -432,6 +436,107 @@ void objective_scale(at::Tensor& x, const at::Tensor& g) {
                       check_rows_f32(g, 1, "objective_scale: g"), cur_stream());
 }
 
+// ---------------------------------------------------------------- differentiable entry points
+// The losses are calls of a few microseconds on the GPU, so their autograd
+// nodes live here: a Python node costs 30 to 40 us a step in calls back into
+// the interpreter (8 x 509 tokens, forward and backward: 97 us).
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+at::Tensor or_undefined(const c10::optional<at::Tensor>& t) { return given(t) ? *t : at::Tensor(); }
+c10::optional<at::Tensor> or_none(const at::Tensor& t) {
+  return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt;
+}
+
+// The gradients are computed outside autograd: they cannot be differentiated again.
+void check_first_order(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the gradient is not differentiable (create_graph)");
+}
+
+struct PolicyLossNode : public torch::autograd::Function<PolicyLossNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logp, const at::Tensor& old,
+                               const at::Tensor& adv, const c10::optional<at::Tensor>& mask,
+                               const c10::optional<at::Tensor>& ref, double low, double high, double kl_coef,
+                               bool per_sequence, bool want) {
+    auto out = policy_fwd(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence, want);
+    if (want) ctx->save_for_backward({*out[3], *out[4], or_undefined(out[5])});
+    ctx->mark_non_differentiable({*out[1], *out[2]});
+    ctx->set_materialize_grads(false);
+    return {*out[0], *out[1], *out[2]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_first_order("policy_loss");
+    const auto saved = ctx->get_saved_variables();
+    variable_list grads(10);
+    if (g[0].defined()) grads[0] = policy_bwd(saved[0], g[0], saved[1], or_none(saved[2]));
+    return grads;
+  }
+};
+
+std::vector<at::Tensor> policy_loss(const at::Tensor& logp, const at::Tensor& old, const at::Tensor& adv,
+                                    const c10::optional<at::Tensor>& mask, const c10::optional<at::Tensor>& ref,
+                                    double low, double high, double kl_coef, bool per_sequence) {
+  return PolicyLossNode::apply(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence,
+                               wants_grad(logp));
+}
+
+struct PreferenceLossNode : public torch::autograd::Function<PreferenceLossNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logp, const c10::optional<at::Tensor>& ref,
+                               const c10::optional<at::Tensor>& mask, double beta, double smoothing, bool average) {
+    auto out = preference_fwd(logp, ref, mask, beta, smoothing, average);
+    ctx->save_for_backward({out[2], or_undefined(mask)});
+    ctx->saved_data["S"] = logp.size(1);
+    ctx->mark_non_differentiable({out[1]});
+    ctx->set_materialize_grads(false);
+    return {out[0], out[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_first_order("preference_loss");
+    const auto saved = ctx->get_saved_variables();
+    variable_list grads(6);
+    if (g[0].defined()) grads[0] = preference_bwd(saved[0], g[0], or_none(saved[1]), ctx->saved_data["S"].toInt());
+    return grads;
+  }
+};
+
+std::vector<at::Tensor> preference_loss(const at::Tensor& logp, const c10::optional<at::Tensor>& ref,
+                                        const c10::optional<at::Tensor>& mask, double beta, double smoothing,
+                                        bool average) {
+  return PreferenceLossNode::apply(logp, ref, mask, beta, smoothing, average);
+}
+
+// The gradient is written in the forward pass, from the one read of the
+// logits, and scaled by the incoming gradient in the backward.
+struct DistillationNode : public torch::autograd::Function<DistillationNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& top,
+                            const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau, bool want) {
+    const auto prep = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau);
+    std::vector<at::Tensor> grad;
+    if (want) grad = grad_like(logits);
+    distill_rows(logits, prep, top.size(1), 0, tau, want ? c10::optional<at::Tensor>(grad[0]) : c10::nullopt);
+    // not save_for_backward: the backward hands the gradient out, it does not keep it
+    if (want) ctx->saved_data["grad"] = grad;
+    return prep[5];
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_first_order("distillation_loss");
+    TORCH_CHECK(ctx->saved_data.count("grad"), "distillation_loss supports one backward pass per forward");
+    std::vector<at::Tensor> grad = ctx->saved_data["grad"].toTensorVector();
+    ctx->saved_data.erase("grad");
+    objective_scale(grad[1], g[0]);
+    variable_list grads(6);
+    grads[0] = grad[0];
+    return grads;
+  }
+};
+
+at::Tensor distillation_loss(const at::Tensor& logits, const at::Tensor& top, const at::Tensor& ids,
+                             const c10::optional<at::Tensor>& mask, double tau) {
+  return DistillationNode::apply(logits, top, ids, mask, tau, wants_grad(logits));
+}
+
 }  // namespace
 
 void register_objectives(pybind11::module& m) {
@@ -442,16 +547,15 @@ void register_objectives(pybind11::module& m) {
         py::arg("e") = py::none(), py::arg("perm") = py::none());
   m.def("logprob_bwd", &logprob_bwd, py::arg("e"), py::arg("stats"), py::arg("lse2"), py::arg("ids"), py::arg("perm"),
         py::arg("logp"), py::arg("g"), py::arg("inv_tau"), py::arg("bn"));
-  m.def("policy_fwd", &policy_fwd, py::arg("logp"), py::arg("old"), py::arg("adv"), py::arg("mask"), py::arg("ref"),
-        py::arg("low"), py::arg("high"), py::arg("kl_coef"), py::arg("per_sequence"), py::arg("want_grad"));
-  m.def("policy_bwd", &policy_bwd, py::arg("coef"), py::arg("g"), py::arg("inv"), py::arg("inv_row"));
-  m.def("preference_fwd", &preference_fwd, py::arg("logp"), py::arg("ref"), py::arg("mask"), py::arg("beta"),
+  m.def("policy_loss", &policy_loss, py::arg("logp"), py::arg("old"), py::arg("adv"), py::arg("mask"), py::arg("ref"),
+        py::arg("low"), py::arg("high"), py::arg("kl_coef"), py::arg("per_sequence"));
+  m.def("preference_loss", &preference_loss, py::arg("logp"), py::arg("ref"), py::arg("mask"), py::arg("beta"),
         py::arg("smoothing"), py::arg("average"));
-  m.def("preference_bwd", &preference_bwd, py::arg("coef"), py::arg("g"), py::arg("mask"), py::arg("S"));
+  m.def("distillation_loss", &distillation_loss, py::arg("logits"), py::arg("top"), py::arg("ids"), py::arg("mask"),
+        py::arg("tau"));
   m.def("distill_prep", &distill_prep, py::arg("top"), py::arg("ids"), py::arg("mask"), py::arg("V"),
         py::arg("inv_tau"));
-  m.def("distill_rows", &distill_rows, py::arg("logits"), py::arg("prep"), py::arg("row0"), py::arg("tau"),
+  m.def("distill_rows", &distill_rows, py::arg("logits"), py::arg("prep"), py::arg("K"), py::arg("row0"), py::arg("tau"),
         py::arg("grad"));
-  m.def("grad_like", &grad_like, py::arg("logits"));
   m.def("objective_scale", &objective_scale, py::arg("x"), py::arg("g"));
 }

@@ -81,10 +81,11 @@ void preference_bwd(const float* coef, const float* g, const uint8_t* mask, int6
 // Teacher entries [T_all, K]: values (bf16 or fp32) and ids (int32 or int64,
 // negative = absent), mask (optional bool [T_all]).  distill_prep fills q, id,
 // live and counters[0] = rows that count; distill_rows then takes a block of
-// T rows of logits, [row0, row0 + T), and the last block of T_all rows writes
-// loss.  grad (optional) may be the logits themselves; the two must be
+// T rows of logits, [row0, row0 + T), in order; the block that ends at T_all
+// writes loss.  grad (optional) may be the logits themselves; the two must be
 // misaligned by the same number of bytes in every row.
 constexpr int kDistillMaxK = 1024;
+constexpr int kDistillMaxCluster = 8;
 struct DistillParams {
   const void* logits;
   void* grad;
@@ -93,17 +94,16 @@ struct DistillParams {
   const uint8_t* mask;
   int64_t ld_top, ld_ids, ld_mask;
   bool top_bf16, ids32;
-  int T, T_all, V, K, cluster;
+  int T, T_all, V, K, Kp, cluster;  // Kp: K rounded up to a multiple of 4
   int64_t row0;
   float tau, inv_tau;
-  float* q;        // [T_all, K]
-  int* id;         // [T_all, K]
+  float* q;        // [T_all, Kp]
+  int* id;         // [T_all, Kp]
   uint8_t* live;   // [T_all]
-  float* row_loss;  // [T_all]
-  int* counters;   // [2]
+  float* row_loss;  // [T_all * kDistillMaxCluster]: shares of a row's loss, cluster by cluster
+  int* counters;   // [1]
   float* loss;
 };
-int64_t distill_max_vocab(bool bf16);
 void distill_prep(const DistillParams& p, cudaStream_t stream);  // T = T_all
 void distill_rows(const DistillParams& p, bool bf16, cudaStream_t stream);
 

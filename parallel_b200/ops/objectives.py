@@ -201,22 +201,6 @@ def _unit_inner(t: torch.Tensor | None) -> torch.Tensor | None:
     return t if t is None or t.stride(-1) == 1 else t.contiguous()
 
 
-class _PolicyLossFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logp, old, adv, mask, ref, low, high, kl_coef, per_sequence):
-        loss, clip, kl, coef, inv, inv_row = ext().policy_fwd(logp, old, adv, mask, ref, low, high, kl_coef,
-                                                              per_sequence, True)
-        ctx.save_for_backward(coef, inv, inv_row)
-        ctx.mark_non_differentiable(clip, kl)
-        return loss, clip, kl
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _clip, _kl):
-        coef, inv, inv_row = ctx.saved_tensors
-        return (ext().policy_bwd(coef, g, inv, inv_row),) + (None,) * 8
-
-
 def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
                 mask: torch.Tensor | None = None, ref_logp: torch.Tensor | None = None, clip_low: float = 0.2,
                 clip_high: float = 0.2, kl_coef: float = 0.0, reduction: str = "token") -> PolicyLoss:
@@ -249,10 +233,8 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Te
     low, high, per_sequence = 1.0 - clip_low, 1.0 + clip_high, reduction == "sequence"
     if not logp.is_cuda:
         return _policy_plain(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence)
-    lp, m = _unit_inner(logp), _unit_inner(mask)
-    if torch.is_grad_enabled() and lp.requires_grad:
-        return PolicyLoss(*_PolicyLossFn.apply(lp, old, adv, m, ref, low, high, float(kl_coef), per_sequence))
-    return PolicyLoss(*ext().policy_fwd(lp, old, adv, m, ref, low, high, float(kl_coef), per_sequence, False)[:3])
+    return PolicyLoss(*ext().policy_loss(_unit_inner(logp), old, adv, _unit_inner(mask), ref, low, high,
+                                         float(kl_coef), per_sequence))
 
 
 def _policy_plain(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence):
@@ -277,22 +259,6 @@ def _policy_plain(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence):
     return PolicyLoss((per * weight).sum(), clipped.to(x.dtype).sum() / n, kl.detach().sum() / n)
 
 
-class _PreferenceLossFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logp, ref, mask, beta, smoothing, average):
-        loss, rewards, coef = ext().preference_fwd(logp, ref, mask, beta, smoothing, average)
-        ctx.save_for_backward(coef, mask)
-        ctx.S = logp.shape[1]
-        ctx.mark_non_differentiable(rewards)
-        return loss, rewards
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _rewards):
-        coef, mask = ctx.saved_tensors
-        return (ext().preference_bwd(coef, g, mask, ctx.S),) + (None,) * 5
-
-
 def preference_loss(logp: torch.Tensor, ref_logp: torch.Tensor | None = None, mask: torch.Tensor | None = None,
                     beta: float = 0.1, label_smoothing: float = 0.0, average: bool = False) -> PreferenceLoss:
     """Loss on pairs of sequences from token log-probabilities, logp fp32 [2P, S].
@@ -312,10 +278,8 @@ def preference_loss(logp: torch.Tensor, ref_logp: torch.Tensor | None = None, ma
     ref = _tokens(ref_logp, logp, "ref_logp")
     if not logp.is_cuda:
         return _preference_plain(logp, ref, mask, beta, label_smoothing, average)
-    lp, m = _unit_inner(logp), _unit_inner(mask)
-    if torch.is_grad_enabled() and lp.requires_grad:
-        return PreferenceLoss(*_PreferenceLossFn.apply(lp, ref, m, float(beta), float(label_smoothing), bool(average)))
-    return PreferenceLoss(*ext().preference_fwd(lp, ref, m, float(beta), float(label_smoothing), bool(average))[:2])
+    return PreferenceLoss(*ext().preference_loss(_unit_inner(logp), ref, _unit_inner(mask), float(beta),
+                                                 float(label_smoothing), bool(average)))
 
 
 def _preference_plain(logp, ref, mask, beta, smoothing, average):
@@ -331,27 +295,6 @@ def _preference_plain(logp, ref, mask, beta, smoothing, average):
 
 
 # ----------------------------------------------------------------- distillation from a teacher's top logits
-class _DistillationFn(torch.autograd.Function):
-    """The gradient is written in the forward pass, from the one read of the
-    logits, and scaled by the incoming gradient in the backward."""
-
-    @staticmethod
-    def forward(ctx, logits, top, ids, mask, tau):
-        prep = ext().distill_prep(top, ids, mask, logits.shape[1], 1.0 / tau)
-        grad, flat = ext().grad_like(logits)
-        ext().distill_rows(logits, prep, 0, tau, grad)
-        ctx.grads = (grad, flat)
-        return prep[-1]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        _one_backward(ctx, "distillation_loss")
-        (grad, flat), ctx.grads = ctx.grads, None
-        ext().objective_scale(flat, g)
-        return grad, None, None, None, None
-
-
 class _LMHeadDistillationFn(torch.autograd.Function):
     """Blocks of logits, overwritten by their gradient, as in ``lm_head_cross_entropy``."""
 
@@ -368,7 +311,7 @@ class _LMHeadDistillationFn(torch.autograd.Function):
             rows = slice(r0, min(T, r0 + block))
             logits = buf[:rows.stop - r0]
             ext().gemm(h[rows], w, logits, False, False, G.EPI_STORE_BF16, 1.0)
-            ext().distill_rows(logits, prep, r0, tau, logits if need_h or need_w else None)
+            ext().distill_rows(logits, prep, top.shape[1], r0, tau, logits if need_h or need_w else None)
             if need_h:
                 _grad_rows(logits, w, dh[rows])
             if need_w:
@@ -431,12 +374,7 @@ def distillation_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_ids: t
     tau = float(temperature)
     if not x.is_cuda:
         return _distillation_plain(x, top, ids, m, tau)
-    x = _unit_inner(x)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _DistillationFn.apply(x, top, ids, m, tau)
-    prep = ext().distill_prep(top, ids, m, x.shape[1], 1.0 / tau)
-    ext().distill_rows(x, prep, 0, tau, None)
-    return prep[-1]
+    return ext().distillation_loss(_unit_inner(x), top, ids, m, tau)
 
 
 def lm_head_distillation(h: torch.Tensor, w: torch.Tensor, top_logits: torch.Tensor, top_ids: torch.Tensor,

@@ -317,8 +317,25 @@ at::Tensor preference_bwd(const at::Tensor& coef, const at::Tensor& g, const c10
 }
 
 // ---------------------------------------------------------------- distillation
-// distill_prep(top [T, K], ids [T, K], mask [T] or None, V, inv_tau) ->
-// [q, id [T, K rounded up to 4], live [T], row_loss, counters [1], loss]
+// Scratch of a distillation, one allocation of 4-byte words: q and id [T, Kp]
+// (Kp: K rounded up to 4), the row losses, the count, the rows' live bytes.
+struct DistillScratch {
+  int64_t T, Kp;
+  explicit DistillScratch(int64_t t, int64_t k) : T(t), Kp((k + 3) / 4 * 4) {}
+  int64_t words() const { return T * (2 * Kp + pb::kDistillMaxCluster) + 1 + (T + 3) / 4; }
+  void fill(pb::DistillParams& p, const at::Tensor& t) const {
+    float* base = t.data_ptr<float>();
+    p.Kp = (int)Kp;
+    p.T_all = (int)T;
+    p.q = base;
+    p.id = reinterpret_cast<int*>(base + T * Kp);
+    p.row_loss = base + 2 * T * Kp;
+    p.counters = reinterpret_cast<int*>(p.row_loss + T * pb::kDistillMaxCluster);
+    p.live = reinterpret_cast<uint8_t*>(p.counters + 1);
+  }
+};
+
+// distill_prep(top [T, K], ids [T, K], mask [T] or None, V, inv_tau) -> [scratch, loss]
 std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& ids,
                                      const c10::optional<at::Tensor>& mask, int64_t V, double inv_tau) {
   TORCH_CHECK(top.is_cuda() && (top.scalar_type() == at::kBFloat16 || top.scalar_type() == at::kFloat) &&
@@ -340,47 +357,43 @@ std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& id
     p.ld_mask = mask->stride(0);
   }
   const c10::cuda::CUDAGuard g(top.device());
-  const auto f32 = top.options().dtype(at::kFloat), i32 = top.options().dtype(at::kInt);
-  const int64_t Kp = (K + 3) / 4 * 4;
-  at::Tensor q = at::empty({T, Kp}, f32), id = at::empty({T, Kp}, i32);
-  at::Tensor live = at::empty({T}, top.options().dtype(at::kByte));
-  at::Tensor row_loss = at::empty({T * pb::kDistillMaxCluster}, f32);
-  at::Tensor counters = at::empty({1}, i32), loss = T ? at::empty({}, f32) : at::zeros({}, f32);
+  const auto f32 = top.options().dtype(at::kFloat);
+  const DistillScratch sc(T, K);
+  at::Tensor scratch = at::empty({sc.words()}, f32), loss = T ? at::empty({}, f32) : at::zeros({}, f32);
+  sc.fill(p, scratch);
   p.top = top.data_ptr();
   p.ids = ids.data_ptr();
   p.ld_top = top.stride(0);
   p.ld_ids = ids.stride(0);
   p.top_bf16 = top.scalar_type() == at::kBFloat16;
   p.ids32 = ids.scalar_type() == at::kInt;
-  p.T = p.T_all = (int)T;
+  p.T = (int)T;
   p.V = (int)V;
   p.K = (int)K;
-  p.Kp = (int)Kp;
   p.inv_tau = (float)inv_tau;
-  p.q = q.data_ptr<float>();
-  p.id = id.data_ptr<int>();
-  p.live = live.data_ptr<uint8_t>();
-  p.counters = counters.data_ptr<int>();
   pb::distill_prep(p, cur_stream());
-  return {q, id, live, row_loss, counters, loss};
+  return {scratch, loss};
 }
 
-// distill_rows(logits [T, V], prep (of all rows), K, row0, tau, grad [T, V] or None): the losses of rows
-// [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss
-void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep, int64_t K, int64_t row0, double tau,
-                  const c10::optional<at::Tensor>& grad) {
+// distill_rows(logits [T, V], prep ([scratch, loss] of all T_all rows), T_all, K, row0, tau, grad [T, V] or None):
+// the losses of rows [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss
+void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep, int64_t T_all, int64_t K, int64_t row0,
+                  double tau, const c10::optional<at::Tensor>& grad) {
   TORCH_CHECK(logits.is_cuda() && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat) &&
                   logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) <= 1),
               "distill: logits must be CUDA bf16 or fp32 [T, V] with unit inner stride");
-  TORCH_CHECK(prep.size() == 6, "distill: what distill_prep returned");
   const bool bf16 = logits.scalar_type() == at::kBFloat16;
-  const int64_t T = logits.size(0), V = logits.size(1), T_all = prep[0].size(0), Kp = prep[0].size(1);
+  const int64_t T = logits.size(0), V = logits.size(1);
   TORCH_CHECK(V >= 1 && V <= kIntMax, "distill: vocabulary");
-  TORCH_CHECK(row0 >= 0 && row0 + T <= T_all && K >= 1 && (K + 3) / 4 * 4 == Kp,
-              "distill: rows or entries other than the teacher's");
+  TORCH_CHECK(row0 >= 0 && row0 + T <= T_all, "distill: rows outside the teacher's");
+  const DistillScratch sc(T_all, K);
+  TORCH_CHECK(prep.size() == 2 && K >= 1 && K <= pb::kDistillMaxK, "distill: what distill_prep returned");
   for (const at::Tensor& t : prep) CHECK_SAME_DEVICE(logits, t);
+  check_rows_f32(prep[0], sc.words(), "distill: scratch");
   if (T == 0) return;
   pb::DistillParams p{};
+  sc.fill(p, prep[0]);
+  p.loss = check_rows_f32(prep[1], 1, "distill: loss");
   const int64_t es = logits.element_size();
   p.logits = logits.data_ptr();
   p.ld = logits.stride(0);
@@ -397,20 +410,11 @@ void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep,
   }
   const c10::cuda::CUDAGuard g(logits.device());
   p.T = (int)T;
-  p.T_all = (int)T_all;
   p.V = (int)V;
   p.K = (int)K;
   p.row0 = row0;
   p.tau = (float)tau;
   p.inv_tau = (float)(1.0 / tau);
-  p.Kp = (int)Kp;
-  p.q = check_rows_f32(prep[0], T_all * Kp, "distill: q");
-  p.id = check_rows_i32(prep[1], T_all * Kp, "distill: id");
-  TORCH_CHECK(prep[2].scalar_type() == at::kByte && prep[2].numel() == T_all, "distill: live");
-  p.live = prep[2].data_ptr<uint8_t>();
-  p.row_loss = check_rows_f32(prep[3], T_all * pb::kDistillMaxCluster, "distill: row_loss");
-  p.counters = check_rows_i32(prep[4], 1, "distill: counters");
-  p.loss = check_rows_f32(prep[5], 1, "distill: loss");
   pb::distill_rows(p, bf16, cur_stream());
 }
 
@@ -515,10 +519,10 @@ struct DistillationNode : public torch::autograd::Function<DistillationNode> {
     const auto prep = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau);
     std::vector<at::Tensor> grad;
     if (want) grad = grad_like(logits);
-    distill_rows(logits, prep, top.size(1), 0, tau, want ? c10::optional<at::Tensor>(grad[0]) : c10::nullopt);
+    distill_rows(logits, prep, top.size(0), top.size(1), 0, tau, want ? c10::optional<at::Tensor>(grad[0]) : c10::nullopt);
     // not save_for_backward: the backward hands the gradient out, it does not keep it
     if (want) ctx->saved_data["grad"] = grad;
-    return prep[5];
+    return prep[1];
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     check_first_order("distillation_loss");
@@ -555,7 +559,7 @@ void register_objectives(pybind11::module& m) {
         py::arg("tau"));
   m.def("distill_prep", &distill_prep, py::arg("top"), py::arg("ids"), py::arg("mask"), py::arg("V"),
         py::arg("inv_tau"));
-  m.def("distill_rows", &distill_rows, py::arg("logits"), py::arg("prep"), py::arg("K"), py::arg("row0"), py::arg("tau"),
+  m.def("distill_rows", &distill_rows, py::arg("logits"), py::arg("prep"), py::arg("T_all"), py::arg("K"), py::arg("row0"), py::arg("tau"),
         py::arg("grad"));
   m.def("objective_scale", &objective_scale, py::arg("x"), py::arg("g"));
 }

@@ -311,7 +311,7 @@ class _LMHeadDistillationFn(torch.autograd.Function):
             rows = slice(r0, min(T, r0 + block))
             logits = buf[:rows.stop - r0]
             ext().gemm(h[rows], w, logits, False, False, G.EPI_STORE_BF16, 1.0)
-            ext().distill_rows(logits, prep, top.shape[1], r0, tau, logits if need_h or need_w else None)
+            ext().distill_rows(logits, prep, T, top.shape[1], r0, tau, logits if need_h or need_w else None)
             if need_h:
                 _grad_rows(logits, w, dh[rows])
             if need_w:

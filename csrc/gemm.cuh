@@ -77,6 +77,14 @@ struct GemmParams {
   int64_t ws_ld = 0;
   bool out_f32 = false;     // kEpiSplitOrdered: C is fp32 (else bf16)
   bool accumulate = false;  // kEpiSplitOrdered: C += result
+  // Rows known on the device only (CTA-pair kernel, no gather or scatter): of the
+  // M rows (live_k: of the K rows of both MN-major operands) the first
+  // live[0] - live_row0 count.  Output tiles beyond them are not computed
+  // (live_k: the sum stops at the end of the 64-row step, so operand rows up to
+  // there must be finite and A's zero; at least one step is taken).
+  const int* live = nullptr;
+  int live_row0 = 0;
+  bool live_k = false;
   const ScatterArgs* scatter = nullptr;  // kEpiStoreBf16 rows to their sequence-parallel owners
   const GatherArgs* gather = nullptr;    // A assembled from sequence-parallel shards in-kernel
 };

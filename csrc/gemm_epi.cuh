@@ -32,10 +32,10 @@ struct EpiArgs {
 // free of bank conflicts.
 constexpr int kEpiBox = 32;
 constexpr int kEpiBoxBytes = kEpiBox * kEpiBox * 2;
-// (8 KB: the SwiGLU epilogue's three bf16 boxes, or two 32 x 32 fp32 boxes)
+// (8 KB: the SwiGLU epilogue's three bf16 boxes, four for the bf16 store, or two 32 x 32 fp32 boxes)
 constexpr int kEpiWarpBytes = 8192;
 constexpr int kEpiBoxF32Bytes = kEpiBox * kEpiBox * 4;
-static_assert(3 * kEpiBoxBytes <= kEpiWarpBytes && 2 * kEpiBoxF32Bytes <= kEpiWarpBytes, "epilogue staging");
+static_assert(4 * kEpiBoxBytes <= kEpiWarpBytes && 2 * kEpiBoxF32Bytes <= kEpiWarpBytes, "epilogue staging");
 
 // Output row pointer of row m for the bf16 store epilogue.
 __device__ __forceinline__ __nv_bfloat16* out_row_bf16(const EpiArgs& ep, int m) {
@@ -236,9 +236,9 @@ __device__ __forceinline__ void epilogue_warp_tma(const EpiArgs& ep, const CUten
     } else {
 #pragma unroll
       for (int j = 0; j < 32; ++j) a[j] *= ep.alpha;
-      // two boxes alternate: chunk c may be staged while chunk c - 1 drains
-      box0 = stage + ((c >> 5) & 1) * kEpiBoxBytes;
-      if (lane == 0) bulk_wait_group_read<1>();
+      // four boxes in turn: chunk c may be staged while chunks c - 3 .. c - 1 drain
+      box0 = stage + ((c >> 5) & 3) * kEpiBoxBytes;
+      if (lane == 0) bulk_wait_group_read<3>();
       __syncwarp();
       if (store) stage_row_swz64(box0, lane, a);
     }

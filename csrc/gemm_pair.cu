@@ -212,7 +212,8 @@ template <int BN, bool A_MN, bool B_MN, bool SWIGLU, bool GATHER>
 __global__ void __launch_bounds__(GATHER ? kThreads + 64 : kThreads, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, EpiArgs ep,
                      int M, int N, int K, int b_up_row, int* err, const __grid_constant__ GatherArgs ga,
-                     int splits, const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR) {
+                     int splits, const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR,
+                     const int* __restrict__ live, int live_row0, bool live_k) {
   pdl_prologue();
   using Cfg = PairCfg<BN>;
   constexpr int STAGES = Cfg::STAGES;
@@ -262,10 +263,16 @@ __global__ void __launch_bounds__(GATHER ? kThreads + 64 : kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  const int tiles_m = (M + 2 * BM_CTA - 1) / (2 * BM_CTA);
+  int rows_m = M, rows_k = K;
+  if (live) {
+    const int n = *live - live_row0;
+    if (live_k) rows_k = min(K, max(1, n));
+    else rows_m = min(M, max(0, n));
+  }
+  const int tiles_m = (rows_m + 2 * BM_CTA - 1) / (2 * BM_CTA);
   const int tiles_n = (N + BN_OUT - 1) / BN_OUT;
   const int num_tiles = tiles_m * tiles_n;
-  const int num_kb = (K + BK - 1) / BK;
+  const int num_kb = (rows_k + BK - 1) / BK;
   // work item w = (tile, K slice): tile = w % num_tiles, slice = w / num_tiles
   const int kb_per = (num_kb + splits - 1) / splits;
   const int num_work = num_tiles * splits;
@@ -513,13 +520,14 @@ void launch_pair(const GemmParams& p, cudaStream_t stream) {
   cfg.gridDim = dim3(2 * clusters, 1, 1);
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, ep, p.M, p.N, p.K, (int)p.b_up_offset, error_word(dev), ga,
-                                   std::max(1, p.splits), tc, tr));
+                                   std::max(1, p.splits), tc, tr, p.live, p.live_row0, p.live_k));
 }
 
 }  // namespace
 
 void gemm_bf16_pair(const GemmParams& p, cudaStream_t stream) {
   if (p.gather) {
+    PB_CHECK(!p.live, "gemm: the gather has no row count on the device");
     // A (the gathered activations) is K-major by construction
     PB_CHECK(!p.a_mn, "gemm: the gathered A operand is K-major");
     PB_CHECK(p.gather->seq_local % 256 == 0 && p.gather->n_blocks == (p.M + 255) / 256 && p.M % 256 == 0 &&
@@ -529,6 +537,8 @@ void gemm_bf16_pair(const GemmParams& p, cudaStream_t stream) {
     if (!p.b_mn) return launch_pair<256, false, false, false, true>(p, stream);
     return launch_pair<256, false, true, false, true>(p, stream);
   }
+  PB_CHECK(!p.live || (!p.scatter && p.epi != kEpiSwiGLU && (!p.live_k || (p.a_mn && p.b_mn && p.splits <= 1))),
+           "gemm: a row count on the device needs plain rows (or MN-major operands and one K slice)");
   if (p.scatter) PB_CHECK(p.epi == kEpiStoreBf16 && p.scatter->nranks <= 8, "gemm: scatter needs the bf16 store epilogue");
   PB_CHECK(p.splits <= 1 || ((p.epi == kEpiAtomicF32 || p.epi == kEpiSplitOrdered || p.epi == kEpiStoreF32) &&
                                !p.gather && !p.scatter),

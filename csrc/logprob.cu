@@ -47,7 +47,8 @@ constexpr int B_BYTES = (BN_MAX / 2) * BK * 2;
 constexpr int STAGES = 6;
 constexpr int kBox = 32;  // E is stored in 32 x 32 boxes of 64-byte rows (64-byte swizzle)
 constexpr int kBoxBytes = kBox * kBox * 2;
-constexpr int EPI_BYTES = 4 * 2 * kBoxBytes;  // two boxes for each of the 4 epilogue warps
+constexpr int kBoxes = 4;     // per epilogue warp: three stores may be draining while one box is filled
+constexpr int EPI_BYTES = 4 * kBoxes * kBoxBytes;
 constexpr int SMEM_BYTES = STAGES * (A_BYTES + B_BYTES) + EPI_BYTES + 1024 + 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -57,6 +58,15 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Column tiles: the first n_full are BN_MAX wide, the others bn2.  Whole waves of
+// wide tiles over the CTA pairs, and what is left over in tiles narrow enough
+// for one more wave: 151,936 columns are 8 waves of 256 on 74 pairs and 384
+// columns, which as two wide tiles cost a ninth wave (one row: 61 -> 54 us).
+__device__ __forceinline__ int tile_start(const LogprobTiles& g, int tn) {
+  return tn < g.n_full ? tn * BN_MAX : g.n_full * BN_MAX + (tn - g.n_full) * g.bn2;
+}
+__device__ __forceinline__ int tile_width(const LogprobTiles& g, int tn) { return tn < g.n_full ? BN_MAX : g.bn2; }
 
 // Wait for this thread's TMEM loads; the registers are operands, so no use of
 // them can move above the wait.
@@ -118,8 +128,8 @@ __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, 
 // whole tile), then the exponentials, 32 x 32 boxes through TMA.
 template <typename Release>
 __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_base, int V, int64_t id, float scale,
-                                                  const CUtensorMap* tmE, uint8_t* stage, int lane, int y0,
-                                                  Release release) {
+                                                  const CUtensorMap* tmE, uint8_t* stage, int& next_box, int lane,
+                                                  int y0, Release release) {
   float m = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < bn; c += 32) {
@@ -145,9 +155,9 @@ __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_
       v[j] = ex2(fmaf(v[j], scale, -ref));
       s += v[j];
     }
-    // two boxes alternate: chunk c is staged while chunk c - 1 drains
-    uint8_t* box = stage + ((c >> 5) & 1) * kBoxBytes;
-    if (lane == 0) bulk_wait_group_read<1>();
+    uint8_t* box = stage + next_box * kBoxBytes;
+    next_box = (next_box + 1) & (kBoxes - 1);
+    if (lane == 0) bulk_wait_group_read<kBoxes - 1>();
     __syncwarp();
     uint8_t* row = box + lane * 64;
 #pragma unroll
@@ -177,9 +187,11 @@ __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_
 template <bool STORE>
 __global__ void __launch_bounds__(kThreads, 1)
     logprob_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                        const __grid_constant__ CUtensorMap tmE, const int64_t* __restrict__ ids,
-                        float2* __restrict__ stats, int T, int V, int H, int bn, float scale, int* err) {
+                        const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ CUtensorMap tmE,
+                        const int64_t* __restrict__ ids, const int* __restrict__ count, int row0,
+                        float2* __restrict__ stats, int T_all, int V, int H, int a_rows, const LogprobTiles geo, float scale, int* err) {
   pdl_prologue();
+  const int T = count ? min(T_all, max(0, *count - row0)) : T_all;  // the rows in front that have a token
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -222,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
 
   const int tiles_m = (T + 2 * BM_CTA - 1) / (2 * BM_CTA);
-  const int tiles_n = (V + bn - 1) / bn;
+  const int tiles_n = geo.n_full + geo.n_rest;
   const int64_t num_tiles = (int64_t)tiles_m * tiles_n;
   const int num_kb = (H + BK - 1) / BK;
   const int n_clusters = gridDim.x >> 1;
@@ -230,32 +242,39 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      const uint32_t stage_bytes = 2 * (A_BYTES + (uint32_t)(bn / 2) * BK * 2);
+      // few rows: a box of the rows that are there (a box mostly out of bounds is
+      // slow to fill: one row 91 us, 64 rows 61 us), and none for the odd CTA.  The
+      // rest of the stage holds anything: rows of A are independent.
+      const uint32_t a_bytes = a_rows < BM_CTA ? (uint32_t)a_rows * BK * 2 : 2 * A_BYTES;
+      const bool load_a = a_rows == BM_CTA || leader;
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int64_t w = cid; w < num_tiles && ok; w += n_clusters) {
         const int tm = (int)(w % tiles_m), tn = (int)(w / tiles_m);
         const int a_row = tm * 2 * BM_CTA + (int)rank * BM_CTA;
-        const int b_row = tn * bn + (int)rank * (bn / 2);
+        const int bn = tile_width(geo, tn);
+        const int b_row = tile_start(geo, tn) + (int)rank * (bn / 2);
+        const CUtensorMap* map_b = tn < geo.n_full ? &tmB : &tmB2;
+        const uint32_t stage_bytes = a_bytes + (uint32_t)bn * BK * 2;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, err)) { ok = false; break; }
           const uint32_t full_even = mapa_shared(smem_u32(&full_bar[stage]), 0);
           if (leader) mbar_arrive_expect_tx(&full_bar[stage], stage_bytes);
-          tma_load_2d_pair(sA + stage * A_BYTES, &tmA, full_even, kb * BK, a_row);
-          tma_load_2d_pair(sB + stage * B_BYTES, &tmB, full_even, kb * BK, b_row);
+          if (load_a) tma_load_2d_pair(sA + stage * A_BYTES, &tmA, full_even, kb * BK, a_row);
+          tma_load_2d_pair(sB + stage * B_BYTES, map_b, full_even, kb * BK, b_row);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
     }
   } else if (warp == 1) {
     if (leader && lane == 0) {
-      const uint32_t idesc = idesc_bf16(2 * BM_CTA, bn, false, false);
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
       bool ok = true;
       for (int64_t w = cid; w < num_tiles && ok; w += n_clusters, ++local) {
+        const uint32_t idesc = idesc_bf16(2 * BM_CTA, tile_width(geo, (int)(w / tiles_m)), false, false);
         const int acc = local & 1;
         const uint32_t acc_phase = (local >> 1) & 1;
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, err)) break;
@@ -278,8 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     const int quarter = warp & 3;
-    uint8_t* stage = sEpi + quarter * 2 * kBoxBytes;
-    int local = 0;
+    uint8_t* stage = sEpi + quarter * kBoxes * kBoxBytes;
+    int local = 0, next_box = 0;
     for (int64_t w = cid; w < num_tiles; w += n_clusters, ++local) {
       const int tm = (int)(w % tiles_m), tn = (int)(w / tiles_m);
       const int acc = local & 1;
@@ -299,11 +318,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         continue;
       }
       const int64_t id = t < T ? ids[t] : -1;
+      const int bn = tile_width(geo, tn), n0 = tile_start(geo, tn);
       float2 st;
       if constexpr (STORE)
-        st = row_stats_store(t_row, bn, tn * bn, V, id, scale, &tmE, stage, lane, y0, release);
+        st = row_stats_store(t_row, bn, n0, V, id, scale, &tmE, stage, next_box, lane, y0, release);
       else
-        st = row_stats(t_row, bn, tn * bn, V, id, scale, release);
+        st = row_stats(t_row, bn, n0, V, id, scale, release);
       if (t < T) stats[(int64_t)t * tiles_n + tn] = st;
     }
     // the box stores must have finished before the kernel's shared memory goes
@@ -419,16 +439,20 @@ __global__ void __launch_bounds__(kFinThreads)
 // ---------------------------------------------------------------- backward
 constexpr int kBwdThreads = 256;
 
-// A warp takes a tile of a row at a time: one factor for bn consecutive
+// A warp takes a tile of a row at a time: one factor for its (256) consecutive
 // entries, 8 of them per lane and step.  The target's own entry is
 // c (1 - p) = -c expm1(logp), which bf16 E could not give where p is near 1.
 __global__ void __launch_bounds__(kBwdThreads)
     logprob_bwd_kernel(__nv_bfloat16* __restrict__ e, int64_t lde, const float2* __restrict__ stats, int tiles,
                        const float* __restrict__ lse2, const float* __restrict__ logp,
-                       const int64_t* __restrict__ ids, const int* __restrict__ perm, const float* __restrict__ g,
-                       float inv_tau, int V, int bn) {
+                       const int64_t* __restrict__ ids, const int* __restrict__ perm,
+                       const int* __restrict__ count, int row0, const float* __restrict__ g, float inv_tau, int V,
+                       const LogprobTiles geo) {
   pdl_prologue();
   const int64_t t = blockIdx.x;
+  // behind the rows with a token: zeros up to the end of the last 64-deep step of
+  // the head gradient's sum over rows, and nothing beyond, which no product reads
+  if (t >= (max(1, *count - row0) + 63) / 64 * 64) return;
   const int64_t id = ids[t];
   const int src = perm[t];  // logp and g are in the caller's row order
   const float c = id < 0 ? 0.f : g[src] * inv_tau;
@@ -438,8 +462,8 @@ __global__ void __launch_bounds__(kBwdThreads)
   const int warps = (int)gridDim.y * (kBwdThreads / 32);
   for (int tile = blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += warps) {
     const float f = id < 0 ? 0.f : -c * ex2(stats[t * tiles + tile].x - l2);
-    const int end = min(V, (tile + 1) * bn);
-    for (int col = tile * bn + lane * 8; col < end; col += 256) {
+    const int start = tile_start(geo, tile), end = min(V, start + tile_width(geo, tile));
+    for (int col = start + lane * 8; col < end; col += 256) {
       uint4* p4 = reinterpret_cast<uint4*>(row + col);
       uint4 u = make_uint4(0u, 0u, 0u, 0u);
       if (id >= 0) {
@@ -464,19 +488,19 @@ __global__ void __launch_bounds__(kBwdThreads)
 // perm its inverse.  The packed rows without a token are zeros, so what stands
 // in them (padding, even NaN) cannot reach the head's gradient, a sum over
 // rows in which their coefficient is 0.
-// A block takes kPackRows rows and counts the ids before them itself (T ids
-// from L2; at T = 8192 a block reads 64 KB), so one launch does it all.
+// A block takes `rows` rows, one a warp at a time, and counts the ids before
+// them itself (T ids from L2), so one launch does it all.
 constexpr int kPackThreads = 256;
-constexpr int kPackRows = 64;
+constexpr int kPackMaxRows = 1024;
 
 __global__ void __launch_bounds__(kPackThreads)
     logprob_pack_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const int64_t* __restrict__ ids, int T,
-                        int H, __nv_bfloat16* __restrict__ hp, int64_t* __restrict__ idp, int* __restrict__ perm,
+                        int H, int rows, __nv_bfloat16* __restrict__ hp, int64_t* __restrict__ idp, int* __restrict__ perm,
                         int* __restrict__ pos, int* __restrict__ count) {
   pdl_prologue();
   __shared__ int s_before[kPackThreads / 32], s_total[kPackThreads / 32];
-  __shared__ int s_pos[kPackRows];
-  const int r0 = blockIdx.x * kPackRows;
+  __shared__ int s_pos[kPackMaxRows];
+  const int r0 = blockIdx.x * rows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int before = 0, total = 0;
   for (int t = threadIdx.x; t < T; t += kPackThreads) {
@@ -501,8 +525,8 @@ __global__ void __launch_bounds__(kPackThreads)
     total += s_total[i];
   }
   if (warp == 0) {
-    for (int i = 0; i < kPackRows; i += 32) {
-      const int t = r0 + i + lane;
+    for (int i = 0; i < rows; i += 32) {
+      const int t = i + lane < rows ? r0 + i + lane : T;
       const int64_t id = t < T ? ids[t] : -1;
       const uint32_t live = __ballot_sync(0xffffffffu, id >= 0);
       const int mine = before + __popc(live & ((1u << lane) - 1u));
@@ -518,11 +542,13 @@ __global__ void __launch_bounds__(kPackThreads)
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) count[0] = total;
   __syncthreads();
-  for (int i = warp; i < kPackRows && r0 + i < T; i += kPackThreads / 32) {
+  for (int i = warp; i < rows && r0 + i < T; i += kPackThreads / 32) {
     const int p = s_pos[i];
     const uint4* src = reinterpret_cast<const uint4*>(h + (int64_t)(r0 + i) * ldh);
     uint4* dst = reinterpret_cast<uint4*>(hp + (int64_t)p * H);
-    for (int k = lane; k < H / 8; k += 32) dst[k] = p < total ? src[k] : make_uint4(0u, 0u, 0u, 0u);
+    const bool has = p < total;
+#pragma unroll 4
+    for (int k = lane; k < H / 8; k += 32) dst[k] = has ? src[k] : make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
@@ -541,8 +567,8 @@ __global__ void __launch_bounds__(256)
 }
 
 template <bool STORE>
-void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& te, const LogprobParams& p, int bn,
-                 float scale, cudaStream_t stream) {
+void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const CUtensorMap& te,
+                 const LogprobParams& p, int a_rows, float scale, cudaStream_t stream) {
   auto kern = logprob_gemm_kernel<STORE>;
   static std::mutex mu;
   static int max_clusters[64] = {0};
@@ -574,20 +600,29 @@ void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap
     }
     clusters = max_clusters[dev & 63];
   }
-  const int64_t tiles = (int64_t)((p.T + 2 * BM_CTA - 1) / (2 * BM_CTA)) * ((p.V + bn - 1) / bn);
+  const int64_t tiles = (int64_t)((p.T + 2 * BM_CTA - 1) / (2 * BM_CTA)) * (p.tiles.n_full + p.tiles.n_rest);
   clusters = (int)std::max<int64_t>(1, std::min<int64_t>(clusters, tiles));
   cfg.gridDim = dim3(2 * clusters, 1, 1);
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, te, p.ids, reinterpret_cast<float2*>(p.stats), p.T, p.V, p.H,
-                                   bn, scale, error_word(dev)));
+  PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, tb2, te, p.ids, p.count, p.row0, reinterpret_cast<float2*>(p.stats),
+                                   p.T, p.V, p.H, a_rows, p.tiles, scale, error_word(dev)));
 }
 
 }  // namespace
 
-int logprob_tile_n(int T, int V) {
-  (void)T;
-  (void)V;
-  return BN_MAX;
+LogprobTiles logprob_tiles(int T, int V) {
+  const int64_t tiles_m = (T + 2 * BM_CTA - 1) / (2 * BM_CTA), pairs = std::max(1, num_sms() / 2);
+  const int wide = V / BN_MAX;  // whole wide tiles
+  const int64_t waves = tiles_m * wide / pairs;
+  LogprobTiles g;
+  g.n_full = (int)std::min<int64_t>(wide, waves * pairs / tiles_m);
+  const int rest = V - g.n_full * BN_MAX;
+  // the narrowest multiple of 32 whose tiles fit one wave
+  g.bn2 = BN_MAX;
+  for (int bn = BN_MAX - 32; bn >= 32; bn -= 32)
+    if (tiles_m * ((rest + bn - 1) / bn) <= pairs) g.bn2 = bn;
+  g.n_rest = (rest + g.bn2 - 1) / g.bn2;
+  return g;
 }
 
 void logprob_fwd(const LogprobParams& p, cudaStream_t stream) {
@@ -596,32 +631,33 @@ void logprob_fwd(const LogprobParams& p, cudaStream_t stream) {
            "logprob: hidden size and row strides must be multiples of 8 elements");
   PB_CHECK((reinterpret_cast<uintptr_t>(p.h) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.w) & 15) == 0,
            "logprob: h and w must be 16-byte aligned");
-  const int bn = p.bn;
-  PB_CHECK(bn >= 32 && bn <= BN_MAX && bn % 32 == 0, "logprob: tile width must be a multiple of 32, at most 256");
   const float scale = kLog2e * p.inv_tau;
-  const CUtensorMap ta = make_tmap_2d_bf16(p.h, p.H, p.T, p.ldh, BK, BM_CTA);
-  const CUtensorMap tb = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, bn / 2);
+  const int a_rows = p.T < BM_CTA ? (p.T + 7) / 8 * 8 : BM_CTA;
+  const CUtensorMap ta = make_tmap_2d_bf16(p.h, p.H, p.T, p.ldh, BK, a_rows);
+  const CUtensorMap tb = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, BN_MAX / 2);
+  const CUtensorMap tb2 = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, p.tiles.bn2 / 2);
   CUtensorMap te{};
   if (p.e) {
     PB_CHECK(p.lde % 8 == 0 && (reinterpret_cast<uintptr_t>(p.e) & 15) == 0, "logprob: E must have 16-byte rows");
     te = make_tmap_2d_bf16_swz(p.e, p.V, p.T, p.lde, kBox, kBox, 64);
-    launch_gemm<true>(ta, tb, te, p, bn, scale, stream);
+    launch_gemm<true>(ta, tb, tb2, te, p, a_rows, scale, stream);
   } else {
-    launch_gemm<false>(ta, tb, te, p, bn, scale, stream);
+    launch_gemm<false>(ta, tb, tb2, te, p, a_rows, scale, stream);
   }
-  const int tiles = (p.V + bn - 1) / bn;
+  const int tiles = p.tiles.n_full + p.tiles.n_rest;
   launch_k(logprob_finish_kernel, p.T, kFinThreads, 0, stream, (const __nv_bfloat16*)p.h, p.ldh,
            (const __nv_bfloat16*)p.w, p.ldw, p.ids, p.perm, (const float2*)p.stats, tiles, p.V, p.H, scale, p.logp, p.lse2);
 }
 
 void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse2, const float* logp, const int64_t* ids,
-                 const int* perm, const float* g, float inv_tau, int T, int V, int bn, cudaStream_t stream) {
+                 const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V,
+                 const LogprobTiles& geo, cudaStream_t stream) {
   if (T == 0) return;
-  const int tiles = (V + bn - 1) / bn;
+  const int tiles = geo.n_full + geo.n_rest;
   // enough blocks for every SM when there are few rows
   const int segs = std::max(1, std::min((tiles + 7) / 8, (8 * num_sms() + T - 1) / T));
   launch_k(logprob_bwd_kernel, dim3(T, segs), kBwdThreads, 0, stream, (__nv_bfloat16*)e, lde, (const float2*)stats,
-           tiles, lse2, logp, ids, perm, g, inv_tau, V, bn);
+           tiles, lse2, logp, ids, perm, count, row0, g, inv_tau, V, geo);
 }
 
 void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, void* hp, int64_t* idp, int* perm,
@@ -629,8 +665,10 @@ void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, 
   PB_CHECK(H % 8 == 0 && ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0 &&
                (reinterpret_cast<uintptr_t>(hp) & 15) == 0,
            "logprob: h must have 16-byte rows");
-  launch_k(logprob_pack_kernel, (T + kPackRows - 1) / kPackRows, kPackThreads, 0, stream, (const __nv_bfloat16*)h, ldh,
-           ids, T, H, (__nv_bfloat16*)hp, idp, perm, pos, count);
+  // 8 rows a block up to 8192 rows; beyond, more, so that all blocks together read at most 8192 ids per row
+  const int rows = std::min(kPackMaxRows, 8 * ((T + 8191) / 8192));
+  launch_k(logprob_pack_kernel, (T + rows - 1) / rows, kPackThreads, 0, stream, (const __nv_bfloat16*)h, ldh, ids, T, H,
+           rows, (__nv_bfloat16*)hp, idp, perm, pos, count);
 }
 
 void logprob_unpack(const void* src, const int* pos, const int* count, int T, int H, void* dst, cudaStream_t stream) {

@@ -24,6 +24,8 @@ std::string num(int64_t n) { return std::to_string(n); }
 #define CHECK_SAME_DEVICE(a, b) \
   TORCH_CHECK((a).device() == (b).device(), #a " and " #b " must be on one device, got ", (a).device().str(), " and ", (b).device().str())
 
+bool given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
+
 void check_rows_bf16(const at::Tensor& t, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.stride(1) == 1, what,
               " must be a 2-D CUDA bf16 tensor with unit inner stride");
@@ -78,12 +80,13 @@ at::Tensor logprob_unpack(const at::Tensor& src, const at::Tensor& pos, const at
   return dst;
 }
 
-// logprob_fwd(h [T, H], w [V, H], ids [T], inv_tau, logp [>= T], e [T, V] or None, perm [T] or None) ->
-// (lse2 [T], stats [T, tiles, 2], tile width); logp of row t goes to logp[perm[t]] (logp[t] without perm)
-std::tuple<at::Tensor, at::Tensor, int64_t> logprob_fwd(const at::Tensor& h, const at::Tensor& w,
-                                                        const at::Tensor& ids, double inv_tau, at::Tensor& logp,
-                                                        const c10::optional<at::Tensor>& e,
-                                                        const c10::optional<at::Tensor>& perm) {
+// logprob_fwd(h [T, H], w [V, H], ids [T], inv_tau, logp [>= T], e [T, V] or None, perm [T] or None, count [1] or
+// None, row0) -> (lse2 [T], stats [T, tiles, 2]); logp of row t goes to logp[perm[t]] (logp[t] without perm).  With
+// count, h holds packed rows from row row0 on, of which the first count[0] have a token.
+std::vector<at::Tensor> logprob_fwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, double inv_tau,
+                                    at::Tensor& logp, const c10::optional<at::Tensor>& e,
+                                    const c10::optional<at::Tensor>& perm, const c10::optional<at::Tensor>& count,
+                                    int64_t row0) {
   check_rows_bf16(h, "logprob: h");
   check_rows_bf16(w, "logprob: w");
   const int64_t T = h.size(0), H = h.size(1), V = w.size(0);
@@ -96,10 +99,10 @@ std::tuple<at::Tensor, at::Tensor, int64_t> logprob_fwd(const at::Tensor& h, con
   CHECK_SAME_DEVICE(h, ids);
   CHECK_SAME_DEVICE(h, logp);
   const c10::cuda::CUDAGuard g(h.device());
-  const int bn = pb::logprob_tile_n((int)T, (int)V);
-  const auto f32 = h.options().dtype(at::kFloat);
-  at::Tensor lse2 = at::empty({T}, f32), stats = at::empty({T, (V + bn - 1) / bn, 2}, f32);
   pb::LogprobParams p{};
+  p.tiles = pb::logprob_tiles((int)T, (int)V);
+  const auto f32 = h.options().dtype(at::kFloat);
+  at::Tensor lse2 = at::empty({T}, f32), stats = at::empty({T, p.tiles.n_full + p.tiles.n_rest, 2}, f32);
   p.h = h.data_ptr();
   p.w = w.data_ptr();
   p.ids = ids.data_ptr<int64_t>();
@@ -108,7 +111,7 @@ std::tuple<at::Tensor, at::Tensor, int64_t> logprob_fwd(const at::Tensor& h, con
   p.lse2 = lse2.data_ptr<float>();
   p.ldh = h.stride(0);
   p.ldw = w.stride(0);
-  if (e.has_value() && e->defined()) {
+  if (given(e)) {
     check_rows_bf16(*e, "logprob: e");
     CHECK_SAME_DEVICE(h, *e);
     TORCH_CHECK(e->size(0) == T && e->size(1) == V && e->stride(0) >= (V + 7) / 8 * 8,
@@ -116,39 +119,44 @@ std::tuple<at::Tensor, at::Tensor, int64_t> logprob_fwd(const at::Tensor& h, con
     p.e = e->data_ptr();
     p.lde = e->stride(0);
   }
-  if (perm.has_value() && perm->defined()) {
+  if (given(perm)) {
     CHECK_SAME_DEVICE(h, *perm);
     p.perm = check_rows_i32(*perm, T, "logprob: perm");
+  }
+  if (given(count)) {
+    CHECK_SAME_DEVICE(h, *count);
+    p.count = check_rows_i32(*count, 1, "logprob: count");
+    p.row0 = (int)row0;
   }
   p.T = (int)T;
   p.V = (int)V;
   p.H = (int)H;
-  p.bn = bn;
   p.inv_tau = (float)inv_tau;
   pb::logprob_fwd(p, cur_stream());
-  return {lse2, stats, bn};
+  return {lse2, stats};
 }
 
-// logprob_bwd(e [T, V], stats, lse2 [T], ids [T], perm [T], logp, g, inv_tau, bn): e becomes the gradient of h w^T;
-// logp and g are in the caller's row order (row perm[t] for row t of e)
+// logprob_bwd(e [T, V], stats, lse2 [T], ids [T], perm [T], count [1], row0, logp, g, inv_tau): e becomes the gradient
+// of h w^T; logp and g are in the caller's row order (row perm[t] for row t of e)
 void logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor& lse2, const at::Tensor& ids,
-                 const at::Tensor& perm, const at::Tensor& logp, const at::Tensor& g, double inv_tau, int64_t bn) {
+                 const at::Tensor& perm, const at::Tensor& count, int64_t row0, const at::Tensor& logp,
+                 const at::Tensor& g, double inv_tau) {
   check_rows_bf16(e, "logprob: e");
   const int64_t T = e.size(0), V = e.size(1);
+  TORCH_CHECK(T >= 1 && V >= 1 && T <= kIntMax / 2 && V <= kIntMax / 2, "logprob: row and vocabulary counts");
   check_ids(ids, T, "logprob: ids");
-  for (const at::Tensor* t : {&stats, &lse2, &ids, &perm, &logp, &g}) CHECK_SAME_DEVICE(e, *t);
+  for (const at::Tensor* t : {&stats, &lse2, &ids, &perm, &count, &logp, &g}) CHECK_SAME_DEVICE(e, *t);
   TORCH_CHECK(logp.numel() == g.numel() && g.numel() >= T, "logprob: logp and g must have one entry per row");
-  TORCH_CHECK(bn >= 32 && bn <= 256 && bn % 32 == 0 && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
-                  stats.numel() == T * ((V + bn - 1) / bn) * 2,
-              "logprob: stats must be the forward's");
+  const c10::cuda::CUDAGuard guard(e.device());
+  const pb::LogprobTiles tiles = pb::logprob_tiles((int)T, (int)V);
+  check_rows_f32(stats, T * (tiles.n_full + tiles.n_rest) * 2, "logprob: stats");
   TORCH_CHECK(e.stride(0) % 8 == 0 && e.stride(0) >= (V + 7) / 8 * 8 &&
                   (reinterpret_cast<uintptr_t>(e.data_ptr()) & 15) == 0,
               "logprob: e must have 16-byte rows with room for whole 8-column groups");
-  const c10::cuda::CUDAGuard guard(e.device());
   pb::logprob_bwd(e.data_ptr(), e.stride(0), stats.data_ptr<float>(), check_rows_f32(lse2, T, "logprob: lse2"),
                   check_rows_f32(logp, logp.numel(), "logprob: logp"), ids.data_ptr<int64_t>(),
-                  check_rows_i32(perm, T, "logprob: perm"), check_rows_f32(g, g.numel(), "logprob: g"),
-                  (float)inv_tau, (int)T, (int)V, (int)bn, cur_stream());
+                  check_rows_i32(perm, T, "logprob: perm"), check_rows_i32(count, 1, "logprob: count"), (int)row0,
+                  check_rows_f32(g, g.numel(), "logprob: g"), (float)inv_tau, (int)T, (int)V, tiles, cur_stream());
 }
 
 // ---------------------------------------------------------------- policy and preference losses
@@ -165,8 +173,6 @@ const uint8_t* check_mask(const at::Tensor& t, int64_t B, int64_t S) {
               "mask must be CUDA bool [", num(B), ", ", num(S), "] with unit inner stride");
   return reinterpret_cast<const uint8_t*>(t.data_ptr<bool>());
 }
-
-bool given(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
 
 struct Chunks {
   int chunk, n;
@@ -548,9 +554,9 @@ void register_objectives(pybind11::module& m) {
   m.def("logprob_pack", &logprob_pack, py::arg("h"), py::arg("ids"));
   m.def("logprob_unpack", &logprob_unpack, py::arg("src"), py::arg("pos"), py::arg("count"));
   m.def("logprob_fwd", &logprob_fwd, py::arg("h"), py::arg("w"), py::arg("ids"), py::arg("inv_tau"), py::arg("logp"),
-        py::arg("e") = py::none(), py::arg("perm") = py::none());
+        py::arg("e") = py::none(), py::arg("perm") = py::none(), py::arg("count") = py::none(), py::arg("row0") = 0);
   m.def("logprob_bwd", &logprob_bwd, py::arg("e"), py::arg("stats"), py::arg("lse2"), py::arg("ids"), py::arg("perm"),
-        py::arg("logp"), py::arg("g"), py::arg("inv_tau"), py::arg("bn"));
+        py::arg("count"), py::arg("row0"), py::arg("logp"), py::arg("g"), py::arg("inv_tau"));
   m.def("policy_loss", &policy_loss, py::arg("logp"), py::arg("old"), py::arg("adv"), py::arg("mask"), py::arg("ref"),
         py::arg("low"), py::arg("high"), py::arg("kl_coef"), py::arg("per_sequence"));
   m.def("preference_loss", &preference_loss, py::arg("logp"), py::arg("ref"), py::arg("mask"), py::arg("beta"),

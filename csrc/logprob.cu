@@ -45,11 +45,7 @@ constexpr int kThreads = 192;
 constexpr int A_BYTES = BM_CTA * BK * 2;
 constexpr int B_BYTES = (BN_MAX / 2) * BK * 2;
 constexpr int STAGES = 6;
-constexpr int kBox = 32;  // E is stored in 32 x 32 boxes of 64-byte rows (64-byte swizzle)
-constexpr int kBoxBytes = kBox * kBox * 2;
-constexpr int kBoxes = 4;     // per epilogue warp: three stores may be draining while one box is filled
-constexpr int EPI_BYTES = 4 * kBoxes * kBoxBytes;
-constexpr int SMEM_BYTES = STAGES * (A_BYTES + B_BYTES) + EPI_BYTES + 1024 + 256;
+constexpr int SMEM_BYTES = STAGES * (A_BYTES + B_BYTES) + 1024 + 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -106,7 +102,7 @@ __device__ __forceinline__ float max32(const float* v) {
 template <typename Release>
 __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, int V, int64_t id, float scale,
                                             Release release) {
-  float m = -INFINITY, s = 0.f;
+  float m = -INFINITY, s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int c = 0; c < bn; c += 32) {
     float v[32];
@@ -116,20 +112,31 @@ __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, 
     mask_cols(v, n_base + c, V, id);
     const float mn = fmaxf(m, max32(v) * scale);
     const float ref = mn == -INFINITY ? 0.f : mn;  // nothing but masked columns so far
-    s *= ex2(m - ref);
+    const float r = ex2(m - ref);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) s += ex2(fmaf(v[j], scale, -ref));
+    for (int q = 0; q < 4; ++q) s[q] *= r;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s[j & 3] += ex2(fmaf(v[j], scale, -ref));
     m = mn;
   }
-  return make_float2(m, s);
+  return make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
+}
+
+// 32 bytes with one store: whole sectors, though every lane is on another row.
+__device__ __forceinline__ void st_32(void* p, const uint32_t* u) {
+  asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]),
+               "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
 }
 
 // The same with E stored: the maximum first (E needs one reference for the
-// whole tile), then the exponentials, 32 x 32 boxes through TMA.
+// whole tile), then the exponentials, straight from registers.  Staging them in
+// shared memory for tile stores put 128 KB more per tile on a shared memory
+// that the MMAs already read at its rate (8192 rows, 6554 with a token:
+// 1605 us; like this 1463).
 template <typename Release>
 __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_base, int V, int64_t id, float scale,
-                                                  const CUtensorMap* tmE, uint8_t* stage, int& next_box, int lane,
-                                                  int y0, Release release) {
+                                                  __nv_bfloat16* e_row, bool row_in, Release release) {
   float m = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < bn; c += 32) {
@@ -141,7 +148,7 @@ __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_
   }
   m *= scale;
   const float ref = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int c = 0; c < bn; c += 32) {
     float v[32];
@@ -153,30 +160,17 @@ __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
       v[j] = ex2(fmaf(v[j], scale, -ref));
-      s += v[j];
+      s[j & 3] += v[j];
     }
-    uint8_t* box = stage + next_box * kBoxBytes;
-    next_box = (next_box + 1) & (kBoxes - 1);
-    if (lane == 0) bulk_wait_group_read<kBoxes - 1>();
-    __syncwarp();
-    uint8_t* row = box + lane * 64;
+    if (row_in && n0 < V) {
+      uint32_t u[16];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint4 u;
-      u.x = pack_bf16x2(v[q * 8 + 0], v[q * 8 + 1]);
-      u.y = pack_bf16x2(v[q * 8 + 2], v[q * 8 + 3]);
-      u.z = pack_bf16x2(v[q * 8 + 4], v[q * 8 + 5]);
-      u.w = pack_bf16x2(v[q * 8 + 6], v[q * 8 + 7]);
-      *reinterpret_cast<uint4*>(row + ((q ^ ((lane >> 1) & 3)) << 4)) = u;
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (n0 < V) tma_store_2d(tmE, box, n0, y0);  // rows and columns past the extents are clipped
-      bulk_commit_group();
+      for (int q = 0; q < 16; ++q) u[q] = pack_bf16x2(v[2 * q], v[2 * q + 1]);
+      st_32(e_row + n0, u);
+      st_32(e_row + n0 + 16, u + 8);
     }
   }
-  return make_float2(m, s);
+  return make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
 }
 
 // Roles per CTA: warp 0 TMA producer, warp 1 TMEM allocator and (even CTA) MMA
@@ -187,7 +181,7 @@ __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_
 template <bool STORE>
 __global__ void __launch_bounds__(kThreads, 1)
     logprob_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                        const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ CUtensorMap tmE,
+                        const __grid_constant__ CUtensorMap tmB2, __nv_bfloat16* __restrict__ e, int64_t lde,
                         const int64_t* __restrict__ ids, const int* __restrict__ count, int row0,
                         float2* __restrict__ stats, int T_all, int V, int H, int a_rows, const LogprobTiles geo, float scale, int* err) {
   pdl_prologue();
@@ -196,8 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * A_BYTES;
-  uint8_t* sEpi = sB + STAGES * B_BYTES;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sEpi + EPI_BYTES);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sB + STAGES * B_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;  // used on the even CTA (256 arrivals: both epilogues)
@@ -297,8 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     const int quarter = warp & 3;
-    uint8_t* stage = sEpi + quarter * kBoxes * kBoxBytes;
-    int local = 0, next_box = 0;
+    int local = 0;
     for (int64_t w = cid; w < num_tiles; w += n_clusters, ++local) {
       const int tm = (int)(w % tiles_m), tn = (int)(w / tiles_m);
       const int acc = local & 1;
@@ -321,13 +313,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int bn = tile_width(geo, tn), n0 = tile_start(geo, tn);
       float2 st;
       if constexpr (STORE)
-        st = row_stats_store(t_row, bn, n0, V, id, scale, &tmE, stage, next_box, lane, y0, release);
+        st = row_stats_store(t_row, bn, n0, V, id, scale, e + (int64_t)t * lde, t < T, release);
       else
         st = row_stats(t_row, bn, n0, V, id, scale, release);
       if (t < T) stats[(int64_t)t * tiles_n + tn] = st;
     }
-    // the box stores must have finished before the kernel's shared memory goes
-    if (STORE && lane == 0) bulk_wait_group<0>();
   }
 
   // On an error path the MMA issuer may have left MMAs in flight: drain them
@@ -438,6 +428,7 @@ __global__ void __launch_bounds__(kFinThreads)
 
 // ---------------------------------------------------------------- backward
 constexpr int kBwdThreads = 256;
+constexpr int kBwdUnroll = 4;
 
 // A warp takes a tile of a row at a time: one factor for its (256) consecutive
 // entries, 8 of them per lane and step.  The target's own entry is
@@ -460,32 +451,51 @@ __global__ void __launch_bounds__(kBwdThreads)
   __nv_bfloat16* row = e + t * lde;
   const int lane = threadIdx.x & 31;
   const int warps = (int)gridDim.y * (kBwdThreads / 32);
-  for (int tile = blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += warps) {
-    const float f = id < 0 ? 0.f : -c * ex2(stats[t * tiles + tile].x - l2);
-    const int start = tile_start(geo, tile), end = min(V, start + tile_width(geo, tile));
+  const float own = id < 0 ? 0.f : -c * expm1f(logp[src]);
+  const float2* st = stats + t * tiles;
+  auto scaled = [&](uint4 u, float f, int col) {
+    uint32_t* p = &u.x;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 x = unpack_bf16x2(p[q]);
+      p[q] = pack_bf16x2(col + 2 * q == id ? own : x.x * f, col + 2 * q + 1 == id ? own : x.y * f);
+    }
+    return u;
+  };
+  int tile = blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5);
+  // wide tiles, kBwdUnroll of them in flight: a tile is one vector a lane
+  for (; tile < geo.n_full; tile += kBwdUnroll * warps) {
+    uint4 u[kBwdUnroll];
+    float f[kBwdUnroll];
+#pragma unroll
+    for (int j = 0; j < kBwdUnroll; ++j) {
+      const int tj = tile + j * warps;
+      if (id >= 0 && tj < geo.n_full) {
+        u[j] = __ldcs(reinterpret_cast<const uint4*>(row + tj * BN_MAX + lane * 8));
+        f[j] = st[tj].x;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kBwdUnroll; ++j) {
+      const int tj = tile + j * warps, col = tj * BN_MAX + lane * 8;
+      if (tj < geo.n_full)
+        *reinterpret_cast<uint4*>(row + col) =
+            id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(u[j], -c * ex2(f[j] - l2), col);
+    }
+  }
+  for (tile = geo.n_full + blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += warps) {
+    const float f = id < 0 ? 0.f : -c * ex2(st[tile].x - l2);
+    const int start = tile_start(geo, tile), end = min(V, start + geo.bn2);
     for (int col = start + lane * 8; col < end; col += 256) {
       uint4* p4 = reinterpret_cast<uint4*>(row + col);
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (id >= 0) {
-        u = *p4;
-        uint32_t* p = &u.x;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float2 x = unpack_bf16x2(p[q]);
-          float a = x.x * f, b = x.y * f;
-          if (col + 2 * q == id) a = -c * expm1f(logp[src]);
-          if (col + 2 * q + 1 == id) b = -c * expm1f(logp[src]);
-          p[q] = pack_bf16x2(a, b);
-        }
-      }
-      *p4 = u;
+      *p4 = id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(*p4, f, col);
     }
   }
 }
 
 // ---------------------------------------------------------------- packing
-// Rows with a token first, in order, then the others: pos[t] is row t's place,
-// perm its inverse.  The packed rows without a token are zeros, so what stands
+// Rows with a token first, in order, then the others: perm[i] is the row at
+// place i.  The packed rows without a token are zeros, so what stands
 // in them (padding, even NaN) cannot reach the head's gradient, a sum over
 // rows in which their coefficient is 0.
 // A block takes `rows` rows, one a warp at a time, and counts the ids before
@@ -496,7 +506,7 @@ constexpr int kPackMaxRows = 1024;
 __global__ void __launch_bounds__(kPackThreads)
     logprob_pack_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const int64_t* __restrict__ ids, int T,
                         int H, int rows, __nv_bfloat16* __restrict__ hp, int64_t* __restrict__ idp, int* __restrict__ perm,
-                        int* __restrict__ pos, int* __restrict__ count) {
+                        int* __restrict__ count) {
   pdl_prologue();
   __shared__ int s_before[kPackThreads / 32], s_total[kPackThreads / 32];
   __shared__ int s_pos[kPackMaxRows];
@@ -533,7 +543,6 @@ __global__ void __launch_bounds__(kPackThreads)
       if (t < T) {
         const int p = id >= 0 ? mine : total + (t - mine);
         s_pos[i + lane] = p;
-        pos[t] = p;
         perm[p] = t;
         idp[p] = id;
       }
@@ -552,23 +561,43 @@ __global__ void __launch_bounds__(kPackThreads)
   }
 }
 
-// dst[t] = src[pos[t]] for rows with a token, 0 for the others; a warp a row.
-__global__ void __launch_bounds__(256)
-    logprob_unpack_kernel(const __nv_bfloat16* __restrict__ src, const int* __restrict__ pos,
-                          const int* __restrict__ count, int T, int H, __nv_bfloat16* __restrict__ dst) {
+// dst[perm[row0 + i]] = the sum over slices, in order, of row i of src - bf16
+// rows (one slice), or the fp32 slabs of a product that was split - for rows
+// with a token, 0 for the others; a block a row.
+template <typename E>
+__global__ void __launch_bounds__(128)
+    logprob_unpack_kernel(const E* __restrict__ src, int slices, const int* __restrict__ perm,
+                          const int* __restrict__ count, int row0, int T, int H, __nv_bfloat16* __restrict__ dst) {
   pdl_prologue();
-  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (t >= T) return;
-  const int p = pos[t];
-  const bool live = p < count[0];
-  const uint4* s = reinterpret_cast<const uint4*>(src + (int64_t)p * H);
-  uint4* d = reinterpret_cast<uint4*>(dst + (int64_t)t * H);
-  for (int k = threadIdx.x & 31; k < H / 8; k += 32) d[k] = live ? s[k] : make_uint4(0u, 0u, 0u, 0u);
+  const int i = blockIdx.x;
+  const bool live = row0 + i < count[0];
+  uint4* d = reinterpret_cast<uint4*>(dst + (int64_t)perm[i] * H);
+  const int64_t slab = (int64_t)T * H;
+  for (int k = threadIdx.x; k < H / 8; k += 128) {
+    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+    if (live) {
+      if constexpr (sizeof(E) == 2) {
+        u = reinterpret_cast<const uint4*>(src + (int64_t)i * H)[k];
+      } else {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = 0; s < slices; ++s) {
+          const float4* p = reinterpret_cast<const float4*>(src + s * slab + (int64_t)i * H) + 2 * k;
+          const float4 a = __ldcs(p), b = __ldcs(p + 1);
+          v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+          v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        }
+        u = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                       pack_bf16x2(v[6], v[7]));
+      }
+    }
+    d[k] = u;
+  }
 }
 
 template <bool STORE>
-void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const CUtensorMap& te,
-                 const LogprobParams& p, int a_rows, float scale, cudaStream_t stream) {
+void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const LogprobParams& p,
+                 int a_rows, float scale, cudaStream_t stream) {
   auto kern = logprob_gemm_kernel<STORE>;
   static std::mutex mu;
   static int max_clusters[64] = {0};
@@ -604,7 +633,7 @@ void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap
   clusters = (int)std::max<int64_t>(1, std::min<int64_t>(clusters, tiles));
   cfg.gridDim = dim3(2 * clusters, 1, 1);
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, tb2, te, p.ids, p.count, p.row0, reinterpret_cast<float2*>(p.stats),
+  PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, tb2, (__nv_bfloat16*)p.e, p.lde, p.ids, p.count, p.row0, reinterpret_cast<float2*>(p.stats),
                                    p.T, p.V, p.H, a_rows, p.tiles, scale, error_word(dev)));
 }
 
@@ -636,13 +665,11 @@ void logprob_fwd(const LogprobParams& p, cudaStream_t stream) {
   const CUtensorMap ta = make_tmap_2d_bf16(p.h, p.H, p.T, p.ldh, BK, a_rows);
   const CUtensorMap tb = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, BN_MAX / 2);
   const CUtensorMap tb2 = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, p.tiles.bn2 / 2);
-  CUtensorMap te{};
   if (p.e) {
-    PB_CHECK(p.lde % 8 == 0 && (reinterpret_cast<uintptr_t>(p.e) & 15) == 0, "logprob: E must have 16-byte rows");
-    te = make_tmap_2d_bf16_swz(p.e, p.V, p.T, p.lde, kBox, kBox, 64);
-    launch_gemm<true>(ta, tb, tb2, te, p, a_rows, scale, stream);
+    PB_CHECK(p.lde % 32 == 0 && (reinterpret_cast<uintptr_t>(p.e) & 63) == 0, "logprob: E must have 64-byte rows");
+    launch_gemm<true>(ta, tb, tb2, p, a_rows, scale, stream);
   } else {
-    launch_gemm<false>(ta, tb, tb2, te, p, a_rows, scale, stream);
+    launch_gemm<false>(ta, tb, tb2, p, a_rows, scale, stream);
   }
   const int tiles = p.tiles.n_full + p.tiles.n_rest;
   launch_k(logprob_finish_kernel, p.T, kFinThreads, 0, stream, (const __nv_bfloat16*)p.h, p.ldh,
@@ -661,19 +688,24 @@ void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse2, co
 }
 
 void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, void* hp, int64_t* idp, int* perm,
-                  int* pos, int* count, cudaStream_t stream) {
+                  int* count, cudaStream_t stream) {
   PB_CHECK(H % 8 == 0 && ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0 &&
                (reinterpret_cast<uintptr_t>(hp) & 15) == 0,
            "logprob: h must have 16-byte rows");
   // 8 rows a block up to 8192 rows; beyond, more, so that all blocks together read at most 8192 ids per row
   const int rows = std::min(kPackMaxRows, 8 * ((T + 8191) / 8192));
   launch_k(logprob_pack_kernel, (T + rows - 1) / rows, kPackThreads, 0, stream, (const __nv_bfloat16*)h, ldh, ids, T, H,
-           rows, (__nv_bfloat16*)hp, idp, perm, pos, count);
+           rows, (__nv_bfloat16*)hp, idp, perm, count);
 }
 
-void logprob_unpack(const void* src, const int* pos, const int* count, int T, int H, void* dst, cudaStream_t stream) {
-  launch_k(logprob_unpack_kernel, (T + 7) / 8, 256, 0, stream, (const __nv_bfloat16*)src, pos, count, T, H,
-           (__nv_bfloat16*)dst);
+void logprob_unpack(const void* src, bool f32, int slices, const int* perm, const int* count, int row0, int T, int H,
+                    void* dst, cudaStream_t stream) {
+  if (f32)
+    launch_k(logprob_unpack_kernel<float>, T, 128, 0, stream, (const float*)src, slices, perm, count, row0, T,
+             H, (__nv_bfloat16*)dst);
+  else
+    launch_k(logprob_unpack_kernel<__nv_bfloat16>, T, 128, 0, stream, (const __nv_bfloat16*)src, 1, perm,
+             count, row0, T, H, (__nv_bfloat16*)dst);
 }
 
 }  // namespace pb

@@ -48,7 +48,7 @@ float* check_rows_f32(const at::Tensor& t, int64_t n, const char* what) {
   return t.data_ptr<float>();
 }
 
-// logprob_pack(h [T, H], ids [T]) -> (packed h, packed ids, perm, pos, count)
+// logprob_pack(h [T, H], ids [T]) -> (packed h, packed ids, perm, count)
 std::vector<at::Tensor> logprob_pack(const at::Tensor& h, const at::Tensor& ids) {
   check_rows_bf16(h, "logprob: h");
   const int64_t T = h.size(0), H = h.size(1);
@@ -58,26 +58,30 @@ std::vector<at::Tensor> logprob_pack(const at::Tensor& h, const at::Tensor& ids)
   const c10::cuda::CUDAGuard g(h.device());
   const auto i32 = h.options().dtype(at::kInt);
   at::Tensor hp = at::empty({T, H}, h.options()), idp = at::empty({T}, ids.options());
-  at::Tensor perm = at::empty({T}, i32), pos = at::empty({T}, i32), count = at::empty({1}, i32);
+  at::Tensor perm = at::empty({T}, i32), count = at::empty({1}, i32);
   pb::logprob_pack(h.data_ptr(), h.stride(0), ids.data_ptr<int64_t>(), (int)T, (int)H, hp.data_ptr(),
-                   idp.data_ptr<int64_t>(), perm.data_ptr<int>(), pos.data_ptr<int>(), count.data_ptr<int>(),
-                   cur_stream());
-  return {hp, idp, perm, pos, count};
+                   idp.data_ptr<int64_t>(), perm.data_ptr<int>(), count.data_ptr<int>(), cur_stream());
+  return {hp, idp, perm, count};
 }
 
-// logprob_unpack(src [T, H], pos, count) -> dst [T, H]
-at::Tensor logprob_unpack(const at::Tensor& src, const at::Tensor& pos, const at::Tensor& count) {
-  check_rows_bf16(src, "logprob: packed rows");
-  TORCH_CHECK(src.is_contiguous() && src.size(1) % 8 == 0, "logprob: packed rows must be contiguous");
-  const int64_t T = src.size(0);
-  CHECK_SAME_DEVICE(src, pos);
+// logprob_unpack(src [slices * T, H] (bf16, one slice, or fp32 slabs), perm [T], count, row0, dst [T_all, H] bf16):
+// dst[perm[i]] = row i of src (its slices added) where packed row row0 + i has a token, else 0
+void logprob_unpack(const at::Tensor& src, const at::Tensor& perm, const at::Tensor& count, int64_t row0,
+                    at::Tensor& dst) {
+  const int64_t T = perm.numel(), H = dst.size(-1);
+  const bool f32 = src.scalar_type() == at::kFloat;
+  TORCH_CHECK(src.is_cuda() && src.is_contiguous() && (f32 || src.scalar_type() == at::kBFloat16) && src.dim() == 2 &&
+                  src.size(1) == H && H % 8 == 0 && T >= 1 && src.size(0) % T == 0 && (f32 || src.size(0) == T),
+              "logprob: packed rows must be contiguous bf16 [T, H] or fp32 slabs [slices * T, H]");
+  TORCH_CHECK(dst.is_contiguous() && dst.scalar_type() == at::kBFloat16 && dst.dim() == 2 && dst.size(0) >= T,
+              "logprob: contiguous bf16 rows to unpack to");
+  CHECK_SAME_DEVICE(src, perm);
   CHECK_SAME_DEVICE(src, count);
+  CHECK_SAME_DEVICE(src, dst);
   const c10::cuda::CUDAGuard g(src.device());
-  at::Tensor dst = at::empty_like(src);
-  pb::logprob_unpack(src.data_ptr(), check_rows_i32(pos, T, "logprob: pos"),
-                     check_rows_i32(count, 1, "logprob: count"), (int)T, (int)src.size(1), dst.data_ptr(),
+  pb::logprob_unpack(src.data_ptr(), f32, (int)(src.size(0) / T), check_rows_i32(perm, T, "logprob: perm"),
+                     check_rows_i32(count, 1, "logprob: count"), (int)row0, (int)T, (int)H, dst.data_ptr(),
                      cur_stream());
-  return dst;
 }
 
 // logprob_fwd(h [T, H], w [V, H], ids [T], inv_tau, logp [>= T], e [T, V] or None, perm [T] or None, count [1] or
@@ -552,7 +556,8 @@ at::Tensor distillation_loss(const at::Tensor& logits, const at::Tensor& top, co
 void register_objectives(pybind11::module& m) {
   namespace py = pybind11;
   m.def("logprob_pack", &logprob_pack, py::arg("h"), py::arg("ids"));
-  m.def("logprob_unpack", &logprob_unpack, py::arg("src"), py::arg("pos"), py::arg("count"));
+  m.def("logprob_unpack", &logprob_unpack, py::arg("src"), py::arg("perm"), py::arg("count"), py::arg("row0"),
+        py::arg("dst"));
   m.def("logprob_fwd", &logprob_fwd, py::arg("h"), py::arg("w"), py::arg("ids"), py::arg("inv_tau"), py::arg("logp"),
         py::arg("e") = py::none(), py::arg("perm") = py::none(), py::arg("count") = py::none(), py::arg("row0") = 0);
   m.def("logprob_bwd", &logprob_bwd, py::arg("e"), py::arg("stats"), py::arg("lse2"), py::arg("ids"), py::arg("perm"),

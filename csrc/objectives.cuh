@@ -40,12 +40,14 @@ void logprob_fwd(const LogprobParams& p, cudaStream_t stream);
 void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse2, const float* logp, const int64_t* ids,
                  const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V,
                  const LogprobTiles& tiles, cudaStream_t stream);
-// hp [T, H]: the rows of h with ids >= 0 in order, then zeros; idp the ids in
-// that order, pos[t] row t's place, perm its inverse, count[0] the rows with a token
+// hp [T, H]: the rows of h with ids >= 0 in order, then zeros; idp the ids and
+// perm the rows in that order, count[0] the rows with a token
 void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, void* hp, int64_t* idp, int* perm,
-                  int* pos, int* count, cudaStream_t stream);
-// dst[t] = src[pos[t]] where row t has a token, else 0
-void logprob_unpack(const void* src, const int* pos, const int* count, int T, int H, void* dst, cudaStream_t stream);
+                  int* count, cudaStream_t stream);
+// dst[perm[i]] = row i of src [T, H] (bf16, or f32: the sum of `slices` such slabs) for the packed rows
+// [row0, row0 + T) with a token, 0 for the others; perm starts at row0
+void logprob_unpack(const void* src, bool f32, int slices, const int* perm, const int* count, int row0, int T, int H,
+                    void* dst, cudaStream_t stream);
 
 // ---- losses over token log-probabilities (objectives.cu); rows b have their
 // own strides, mask is bool bytes (optional).  chunk: objective_chunk(rows, S),

@@ -53,7 +53,7 @@ class _LMHeadLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, ids, inv_tau, max_block_bytes):
         T, V = h.shape[0], w.shape[0]
-        hp, idp, perm, pos, count = ext().logprob_pack(h, ids)
+        hp, idp, perm, count = ext().logprob_pack(h, ids)
         logp = torch.empty(T, device=h.device, dtype=torch.float32)
         block = _block_rows(T, V, max_block_bytes)
         e = _exp_buffer(block, V, h.device)
@@ -64,7 +64,7 @@ class _LMHeadLogProbsFn(torch.autograd.Function):
             lses.append(ext().logprob_fwd(hp[rows], w, idp[rows], inv_tau, logp, None, perm[rows], count, r0)[0])
         # kept outside save_for_backward: e is overwritten by the backward
         ctx.kept = (e, stats, lses)
-        ctx.save_for_backward(hp, w, idp, perm, pos, count, logp)
+        ctx.save_for_backward(hp, w, idp, perm, count, logp)
         ctx.inv_tau, ctx.block = inv_tau, block
         return logp
 
@@ -72,12 +72,12 @@ class _LMHeadLogProbsFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         _one_backward(ctx, "lm_head_log_probs")
-        hp, w, idp, perm, pos, count, logp = ctx.saved_tensors
+        hp, w, idp, perm, count, logp = ctx.saved_tensors
         (e, stats, lses), ctx.kept = ctx.kept, None
         need_h, need_w = ctx.needs_input_grad[:2]
         T, (V, H) = hp.shape[0], w.shape
         g = g.contiguous()
-        dhp = torch.empty_like(hp) if need_h else None
+        dh = torch.empty_like(hp) if need_h else None
         single = ctx.block >= T
         # one row block: the head's gradient is rounded once by its product; several
         # blocks add up in fp32 first
@@ -90,10 +90,9 @@ class _LMHeadLogProbsFn(torch.autograd.Function):
                 _, stats = ext().logprob_fwd(hp[rows], w, idp[rows], ctx.inv_tau, again, e, perm[rows], count, r0)
             ext().logprob_bwd(e, stats, lses[i], idp[rows], perm[rows], count, r0, logp, g, ctx.inv_tau)
             if need_h:
-                _grad_rows(e, w, dhp[rows], count, r0)
+                ext().logprob_unpack(_grad_rows(e, w, count, r0), perm[rows], count, r0, dh)
             if need_w:
                 _grad_head(e, hp[rows], dw, r0 > 0, count, r0)
-        dh = ext().logprob_unpack(dhp, pos, count) if need_h else None
         if need_w and not single:
             out = torch.empty(V, H, device=hp.device, dtype=w.dtype)
             ext().cast_f32_to_bf16(dw, out)
@@ -101,21 +100,20 @@ class _LMHeadLogProbsFn(torch.autograd.Function):
         return dh, dw, None, None, None
 
 
-def _grad_rows(dl: torch.Tensor, w: torch.Tensor, out: torch.Tensor, live=None, row0: int = 0) -> None:
-    """``out = dl @ w`` over the vocabulary, for the rows that ``live`` (a
-    device count over all rows, of which dl starts at row0) says count.
+def _grad_rows(dl: torch.Tensor, w: torch.Tensor, live: torch.Tensor, row0: int) -> torch.Tensor:
+    """``dl @ w`` over the vocabulary, for the rows that ``live`` (a device
+    count over all rows, of which dl starts at row0) says count: bf16 [T, H],
+    or the fp32 slabs [slices * T, H] that are still to be added.
 
     A few rows make few output tiles with a long sum over the vocabulary: K
-    slices spread them over the SMs, each slice an fp32 slab, added in slice
-    order.  The slice count is the cheapest of the wave model of ``gemm``."""
+    slices spread them over the SMs, each slice a slab.  The slice count is
+    the cheapest of the wave model of ``gemm``."""
     (T, V), H = dl.shape, w.shape[1]
     splits = _row_splits(T, H, V)
-    if splits == 1:
-        ext().gemm(dl, w, out, False, True, G.EPI_STORE_BF16, 1.0, live=live, live_row0=row0)
-        return
-    slabs = torch.empty(splits * T, H, device=dl.device, dtype=torch.float32)
-    ext().gemm(dl, w, slabs, False, True, G.EPI_STORE_F32, 1.0, splits=splits, live=live, live_row0=row0)
-    ext().sum_slices(slabs.view(splits, T * H), out.view(-1), False)
+    out = torch.empty(splits * T, H, device=dl.device, dtype=torch.bfloat16 if splits == 1 else torch.float32)
+    ext().gemm(dl, w, out, False, True, G.EPI_STORE_BF16 if splits == 1 else G.EPI_STORE_F32, 1.0, splits=splits,
+               live=live, live_row0=row0)
+    return out
 
 
 def _row_splits(T: int, H: int, V: int, slots: int | None = None) -> int:
@@ -135,9 +133,9 @@ def _row_splits(T: int, H: int, V: int, slots: int | None = None) -> int:
     return best
 
 
-def _grad_head(dl: torch.Tensor, h: torch.Tensor, out: torch.Tensor, accumulate: bool, live=None,
-               row0: int = 0) -> None:
-    """``out (+)= dl.T @ h`` over the rows that count, out bf16 or (over several row blocks) fp32."""
+def _grad_head(dl: torch.Tensor, h: torch.Tensor, out: torch.Tensor, accumulate: bool,
+               live: torch.Tensor | None = None, row0: int = 0) -> None:
+    """``out (+)= dl.T @ h`` over the rows (that count), out bf16 or (over several row blocks) fp32."""
     if out.dtype == torch.bfloat16:
         epi = G.EPI_STORE_BF16
     else:
@@ -189,7 +187,7 @@ def lm_head_log_probs(h: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, tempe
         return _LMHeadLogProbsFn.apply(h2, w, flat, inv_tau, max_block_bytes).view(ids.shape)
     logp = torch.empty(flat.shape, device=h.device, dtype=torch.float32)
     if flat.numel() >= _PACK_ROWS:
-        hp, idp, perm, _, count = ext().logprob_pack(h2, flat)
+        hp, idp, perm, count = ext().logprob_pack(h2, flat)
         ext().logprob_fwd(hp, w, idp, inv_tau, logp, None, perm, count)
     else:
         ext().logprob_fwd(h2, w, flat, inv_tau, logp)
@@ -352,7 +350,7 @@ class _LMHeadDistillationFn(torch.autograd.Function):
             ext().gemm(h[rows], w, logits, False, False, G.EPI_STORE_BF16, 1.0)
             ext().distill_rows(logits, prep, T, top.shape[1], r0, tau, logits if need_h or need_w else None)
             if need_h:
-                _grad_rows(logits, w, dh[rows])
+                ext().gemm(logits, w, dh[rows], False, True, G.EPI_STORE_BF16, 1.0)
             if need_w:
                 _grad_head(logits, h[rows], dw, accumulate=r0 > 0)
         if need_w and block < T:

@@ -4,7 +4,7 @@
 //   logprob_gemm    CTA-pair tcgen05 GEMM h w^T whose epilogue turns each row
 //                   of an output tile into (max, sum of 2^(x - max)) of
 //                   x = l * log2(e), the target column left out; under a
-//                   gradient it also stores E = bf16(2^(x - tile max)).
+//                   gradient it also stores E = 2^(x - tile max) in 16 bits.
 //   logprob_finish  per row: the target logit as its own dot product, the
 //                   merge of the row's tile statistics, logp and the row's
 //                   base-2 log-sum-exp.
@@ -21,9 +21,9 @@
 // of that loss shows; it is added back (kTruncation).
 //
 // E is relative to the tile's own maximum, which is known when the tile is
-// stored, while the row's log-sum-exp is not: an entry keeps 8 bits of its
-// probability whatever its size, and the backward is one multiplication per
-// entry (the factor 2^(tile max - lse2) is shared by a tile's row) in a pass
+// stored, while the row's log-sum-exp is not: an entry keeps 10 bits of its
+// probability whatever its size (pack_e), and the backward is one multiplication
+// per entry (the factor 2^(tile max - lse2) is shared by a tile's row) in a pass
 // bound by memory.  bf16 logits would lose |l| / 256 of the exponent instead.
 #include <cuda_bf16.h>
 #include <math.h>
@@ -44,7 +44,7 @@ constexpr int BN_MAX = 256;
 constexpr int kThreads = 192;
 constexpr int A_BYTES = BM_CTA * BK * 2;
 constexpr int B_BYTES = (BN_MAX / 2) * BK * 2;
-constexpr int STAGES = 6;
+constexpr int STAGES = 7;
 constexpr int SMEM_BYTES = STAGES * (A_BYTES + B_BYTES) + 1024 + 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -128,6 +128,18 @@ __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, 
   return make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
 }
 
+// Two values of [0, 2) in 16 bits each: a float's sign and upper exponent bit
+// are 0 there, so 7 bits of exponent and 9 of mantissa remain (bf16 has 7 of
+// mantissa); rounded to nearest.  NaN does not survive, nor need it: the row's
+// sum has it, and with that every gradient of the row.
+__device__ __forceinline__ uint32_t pack_e(float a, float b) {
+  // bits 29..14, moved to the upper half with the rounding's half added
+  return __byte_perm(__float_as_uint(a) * 4u + 0x8000u, __float_as_uint(b) * 4u + 0x8000u, 0x7632);
+}
+__device__ __forceinline__ float2 unpack_e(uint32_t u) {
+  return make_float2(__uint_as_float((u << 14) & 0x3fffc000u), __uint_as_float((u >> 2) & 0x3fffc000u));
+}
+
 // 32 bytes with one store: whole sectors, though every lane is on another row.
 __device__ __forceinline__ void st_32(void* p, const uint32_t* u) {
   asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]),
@@ -171,7 +183,7 @@ __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_
     if (row_in && n0 < V) {
       uint32_t u[16];
 #pragma unroll
-      for (int q = 0; q < 16; ++q) u[q] = pack_bf16x2(v[2 * q], v[2 * q + 1]);
+      for (int q = 0; q < 16; ++q) u[q] = pack_e(v[2 * q], v[2 * q + 1]);
       st_32(e_row + n0, u);
       st_32(e_row + n0 + 16, u + 8);
     }
@@ -438,7 +450,7 @@ constexpr int kBwdUnroll = 4;
 
 // A warp takes a tile of a row at a time: one factor for its (256) consecutive
 // entries, 8 of them per lane and step.  The target's own entry is
-// c (1 - p) = -c expm1(logp), which bf16 E could not give where p is near 1.
+// c (1 - p) = -c expm1(logp), which E could not give where p is near 1.
 __global__ void __launch_bounds__(kBwdThreads)
     logprob_bwd_kernel(__nv_bfloat16* __restrict__ e, int64_t lde, const float2* __restrict__ stats, int tiles,
                        const float* __restrict__ lse2, const float* __restrict__ logp,
@@ -463,7 +475,7 @@ __global__ void __launch_bounds__(kBwdThreads)
     uint32_t* p = &u.x;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float2 x = unpack_bf16x2(p[q]);
+      const float2 x = unpack_e(p[q]);
       p[q] = pack_bf16x2(col + 2 * q == id ? own : x.x * f, col + 2 * q + 1 == id ? own : x.y * f);
     }
     return u;

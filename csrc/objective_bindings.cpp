@@ -8,6 +8,8 @@
 #include <string>
 #include <vector>
 
+#include "gemm.cuh"
+#include "host_util.h"
 #include "objectives.cuh"
 
 namespace {
@@ -469,6 +471,162 @@ void check_first_order(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the gradient is not differentiable (create_graph)");
 }
 
+// Rows of a [rows, V] 16-bit block of at most max_bytes: whole 256-row tiles, one at least.
+int64_t block_rows(int64_t T, int64_t V, int64_t max_bytes) {
+  return std::max<int64_t>(1, std::min(T, std::max<int64_t>(256, max_bytes / (V * 2) / 256 * 256)));
+}
+
+at::Tensor rows_of(const at::Tensor& t, int64_t r0, int64_t n) { return r0 == 0 && n == t.size(0) ? t : t.narrow(0, r0, n); }
+
+// K slices of dl @ w over the vocabulary.  A few rows make few output tiles with
+// a long sum: slices spread them over the SM pairs, each into an fp32 slab that
+// the unpacking adds in slice order.  The cheapest count by a wave model:
+// ceil(tiles s / pairs) / s of a tile's time at 22 TFLOP/s a pair, and the
+// slabs' round trip at 5 TB/s (8192 x 1024 over 151936: 1753 us in one slice,
+// 1472 + 24 in 4; 333 x 4096: 860 -> 406 + 22).
+int grad_rows_slices(int64_t T, int64_t H, int64_t V) {
+  const int64_t pairs = std::max(1, pb::num_sms() / 2);
+  const int64_t tiles = ((T + 255) / 256) * ((H + 255) / 256);
+  const double t_tile = 2.0 * 256 * 256 * (double)V / 22e12;
+  auto cost = [&](int64_t s) {
+    return (double)((tiles * s + pairs - 1) / pairs) / s * t_tile + (s == 1 ? 0.0 : 2.0 * s * T * H * 4 / 5e12);
+  };
+  int best = 1;
+  for (int s = 2; s <= 16 && V / s >= 1024; ++s)  // at least 16 steps of 64 a slice: none is empty
+    if (cost(s) < 0.97 * cost(best)) best = s;
+  return best;
+}
+
+// dl [T, V] @ w [V, H] for the rows that count: bf16 [T, H], or fp32 slabs [slices * T, H]
+at::Tensor grad_rows(const at::Tensor& dl, const at::Tensor& w, const at::Tensor& count, int64_t row0) {
+  const int64_t T = dl.size(0), V = w.size(0), H = w.size(1);
+  const int slices = grad_rows_slices(T, H, V);
+  at::Tensor out = at::empty({slices * T, H}, dl.options().dtype(slices == 1 ? at::kBFloat16 : at::kFloat));
+  pb::GemmParams p{};
+  p.A = dl.data_ptr();
+  p.B = w.data_ptr();
+  p.C = out.data_ptr();
+  p.lda = dl.stride(0);
+  p.ldb = w.stride(0);
+  p.ldc = H;
+  p.M = (int)T;
+  p.N = (int)H;
+  p.K = (int)V;
+  p.b_mn = true;
+  p.alpha = 1.f;
+  p.epi = slices == 1 ? pb::kEpiStoreBf16 : pb::kEpiStoreF32;
+  p.splits = slices;
+  p.live = count.data_ptr<int>();
+  p.live_row0 = (int)row0;
+  pb::gemm_bf16(p, cur_stream());
+  return out;
+}
+
+// out (+)= dl^T h over the rows that count; out bf16, or fp32 where several row blocks add up
+void grad_head(const at::Tensor& dl, const at::Tensor& h, at::Tensor& out, bool accumulate, const at::Tensor& count,
+               int64_t row0) {
+  pb::GemmParams p{};
+  p.A = dl.data_ptr();
+  p.B = h.data_ptr();
+  p.C = out.data_ptr();
+  p.lda = dl.stride(0);
+  p.ldb = h.stride(0);
+  p.ldc = out.stride(0);
+  p.M = (int)out.size(0);
+  p.N = (int)out.size(1);
+  p.K = (int)dl.size(0);
+  p.a_mn = p.b_mn = true;
+  p.alpha = 1.f;
+  p.epi = out.scalar_type() == at::kBFloat16 ? pb::kEpiStoreBf16 : accumulate ? pb::kEpiAccumF32 : pb::kEpiStoreF32;
+  p.live = count.data_ptr<int>();
+  p.live_row0 = (int)row0;
+  p.live_k = true;
+  pb::gemm_bf16(p, cur_stream());
+}
+
+// The forward keeps 16-bit exponentials of the logits (not the logits) for at
+// most max_block_bytes; the backward scales them in place into the logits'
+// gradient and multiplies it with the head and the hidden states.  Rows beyond
+// that are scored without storing and run through the forward kernel again in
+// the backward, block by block.  All of it works on packed rows: those with a
+// token in front, zeros behind.
+struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids,
+                            double inv_tau, int64_t max_block_bytes) {
+    const c10::cuda::CUDAGuard guard(h.device());
+    const int64_t T = h.size(0), V = w.size(0);
+    const auto packed = logprob_pack(h, ids);  // rows, ids, perm, count
+    at::Tensor logp = at::empty({T}, h.options().dtype(at::kFloat));
+    const int64_t block = block_rows(T, V, max_block_bytes);
+    std::vector<at::Tensor> kept{at::empty({block, (V + 63) / 64 * 64}, h.options()).narrow(1, 0, V)};
+    for (int64_t r0 = 0; r0 < T; r0 += block) {
+      const int64_t n = std::min(block, T - r0);
+      const auto out = logprob_fwd(rows_of(packed[0], r0, n), w, rows_of(packed[1], r0, n), inv_tau, logp,
+                                   r0 == 0 ? c10::optional<at::Tensor>(kept[0]) : c10::nullopt,
+                                   rows_of(packed[2], r0, n), packed[3], r0);
+      if (r0 == 0) kept.push_back(out[1]);
+      kept.push_back(out[0]);
+    }
+    // not save_for_backward: the backward overwrites the exponentials
+    ctx->saved_data["kept"] = kept;
+    ctx->save_for_backward({packed[0], w, packed[1], packed[2], packed[3], logp});
+    ctx->saved_data["inv_tau"] = inv_tau;
+    ctx->saved_data["block"] = block;
+    return logp;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_first_order("lm_head_log_probs");
+    TORCH_CHECK(ctx->saved_data.count("kept"), "lm_head_log_probs supports one backward pass per forward");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &hp = saved[0], &w = saved[1], &idp = saved[2], &perm = saved[3], &count = saved[4],
+                     &logp = saved[5];
+    std::vector<at::Tensor> kept = ctx->saved_data["kept"].toTensorVector();
+    ctx->saved_data.erase("kept");
+    const double inv_tau = ctx->saved_data["inv_tau"].toDouble();
+    const int64_t block = ctx->saved_data["block"].toInt(), T = hp.size(0), V = w.size(0), H = w.size(1);
+    const c10::cuda::CUDAGuard guard(hp.device());
+    const at::Tensor g = grads[0].contiguous();
+    at::Tensor dh, dw;
+    if (ctx->needs_input_grad(0)) dh = at::empty({T, H}, hp.options());
+    // one row block: the head's gradient is rounded once by its product; several add up in fp32 first
+    if (ctx->needs_input_grad(1)) dw = at::empty({V, H}, block >= T ? w.options() : w.options().dtype(at::kFloat));
+    at::Tensor e = kept[0], stats = kept[1];
+    for (int64_t r0 = 0, i = 2; r0 < T; r0 += block, ++i) {
+      const int64_t n = std::min(block, T - r0);
+      const at::Tensor rows = rows_of(hp, r0, n), ids = rows_of(idp, r0, n), pm = rows_of(perm, r0, n);
+      if (r0) {
+        e = rows_of(e, 0, n);
+        at::Tensor again = at::empty_like(logp);  // the forward's logp stands
+        stats = logprob_fwd(rows, w, ids, inv_tau, again, e, pm, count, r0)[1];
+      }
+      logprob_bwd(e, stats, kept[i], ids, pm, count, r0, logp, g, inv_tau);
+      if (dh.defined()) logprob_unpack(grad_rows(e, w, count, r0), pm, count, r0, dh);
+      if (dw.defined()) grad_head(e, rows, dw, r0 > 0, count, r0);
+    }
+    return {dh, dw.defined() ? dw.to(w.scalar_type()) : dw, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// Scoring packs the rows from this many on: below, packing (5 us) would save a part of one to three row tiles.
+constexpr int64_t kPackRows = 768;
+
+at::Tensor lm_head_log_probs(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, double inv_tau,
+                             int64_t max_block_bytes) {
+  check_rows_bf16(h, "lm_head_log_probs: h");
+  check_rows_bf16(w, "lm_head_log_probs: w");
+  if (wants_grad(h) || wants_grad(w)) return LogProbsNode::apply(h, w, ids, inv_tau, max_block_bytes);
+  const c10::cuda::CUDAGuard guard(h.device());
+  at::Tensor logp = at::empty({h.size(0)}, h.options().dtype(at::kFloat));
+  if (h.size(0) >= kPackRows) {
+    const auto packed = logprob_pack(h, ids);
+    logprob_fwd(packed[0], w, packed[1], inv_tau, logp, c10::nullopt, packed[2], packed[3], 0);
+  } else {
+    logprob_fwd(h, w, ids, inv_tau, logp, c10::nullopt, c10::nullopt, c10::nullopt, 0);
+  }
+  return logp;
+}
+
 struct PolicyLossNode : public torch::autograd::Function<PolicyLossNode> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logp, const at::Tensor& old,
                                const at::Tensor& adv, const c10::optional<at::Tensor>& mask,
@@ -555,13 +713,8 @@ at::Tensor distillation_loss(const at::Tensor& logits, const at::Tensor& top, co
 
 void register_objectives(pybind11::module& m) {
   namespace py = pybind11;
-  m.def("logprob_pack", &logprob_pack, py::arg("h"), py::arg("ids"));
-  m.def("logprob_unpack", &logprob_unpack, py::arg("src"), py::arg("perm"), py::arg("count"), py::arg("row0"),
-        py::arg("dst"));
-  m.def("logprob_fwd", &logprob_fwd, py::arg("h"), py::arg("w"), py::arg("ids"), py::arg("inv_tau"), py::arg("logp"),
-        py::arg("e") = py::none(), py::arg("perm") = py::none(), py::arg("count") = py::none(), py::arg("row0") = 0);
-  m.def("logprob_bwd", &logprob_bwd, py::arg("e"), py::arg("stats"), py::arg("lse2"), py::arg("ids"), py::arg("perm"),
-        py::arg("count"), py::arg("row0"), py::arg("logp"), py::arg("g"), py::arg("inv_tau"));
+  m.def("lm_head_log_probs", &lm_head_log_probs, py::arg("h"), py::arg("w"), py::arg("ids"), py::arg("inv_tau"),
+        py::arg("max_block_bytes"));
   m.def("policy_loss", &policy_loss, py::arg("logp"), py::arg("old"), py::arg("adv"), py::arg("mask"), py::arg("ref"),
         py::arg("low"), py::arg("high"), py::arg("kl_coef"), py::arg("per_sequence"));
   m.def("preference_loss", &preference_loss, py::arg("logp"), py::arg("ref"), py::arg("mask"), py::arg("beta"),

@@ -13,7 +13,7 @@ namespace pb {
 // h [T, H] and w [V, H] bf16; ids [T] (negative: no token, logp 0).
 // stats [T, tiles, 2] fp32: per row and tile of vocabulary columns the maximum
 // and sum of 2^(x - max), x = l log2(e), target left out.
-// e (optional, bf16 [T, lde >= V]): 2^(x - tile max).
+// e (optional, 16-bit [T, lde >= V]): 2^(x - tile max), in a format of logprob.cu.
 struct LogprobTiles {
   int n_full, n_rest, bn2;  // n_full tiles of 256 columns, then n_rest of bn2
 };
@@ -35,7 +35,7 @@ struct LogprobParams {
   float inv_tau;
 };
 void logprob_fwd(const LogprobParams& p, cudaStream_t stream);
-// e becomes the gradient of the raw logits h w^T given g = d loss / d logp
+// e becomes the gradient (bf16) of the raw logits h w^T given g = d loss / d logp
 // (row t of e has its logp and g in row perm[t]; e starts at packed row row0)
 void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse2, const float* logp, const int64_t* ids,
                  const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V,

@@ -42,107 +42,6 @@ def _rows_bf16(t: torch.Tensor, what: str) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------- log-probabilities through the LM head
-class _LMHeadLogProbsFn(torch.autograd.Function):
-    """The forward keeps bf16 exponentials of the logits (not the logits) for
-    at most ``max_block_bytes``; the backward scales them in place into the
-    logits' gradient and multiplies it with the head and the hidden states.
-    Rows beyond that are scored without storing and run through the forward
-    kernel again in the backward, block by block.  All of it works on the
-    packed rows: those with a token in front, zeros behind."""
-
-    @staticmethod
-    def forward(ctx, h, w, ids, inv_tau, max_block_bytes):
-        T, V = h.shape[0], w.shape[0]
-        hp, idp, perm, count = ext().logprob_pack(h, ids)
-        logp = torch.empty(T, device=h.device, dtype=torch.float32)
-        block = _block_rows(T, V, max_block_bytes)
-        e = _exp_buffer(block, V, h.device)
-        lse2, stats = ext().logprob_fwd(hp[:block], w, idp[:block], inv_tau, logp, e, perm[:block], count)
-        lses = [lse2]
-        for r0 in range(block, T, block):
-            rows = slice(r0, min(T, r0 + block))
-            lses.append(ext().logprob_fwd(hp[rows], w, idp[rows], inv_tau, logp, None, perm[rows], count, r0)[0])
-        # kept outside save_for_backward: e is overwritten by the backward
-        ctx.kept = (e, stats, lses)
-        ctx.save_for_backward(hp, w, idp, perm, count, logp)
-        ctx.inv_tau, ctx.block = inv_tau, block
-        return logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        _one_backward(ctx, "lm_head_log_probs")
-        hp, w, idp, perm, count, logp = ctx.saved_tensors
-        (e, stats, lses), ctx.kept = ctx.kept, None
-        need_h, need_w = ctx.needs_input_grad[:2]
-        T, (V, H) = hp.shape[0], w.shape
-        g = g.contiguous()
-        dh = torch.empty_like(hp) if need_h else None
-        single = ctx.block >= T
-        # one row block: the head's gradient is rounded once by its product; several
-        # blocks add up in fp32 first
-        dw = torch.empty(V, H, device=hp.device, dtype=w.dtype if single else torch.float32) if need_w else None
-        for i, r0 in enumerate(range(0, T, ctx.block)):
-            rows = slice(r0, min(T, r0 + ctx.block))
-            if r0:
-                e = e[:rows.stop - r0]
-                again = torch.empty_like(logp)  # the forward's logp stands
-                _, stats = ext().logprob_fwd(hp[rows], w, idp[rows], ctx.inv_tau, again, e, perm[rows], count, r0)
-            ext().logprob_bwd(e, stats, lses[i], idp[rows], perm[rows], count, r0, logp, g, ctx.inv_tau)
-            if need_h:
-                ext().logprob_unpack(_grad_rows(e, w, count, r0), perm[rows], count, r0, dh)
-            if need_w:
-                _grad_head(e, hp[rows], dw, r0 > 0, count, r0)
-        if need_w and not single:
-            out = torch.empty(V, H, device=hp.device, dtype=w.dtype)
-            ext().cast_f32_to_bf16(dw, out)
-            dw = out
-        return dh, dw, None, None, None
-
-
-def _grad_rows(dl: torch.Tensor, w: torch.Tensor, live: torch.Tensor, row0: int) -> torch.Tensor:
-    """``dl @ w`` over the vocabulary, for the rows that ``live`` (a device
-    count over all rows, of which dl starts at row0) says count: bf16 [T, H],
-    or the fp32 slabs [slices * T, H] that are still to be added.
-
-    A few rows make few output tiles with a long sum over the vocabulary: K
-    slices spread them over the SMs, each slice a slab.  The slice count is
-    the cheapest of the wave model of ``gemm``."""
-    (T, V), H = dl.shape, w.shape[1]
-    splits = _row_splits(T, H, V)
-    out = torch.empty(splits * T, H, device=dl.device, dtype=torch.bfloat16 if splits == 1 else torch.float32)
-    ext().gemm(dl, w, out, False, True, G.EPI_STORE_BF16 if splits == 1 else G.EPI_STORE_F32, 1.0, splits=splits,
-               live=live, live_row0=row0)
-    return out
-
-
-def _row_splits(T: int, H: int, V: int, slots: int | None = None) -> int:
-    slots = slots or G._pair_slots()
-    tiles = ((T + 255) // 256) * ((H + 255) // 256)
-    t_tile = 2.0 * 256 * 256 * V / G._PAIR_TFLOPS
-
-    def cost(s):
-        slab = 0.0 if s == 1 else 2.0 * s * T * H * 4 / G._SLAB_BYTES_PER_S
-        return -(-tiles * s // slots) / s * t_tile + slab
-
-    best = 1
-    for s in range(2, 17):
-        # every slice has work: at least 16 steps of 64, and none is empty
-        if V // s >= 1024 and cost(s) < 0.97 * cost(best):
-            best = s
-    return best
-
-
-def _grad_head(dl: torch.Tensor, h: torch.Tensor, out: torch.Tensor, accumulate: bool,
-               live: torch.Tensor | None = None, row0: int = 0) -> None:
-    """``out (+)= dl.T @ h`` over the rows (that count), out bf16 or (over several row blocks) fp32."""
-    if out.dtype == torch.bfloat16:
-        epi = G.EPI_STORE_BF16
-    else:
-        epi = G.EPI_ACCUM_F32 if accumulate else G.EPI_STORE_F32
-    ext().gemm(dl, h, out, True, True, epi, 1.0, live=live, live_row0=row0, live_k=live is not None)
-
-
 def _block_rows(T: int, V: int, max_block_bytes: int) -> int:
     """Rows of a [rows, V] bf16 block of at most ``max_block_bytes`` (whole
     256-row tiles, one at least)."""
@@ -152,11 +51,6 @@ def _block_rows(T: int, V: int, max_block_bytes: int) -> int:
 def _exp_buffer(rows: int, V: int, device) -> torch.Tensor:
     """bf16 [rows, V] with 128-byte aligned rows."""
     return torch.empty(rows, (V + 63) // 64 * 64, device=device, dtype=torch.bfloat16)[:, :V]
-
-
-# Scoring packs the rows that have a token (prompts and padding have none) from
-# this many rows on: below, it would save a fraction of one or two row tiles.
-_PACK_ROWS = 768
 
 
 def lm_head_log_probs(h: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, temperature: float = 1.0,
@@ -182,16 +76,7 @@ def lm_head_log_probs(h: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, tempe
     if flat.numel() == 0:
         return (h2.float().sum(-1) + w[:0].float().sum()).view(ids.shape)
     h2, w = _rows_bf16(h2, "h"), _rows_bf16(w, "w")
-    inv_tau = 1.0 / float(temperature)
-    if torch.is_grad_enabled() and (h2.requires_grad or w.requires_grad):
-        return _LMHeadLogProbsFn.apply(h2, w, flat, inv_tau, max_block_bytes).view(ids.shape)
-    logp = torch.empty(flat.shape, device=h.device, dtype=torch.float32)
-    if flat.numel() >= _PACK_ROWS:
-        hp, idp, perm, count = ext().logprob_pack(h2, flat)
-        ext().logprob_fwd(hp, w, idp, inv_tau, logp, None, perm, count)
-    else:
-        ext().logprob_fwd(h2, w, flat, inv_tau, logp)
-    return logp.view(ids.shape)
+    return ext().lm_head_log_probs(h2, w, flat, 1.0 / float(temperature), int(max_block_bytes)).view(ids.shape)
 
 
 def _log_probs_plain(h, w, ids, temperature):
@@ -352,7 +237,8 @@ class _LMHeadDistillationFn(torch.autograd.Function):
             if need_h:
                 ext().gemm(logits, w, dh[rows], False, True, G.EPI_STORE_BF16, 1.0)
             if need_w:
-                _grad_head(logits, h[rows], dw, accumulate=r0 > 0)
+                epi = G.EPI_STORE_BF16 if block >= T else G.EPI_ACCUM_F32 if r0 else G.EPI_STORE_F32
+                ext().gemm(logits, h[rows], dw, True, True, epi, 1.0)
         if need_w and block < T:
             out = torch.empty(V, H, device=h.device, dtype=w.dtype)
             ext().cast_f32_to_bf16(dw, out)

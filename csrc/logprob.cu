@@ -102,32 +102,6 @@ __device__ __forceinline__ float max32(const float* v) {
   return m;
 }
 
-// Statistics of one accumulator row (one thread) of `bn` columns from TMEM:
-// running maximum and sum over 32-column chunks.  `release` runs after the
-// last TMEM read.
-template <typename Release>
-__device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, int V, int64_t id, float scale,
-                                            Release release) {
-  float m = -INFINITY, s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-  for (int c = 0; c < bn; c += 32) {
-    float v[32];
-    tmem_ld32(t_row + c, v);
-    wait_ld(v);
-    if (c + 32 >= bn) release();
-    mask_cols(v, n_base + c, V, id);
-    const float mn = fmaxf(m, max32(v) * scale);
-    const float ref = mn == -INFINITY ? 0.f : mn;  // nothing but masked columns so far
-    const float r = ex2(m - ref);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) s[q] *= r;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) s[j & 3] += ex2(fmaf(v[j], scale, -ref));
-    m = mn;
-  }
-  return make_float2(m, (s[0] + s[1]) + (s[2] + s[3]));
-}
-
 // Two values of [0, 2) in 16 bits each: a float's sign and upper exponent bit
 // are 0 there, so 7 bits of exponent and 9 of mantissa remain (bf16 has 7 of
 // mantissa); rounded to nearest.  NaN does not survive, nor need it: the row's
@@ -147,14 +121,18 @@ __device__ __forceinline__ void st_32(void* p, const uint32_t* u) {
                : "memory");
 }
 
-// The same with E stored: the maximum first (E needs one reference for the
-// whole tile), then the exponentials, straight from registers.  Staging them in
-// shared memory for tile stores put 128 KB more per tile on a shared memory
-// that the MMAs already read at its rate (8192 rows, 6554 with a token:
-// 1605 us; like this 1463).
-template <typename Release>
-__device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_base, int V, int64_t id, float scale,
-                                                  __nv_bfloat16* e_row, bool row_in, Release release) {
+// Statistics of one accumulator row (one thread) of `bn` columns from TMEM: the
+// maximum first (E needs one reference for the whole tile), then the sum of the
+// exponentials, which under a gradient (STORE) also go to E, straight from
+// registers.  Staging them in shared memory for tile stores put 128 KB more per
+// tile on a shared memory that the MMAs already read at its rate (8192 rows,
+// 6554 with a token: 1605 us; like this 1463).  Scoring takes the same two
+// passes, although a running maximum would do: the log-probabilities then are
+// the same bits as in training, and a policy's ratio to itself is exactly 1.
+// `release` runs after the last TMEM read.
+template <bool STORE, typename Release>
+__device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, int V, int64_t id, float scale,
+                                            __nv_bfloat16* e_row, bool row_in, Release release) {
   float m = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < bn; c += 32) {
@@ -165,7 +143,7 @@ __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_
     m = fmaxf(m, max32(v));
   }
   m *= scale;
-  const float ref = m == -INFINITY ? 0.f : m;
+  const float ref = m == -INFINITY ? 0.f : m;  // nothing but masked columns
   float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int c = 0; c < bn; c += 32) {
@@ -180,7 +158,7 @@ __device__ __forceinline__ float2 row_stats_store(uint32_t t_row, int bn, int n_
       v[j] = ex2(fmaf(v[j], scale, -ref));
       s[j & 3] += v[j];
     }
-    if (row_in && n0 < V) {
+    if (STORE && row_in && n0 < V) {
       uint32_t u[16];
 #pragma unroll
       for (int q = 0; q < 16; ++q) u[q] = pack_e(v[2 * q], v[2 * q + 1]);
@@ -329,11 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int64_t id = t < T ? ids[t] : -1;
       const int bn = tile_width(geo, tn), n0 = tile_start(geo, tn);
-      float2 st;
-      if constexpr (STORE)
-        st = row_stats_store(t_row, bn, n0, V, id, scale, e + (int64_t)t * lde, t < T, release);
-      else
-        st = row_stats(t_row, bn, n0, V, id, scale, release);
+      const float2 st = row_stats<STORE>(t_row, bn, n0, V, id, scale, e + (int64_t)t * lde, t < T, release);
       if (t < T) stats[(int64_t)t * tiles_n + tn] = st;
     }
   }

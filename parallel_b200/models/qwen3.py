@@ -23,6 +23,7 @@ import torch.nn as nn
 
 from ..ops import functional as Fx
 from ..ops import moe as MoE
+from ..ops import objectives as Obj
 from .config import ModelConfig
 
 
@@ -51,6 +52,7 @@ class ParallelContext:
 class CausalLMOutput:
     loss: Optional[torch.Tensor] = None
     logits: Optional[torch.Tensor] = None
+    log_probs: Optional[torch.Tensor] = None  # of ``targets``, fp32 [B, S]
     aux_loss: Optional[torch.Tensor] = None
     router_logits: Optional[tuple] = None
     hidden_states: Optional[torch.Tensor] = None
@@ -335,8 +337,22 @@ class Qwen3ForCausalLM(nn.Module):
                         p.normal_(0.0, std)
 
     def forward(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None, shift_labels: bool = True,
-                return_logits: bool = False, output_router_logits: bool | None = None) -> CausalLMOutput:
+                return_logits: bool = False, output_router_logits: bool | None = None,
+                targets: torch.Tensor | None = None, teacher: tuple | None = None,
+                temperature: float = 1.0) -> CausalLMOutput:
+        """``labels`` gives ``loss`` (mean cross-entropy).  For post-training, without materialised logits:
+        ``targets`` [B, S] (-100 = none) gives ``log_probs``, where targets[b, t] is the token that position t
+        predicts (not shifted here); ``teacher`` = (top_logits, top_ids, mask or None), [B, S, K] and [B, S],
+        gives ``loss`` (distillation).  ``temperature`` divides the logits of both."""
         ctx = self.ctx
+        if targets is not None or teacher is not None:
+            if ctx.tp_size > 1:
+                raise NotImplementedError("targets / teacher need the whole vocabulary on each rank (no tensor "
+                                          "parallelism)")
+            if labels is not None:
+                raise ValueError("one objective per forward pass: labels, or targets, or teacher")
+            if targets is not None and teacher is not None:
+                raise ValueError("one objective per forward pass: labels, or targets, or teacher")
         B, S = input_ids.shape
         inv_freq = self.model.rotary_emb.inv_freq
         for layer in self.model.layers:
@@ -373,12 +389,20 @@ class Qwen3ForCausalLM(nn.Module):
         if labels is not None:
             y = Fx.shift_labels(labels) if shift_labels else labels
             out.loss = Fx.lm_head_cross_entropy(x.reshape(B * S, -1), self.lm_head.weight, y, tied=tied)
+        elif targets is not None:
+            out.log_probs = Obj.lm_head_log_probs(x, self.lm_head.weight, targets, temperature=temperature)
+        elif teacher is not None:
+            top_logits, top_ids, mask = teacher
+            out.loss = Obj.lm_head_distillation(x, self.lm_head.weight, top_logits, top_ids, mask=mask,
+                                                temperature=temperature)
+        if labels is not None or targets is not None or teacher is not None:
             if self.config.is_moe and (self.config.output_router_logits if output_router_logits is None
                                        else output_router_logits) and router_logits:
                 out.aux_loss = MoE.load_balancing_loss(router_logits, self.config.num_experts,
                                                        self.config.num_experts_per_tok)
-                out.loss = out.loss + self.config.router_aux_loss_coef * out.aux_loss
-        if return_logits or labels is None:
+                if out.loss is not None:  # with targets the caller's loss adds it
+                    out.loss = out.loss + self.config.router_aux_loss_coef * out.aux_loss
+        if return_logits or (labels is None and targets is None and teacher is None):
             out.logits = self.lm_head(x)
         out.hidden_states = x
         return out

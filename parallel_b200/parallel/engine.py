@@ -139,15 +139,40 @@ class ParallelEngine:
 
     # ------------------------------------------------------------------ fwd / bwd
     def forward(self, x, y):
+        return self._run_forward(x, labels=y)
+
+    def log_probs(self, x, targets, temperature: float = 1.0):
+        """Log-probabilities of ``targets`` [B, S] (the token each position
+        predicts, -100 = none) under the model: the outputs' ``log_probs``,
+        fp32 [B, S].  Under ``torch.no_grad()`` this scores a batch (a
+        reference or the sampling policy); otherwise a loss on them
+        (``ops.objectives.policy_loss``, ``preference_loss``) goes to
+        ``backward`` as any other."""
+        self._refuse_model_parallel("log_probs")
+        return self._run_forward(x, targets=targets, temperature=temperature)
+
+    def distill(self, x, top_logits, top_ids, mask=None, temperature: float = 1.0):
+        """Forward pass whose ``loss`` is the distillation from a teacher's top
+        logits [B, S, K] and their ids (``ops.objectives.lm_head_distillation``)."""
+        self._refuse_model_parallel("distill")
+        return self._run_forward(x, teacher=(top_logits, top_ids, mask), temperature=temperature)
+
+    def _refuse_model_parallel(self, what: str) -> None:
+        if self.mp_wrapper.is_active:
+            raise NotImplementedError(f"{what} needs the whole vocabulary on each rank; model parallelism shards it")
+
+    def _run_forward(self, x, labels=None, **objective):
         self._reset_peak()
         with collective_phase("forward"):
             with torch.autocast(device_type=self.device.type, dtype=self.amp_dtype,
                                 enabled=self.use_amp and self.device.type == "cuda"):
                 if self.mp_wrapper.is_active:
                     outputs = self.model(input_ids=x)
-                    outputs.loss = self.mp_wrapper.training_loss(outputs, y)
+                    outputs.loss = self.mp_wrapper.training_loss(outputs, labels)
+                elif objective:
+                    outputs = self.model(input_ids=x, **objective)
                 else:
-                    outputs = self.model(input_ids=x, labels=y)
+                    outputs = self.model(input_ids=x, labels=labels)
         self._forward_peak_memory_allocated = max(self._forward_peak_memory_allocated, self._peak())
         return outputs
 

@@ -150,3 +150,99 @@ def test_lm_head_distillation_plain_and_refusals():
         O.distillation_loss(x, top, ids.float())
     with pytest.raises(ValueError):
         O.lm_head_distillation(h, w[:, :4], top, ids)
+
+
+@pytest.mark.parametrize("objective", ["policy", "preference", "distill"])
+def test_post_training_example_on_cpu(objective):
+    """The example's loop through the engine: the loss falls, and the first step's statistics are those of a policy
+    that still is its own reference."""
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "post_training.py")
+    spec = importlib.util.spec_from_file_location("post_training", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    history = mod.main([objective, "--steps", "4", "--device", "cpu"])
+    assert history[-1]["loss"] < history[0]["loss"]
+    if objective == "policy":
+        assert history[0]["kl"] == 0 and history[0]["clipped"] == 0
+    if objective == "preference":
+        assert abs(history[0]["loss"] - 0.6931) < 1e-3 and history[-1]["reward_gap"] > 0
+
+
+def test_model_objectives_match_its_logits_and_refuse_mixtures():
+    from parallel_b200.models.config import resolve_config
+    from parallel_b200.models.qwen3 import build_model
+
+    m = build_model(resolve_config("tiny-qwen3"), dtype=torch.float32, seed=0)
+    x = torch.randint(0, 1024, (2, 9), generator=torch.Generator().manual_seed(0))
+    targets = torch.randint(0, 1024, (2, 9), generator=torch.Generator().manual_seed(1))
+    targets[0, :3] = -100
+    logits = m(input_ids=x).logits
+    out = m(input_ids=x, targets=targets, temperature=0.8)
+    want = torch.log_softmax(logits / 0.8, -1).gather(-1, targets.clamp_min(0)[..., None])[..., 0]
+    assert out.logits is None and out.loss is None
+    assert torch.allclose(out.log_probs, want.masked_fill(targets < 0, 0.0), atol=1e-5)
+    top = logits.detach().topk(4, dim=-1)
+    out = m(input_ids=x, teacher=(top.values, top.indices, targets >= 0), temperature=2.0)
+    ref = O.distillation_loss(logits, top.values, top.indices, mask=targets >= 0, temperature=2.0)
+    assert torch.allclose(out.loss, ref, atol=1e-6) and out.logits is None
+    with pytest.raises(ValueError):
+        m(input_ids=x, labels=x, targets=targets)
+    with pytest.raises(ValueError):
+        m(input_ids=x, targets=targets, teacher=(top.values, top.indices, None))
+
+
+def _fsdp_preference_worker(rank, world, out):
+    """Each rank holds one pair (two sequences) of the batch; four preference steps under FSDP."""
+    from dist_utils import cpu_cfg
+    from parallel_b200.models.config import resolve_config
+    from parallel_b200.models.qwen3 import build_model
+    from parallel_b200.parallel.engine import ParallelEngine
+    from parallel_b200.state import ParallelConfig
+
+    cfg = cpu_cfg(**{"parallel.dp_shard": world, "engine.activation_checkpoint": "true"})
+    pc = ParallelConfig(cfg)
+    pc.set_device_mesh("cpu")
+    m = build_model(resolve_config("tiny-qwen3"), dtype=torch.float32, seed=0)
+    eng = ParallelEngine(m, None, pc, cfg, torch.device("cpu"))
+    tok = torch.randint(0, 1024, (2 * world, 33), generator=torch.Generator().manual_seed(5))
+    mine = tok[[rank, world + rank]]  # the chosen and the rejected sequence of this rank's pair
+    x, y = mine[:, :-1], mine[:, 1:]
+    with torch.no_grad():
+        ref = eng.log_probs(x, y).log_probs
+    losses = []
+    for _ in range(4):
+        loss = O.preference_loss(eng.log_probs(x, y).log_probs, ref_logp=ref).loss
+        eng.backward(loss)
+        eng.step()
+        losses.append(eng.reduce_loss(loss.detach().clone()).item())
+    if rank == 0:
+        torch.save({"losses": losses}, out)
+
+
+def test_preference_training_under_fsdp_equals_one_process(tmp_path):
+    from dist_utils import run_ranks
+
+    out = str(tmp_path / "out.pt")
+    run_ranks(_fsdp_preference_worker, 2, out)
+    sharded = torch.load(out, weights_only=False)
+
+    from parallel_b200.models.config import resolve_config
+    from parallel_b200.models.qwen3 import build_model
+    from parallel_b200.parallel.optim import FusedAdamW
+
+    m = build_model(resolve_config("tiny-qwen3"), dtype=torch.float32, seed=0)
+    opt = FusedAdamW(list(m.parameters()), lr=1e-3, betas=(0.9, 0.999), weight_decay=0.01)
+    tok = torch.randint(0, 1024, (4, 33), generator=torch.Generator().manual_seed(5))
+    x, y = tok[:, :-1], tok[:, 1:]
+    with torch.no_grad():
+        ref = m(input_ids=x, targets=y).log_probs
+    for want in sharded["losses"]:
+        loss = O.preference_loss(m(input_ids=x, targets=y).log_probs, ref_logp=ref).loss
+        loss.backward()
+        torch.nn.utils.clip_grad_norm_(list(m.parameters()), 1.0)
+        opt.step()
+        opt.zero_grad(set_to_none=True)
+        assert abs(loss.item() - want) < 1e-5

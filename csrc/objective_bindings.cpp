@@ -202,15 +202,16 @@ std::vector<c10::optional<at::Tensor>> policy_fwd(const at::Tensor& logp, const 
   pb::PolicyParams p{};
   p.logp = check_tokens(logp, B, S, "policy_fwd: logp");
   p.old = check_tokens(old, B, S, "policy_fwd: old log-probabilities");
-  TORCH_CHECK(adv.is_cuda() && adv.scalar_type() == at::kFloat && adv.dim() == 2 && adv.size(0) == B && adv.size(1) == S,
-              "policy_fwd: advantages must be CUDA fp32 [B, S] (any strides)");
+  TORCH_CHECK(adv.is_cuda() && adv.scalar_type() == at::kFloat && adv.dim() == 2 && adv.size(0) == B &&
+                  (adv.size(1) == S || adv.size(1) == 1),
+              "policy_fwd: advantages must be CUDA fp32 [B, S] (any strides) or [B, 1]");
   CHECK_SAME_DEVICE(logp, old);
   CHECK_SAME_DEVICE(logp, adv);
   p.adv = adv.data_ptr<float>();
   p.ld_logp = logp.stride(0);
   p.ld_old = old.stride(0);
   p.adv_sb = adv.stride(0);
-  p.adv_ss = adv.stride(1);
+  p.adv_ss = adv.size(1) == S ? adv.stride(1) : 0;
   if (given(mask)) {
     CHECK_SAME_DEVICE(logp, *mask);
     p.mask = check_mask(*mask, B, S);
@@ -631,9 +632,9 @@ struct PolicyLossNode : public torch::autograd::Function<PolicyLossNode> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logp, const at::Tensor& old,
                                const at::Tensor& adv, const c10::optional<at::Tensor>& mask,
                                const c10::optional<at::Tensor>& ref, double low, double high, double kl_coef,
-                               bool per_sequence, bool want) {
-    auto out = policy_fwd(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence, want);
-    if (want) ctx->save_for_backward({*out[3], *out[4], or_undefined(out[5])});
+                               bool per_sequence) {
+    auto out = policy_fwd(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence, true);
+    ctx->save_for_backward({*out[3], *out[4], or_undefined(out[5])});
     ctx->mark_non_differentiable({*out[1], *out[2]});
     ctx->set_materialize_grads(false);
     return {*out[0], *out[1], *out[2]};
@@ -641,7 +642,7 @@ struct PolicyLossNode : public torch::autograd::Function<PolicyLossNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     check_first_order("policy_loss");
     const auto saved = ctx->get_saved_variables();
-    variable_list grads(10);
+    variable_list grads(9);  // to logp alone
     if (g[0].defined()) grads[0] = policy_bwd(saved[0], g[0], saved[1], or_none(saved[2]));
     return grads;
   }
@@ -650,8 +651,11 @@ struct PolicyLossNode : public torch::autograd::Function<PolicyLossNode> {
 std::vector<at::Tensor> policy_loss(const at::Tensor& logp, const at::Tensor& old, const at::Tensor& adv,
                                     const c10::optional<at::Tensor>& mask, const c10::optional<at::Tensor>& ref,
                                     double low, double high, double kl_coef, bool per_sequence) {
-  return PolicyLossNode::apply(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence,
-                               wants_grad(logp));
+  if (!wants_grad(logp)) {
+    const auto out = policy_fwd(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence, false);
+    return {*out[0], *out[1], *out[2]};
+  }
+  return PolicyLossNode::apply(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence);
 }
 
 struct PreferenceLossNode : public torch::autograd::Function<PreferenceLossNode> {
@@ -676,6 +680,10 @@ struct PreferenceLossNode : public torch::autograd::Function<PreferenceLossNode>
 std::vector<at::Tensor> preference_loss(const at::Tensor& logp, const c10::optional<at::Tensor>& ref,
                                         const c10::optional<at::Tensor>& mask, double beta, double smoothing,
                                         bool average) {
+  if (!wants_grad(logp)) {
+    const auto out = preference_fwd(logp, ref, mask, beta, smoothing, average);
+    return {out[0], out[1]};
+  }
   return PreferenceLossNode::apply(logp, ref, mask, beta, smoothing, average);
 }
 
@@ -683,13 +691,12 @@ std::vector<at::Tensor> preference_loss(const at::Tensor& logp, const c10::optio
 // logits, and scaled by the incoming gradient in the backward.
 struct DistillationNode : public torch::autograd::Function<DistillationNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& top,
-                            const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau, bool want) {
+                            const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau) {
     const auto prep = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau);
-    std::vector<at::Tensor> grad;
-    if (want) grad = grad_like(logits);
-    distill_rows(logits, prep, top.size(0), top.size(1), 0, tau, want ? c10::optional<at::Tensor>(grad[0]) : c10::nullopt);
+    const std::vector<at::Tensor> grad = grad_like(logits);
+    distill_rows(logits, prep, top.size(0), top.size(1), 0, tau, grad[0]);
     // not save_for_backward: the backward hands the gradient out, it does not keep it
-    if (want) ctx->saved_data["grad"] = grad;
+    ctx->saved_data["grad"] = grad;
     return prep[1];
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -698,7 +705,7 @@ struct DistillationNode : public torch::autograd::Function<DistillationNode> {
     std::vector<at::Tensor> grad = ctx->saved_data["grad"].toTensorVector();
     ctx->saved_data.erase("grad");
     objective_scale(grad[1], g[0]);
-    variable_list grads(6);
+    variable_list grads(5);
     grads[0] = grad[0];
     return grads;
   }
@@ -706,7 +713,12 @@ struct DistillationNode : public torch::autograd::Function<DistillationNode> {
 
 at::Tensor distillation_loss(const at::Tensor& logits, const at::Tensor& top, const at::Tensor& ids,
                              const c10::optional<at::Tensor>& mask, double tau) {
-  return DistillationNode::apply(logits, top, ids, mask, tau, wants_grad(logits));
+  if (!wants_grad(logits)) {
+    const auto prep = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau);
+    distill_rows(logits, prep, top.size(0), top.size(1), 0, tau, c10::nullopt);
+    return prep[1];
+  }
+  return DistillationNode::apply(logits, top, ids, mask, tau);
 }
 
 }  // namespace

@@ -101,14 +101,13 @@ class PreferenceLoss(NamedTuple):
 
 
 def _tokens(t: torch.Tensor | None, like: torch.Tensor, what: str) -> torch.Tensor | None:
-    """fp32 [B, S] without gradient, rows of unit inner stride."""
+    """[B, S] of logp's type, rows of unit inner stride."""
     if t is None:
         return None
     if t.dtype != like.dtype:
         raise TypeError(f"{what} must be {like.dtype}, got {t.dtype}")
     if t.shape != like.shape:
         raise ValueError(f"{what} {tuple(t.shape)} must have logp's shape {tuple(like.shape)}")
-    t = t.detach()
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
@@ -143,18 +142,16 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Te
     if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0):
         raise ValueError(f"clip range: 0 <= clip_low <= 1 and clip_high >= 0, got {clip_low} and {clip_high}")
     B, S = logp.shape
-    adv = advantages.detach()
-    if adv.dim() == 1:
-        adv = adv[:, None]
+    adv = advantages if advantages.dim() != 1 else advantages[:, None]
     if adv.dtype != logp.dtype:
         raise TypeError(f"advantages must be {logp.dtype}, got {adv.dtype}")
     if tuple(adv.shape) not in ((B, S), (B, 1)):
         raise ValueError(f"advantages {tuple(advantages.shape)}: [{B}, {S}], [{B}, 1] or [{B}] expected")
-    adv = adv.expand(B, S)
     old, ref = _tokens(old_logp, logp, "old_logp"), _tokens(ref_logp, logp, "ref_logp")
     low, high, per_sequence = 1.0 - clip_low, 1.0 + clip_high, reduction == "sequence"
     if not logp.is_cuda:
-        return _policy_plain(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence)
+        return _policy_plain(logp, old.detach(), adv.detach().expand(B, S), mask,
+                             None if ref is None else ref.detach(), low, high, kl_coef, per_sequence)
     return PolicyLoss(*ext().policy_loss(_unit_inner(logp), old, adv, _unit_inner(mask), ref, low, high,
                                          float(kl_coef), per_sequence))
 
@@ -199,7 +196,7 @@ def preference_loss(logp: torch.Tensor, ref_logp: torch.Tensor | None = None, ma
         raise ValueError(f"0 <= label_smoothing <= 1 and a finite beta, got {label_smoothing} and {beta}")
     ref = _tokens(ref_logp, logp, "ref_logp")
     if not logp.is_cuda:
-        return _preference_plain(logp, ref, mask, beta, label_smoothing, average)
+        return _preference_plain(logp, None if ref is None else ref.detach(), mask, beta, label_smoothing, average)
     return PreferenceLoss(*ext().preference_loss(_unit_inner(logp), ref, _unit_inner(mask), float(beta),
                                                  float(label_smoothing), bool(average)))
 
@@ -274,8 +271,11 @@ def _check_teacher(rows, top_logits, top_ids, mask, temperature):
     if mask is not None and (mask.dtype != torch.bool or mask.shape != rows):
         raise ValueError(f"mask must be bool {tuple(rows)}, got {mask.dtype} {tuple(mask.shape)}")
     K = top_logits.shape[-1]
-    top, ids = _unit_inner(top_logits.detach().reshape(-1, K)), _unit_inner(top_ids.reshape(-1, K))
-    return top, ids, None if mask is None else mask.reshape(-1)
+    top, ids = top_logits.detach(), top_ids
+    if top.dim() != 2:
+        top, ids = top.reshape(-1, K), ids.reshape(-1, K)
+    top, ids = _unit_inner(top), _unit_inner(ids)
+    return top, ids, mask if mask is None or mask.dim() == 1 else mask.reshape(-1)
 
 
 def distillation_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_ids: torch.Tensor,
@@ -293,7 +293,7 @@ def distillation_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_ids: t
     An id >= V makes the loss NaN (an ``IndexError`` on CPU).  The gradient
     goes to logits alone; one backward pass per forward."""
     top, ids, m = _check_teacher(logits.shape[:-1], top_logits, top_ids, mask, temperature)
-    x = logits.reshape(-1, logits.shape[-1])
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     tau = float(temperature)
     if not x.is_cuda:
         return _distillation_plain(x, top, ids, m, tau)

@@ -740,3 +740,21 @@ def test_objectives_replay_in_a_cuda_graph():
         want = step()
         _synced()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_only_the_first_argument_gets_a_gradient():
+    """Old and reference log-probabilities, advantages and teachers that carry a graph of their own get none."""
+    from parallel_b200.ops import objectives as O
+
+    B, S = 4, 40
+    leaf = torch.randn(B, S, device="cuda", requires_grad=True)
+    other = torch.randn(B, S, device="cuda", requires_grad=True)
+    for fn in (lambda lp: O.policy_loss(lp, other, other, ref_logp=other, kl_coef=0.1).loss,
+               lambda lp: O.policy_loss(lp, other, other[:, :1], ref_logp=other, reduction="sequence").loss,
+               lambda lp: O.preference_loss(lp, ref_logp=other).loss,
+               lambda lp: O.distillation_loss(lp, other[:, :3], torch.arange(3, device="cuda").expand(B, 3))):
+        leaf.grad = other.grad = None
+        fn(leaf).backward()
+        assert leaf.grad is not None and other.grad is None
+        assert not fn(leaf.detach()).requires_grad
+    _synced()

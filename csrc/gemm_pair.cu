@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(GATHER ? kThreads + 64 : kThreads, 1)
       } else if (!SWIGLU && ep.tma == 3) {
         gemm_detail::epilogue_row_direct<BN>(ep, t_row, m, M, N, tn * BN_OUT, [&] {
           tc_fence_before();
-          mbar_arrive_cluster(tempty);
+          mbar_arrive_cluster_relaxed(tempty);
         });
       } else if (ep.tma) {
         gemm_detail::epilogue_warp_tma<BN, SWIGLU>(ep, &tmC, &tmR, t_row, stage, lane, m - lane, M, N, tn * BN_OUT,

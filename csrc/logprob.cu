@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t tempty = mapa_shared(smem_u32(&tempty_bar[acc]), 0);
       auto release = [&] {
         tc_fence_before();
-        mbar_arrive_cluster(tempty);
+        mbar_arrive_cluster_relaxed(tempty);
       };
       if (y0 >= T) {  // no row of this warp is in range
         release();

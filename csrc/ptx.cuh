@@ -353,6 +353,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// The same without release ordering, for a thread that hands back accumulator
+// columns it has finished reading (tcgen05.wait::ld) while its global stores are
+// still on their way: a release would wait for those stores.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // 2-D tiled TMA load into this CTA's shared memory whose completion is
 // signalled on an mbarrier of either CTA of the pair (cluster address).
 // No multicast.

@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) distill_prep_kernel(const Dis
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) {
     p.live[t] = any ? 1 : 0;
+    if (p.key) p.key[t] = any ? 0 : -1;
     if (any) atomicAdd(p.counters, 1);
   }
   if (!any) return;
@@ -215,7 +216,14 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const Dist
   const int C = p.cluster;
   const int rank = C == 1 ? 0 : (int)cluster_ctarank();
   const int64_t t = blockIdx.x / C;  // row of this block of logits
-  const int64_t tg = p.row0 + t;     // row of the teacher's entries and of the loss
+  // Packed rows: those behind the last 64-deep step of a sum over the rows that
+  // count are neither read nor written.
+  if (p.perm && p.row0 + t >= (max(p.counters[0], (int)p.row0 + 1) + 63) / 64 * 64) {
+    if (threadIdx.x == 0) p.row_loss[(int64_t)p.perm[p.row0 + t] * C + rank] = 0.f;
+    return;
+  }
+  // row of the teacher's entries and of the loss
+  const int64_t tg = p.perm ? p.perm[p.row0 + t] : p.row0 + t;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const E* row = reinterpret_cast<const E*>(p.logits) + t * p.ld;
   E* out = p.grad ? reinterpret_cast<E*>(p.grad) + t * p.ld_grad : nullptr;
@@ -431,10 +439,11 @@ void distill_prep(const DistillParams& p, cudaStream_t stream) {
 void distill_rows(const DistillParams& p0, bool bf16, cudaStream_t stream) {
   PB_CHECK(p0.K <= kDistillMaxK && (int64_t)p0.T * kMaxCluster < ((int64_t)1 << 31), "distill: too many rows or entries");
   DistillParams p = p0;
-  // a CTA per row, or a cluster while that leaves SMs idle and each CTA still has 2 vectors a thread
+  // a CTA per row, or a cluster while that leaves SMs idle and each CTA still has 2 vectors a thread; by all
+  // rows, so that the blocks of one call write their shares of row_loss alike
   const int nvec = p.V / (bf16 ? 8 : 4);
   p.cluster = 1;
-  while (p.cluster < kMaxCluster && 2 * p.cluster * (int64_t)p.T <= 2 * num_sms() &&
+  while (p.cluster < kMaxCluster && 2 * p.cluster * (int64_t)p.T_all <= 2 * num_sms() &&
          nvec / p.cluster >= 4 * kRowThreads)
     p.cluster *= 2;
   if (bf16)

@@ -331,7 +331,7 @@ at::Tensor preference_bwd(const at::Tensor& coef, const at::Tensor& g, const c10
 
 // ---------------------------------------------------------------- distillation
 // Scratch of a distillation, one allocation of 4-byte words: q and id [T, Kp]
-// (Kp: K rounded up to 4), the row losses, the count, the rows' live bytes.
+// (Kp: K rounded up to 4), the row losses, the count of rows, their live bytes.
 struct DistillScratch {
   int64_t T, Kp;
   explicit DistillScratch(int64_t t, int64_t k) : T(t), Kp((k + 3) / 4 * 4) {}
@@ -350,7 +350,8 @@ struct DistillScratch {
 
 // distill_prep(top [T, K], ids [T, K], mask [T] or None, V, inv_tau) -> [scratch, loss]
 std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& ids,
-                                     const c10::optional<at::Tensor>& mask, int64_t V, double inv_tau) {
+                                     const c10::optional<at::Tensor>& mask, int64_t V, double inv_tau,
+                                     int64_t* key = nullptr) {
   TORCH_CHECK(top.is_cuda() && (top.scalar_type() == at::kBFloat16 || top.scalar_type() == at::kFloat) &&
                   top.dim() == 2 && (top.stride(1) == 1 || top.size(1) <= 1),
               "distill: teacher logits must be CUDA bf16 or fp32 [T, K] with unit inner stride");
@@ -384,14 +385,16 @@ std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& id
   p.V = (int)V;
   p.K = (int)K;
   p.inv_tau = (float)inv_tau;
+  p.key = key;
   pb::distill_prep(p, cur_stream());
   return {scratch, loss};
 }
 
 // distill_rows(logits [T, V], prep ([scratch, loss] of all T_all rows), T_all, K, row0, tau, grad [T, V] or None):
-// the losses of rows [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss
+// the losses of rows [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss; with perm,
+// row i of the logits is row perm[i] of the teacher's
 void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep, int64_t T_all, int64_t K, int64_t row0,
-                  double tau, const c10::optional<at::Tensor>& grad) {
+                  double tau, const c10::optional<at::Tensor>& grad, const int* perm = nullptr) {
   TORCH_CHECK(logits.is_cuda() && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat) &&
                   logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) <= 1),
               "distill: logits must be CUDA bf16 or fp32 [T, V] with unit inner stride");
@@ -426,6 +429,7 @@ void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep,
   p.V = (int)V;
   p.K = (int)K;
   p.row0 = row0;
+  p.perm = perm;
   p.tau = (float)tau;
   p.inv_tau = (float)(1.0 / tau);
   pb::distill_rows(p, bf16, cur_stream());
@@ -721,6 +725,86 @@ at::Tensor distillation_loss(const at::Tensor& logits, const at::Tensor& top, co
   return DistillationNode::apply(logits, top, ids, mask, tau);
 }
 
+// Distillation through the LM head: blocks of bf16 logits of the packed rows
+// (those that count in front, zeros behind, as in LogProbsNode), overwritten by
+// their gradient, which the two products turn into those of h and w at once.
+struct HeadDistillationNode : public torch::autograd::Function<HeadDistillationNode> {
+  static at::Tensor run(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& top,
+                        const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau, int64_t max_block_bytes,
+                        bool need_h, bool need_w) {
+    const c10::cuda::CUDAGuard guard(h.device());
+    const int64_t T = h.size(0), V = w.size(0), H = w.size(1), K = top.size(1);
+    TORCH_CHECK(H == h.size(1) && top.size(0) == T, "lm_head_distillation: shapes");
+    CHECK_SAME_DEVICE(h, w);
+    CHECK_SAME_DEVICE(h, top);
+    at::Tensor key = at::empty({T}, h.options().dtype(at::kLong));
+    const auto prep = distill_prep(top, ids, mask, V, 1.0 / tau, key.data_ptr<int64_t>());
+    const auto packed = logprob_pack(h, key);  // rows, keys, perm, count
+    const at::Tensor &hp = packed[0], &perm = packed[2], &count = packed[3];
+    const int64_t block = block_rows(T, V, max_block_bytes);
+    const at::Tensor buf = at::empty({block, (V + 63) / 64 * 64}, h.options()).narrow(1, 0, V);
+    at::Tensor dh, dw;
+    if (need_h) dh = at::empty({T, H}, h.options());
+    if (need_w) dw = at::empty({V, H}, block >= T ? w.options() : w.options().dtype(at::kFloat));
+    for (int64_t r0 = 0; r0 < T; r0 += block) {
+      const int64_t n = std::min(block, T - r0);
+      const at::Tensor logits = rows_of(buf, 0, n), rows = rows_of(hp, r0, n), pm = rows_of(perm, r0, n);
+      pb::GemmParams p{};
+      p.A = rows.data_ptr();
+      p.B = w.data_ptr();
+      p.C = logits.data_ptr();
+      p.lda = rows.stride(0);
+      p.ldb = w.stride(0);
+      p.ldc = buf.stride(0);
+      p.M = (int)n;
+      p.N = (int)V;
+      p.K = (int)H;
+      p.alpha = 1.f;
+      p.epi = pb::kEpiStoreBf16;
+      p.live = count.data_ptr<int>();
+      p.live_row0 = (int)r0;
+      pb::gemm_bf16(p, cur_stream());
+      distill_rows(logits, prep, T, K, r0, tau, need_h || need_w ? c10::optional<at::Tensor>(logits) : c10::nullopt,
+                   perm.data_ptr<int>());
+      if (need_h) logprob_unpack(grad_rows(logits, w, count, r0), pm, count, r0, dh);
+      if (need_w) grad_head(logits, rows, dw, r0 > 0, count, r0);
+    }
+    if (ctx) {
+      // not save_for_backward: the backward hands the gradients out
+      ctx->saved_data["grads"] =
+          std::vector<at::Tensor>{need_h ? dh : at::empty({0}, h.options()),
+                                  need_w ? dw.to(w.scalar_type()) : at::empty({0}, h.options())};
+      ctx->saved_data["need_h"] = need_h;
+      ctx->saved_data["need_w"] = need_w;
+    }
+    return prep[1];
+  }
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& top,
+                            const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau,
+                            int64_t max_block_bytes) {
+    return run(ctx, h, w, top, ids, mask, tau, max_block_bytes, h.requires_grad(), w.requires_grad());
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_first_order("lm_head_distillation");
+    TORCH_CHECK(ctx->saved_data.count("grads"), "lm_head_distillation supports one backward pass per forward");
+    std::vector<at::Tensor> grads = ctx->saved_data["grads"].toTensorVector();
+    ctx->saved_data.erase("grads");
+    variable_list out(7);
+    if (ctx->saved_data["need_h"].toBool()) out[0] = grads[0];
+    if (ctx->saved_data["need_w"].toBool()) out[1] = grads[1];
+    for (at::Tensor& t : grads) objective_scale(t, g[0]);
+    return out;
+  }
+};
+
+at::Tensor lm_head_distillation(const at::Tensor& h, const at::Tensor& w, const at::Tensor& top, const at::Tensor& ids,
+                                const c10::optional<at::Tensor>& mask, double tau, int64_t max_block_bytes) {
+  check_rows_bf16(h, "lm_head_distillation: h");
+  check_rows_bf16(w, "lm_head_distillation: w");
+  if (wants_grad(h) || wants_grad(w)) return HeadDistillationNode::apply(h, w, top, ids, mask, tau, max_block_bytes);
+  return HeadDistillationNode::run(nullptr, h, w, top, ids, mask, tau, max_block_bytes, false, false);
+}
+
 }  // namespace
 
 void register_objectives(pybind11::module& m) {
@@ -733,9 +817,6 @@ void register_objectives(pybind11::module& m) {
         py::arg("smoothing"), py::arg("average"));
   m.def("distillation_loss", &distillation_loss, py::arg("logits"), py::arg("top"), py::arg("ids"), py::arg("mask"),
         py::arg("tau"));
-  m.def("distill_prep", &distill_prep, py::arg("top"), py::arg("ids"), py::arg("mask"), py::arg("V"),
-        py::arg("inv_tau"));
-  m.def("distill_rows", &distill_rows, py::arg("logits"), py::arg("prep"), py::arg("T_all"), py::arg("K"), py::arg("row0"), py::arg("tau"),
-        py::arg("grad"));
-  m.def("objective_scale", &objective_scale, py::arg("x"), py::arg("g"));
+  m.def("lm_head_distillation", &lm_head_distillation, py::arg("h"), py::arg("w"), py::arg("top"), py::arg("ids"),
+        py::arg("mask"), py::arg("tau"), py::arg("max_block_bytes"));
 }

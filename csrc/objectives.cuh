@@ -105,6 +105,8 @@ struct DistillParams {
   bool top_bf16, ids32;
   int T, T_all, V, K, Kp, cluster;  // Kp: K rounded up to a multiple of 4
   int64_t row0;
+  const int* perm;  // optional: row i of the logits is row perm[i] of the teacher's, those that count first
+  int64_t* key;     // optional [T_all]: 0 for a row that counts, else -1 (what logprob_pack packs by)
   float tau, inv_tau;
   float* q;        // [T_all, Kp]
   int* id;         // [T_all, Kp]

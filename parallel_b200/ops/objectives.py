@@ -19,16 +19,8 @@ from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
-from . import gemm as G
 from ._ext import ext
-
-
-def _one_backward(ctx, what: str) -> None:
-    if getattr(ctx, "consumed", False):
-        raise RuntimeError(f"{what} supports one backward pass per forward")
-    ctx.consumed = True
 
 
 def _rows_bf16(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -42,17 +34,6 @@ def _rows_bf16(t: torch.Tensor, what: str) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------- log-probabilities through the LM head
-def _block_rows(T: int, V: int, max_block_bytes: int) -> int:
-    """Rows of a [rows, V] bf16 block of at most ``max_block_bytes`` (whole
-    256-row tiles, one at least)."""
-    return max(1, min(T, max(256, int(max_block_bytes // (V * 2)) // 256 * 256)))
-
-
-def _exp_buffer(rows: int, V: int, device) -> torch.Tensor:
-    """bf16 [rows, V] with 128-byte aligned rows."""
-    return torch.empty(rows, (V + 63) // 64 * 64, device=device, dtype=torch.bfloat16)[:, :V]
-
-
 def lm_head_log_probs(h: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, temperature: float = 1.0,
                       max_block_bytes: int = 6 << 30) -> torch.Tensor:
     """fp32 ``log_softmax(h @ w.T / temperature)[..., ids]``, shaped as ``ids``.
@@ -214,46 +195,6 @@ def _preference_plain(logp, ref, mask, beta, smoothing, average):
 
 
 # ----------------------------------------------------------------- distillation from a teacher's top logits
-class _LMHeadDistillationFn(torch.autograd.Function):
-    """Blocks of logits, overwritten by their gradient, as in ``lm_head_cross_entropy``."""
-
-    @staticmethod
-    def forward(ctx, h, w, top, ids, mask, tau, max_block_bytes):
-        (T, H), V = h.shape, w.shape[0]
-        need_h, need_w = ctx.needs_input_grad[:2]
-        prep = ext().distill_prep(top, ids, mask, V, 1.0 / tau)
-        block = _block_rows(T, V, max_block_bytes)
-        buf = _exp_buffer(block, V, h.device)
-        dh = torch.empty(T, H, device=h.device, dtype=h.dtype) if need_h else None
-        dw = torch.empty(V, H, device=h.device, dtype=w.dtype if block >= T else torch.float32) if need_w else None
-        for r0 in range(0, T, block):
-            rows = slice(r0, min(T, r0 + block))
-            logits = buf[:rows.stop - r0]
-            ext().gemm(h[rows], w, logits, False, False, G.EPI_STORE_BF16, 1.0)
-            ext().distill_rows(logits, prep, T, top.shape[1], r0, tau, logits if need_h or need_w else None)
-            if need_h:
-                ext().gemm(logits, w, dh[rows], False, True, G.EPI_STORE_BF16, 1.0)
-            if need_w:
-                epi = G.EPI_STORE_BF16 if block >= T else G.EPI_ACCUM_F32 if r0 else G.EPI_STORE_F32
-                ext().gemm(logits, h[rows], dw, True, True, epi, 1.0)
-        if need_w and block < T:
-            out = torch.empty(V, H, device=h.device, dtype=w.dtype)
-            ext().cast_f32_to_bf16(dw, out)
-            dw = out
-        ctx.grads = (dh, dw)
-        return prep[-1]
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        _one_backward(ctx, "lm_head_distillation")
-        (dh, dw), ctx.grads = ctx.grads, None
-        for t in (dh, dw):
-            if t is not None:
-                ext().objective_scale(t, g)
-        return dh, dw, None, None, None, None, None
-
-
 def _check_teacher(rows, top_logits, top_ids, mask, temperature):
     """Teacher entries as [T, K] and the mask as [T] for `rows` (the leading shape of the student's rows)."""
     if not temperature > 0.0:
@@ -314,9 +255,7 @@ def lm_head_distillation(h: torch.Tensor, w: torch.Tensor, top_logits: torch.Ten
     if h2.shape[0] == 0:
         return h2.float().sum() + w[:0].float().sum()
     h2, w = _rows_bf16(h2, "h"), _rows_bf16(w, "w")
-    if not torch.is_grad_enabled():
-        h2, w = h2.detach(), w.detach()
-    return _LMHeadDistillationFn.apply(h2, w, top, ids, m, tau, max_block_bytes)
+    return ext().lm_head_distillation(h2, w, top, ids, m, tau, int(max_block_bytes))
 
 
 def _distillation_plain(x, top, ids, mask, tau):

@@ -216,6 +216,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc_pair(tmem_slot, 2 * BN_MAX);
     tmem_relinquish_pair();
   }
+  if (a_rows < BM_CTA) {
+    // few rows: the rest of A is multiplied too, and zeros cost the least power
+    // (one row, thousands of calls in a row: 72 us, with this 66.5)
+    for (int i = threadIdx.x; i < STAGES * A_BYTES / 16; i += kThreads)
+      reinterpret_cast<uint4*>(sA)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // barriers of both CTAs initialised before any cross-CTA use
@@ -233,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       // few rows: a box of the rows that are there (a box mostly out of bounds is
       // slow to fill: one row 91 us, 64 rows 61 us), and none for the odd CTA.  The
-      // rest of the stage holds anything: rows of A are independent.
+      // rest of the stage stays zero.
       const uint32_t a_bytes = a_rows < BM_CTA ? (uint32_t)a_rows * BK * 2 : 2 * A_BYTES;
       const bool load_a = a_rows == BM_CTA || leader;
       int stage = 0;

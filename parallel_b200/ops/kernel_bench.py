@@ -1,6 +1,6 @@
 """Micro-benchmarks of the sm_100a kernels at the Qwen3-0.6B training shapes.
 
-    python -m parallel_b200.ops.kernel_bench attn_fwd|attn_bwd|ce|gemm|gemm_vs_cublas|gemm_swiglu|gemm_residual|moe_layer|rmsnorm_bwd|qknorm|qknorm_bwd|wgrad_split|all [--iters N]
+    python -m parallel_b200.ops.kernel_bench attn_fwd|attn_bwd|ce|gemm|gemm_vs_cublas|gemm_swiglu|gemm_residual|moe_layer|rmsnorm_bwd|qknorm|qknorm_bwd|wgrad_split|log_probs_score|log_probs_train|distill|policy|preference|all [--iters N]
 
 Each case runs a few warm-up launches, then times ``--iters`` launches with
 CUDA events on the current stream and prints the time per launch and the
@@ -303,10 +303,81 @@ def case_moe_layer(warmup, iters):
             f"torch._grouped_mm path {t_torch:.1f} us, speedup {t_torch / t_ours:.2f}x")
 
 
+VOCAB = 151936
+
+
+def _head(T):
+    """Hidden states, LM head (logits of standard deviation 2.5) and ids with a fifth of the rows without a token."""
+    w = (torch.randn(VOCAB, H, device="cuda") * 2.5 / math.sqrt(H)).to(torch.bfloat16)
+    ids = torch.randint(0, VOCAB, (T,), device="cuda")
+    h = (torch.randn(T, H, device="cuda") + 10 * torch.rand(T, 1, device="cuda") * w[ids].float() / 2.5)
+    return h.to(torch.bfloat16), w, ids.masked_fill(torch.rand(T, device="cuda") < 0.2, -100)
+
+
+def case_log_probs_score(warmup, iters):
+    from .objectives import lm_head_log_probs
+
+    T = B * S
+    h, w, ids = _head(T)
+    us = _time(lambda: lm_head_log_probs(h, w, ids), warmup, iters)
+    live = int((ids >= 0).sum())
+    return f"log-probs, scored: {T} rows ({live} with a token) x {VOCAB}, H {H}: {us:.1f} us, {2 * live * VOCAB * H / us / 1e6:.0f} TF/s"
+
+
+def case_log_probs_train(warmup, iters):
+    from .objectives import lm_head_log_probs
+
+    T = B * S
+    h, w, ids = _head(T)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    g = torch.randn(T, device="cuda") / T
+    us = _time(lambda: torch.autograd.grad(lm_head_log_probs(h, w, ids), (h, w), g), warmup, iters)
+    live = int((ids >= 0).sum())
+    return f"log-probs, forward + backward: {T} rows ({live} with a token) x {VOCAB}, H {H}: {us:.1f} us, {6 * live * VOCAB * H / us / 1e6:.0f} TF/s"
+
+
+def case_distill(warmup, iters):
+    from .objectives import distillation_loss
+
+    T, K = B * S, 64
+    logits = (torch.randn(T, VOCAB, device="cuda") * 2.5).to(torch.bfloat16).requires_grad_(True)
+    top, ids = 10 * torch.rand(T, K, device="cuda"), torch.randint(0, VOCAB, (T, K), device="cuda")
+    us = _time(lambda: torch.autograd.grad(distillation_loss(logits, top, ids, temperature=2.0), logits), warmup, iters)
+    return f"distillation, forward + backward: {T} x {VOCAB} bf16, {K} entries: {us:.1f} us, {4 * T * VOCAB / us / 1e3:.0f} GB/s"
+
+
+def _token_rows(rows, cols):
+    lp = -torch.rand(rows, cols, device="cuda")
+    return lp, lp + 0.1 * torch.randn(rows, cols, device="cuda"), torch.rand(rows, cols, device="cuda") < 0.8
+
+
+def case_policy(warmup, iters):
+    from .objectives import policy_loss
+
+    lp, old, mask = _token_rows(512, 4096)
+    adv = torch.randn(512, 4096, device="cuda")
+    lp.requires_grad_(True)
+    us = _time(lambda: torch.autograd.grad(policy_loss(lp, old, adv, mask=mask, ref_logp=old, kl_coef=0.05).loss, lp),
+               warmup, iters)
+    return f"policy loss, forward + backward: 512 x 4096: {us:.1f} us, {21 * lp.numel() / us / 1e3:.0f} GB/s"
+
+
+def case_preference(warmup, iters):
+    from .objectives import preference_loss
+
+    lp, ref, mask = _token_rows(512, 4096)
+    lp.requires_grad_(True)
+    us = _time(lambda: torch.autograd.grad(preference_loss(lp, ref_logp=ref, mask=mask).loss, lp), warmup, iters)
+    return f"preference loss, forward + backward: 256 pairs x 4096: {us:.1f} us, {13 * lp.numel() / us / 1e3:.0f} GB/s"
+
+
 CASES = {"attn_fwd": case_attn_fwd, "moe_layer": case_moe_layer, "ce": case_ce, "gemm_vs_cublas": case_gemm_vs_cublas,
          "wgrad_oproj": case_wgrad_oproj, "wgrad_oproj_cublas": case_wgrad_oproj_cublas, "attn_bwd": case_attn_bwd, "gemm": case_gemm, "gemm_swiglu": case_gemm_swiglu,
          "gemm_residual": case_gemm_residual, "rmsnorm_bwd": case_rmsnorm_bwd, "qknorm": case_qknorm,
-         "qknorm_bwd": case_qknorm_bwd, "wgrad_split": case_wgrad_split}
+         "qknorm_bwd": case_qknorm_bwd, "wgrad_split": case_wgrad_split, "log_probs_score": case_log_probs_score,
+         "log_probs_train": case_log_probs_train, "distill": case_distill, "policy": case_policy,
+         "preference": case_preference}
 
 
 def main(argv=None):

@@ -1,8 +1,10 @@
 // Losses over token log-probabilities [B, S] (fp32): the clipped policy loss
 // with a KL term and the preference loss over pairs of sequences.
 //
-// Both are bound by launch latency up to some 100k tokens and by memory above
-// (17 / 9 bytes read per token).  One launch forward, one backward: a warp
+// Both are bound by latency up to some 100k tokens (one launch each way: 6 + 3
+// us on the GPU for 8 x 509 tokens, inside some 75 us of a call's host time) and
+// by memory far above (17 / 9 bytes read per token; 2M tokens: 21.5 + 3.6 us
+// for the policy loss, 16 + 3.4 for the preference loss).  One launch forward, one backward: a warp
 // sums a chunk of one row, writes the chunk's partial sums, and the last
 // block to finish adds the partials in chunk order (fp64), so the results
 // have the same bits on every run.  Positions outside the mask are never
@@ -19,6 +21,7 @@ namespace pb {
 namespace {
 
 constexpr int kWarps = 8;          // per block when there are many units
+constexpr int kAhead = 4;          // tokens a lane loads before it uses the first
 constexpr int kOneBlockUnits = 32;  // up to this many units one block does it all, without a ticket
 
 __device__ __forceinline__ float warp_add(float v) {
@@ -27,17 +30,26 @@ __device__ __forceinline__ float warp_add(float v) {
   return v;
 }
 
-// Sum of one double per thread over the block; the same order on every run.
-// Every thread gets the sum; `sh` holds 32 doubles.
-__device__ __forceinline__ double block_add(double v, double* sh) {
+// Sums of K doubles per thread over the block, valid in thread 0; the same
+// order on every run.  sh: [32][K].
+template <int K>
+__device__ __forceinline__ void block_add(double (&v)[K], double (*sh)[K]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)(blockDim.x >> 5);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < K; ++k) sh[warp][k] = v[k];
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0;
-  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) v += sh[i];
-  return v;
+  if (warp != 0) return;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = lane < warps ? sh[lane][k] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
 }
 
 // True in every thread of the last block to arrive (ticket zeroed before the
@@ -71,29 +83,44 @@ __global__ void __launch_bounds__(1024) policy_fwd_kernel(const PolicyParams p) 
     const float* adv = p.adv + b * p.adv_sb;
     const uint8_t* mask = p.mask ? p.mask + b * p.ld_mask : nullptr;
     float loss = 0.f, n = 0.f, clip = 0.f, kl = 0.f;
-#pragma unroll 4
-    for (int64_t s = s0 + lane; s < s1; s += 32) {
-      float coef = 0.f;
-      if (!mask || mask[s]) {
-        const float l = lp[s], a = adv[s * p.adv_ss];
-        const float r = expf(l - old[s]);
-        const float u = r * a;
-        const float c = fminf(fmaxf(r, p.low), p.high) * a;
-        const bool clipped = u > c;  // false for NaN: u carries it on
-        float per = clipped ? -c : -u;
-        coef = clipped ? 0.f : -u;
-        if (ref) {
-          const float x = ref[s] - l;
-          const float e = expm1f(x);  // exp(x) - 1 - x without the cancellation at small x
-          kl += e - x;
-          per += p.kl_coef * (e - x);
-          coef -= p.kl_coef * e;
+    // kAhead tokens a lane at a time: all their loads first, whatever the mask says
+    // (what is outside it is dropped), then the arithmetic
+    for (int64_t sb = s0 + lane; sb < s1; sb += 32 * kAhead) {
+      float l[kAhead], a[kAhead], o[kAhead], rl[kAhead];
+      bool on[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t s = sb + 32 * j;
+        on[j] = s < s1;
+        l[j] = a[j] = o[j] = rl[j] = 0.f;
+        if (s < s1) {
+          if (mask) on[j] = __ldg(mask + s) != 0;
+          l[j] = __ldg(lp + s);
+          a[j] = __ldg(adv + s * p.adv_ss);
+          o[j] = __ldg(old + s);
+          if (ref) rl[j] = __ldg(ref + s);
         }
-        loss += per;
-        n += 1.f;
-        clip += clipped ? 1.f : 0.f;
       }
-      if (p.coef) p.coef[b * p.S + s] = coef;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float r = expf(l[j] - o[j]);
+        const float u = r * a[j];
+        const float c = fminf(fmaxf(r, p.low), p.high) * a[j];
+        const bool clipped = u > c;  // false for NaN: u carries it on
+        float per = clipped ? -c : -u, coef = clipped ? 0.f : -u;
+        if (ref) {
+          const float x = rl[j] - l[j];
+          const float e = expm1f(x), k = e - x;  // exp(x) - 1 - x without the cancellation at small x
+          per += p.kl_coef * k;
+          coef -= p.kl_coef * e;
+          kl += on[j] ? k : 0.f;
+        }
+        loss += on[j] ? per : 0.f;
+        n += on[j] ? 1.f : 0.f;
+        clip += on[j] && clipped ? 1.f : 0.f;
+        const int64_t s = sb + 32 * j;
+        if (p.coef && s < s1) p.coef[b * p.S + s] = on[j] ? coef : 0.f;
+      }
     }
     loss = warp_add(loss);
     n = warp_add(n);
@@ -102,48 +129,43 @@ __global__ void __launch_bounds__(1024) policy_fwd_kernel(const PolicyParams p) 
     if (lane == 0) p.parts[unit] = make_float4(loss, n, clip, kl);
   }
   if (!last_block(p.ticket)) return;
-  __shared__ double sh[32];
-  double loss = 0.0, n = 0.0, clip = 0.0, kl = 0.0;
+  __shared__ double sh[32][5];
+  double v[5] = {0.0, 0.0, 0.0, 0.0, 0.0};  // loss, tokens, clipped, kl, rows with a token
   if (!p.per_sequence) {
     for (int64_t i = threadIdx.x; i < units; i += blockDim.x) {
-      const float4 v = __ldcg(p.parts + i);
-      loss += v.x;
-      n += v.y;
-      clip += v.z;
-      kl += v.w;
+      const float4 q = __ldcg(p.parts + i);
+      v[0] += q.x;
+      v[1] += q.y;
+      v[2] += q.z;
+      v[3] += q.w;
     }
   } else {
-    double live = 0.0;
     for (int64_t b = threadIdx.x; b < p.B; b += blockDim.x) {
       double row = 0.0, rn = 0.0;
+#pragma unroll 8
       for (int c = 0; c < p.nchunk; ++c) {
-        const float4 v = __ldcg(p.parts + b * p.nchunk + c);
-        row += v.x;
-        rn += v.y;
-        clip += v.z;
-        kl += v.w;
+        const float4 q = __ldcg(p.parts + b * p.nchunk + c);
+        row += q.x;
+        rn += q.y;
+        v[2] += q.z;
+        v[3] += q.w;
       }
       if (rn > 0.0) {
-        loss += row / rn;
-        live += 1.0;
+        v[0] += row / rn;
+        v[4] += 1.0;
       }
-      n += rn;
+      v[1] += rn;
       p.inv_row[b] = rn > 0.0 ? (float)(1.0 / rn) : 0.f;
     }
-    live = block_add(live, sh);
-    if (threadIdx.x == 0) p.inv[0] = (float)(1.0 / fmax(live, 1.0));
-    loss /= fmax(live, 1.0);
   }
-  loss = block_add(loss, sh);
-  n = block_add(n, sh);
-  clip = block_add(clip, sh);
-  kl = block_add(kl, sh);
+  block_add(v, sh);
   if (threadIdx.x == 0) {
-    const double inv = 1.0 / fmax(n, 1.0);
-    if (!p.per_sequence) p.inv[0] = (float)inv;
-    p.loss[0] = (float)(p.per_sequence ? loss : loss * inv);
-    p.clip[0] = (float)(clip * inv);
-    p.kl[0] = (float)(kl * inv);
+    const double per_token = 1.0 / fmax(v[1], 1.0);
+    const double inv = p.per_sequence ? 1.0 / fmax(v[4], 1.0) : per_token;
+    p.inv[0] = (float)inv;
+    p.loss[0] = (float)(v[0] * inv);
+    p.clip[0] = (float)(v[2] * per_token);
+    p.kl[0] = (float)(v[3] * per_token);
   }
 }
 
@@ -179,11 +201,24 @@ __global__ void __launch_bounds__(1024) preference_fwd_kernel(const PreferencePa
     const float* ref = p.ref ? p.ref + b * p.ld_ref : nullptr;
     const uint8_t* mask = p.mask ? p.mask + b * p.ld_mask : nullptr;
     float d = 0.f, n = 0.f;
-#pragma unroll 4
-    for (int64_t s = s0 + lane; s < s1; s += 32) {
-      if (!mask || mask[s]) {
-        d += lp[s] - (ref ? ref[s] : 0.f);
-        n += 1.f;
+    for (int64_t sb = s0 + lane; sb < s1; sb += 32 * kAhead) {
+      float l[kAhead], r[kAhead];
+      bool on[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t s = sb + 32 * j;
+        on[j] = s < s1;
+        l[j] = r[j] = 0.f;
+        if (s < s1) {
+          if (mask) on[j] = __ldg(mask + s) != 0;
+          l[j] = __ldg(lp + s);
+          if (ref) r[j] = __ldg(ref + s);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        d += on[j] ? l[j] - r[j] : 0.f;
+        n += on[j] ? 1.f : 0.f;
       }
     }
     d = warp_add(d);
@@ -191,14 +226,15 @@ __global__ void __launch_bounds__(1024) preference_fwd_kernel(const PreferencePa
     if (lane == 0) p.parts[unit] = make_float2(d, n);
   }
   if (!last_block(p.ticket)) return;
-  __shared__ double sh[32];
-  double loss = 0.0;
+  __shared__ double sh[32][1];
+  double loss[1] = {0.0};
   for (int i = threadIdx.x; i < p.P; i += blockDim.x) {
     double r[2], w[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {  // the chosen row, the rejected row
       const int64_t b = i + (int64_t)k * p.P;
       double d = 0.0, n = 0.0;
+#pragma unroll 8
       for (int c = 0; c < p.nchunk; ++c) {
         const float2 v = __ldcg(p.parts + b * p.nchunk + c);
         d += v.x;
@@ -212,7 +248,7 @@ __global__ void __launch_bounds__(1024) preference_fwd_kernel(const PreferencePa
     const float soft = log1pf(expf(-fabsf(gap)));  // -log sigmoid(x) = soft + max(-x, 0)
     const float neg = gap < 0.f ? -gap : 0.f, pos = gap > 0.f ? gap : 0.f;
     const float e = p.smoothing;
-    loss += (double)((1.f - e) * (soft + neg) + e * (soft + pos));
+    loss[0] += (double)((1.f - e) * (soft + neg) + e * (soft + pos));
     // sigmoid(-gap) and sigmoid(gap), each without cancellation
     const float t = expf(-fabsf(gap));
     const float small = t / (1.f + t), big = 1.f / (1.f + t);
@@ -221,8 +257,8 @@ __global__ void __launch_bounds__(1024) preference_fwd_kernel(const PreferencePa
     p.coef[i] = (float)(w[0] * (double)dgap);
     p.coef[i + p.P] = (float)(-w[1] * (double)dgap);
   }
-  loss = block_add(loss, sh);
-  if (threadIdx.x == 0) p.loss[0] = (float)(loss / (double)p.P);
+  block_add(loss, sh);
+  if (threadIdx.x == 0) p.loss[0] = (float)(loss[0] / (double)p.P);
 }
 
 // out = g * coef[row] inside the mask, 0 outside
@@ -245,11 +281,13 @@ int unit_blocks(int64_t units) { return (int)((units + kWarps - 1) / kWarps); }
 
 }  // namespace
 
-// Tokens of a row that one warp sums: long enough to amortise its reduction,
-// short enough that a small batch still covers the SMs (8 warps on each).
+// Tokens of a row that one warp sums: the longest that still gives each SM 16
+// warps, whose loads hide one another's latency, while the last block has few
+// partials to add (policy forward, 512 x 4096, inputs not in L2: 32.7 us with
+// 1024 tokens a warp, 21.5 with 512, 24.7 with 256).
 int objective_chunk(int64_t rows, int64_t S) {
   int chunk = 1024;
-  while (chunk > 128 && rows * ((S + chunk - 1) / chunk) < (int64_t)8 * num_sms()) chunk /= 2;
+  while (chunk > 128 && rows * ((S + chunk - 1) / chunk) < (int64_t)16 * num_sms()) chunk /= 2;
   return chunk;
 }
 

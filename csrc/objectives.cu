@@ -4,11 +4,11 @@
 // Both are bound by latency up to some 100k tokens (one launch each way: 6 + 3
 // us on the GPU for 8 x 509 tokens, inside some 75 us of a call's host time) and
 // by memory far above (17 / 9 bytes read per token; 2M tokens: 21.5 + 3.6 us
-// for the policy loss, 16 + 3.4 for the preference loss).  One launch forward, one backward: a warp
-// sums a chunk of one row, writes the chunk's partial sums, and the last
-// block to finish adds the partials in chunk order (fp64), so the results
-// have the same bits on every run.  Positions outside the mask are never
-// part of an operation: they may hold anything.
+// for the policy loss, 16 + 3.4 for the preference loss).  A warp sums a chunk
+// of one row and writes the chunk's partial sums, and the last block to finish
+// adds the partials in chunk order (fp64), so the results have the same bits on
+// every run.  What stands outside the mask is dropped by selection, never by a
+// product: it may be anything.
 #include <math.h>
 
 #include <algorithm>

@@ -64,7 +64,8 @@ __device__ __forceinline__ float ex2(float x) {
 // Column tiles: the first n_full are BN_MAX wide, the others bn2.  Whole waves of
 // wide tiles over the CTA pairs, and what is left over in tiles narrow enough
 // for one more wave: 151,936 columns are 8 waves of 256 on 74 pairs and 384
-// columns, which as two wide tiles cost a ninth wave (one row: 61 -> 54 us).
+// columns, which as two wide tiles cost a ninth wave (64 rows, H 1024: 62.2 ->
+// 60.1 us; 8 rows of V 10000: 12.6 -> 11.6; 333 rows, H 4096: 435 -> 439).
 __device__ __forceinline__ int tile_start(const LogprobTiles& g, int tn) {
   return tn < g.n_full ? tn * BN_MAX : g.n_full * BN_MAX + (tn - g.n_full) * g.bn2;
 }
@@ -179,7 +180,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     logprob_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmB2, __nv_bfloat16* __restrict__ e, int64_t lde,
                         const int64_t* __restrict__ ids, const int* __restrict__ count, int row0,
-                        float2* __restrict__ stats, int T_all, int V, int H, int a_rows, const LogprobTiles geo, float scale, int* err) {
+                        float2* __restrict__ stats, int T_all, int V, int H, int a_rows, const LogprobTiles geo,
+                        float scale, int* err) {
   pdl_prologue();
   const int T = count ? min(T_all, max(0, *count - row0)) : T_all;  // the rows in front that have a token
   extern __shared__ uint8_t smem_raw[];
@@ -245,6 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool load_a = a_rows == BM_CTA || leader;
       int stage = 0;
       uint32_t phase = 0;
+      uint32_t issued = 0, last = 0;  // bit s: copies were issued to stage s; the parity of its last phase
       bool ok = true;
       for (int64_t w = cid; w < num_tiles && ok; w += n_clusters) {
         const int tm = (int)(w % tiles_m), tn = (int)(w / tiles_m);
@@ -259,8 +262,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (leader) mbar_arrive_expect_tx(&full_bar[stage], stage_bytes);
           if (load_a) tma_load_2d_pair(sA + stage * A_BYTES, &tmA, full_even, kb * BK, a_row);
           tma_load_2d_pair(sB + stage * B_BYTES, map_b, full_even, kb * BK, b_row);
+          issued |= 1u << stage;
+          last = (last & ~(1u << stage)) | (phase << stage);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
+      }
+      // After an error nobody may have waited for the last copies of the pair (they
+      // complete on the even CTA): do so, bounded, before the shared memory goes.
+      if (leader && *((volatile int*)err) != 0) {
+        const uint64_t t0 = globaltimer();
+        for (int s = 0; s < STAGES; ++s)
+          while ((issued >> s & 1u) && !mbar_try_wait(smem_u32(&full_bar[s]), last >> s & 1u) &&
+                 globaltimer() - t0 < 100000000ull) {
+          }
       }
     }
   } else if (warp == 1) {
@@ -340,9 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kFinThreads = 128;
 
 // One block per row of h; its log-probability goes to row perm[t] (t without
-// perm).  dot in 64 bits (bf16 products are exact in fp32; eight
-// of them are added in fp32, the rest in double), then the tile statistics:
-// with d = m - x_id (base 2), logp = -log(1 + s 2^d), written so that neither
+// perm).  dot in 64 bits (bf16 products are exact in fp32; eight of them are
+// added in fp32, the rest in double), then the tile statistics: with d = m - x_id (base 2), logp = -log(1 + s 2^d), written so that neither
 // a large nor a small d loses digits.
 __global__ void __launch_bounds__(kFinThreads)
     logprob_finish_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const __nv_bfloat16* __restrict__ w,

@@ -653,6 +653,49 @@ def test_lm_head_distillation(T, V, blocks):
     assert torch.equal(dh[~mask], torch.zeros_like(dh[~mask]))
 
 
+# ----------------------------------------------------------------- offsets past 32 bits
+def test_more_than_2_to_the_31_logits():
+    """15,000 rows of a 151,936 vocabulary: 2.28e9 exponentials, logits and gradients, checked where offsets are
+    largest and in a head-gradient column that every row reaches."""
+    from parallel_b200.ops import objectives as O
+
+    T, H, V = 15000, 64, 151936
+    h, w, ids, g = _head_inputs(T, H, V, ignored=0.0, seed=41)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    logp = O.lm_head_log_probs(h, w, ids, max_block_bytes=8 << 30)
+    dh, dw = torch.autograd.grad(logp, (h, w), g)
+    _synced()
+    rows = torch.cat([torch.arange(4), torch.arange(T - 300, T)]).cuda()
+    ref, rdh, _, top = _head_reference(h.detach()[rows], w.detach(), ids[rows], g[rows], 1.0)
+    assert (logp[rows].double() - ref).abs().max().item() <= (H / 16 + 8) * 2.0 ** -23 * (top + 4)
+    assert _err(dh[rows], rdh) <= GRAD_TOL
+    # the head's gradient at the last token and at one that is some row's target
+    for v in (V - 1, int(ids[T - 1])):
+        p = (h.detach().double() @ w.detach()[v].double()
+             - (h.detach().double() * w.detach()[ids].double()).sum(1) + logp.double()).exp()
+        want = (g.double() * ((ids == v).double() - p))[:, None].mul(h.detach().double()).sum(0)
+        size = (g.double() * ((ids == v).double() + p))[:, None].mul(h.detach().double()).norm()
+        assert (dw[v].double() - want).norm().item() <= GRAD_TOL * (want.norm().item() + size.item())
+    del logp, dh, dw, h, w
+    torch.cuda.empty_cache()
+
+    gen = torch.Generator(device="cuda").manual_seed(42)
+    x = torch.randn(T, V, device="cuda", generator=gen, dtype=torch.bfloat16)
+    tid = torch.randint(0, V, (T, 4), device="cuda", generator=gen)
+    teacher = 4 * torch.rand(T, 4, device="cuda", generator=gen)
+    mask = torch.zeros(T, dtype=torch.bool, device="cuda")
+    mask[rows] = True
+    x.requires_grad_(True)
+    loss = O.distillation_loss(x, teacher, tid, mask=mask)
+    (grad,) = torch.autograd.grad(loss, x)
+    _synced()
+    ref, rgrad = _distill_reference(x.detach()[rows], teacher[rows], tid[rows], mask[rows], 1.0)
+    assert abs(loss.item() - ref.item()) <= 100 * F32 * (ref.item() + 40)
+    assert ((grad[rows].double() - rgrad).abs() <= 2.0 ** -8 * rgrad.abs() + 100 * F32 / rows.numel()).all()
+    assert not grad[4:T - 300].any()
+
+
 # ----------------------------------------------------------------- together, as they are used
 @pytest.mark.parametrize("name", ["small-qwen3", "small-qwen3-moe"])
 def test_model_objectives_match_its_logits(name):

@@ -53,9 +53,8 @@ constexpr int kPrepWarps = 8;
 __device__ __forceinline__ float teacher_value(const DistillParams& p, int64_t t, int k, int64_t id) {
   // an id past the vocabulary has no probability: NaN, and so is the loss
   if (id >= p.V) return NAN;
-  const float v = p.top_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.top)[t * p.ld_top + k])
-                             : reinterpret_cast<const float*>(p.top)[t * p.ld_top + k];
-  return v * p.inv_tau;
+  return p.top_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.top)[t * p.ld_top + k])
+                    : reinterpret_cast<const float*>(p.top)[t * p.ld_top + k];
 }
 
 __device__ __forceinline__ int64_t teacher_id(const DistillParams& p, int64_t t, int k) {
@@ -94,7 +93,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) distill_prep_kernel(const Dis
   float s = 0.f;
   for (int k = lane; k < p.K; k += 32) {
     const int64_t id = teacher_id(p, t, k);
-    if (id >= 0) s += expf(teacher_value(p, t, k, id) - m);
+    if (id >= 0) s += expf((teacher_value(p, t, k, id) - m) * p.inv_tau);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -102,7 +101,7 @@ __global__ void __launch_bounds__(32 * kPrepWarps) distill_prep_kernel(const Dis
   const float inv = 1.f / s;
   for (int k = lane; k < p.K; k += 32) {
     const int64_t id = teacher_id(p, t, k);
-    p.q[t * p.Kp + k] = id >= 0 ? expf(teacher_value(p, t, k, id) - m) * inv : 0.f;
+    p.q[t * p.Kp + k] = id >= 0 ? expf((teacher_value(p, t, k, id) - m) * p.inv_tau) * inv : 0.f;
     p.id[t * p.Kp + k] = id >= 0 && id < p.V ? (int)id : -1;
   }
   for (int k = p.K + lane; k < p.Kp; k += 32) {
@@ -131,40 +130,51 @@ __device__ __forceinline__ void st_cluster_f2(float2* p, uint32_t rank, float2 v
 }
 
 // A 16-byte vector of a row: its maximum, its sum of exponentials, its
-// gradient.  ref: the reference maximum; k2 = log2(e) / tau.
+// gradient.  ref: the reference maximum; k2 = log2(e) / tau.  Exponents are
+// (l - ref) k2, the difference exact near the reference; for bf16 a single
+// multiply-add l k2 - ref k2 where its addend is small enough (near): below 1024
+// the addend is rounded by at most 2^-15, and for the type's lowest value, with
+// which columns are masked, it would overflow.
 template <typename E>
 struct Vec;
+constexpr float kNear = 1024.f;
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
   static __device__ __forceinline__ uint4 lowest() {
     return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
   }
+  static __device__ __forceinline__ bool near(float ref, float k2) { return fabsf(ref) * k2 < kNear; }
   static __device__ __forceinline__ float max(const uint4& u) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
     const float2 t = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
     return fmaxf(t.x, t.y);
   }
-  // exponents as one multiply-add, its addend rounded to 2^-24 of some 40 units: 2e-6 of a value of 2^-8
+  template <bool NEAR>
+  static __device__ __forceinline__ float exponent(float l, float ref, float k2, float c) {
+    return NEAR ? fmaf(l, k2, c) : fmaf(l - ref, k2, c);
+  }
+  template <bool NEAR>
   static __device__ __forceinline__ void sum(const uint4& u, float ref, float k2, float* s) {
     const uint32_t* w = &u.x;
-    const float c = -ref * k2;
+    const float c = NEAR ? -ref * k2 : 0.f;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      s[q] += ex2(fmaf(__uint_as_float(w[q] << 16), k2, c));
-      s[q] += ex2(fmaf(__uint_as_float(w[q] & 0xffff0000u), k2, c));
+      s[q] += ex2(exponent<NEAR>(__uint_as_float(w[q] << 16), ref, k2, c));
+      s[q] += ex2(exponent<NEAR>(__uint_as_float(w[q] & 0xffff0000u), ref, k2, c));
     }
   }
   // f exp((l - ref) / tau), lf = log2(f) inside the exponent
+  template <bool NEAR>
   static __device__ __forceinline__ uint4 grad(const uint4& u, float ref, float k2, float, float lf) {
-    const float c = fmaf(-ref, k2, lf);
+    const float c = NEAR ? fmaf(-ref, k2, lf) : lf;
     const uint32_t* w = &u.x;
     uint4 g;
     uint32_t* o = &g.x;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      o[q] = pack_bf16x2(ex2(fmaf(__uint_as_float(w[q] << 16), k2, c)),
-                         ex2(fmaf(__uint_as_float(w[q] & 0xffff0000u), k2, c)));
+      o[q] = pack_bf16x2(ex2(exponent<NEAR>(__uint_as_float(w[q] << 16), ref, k2, c)),
+                         ex2(exponent<NEAR>(__uint_as_float(w[q] & 0xffff0000u), ref, k2, c)));
     return g;
   }
 };
@@ -178,12 +188,14 @@ struct Vec<float> {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)),
                  fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
-  // the difference first: exact near the reference
+  static __device__ __forceinline__ bool near(float, float) { return false; }
+  template <bool>
   static __device__ __forceinline__ void sum(const uint4& u, float ref, float k2, float* s) {
     const uint32_t* w = &u.x;
 #pragma unroll
     for (int q = 0; q < 4; ++q) s[q] += ex2((__uint_as_float(w[q]) - ref) * k2);
   }
+  template <bool>
   static __device__ __forceinline__ uint4 grad(const uint4& u, float ref, float k2, float f, float) {
     const uint32_t* w = &u.x;
     uint4 g;
@@ -286,8 +298,13 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const Dist
 #pragma unroll
     for (int q = 0; q < 4; ++q) s[q] *= r;
     m = mn;
+    if (VE::near(ref, k2)) {
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) VE::sum(u[j], ref, k2, s);
+      for (int j = 0; j < kUnroll; ++j) VE::template sum<true>(u[j], ref, k2, s);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j) VE::template sum<false>(u[j], ref, k2, s);
+    }
   };
   constexpr int kStep = kUnroll * kRowThreads;
   load(ua, tid);
@@ -333,10 +350,13 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const Dist
 
   if (out) {  // second pass: the gradient of the softmax
     const float lf = log2f(f);
+    const bool near = VE::near(m, k2);
     auto store = [&](const uint4* u, int i0) {
 #pragma unroll
       for (int j = 0; j < kUnroll; ++j)
-        if (i0 + j * kRowThreads < nv) __stcs(vout + i0 + j * kRowThreads, VE::grad(u[j], m, k2, f, lf));
+        if (i0 + j * kRowThreads < nv)
+          __stcs(vout + i0 + j * kRowThreads,
+                 near ? VE::template grad<true>(u[j], m, k2, f, lf) : VE::template grad<false>(u[j], m, k2, f, lf));
     };
     for (int i0 = tid; i0 < nv; i0 += 2 * kStep) {
       again(ub, i0 + kStep);

@@ -653,6 +653,67 @@ def test_lm_head_distillation(T, V, blocks):
     assert torch.equal(dh[~mask], torch.zeros_like(dh[~mask]))
 
 
+# ----------------------------------------------------------------- values at the ends of the types
+@pytest.mark.parametrize("V", [40, 1003, 40000])
+@pytest.mark.parametrize("tau", [0.5, 1.0, 4.0])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_of_logits_masked_with_the_lowest_value(V, tau, dtype):
+    """Masks of the type's lowest value: columns in front and behind, all but one, all; and the same for a teacher."""
+    from parallel_b200.ops import objectives as O
+
+    K, low = 5, torch.finfo(dtype).min
+    g = torch.Generator(device="cuda").manual_seed(V)
+    logits = torch.randn(6, V, device="cuda", generator=g).to(dtype)
+    logits[0, 10:] = low
+    logits[1, : V - 10] = low
+    logits[2, V // 2 + 1:] = low
+    logits[2, : V // 2] = low
+    logits[3] = low  # nothing left: uniform
+    top = 3 * torch.rand(6, K, device="cuda", generator=g)
+    ids = torch.randint(0, 10, (6, K), device="cuda", generator=g)
+    ids[1] += V - 10
+    ids[2] = V // 2
+    top[4] = torch.finfo(torch.float32).min  # one value for all entries
+    top[5, 1:] = torch.finfo(torch.float32).min
+    x = logits.clone().requires_grad_(True)
+    loss = O.distillation_loss(x, top, ids, temperature=tau)
+    (grad,) = torch.autograd.grad(loss, x)
+    _synced()
+    ref, rgrad = _distill_reference(logits, top, ids, torch.ones(6, dtype=torch.bool, device="cuda"), tau)
+    tol = 100 * F32
+    assert abs(loss.item() - ref.item()) <= tol * tau ** 2 * (abs(ref.item()) + 40)
+    rounding = 2.0 ** -8 if dtype == torch.bfloat16 else tol
+    assert ((grad.double() - rgrad).abs() <= rounding * rgrad.abs() + tol * tau / 6).all()
+
+
+@pytest.mark.parametrize("V", [333, 40000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_of_large_logits(V, dtype):
+    """|logit| / temperature up to 1e8: what counts are differences to the maximum, and these are exact."""
+    from parallel_b200.ops import objectives as O
+
+    T, K = 24, 4
+    g = torch.Generator(device="cuda").manual_seed(V)
+    # rows of 2^0, 2^1, ... times a mantissa: in bf16 neighbours at the top are 2^-7 of the logit apart
+    size = 2.0 ** torch.arange(T, device="cuda")[:, None]
+    logits = (size * (1 + torch.rand(T, V, device="cuda", generator=g))).to(dtype)
+    logits[::2] = -logits[::2]
+    ids = logits.float().topk(K, dim=1).indices
+    top = torch.rand(T, K, device="cuda", generator=g)
+    for tau in (1.0, 0.125):
+        x = logits.clone().requires_grad_(True)
+        loss = O.distillation_loss(x, top, ids, temperature=tau)
+        (grad,) = torch.autograd.grad(loss, x)
+        _synced()
+        ref, rgrad = _distill_reference(logits, top, ids, torch.ones(T, dtype=torch.bool, device="cuda"), tau)
+        # differences of up to 40 units matter in the exponentials; in the loss all do, off by 2^-22 of themselves.
+        # bf16: one multiply-add up to exponents of 1024 (base 2), its addend rounded to 2^-15
+        tol = 100 * F32 + (2.0 ** -15 if dtype == torch.bfloat16 else 0.0)
+        assert abs(loss.item() - ref.item()) <= tol * tau ** 2 * (abs(ref.item()) / tau ** 2 + 40)
+        rounding = 2.0 ** -8 + tol if dtype == torch.bfloat16 else tol
+        assert ((grad.double() - rgrad).abs() <= rounding * rgrad.abs() + tol * tau / T).all()
+
+
 # ----------------------------------------------------------------- offsets past 32 bits
 def test_more_than_2_to_the_31_logits():
     """15,000 rows of a 151,936 vocabulary: 2.28e9 exponentials, logits and gradients, checked where offsets are

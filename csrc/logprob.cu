@@ -2,16 +2,20 @@
 // logits: logp[t] = l_id - log sum_v exp(l_v), l_v = (h_t . w_v) / temperature.
 //
 //   logprob_gemm    CTA-pair tcgen05 GEMM h w^T whose epilogue turns each row
-//                   of an output tile into (max, sum of 2^(x - max)) of
-//                   x = l * log2(e), the target column left out; under a
+//                   of an output tile into (max, sum of 2^(x - max)), x the
+//                   logit in base 2, the target column left out; under a
 //                   gradient it also stores E = 2^(x - tile max) in 16 bits.
 //   logprob_finish  per row: the target logit as its own dot product, the
 //                   merge of the row's tile statistics, logp and the row's
-//                   base-2 log-sum-exp.
+//                   base-2 log-sum-exp above its maximum.
 //   logprob_pack    (under a gradient) brings the rows that have a token to the
 //                   front; logprob_unpack takes their gradients back.
 //   logprob_bwd     in place over E: the gradient of the logits,
 //                   dl_v = c ([v = id] - 2^(x_v - lse2)), c = dlogp / temperature.
+//
+// Maxima are kept as they come from the tensor core, unscaled, and only
+// differences of them are scaled, so no digit of an exponent is lost however
+// large the logits are.
 //
 // The target logit is kept out of the sums and summed on its own in 64 bits,
 // and logp = -log1p(sum of the others / target): the tensor core truncates as
@@ -23,7 +27,7 @@
 // E is relative to the tile's own maximum, which is known when the tile is
 // stored, while the row's log-sum-exp is not: an entry keeps 10 bits of its
 // probability whatever its size (pack_e), and the backward is one multiplication
-// per entry (the factor 2^(tile max - lse2) is shared by a tile's row) in a pass
+// per entry (the factor 2^(tile max - lse2), shared by a tile's row) in a pass
 // bound by memory.  bf16 logits would lose |l| / 256 of the exponent instead.
 #include <cuda_bf16.h>
 #include <math.h>
@@ -122,6 +126,15 @@ __device__ __forceinline__ void st_32(void* p, const uint32_t* u) {
                : "memory");
 }
 
+// a, b -> (a - m) scale, (b - m) scale, two at a time (8192 rows, 6554 with a
+// token, forward and backward: 5040 us, as with one multiply-add each and a
+// rounded m scale; one at a time 5200)
+__device__ __forceinline__ void scaled_diff(float& a, float& b, float m, float scale) {
+  const float2 d = __fmul2_rn(__fadd2_rn(make_float2(a, b), make_float2(-m, -m)), make_float2(scale, scale));
+  a = d.x;
+  b = d.y;
+}
+
 // Statistics of one accumulator row (one thread) of `bn` columns from TMEM: the
 // maximum first (E needs one reference for the whole tile), then the sum of the
 // exponentials, which under a gradient (STORE) also go to E, straight from
@@ -143,7 +156,6 @@ __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, 
     mask_cols(v, n_base + c, V, id);
     m = fmaxf(m, max32(v));
   }
-  m *= scale;
   const float ref = m == -INFINITY ? 0.f : m;  // nothing but masked columns
   float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
@@ -155,9 +167,12 @@ __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, 
     const int n0 = n_base + c;
     mask_cols(v, n0, V, id);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      v[j] = ex2(fmaf(v[j], scale, -ref));
+    for (int j = 0; j < 32; j += 2) {
+      scaled_diff(v[j], v[j + 1], ref, scale);
+      v[j] = ex2(v[j]);
+      v[j + 1] = ex2(v[j + 1]);
       s[j & 3] += v[j];
+      s[(j & 3) + 1] += v[j + 1];
     }
     if (STORE && row_in && n0 < V) {
       uint32_t u[16];
@@ -355,13 +370,14 @@ constexpr int kFinThreads = 128;
 
 // One block per row of h; its log-probability goes to row perm[t] (t without
 // perm).  dot in 64 bits (bf16 products are exact in fp32; eight of them are
-// added in fp32, the rest in double), then the tile statistics: with d = m - x_id (base 2), logp = -log(1 + s 2^d), written so that neither
-// a large nor a small d loses digits.
+// added in fp32, the rest in double), then the tile statistics: with d = m -
+// x_id (base 2), logp = -log(1 + s 2^d), written so that neither a large nor a
+// small d loses digits.  lse: the row's maximum m, unscaled, and lse2 - m.
 __global__ void __launch_bounds__(kFinThreads)
     logprob_finish_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const __nv_bfloat16* __restrict__ w,
                           int64_t ldw, const int64_t* __restrict__ ids, const int* __restrict__ perm,
-                          const float2* __restrict__ stats, int tiles, int V, int H, float scale,
-                          float* __restrict__ logp, float* __restrict__ lse2) {
+                          const float2* __restrict__ stats, int tiles, int V, int H, float scale, float scale_mma,
+                          float* __restrict__ logp, float2* __restrict__ lse) {
   pdl_prologue();
   const int64_t t = blockIdx.x;
   const int64_t out = perm ? perm[t] : t;
@@ -370,7 +386,7 @@ __global__ void __launch_bounds__(kFinThreads)
     // no token: 0.  An id past the vocabulary has no log-probability: NaN.
     if (threadIdx.x == 0) {
       logp[out] = id < 0 ? 0.f : NAN;
-      lse2[t] = id < 0 ? 0.f : NAN;
+      lse[t] = id < 0 ? make_float2(0.f, 0.f) : make_float2(NAN, NAN);
     }
     return;
   }
@@ -399,7 +415,7 @@ __global__ void __launch_bounds__(kFinThreads)
       s += v.y;  // 0, or the NaN of a NaN logit
       continue;
     }
-    s = s * ex2(m - mn) + v.y * ex2(v.x - mn);
+    s = s * ex2((m - mn) * scale_mma) + v.y * ex2((v.x - mn) * scale_mma);
     m = mn;
   }
   __shared__ double sd[kFinThreads / 32];
@@ -409,7 +425,7 @@ __global__ void __launch_bounds__(kFinThreads)
     dot += __shfl_xor_sync(0xffffffffu, dot, o);
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
     const float mn = fmaxf(m, m2);
-    s = mn == -INFINITY ? s + s2 : s * ex2(m - mn) + s2 * ex2(m2 - mn);
+    s = mn == -INFINITY ? s + s2 : s * ex2((m - mn) * scale_mma) + s2 * ex2((m2 - mn) * scale_mma);
     m = mn;
   }
   const int wp = threadIdx.x >> 5;
@@ -424,18 +440,27 @@ __global__ void __launch_bounds__(kFinThreads)
   for (int i = 1; i < kFinThreads / 32; ++i) {
     dot += sd[i];
     const float mn = fmaxf(m, sm[i]);
-    s = mn == -INFINITY ? s + ss[i] : s * ex2(m - mn) + ss[i] * ex2(sm[i] - mn);
+    s = mn == -INFINITY ? s + ss[i] : s * ex2((m - mn) * scale_mma) + ss[i] * ex2((sm[i] - mn) * scale_mma);
     m = mn;
   }
   const double x_id = dot * (double)scale;
-  const float d = (float)((double)m - x_id);
-  float lp;
-  if (d <= 0.f)
+  const float d = (float)((double)m * (double)scale_mma - x_id);
+  float lp, above;
+  if (d <= 0.f) {
     lp = -log1pf(s * exp2f(d));
-  else
-    lp = -(d * kLn2 + logf(s + exp2f(-d)));
+    above = -d - lp * kLog2e;
+  } else {
+    const float all = s + exp2f(-d);
+    lp = -(d * kLn2 + logf(all));
+    above = log2f(all);
+  }
+  if (x_id == INFINITY) lp = above = NAN;
+  if (m == -INFINITY) {  // no other token
+    m = 0.f;
+    above = (float)x_id - lp;  // lp: 0, or NaN
+  }
   logp[out] = lp;
-  lse2[t] = (float)(x_id - (double)lp * (double)kLog2e);
+  lse[t] = make_float2(m, above);
 }
 
 // ---------------------------------------------------------------- backward
@@ -447,7 +472,7 @@ constexpr int kBwdUnroll = 4;
 // c (1 - p) = -c expm1(logp), which E could not give where p is near 1.
 __global__ void __launch_bounds__(kBwdThreads)
     logprob_bwd_kernel(__nv_bfloat16* __restrict__ e, int64_t lde, const float2* __restrict__ stats, int tiles,
-                       const float* __restrict__ lse2, const float* __restrict__ logp,
+                       const float2* __restrict__ lse, float scale_mma, const float* __restrict__ logp,
                        const int64_t* __restrict__ ids, const int* __restrict__ perm,
                        const int* __restrict__ count, int row0, const float* __restrict__ g, float inv_tau, int V,
                        const LogprobTiles geo) {
@@ -459,7 +484,7 @@ __global__ void __launch_bounds__(kBwdThreads)
   const int64_t id = ids[t];
   const int src = perm[t];  // logp and g are in the caller's row order
   const float c = id < 0 ? 0.f : g[src] * inv_tau;
-  const float l2 = lse2[t];
+  const float2 top = lse[t];
   __nv_bfloat16* row = e + t * lde;
   const int lane = threadIdx.x & 31;
   const int warps = (int)gridDim.y * (kBwdThreads / 32);
@@ -492,11 +517,11 @@ __global__ void __launch_bounds__(kBwdThreads)
       const int tj = tile + j * warps, col = tj * BN_MAX + lane * 8;
       if (tj < geo.n_full)
         *reinterpret_cast<uint4*>(row + col) =
-            id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(u[j], -c * ex2(f[j] - l2), col);
+            id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(u[j], -c * ex2(fmaf(f[j] - top.x, scale_mma, -top.y)), col);
     }
   }
   for (tile = geo.n_full + blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += warps) {
-    const float f = id < 0 ? 0.f : -c * ex2(st[tile].x - l2);
+    const float f = id < 0 ? 0.f : -c * ex2(fmaf(st[tile].x - top.x, scale_mma, -top.y));
     const int start = tile_start(geo, tile), end = min(V, start + geo.bn2);
     for (int col = start + lane * 8; col < end; col += 256) {
       uint4* p4 = reinterpret_cast<uint4*>(row + col);
@@ -649,6 +674,12 @@ void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap
                                    p.T, p.V, p.H, a_rows, p.tiles, scale, error_word(dev)));
 }
 
+// Base-2 logit per unit of the tensor core's dot product: what its truncation
+// takes is given back on average (kTruncation).
+float mma_scale(float inv_tau, int H) {
+  return (float)((double)kLog2e * inv_tau * (1.0 + kTruncation * ((H + 15) / 16)));
+}
+
 }  // namespace
 
 LogprobTiles logprob_tiles(int T, int V) {
@@ -673,9 +704,7 @@ void logprob_fwd(const LogprobParams& p, cudaStream_t stream) {
   PB_CHECK((reinterpret_cast<uintptr_t>(p.h) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.w) & 15) == 0,
            "logprob: h and w must be 16-byte aligned");
   const float scale = kLog2e * p.inv_tau;
-  // What the tensor core's truncation takes from a logit is given back on average
-  // (kTruncation, above); the target logit does not come from it.
-  const float scale_mma = (float)((double)kLog2e * p.inv_tau * (1.0 + kTruncation * ((p.H + 15) / 16)));
+  const float scale_mma = mma_scale(p.inv_tau, p.H);  // the target logit does not come from the tensor core
   const int a_rows = p.T < BM_CTA ? (p.T + 7) / 8 * 8 : BM_CTA;
   const CUtensorMap ta = make_tmap_2d_bf16(p.h, p.H, p.T, p.ldh, BK, a_rows);
   const CUtensorMap tb = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, BN_MAX / 2);
@@ -688,18 +717,19 @@ void logprob_fwd(const LogprobParams& p, cudaStream_t stream) {
   }
   const int tiles = p.tiles.n_full + p.tiles.n_rest;
   launch_k(logprob_finish_kernel, p.T, kFinThreads, 0, stream, (const __nv_bfloat16*)p.h, p.ldh,
-           (const __nv_bfloat16*)p.w, p.ldw, p.ids, p.perm, (const float2*)p.stats, tiles, p.V, p.H, scale, p.logp, p.lse2);
+           (const __nv_bfloat16*)p.w, p.ldw, p.ids, p.perm, (const float2*)p.stats, tiles, p.V, p.H, scale,
+           scale_mma, p.logp, reinterpret_cast<float2*>(p.lse));
 }
 
-void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse2, const float* logp, const int64_t* ids,
-                 const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V,
+void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse, const float* logp, const int64_t* ids,
+                 const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V, int H,
                  const LogprobTiles& geo, cudaStream_t stream) {
   if (T == 0) return;
   const int tiles = geo.n_full + geo.n_rest;
   // enough blocks for every SM when there are few rows
   const int segs = std::max(1, std::min((tiles + 7) / 8, (8 * num_sms() + T - 1) / T));
   launch_k(logprob_bwd_kernel, dim3(T, segs), kBwdThreads, 0, stream, (__nv_bfloat16*)e, lde, (const float2*)stats,
-           tiles, lse2, logp, ids, perm, count, row0, g, inv_tau, V, geo);
+           tiles, (const float2*)lse, mma_scale(inv_tau, H), logp, ids, perm, count, row0, g, inv_tau, V, geo);
 }
 
 void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, void* hp, int64_t* idp, int* perm,

@@ -87,7 +87,7 @@ void logprob_unpack(const at::Tensor& src, const at::Tensor& perm, const at::Ten
 }
 
 // logprob_fwd(h [T, H], w [V, H], ids [T], inv_tau, logp [>= T], e [T, V] or None, perm [T] or None, count [1] or
-// None, row0) -> (lse2 [T], stats [T, tiles, 2]); logp of row t goes to logp[perm[t]] (logp[t] without perm).  With
+// None, row0) -> (lse [T, 2], stats [T, tiles, 2]); logp of row t goes to logp[perm[t]] (logp[t] without perm).  With
 // count, h holds packed rows from row row0 on, of which the first count[0] have a token.
 std::vector<at::Tensor> logprob_fwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, double inv_tau,
                                     at::Tensor& logp, const c10::optional<at::Tensor>& e,
@@ -108,13 +108,13 @@ std::vector<at::Tensor> logprob_fwd(const at::Tensor& h, const at::Tensor& w, co
   pb::LogprobParams p{};
   p.tiles = pb::logprob_tiles((int)T, (int)V);
   const auto f32 = h.options().dtype(at::kFloat);
-  at::Tensor lse2 = at::empty({T}, f32), stats = at::empty({T, p.tiles.n_full + p.tiles.n_rest, 2}, f32);
+  at::Tensor lse = at::empty({T, 2}, f32), stats = at::empty({T, p.tiles.n_full + p.tiles.n_rest, 2}, f32);
   p.h = h.data_ptr();
   p.w = w.data_ptr();
   p.ids = ids.data_ptr<int64_t>();
   p.stats = stats.data_ptr<float>();
   p.logp = logp.data_ptr<float>();
-  p.lse2 = lse2.data_ptr<float>();
+  p.lse = lse.data_ptr<float>();
   p.ldh = h.stride(0);
   p.ldw = w.stride(0);
   if (given(e)) {
@@ -139,19 +139,19 @@ std::vector<at::Tensor> logprob_fwd(const at::Tensor& h, const at::Tensor& w, co
   p.H = (int)H;
   p.inv_tau = (float)inv_tau;
   pb::logprob_fwd(p, cur_stream());
-  return {lse2, stats};
+  return {lse, stats};
 }
 
-// logprob_bwd(e [T, V], stats, lse2 [T], ids [T], perm [T], count [1], row0, logp, g, inv_tau): e becomes the gradient
+// logprob_bwd(e [T, V], stats, lse [T, 2], ids [T], perm [T], count [1], row0, logp, g, inv_tau, H): e becomes the gradient
 // of h w^T; logp and g are in the caller's row order (row perm[t] for row t of e)
-void logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor& lse2, const at::Tensor& ids,
+void logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor& lse, const at::Tensor& ids,
                  const at::Tensor& perm, const at::Tensor& count, int64_t row0, const at::Tensor& logp,
-                 const at::Tensor& g, double inv_tau) {
+                 const at::Tensor& g, double inv_tau, int64_t H) {
   check_rows_bf16(e, "logprob: e");
   const int64_t T = e.size(0), V = e.size(1);
   TORCH_CHECK(T >= 1 && V >= 1 && T <= kIntMax / 2 && V <= kIntMax / 2, "logprob: row and vocabulary counts");
   check_ids(ids, T, "logprob: ids");
-  for (const at::Tensor* t : {&stats, &lse2, &ids, &perm, &count, &logp, &g}) CHECK_SAME_DEVICE(e, *t);
+  for (const at::Tensor* t : {&stats, &lse, &ids, &perm, &count, &logp, &g}) CHECK_SAME_DEVICE(e, *t);
   TORCH_CHECK(logp.numel() == g.numel() && g.numel() >= T, "logprob: logp and g must have one entry per row");
   const c10::cuda::CUDAGuard guard(e.device());
   const pb::LogprobTiles tiles = pb::logprob_tiles((int)T, (int)V);
@@ -159,10 +159,10 @@ void logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor& lse2,
   TORCH_CHECK(e.stride(0) % 8 == 0 && e.stride(0) >= (V + 7) / 8 * 8 &&
                   (reinterpret_cast<uintptr_t>(e.data_ptr()) & 15) == 0,
               "logprob: e must have 16-byte rows with room for whole 8-column groups");
-  pb::logprob_bwd(e.data_ptr(), e.stride(0), stats.data_ptr<float>(), check_rows_f32(lse2, T, "logprob: lse2"),
+  pb::logprob_bwd(e.data_ptr(), e.stride(0), stats.data_ptr<float>(), check_rows_f32(lse, T * 2, "logprob: lse"),
                   check_rows_f32(logp, logp.numel(), "logprob: logp"), ids.data_ptr<int64_t>(),
                   check_rows_i32(perm, T, "logprob: perm"), check_rows_i32(count, 1, "logprob: count"), (int)row0,
-                  check_rows_f32(g, g.numel(), "logprob: g"), (float)inv_tau, (int)T, (int)V, tiles, cur_stream());
+                  check_rows_f32(g, g.numel(), "logprob: g"), (float)inv_tau, (int)T, (int)V, (int)H, tiles, cur_stream());
 }
 
 // ---------------------------------------------------------------- policy and preference losses
@@ -605,7 +605,7 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
         at::Tensor again = at::empty_like(logp);  // the forward's logp stands
         stats = logprob_fwd(rows, w, ids, inv_tau, again, e, pm, count, r0)[1];
       }
-      logprob_bwd(e, stats, kept[i], ids, pm, count, r0, logp, g, inv_tau);
+      logprob_bwd(e, stats, kept[i], ids, pm, count, r0, logp, g, inv_tau, H);
       if (dh.defined()) logprob_unpack(grad_rows(e, w, count, r0), pm, count, r0, dh);
       if (dw.defined()) grad_head(e, rows, dw, r0 > 0, count, r0);
     }

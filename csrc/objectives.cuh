@@ -12,7 +12,8 @@ namespace pb {
 // ---- log-probabilities of given tokens (logprob.cu)
 // h [T, H] and w [V, H] bf16; ids [T] (negative: no token, logp 0).
 // stats [T, tiles, 2] fp32: per row and tile of vocabulary columns the maximum
-// and sum of 2^(x - max), x = l log2(e), target left out.
+// of h . w and the sum of 2^(x - x at the maximum), x the logit in base 2, target
+// left out.
 // e (optional, 16-bit [T, lde >= V]): 2^(x - tile max), in a format of logprob.cu.
 struct LogprobTiles {
   int n_full, n_rest, bn2;  // n_full tiles of 256 columns, then n_rest of bn2
@@ -27,7 +28,7 @@ struct LogprobParams {
   int row0;
   float* stats;
   float* logp;
-  float* lse2;  // base-2 log-sum-exp of row t
+  float* lse;  // [T, 2]: the maximum of h . w over row t's tiles, the row's base-2 log-sum-exp above it
   void* e;
   int64_t ldh, ldw, lde;
   int T, V, H;
@@ -37,8 +38,8 @@ struct LogprobParams {
 void logprob_fwd(const LogprobParams& p, cudaStream_t stream);
 // e becomes the gradient (bf16) of the raw logits h w^T given g = d loss / d logp
 // (row t of e has its logp and g in row perm[t]; e starts at packed row row0)
-void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse2, const float* logp, const int64_t* ids,
-                 const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V,
+void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse, const float* logp, const int64_t* ids,
+                 const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V, int H,
                  const LogprobTiles& tiles, cudaStream_t stream);
 // hp [T, H]: the rows of h with ids >= 0 in order, then zeros; idp the ids and
 // perm the rows in that order, count[0] the rows with a token

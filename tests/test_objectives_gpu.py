@@ -713,6 +713,63 @@ def test_distillation_of_large_logits(V, dtype):
         rounding = 2.0 ** -8 + tol if dtype == torch.bfloat16 else tol
         assert ((grad.double() - rgrad).abs() <= rounding * rgrad.abs() + tol * tau / T).all()
 
+@pytest.mark.parametrize("power", [0, 4, 8, 10, 11])
+@pytest.mark.parametrize("V", [40, 1003])
+def test_lm_head_log_probs_gradient_of_large_logits(power, V):
+    """Logits of 2^(2 power) and a small whole number: exact in 24 bits, so their gradient hangs on the
+    differences alone.  The target has a probability of about exp(-90): its logit is not part of the others' sum."""
+    from parallel_b200.ops import objectives as O
+
+    T, H = 20, 64
+    g = torch.Generator(device="cuda").manual_seed(power)
+    big = 2.0 ** power
+    h = torch.zeros(T, H, device="cuda")
+    w = torch.zeros(V, H, device="cuda")
+    h[:, 0] = big * (1 + torch.arange(T, device="cuda") / 32)  # 6 bits of mantissa
+    w[:, 0] = big
+    h[:, 1:9] = torch.randint(-2, 3, (T, 8), device="cuda", generator=g).float()
+    w[:, 1:9] = torch.randint(-1, 2, (V, 8), device="cuda", generator=g).float()
+    ids = torch.arange(T, device="cuda")
+    w[ids, 9 + ids] = -64.0  # column 9 + t lowers the target of row t, and it alone
+    h[ids, 9 + ids] = 1.5
+    h, w = h.bfloat16().requires_grad_(True), w.bfloat16().requires_grad_(True)
+    logp = O.lm_head_log_probs(h, w, ids)
+    dh, dw = torch.autograd.grad(logp.sum(), (h, w))
+    _synced()
+    ref, rdh, rdw, top = _head_reference(h, w, ids, torch.ones(T, device="cuda"), 1.0)
+    # logp: the truncation given back to the others, at most 1 / 2^24 per 16-deep step, and fp32
+    assert (logp.double() - ref).abs().max().item() <= (H / 16 + 8) * 2.0 ** -23 * (top + 4)
+    # column 9 + t of dh: -64 x (gradient of the target's logit = 1); column 9 + t of dw sums 1.5 x that of row t
+    assert _err(dh[:, 1:], rdh[:, 1:]) <= GRAD_TOL
+    assert _err(dw[:, 9:9 + T], rdw[:, 9:9 + T]) <= GRAD_TOL and _err(dw[:, 1:9], rdw[:, 1:9]) <= GRAD_TOL
+    # every vocabulary entry on its own: what row t alone sends it, over the hidden state's columns 9 and up
+    want = -torch.softmax(h.detach().double() @ w.detach().double().t(), 1)
+    want[ids, ids] += 1
+    got = dw[:, 9:9 + T].t().double() / 1.5
+    assert ((got - want).abs() <= GRAD_TOL * want.abs() + 1e-12).all()
+
+
+def test_lm_head_log_probs_one_logit_above_all():
+    """Logits of 2^14 to 2^31, far apart: the whole probability stands at the largest one."""
+    from parallel_b200.ops import objectives as O
+
+    T, H, V = 64, 64, 1003
+    g = torch.Generator(device="cuda").manual_seed(0)
+    h, w = torch.zeros(T, H, device="cuda"), torch.zeros(V, H, device="cuda")
+    h[:, 0] = 2.0 ** (torch.arange(T, device="cuda") % 16) * (1 + torch.rand(T, device="cuda", generator=g))
+    w[:, 0] = 2.0 ** 14 * (1 + torch.rand(V, device="cuda", generator=g))
+    best = 700
+    w[best, 0] = 2.0 ** 15 * 1.5
+    ids = torch.randint(0, best, (T,), device="cuda", generator=g)
+    h, w = h.bfloat16().requires_grad_(True), w.bfloat16()
+    logp = O.lm_head_log_probs(h, w, ids)
+    (dh,) = torch.autograd.grad(logp.sum(), h)
+    _synced()
+    want = w[ids].double() - w[best].double()  # the gradient: the target's row of the head less the best one's
+    size = h.detach()[:, 0].double() * w[best, 0].double()
+    assert ((logp.double() - want[:, 0] * h.detach()[:, 0].double()).abs() <= (H / 16 + 8) * 2.0 ** -23 * size).all()
+    assert _err(dh, want) <= GRAD_TOL
+
 
 # ----------------------------------------------------------------- offsets past 32 bits
 def test_more_than_2_to_the_31_logits():

@@ -620,6 +620,7 @@ at::Tensor lm_head_log_probs(const at::Tensor& h, const at::Tensor& w, const at:
                              int64_t max_block_bytes) {
   check_rows_bf16(h, "lm_head_log_probs: h");
   check_rows_bf16(w, "lm_head_log_probs: w");
+  TORCH_CHECK(w.size(0) >= 1, "lm_head_log_probs: an empty vocabulary");
   if (wants_grad(h) || wants_grad(w)) return LogProbsNode::apply(h, w, ids, inv_tau, max_block_bytes);
   const c10::cuda::CUDAGuard guard(h.device());
   at::Tensor logp = at::empty({h.size(0)}, h.options().dtype(at::kFloat));

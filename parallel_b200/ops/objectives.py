@@ -25,12 +25,24 @@ from ._ext import ext
 
 def _rows_bf16(t: torch.Tensor, what: str) -> torch.Tensor:
     """``t`` as bf16 rows that TMA can read: unit inner stride, 16-byte row
-    stride and base (a copy if it has another layout)."""
+    stride and base, no row inside another (a copy if it has another layout)."""
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{what} must be bfloat16 on CUDA, got {t.dtype}")
-    if t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+    if t.stride(-1) != 1 or t.stride(0) % 8 or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
+
+
+def _check_temperature(temperature) -> None:
+    if not 0.0 < temperature < math.inf:
+        raise ValueError(f"temperature has to be positive and finite, got {temperature}")
+
+
+def _check_head(h: torch.Tensor, w: torch.Tensor) -> None:
+    if w.dim() != 2 or h.dim() < 1 or h.shape[-1] != w.shape[1]:
+        raise ValueError(f"h {tuple(h.shape)} and w {tuple(w.shape)} must share their last dimension")
+    if w.numel() == 0:
+        raise ValueError(f"w {tuple(w.shape)} has no entry")
 
 
 # ----------------------------------------------------------------- log-probabilities through the LM head
@@ -44,10 +56,8 @@ def lm_head_log_probs(h: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, tempe
     gives NaN (an ``IndexError`` on CPU).  The gradient goes to h and w; one
     backward pass per forward.  ``max_block_bytes`` bounds the [rows, V] block
     held between forward and backward; rows beyond it are computed twice."""
-    if not temperature > 0.0:
-        raise ValueError(f"temperature has to be positive, got {temperature}")
-    if w.dim() != 2 or h.shape[-1] != w.shape[1]:
-        raise ValueError(f"h {tuple(h.shape)} and w {tuple(w.shape)} must share their last dimension")
+    _check_temperature(temperature)
+    _check_head(h, w)
     if ids.dtype != torch.int64 or ids.numel() * h.shape[-1] != h.numel():
         raise ValueError(f"ids must be int64 with one entry per row of h, got {ids.dtype} {tuple(ids.shape)} for "
                          f"{tuple(h.shape)}")
@@ -197,8 +207,7 @@ def _preference_plain(logp, ref, mask, beta, smoothing, average):
 # ----------------------------------------------------------------- distillation from a teacher's top logits
 def _check_teacher(rows, top_logits, top_ids, mask, temperature):
     """Teacher entries as [T, K] and the mask as [T] for `rows` (the leading shape of the student's rows)."""
-    if not temperature > 0.0:
-        raise ValueError(f"temperature has to be positive, got {temperature}")
+    _check_temperature(temperature)
     if top_logits.shape[:-1] != rows or top_ids.shape != top_logits.shape or top_logits.dim() < 1:
         raise ValueError(f"teacher logits {tuple(top_logits.shape)} and ids {tuple(top_ids.shape)}: "
                          f"[{', '.join(str(r) for r in rows)}, K] expected")
@@ -225,10 +234,10 @@ def distillation_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_ids: t
 
     logits [..., V] (bf16 or fp32) are the student's; top_logits [..., K]
     (bf16 or fp32) and top_ids [..., K] (int64 or int32) the teacher's highest
-    logits and their tokens, an id < 0 marking an absent entry.  With
-    q = softmax(top_logits / temperature) over the entries present and
-    p = softmax(logits / temperature) over the vocabulary, a row's loss is
-    ``temperature^2 sum_k q_k (log q_k - log p[id_k])``; an id that comes
+    logits and their tokens, an id < 0 marking an absent entry (K at most 1024
+    on CUDA).  With q = softmax(top_logits / temperature) over the entries
+    present and p = softmax(logits / temperature) over the vocabulary, a row's
+    loss is ``temperature^2 sum_k q_k (log q_k - log p[id_k])``; an id that comes
     twice counts twice.  Rows outside mask (bool [...]) and rows without an
     entry do not count, and may hold anything; without any row the loss is 0.
     An id >= V makes the loss NaN (an ``IndexError`` on CPU).  The gradient
@@ -246,8 +255,7 @@ def lm_head_distillation(h: torch.Tensor, w: torch.Tensor, top_logits: torch.Ten
                          max_block_bytes: int = 6 << 30) -> torch.Tensor:
     """``distillation_loss(h @ w.T, ...)`` for hidden states h [..., H] and the LM head w [V, H], with at most
     ``max_block_bytes`` of bf16 logits held at a time; the gradient goes to h and w."""
-    if w.dim() != 2 or h.shape[-1] != w.shape[1]:
-        raise ValueError(f"h {tuple(h.shape)} and w {tuple(w.shape)} must share their last dimension")
+    _check_head(h, w)
     top, ids, m = _check_teacher(h.shape[:-1], top_logits, top_ids, mask, temperature)
     h2, tau = h.reshape(-1, h.shape[-1]), float(temperature)
     if not h2.is_cuda:

@@ -36,6 +36,19 @@ def test_log_probs_refusals():
     assert O.lm_head_log_probs(h[:0], w, ids[:0]).shape == (0,)
 
 
+def test_log_probs_refuse_an_empty_head_and_a_temperature_without_end():
+    h, w, ids = torch.randn(4, 8), torch.randn(9, 8), torch.full((4,), -100)
+    for bad in (dict(w=w[:0]), dict(h=h[:, :0], w=w[:, :0]), dict(temperature=float("inf")),
+                dict(temperature=float("nan"))):
+        with pytest.raises(ValueError):
+            O.lm_head_log_probs(**{**dict(h=h, w=w, ids=ids), **bad})
+    top, tid = torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    with pytest.raises(ValueError):
+        O.lm_head_distillation(h, w[:0], top, tid)
+    with pytest.raises(ValueError):
+        O.distillation_loss(h, top, tid, temperature=float("inf"))
+
+
 def _differences(fn, x):
     """Autograd against central differences in 64 bits along a random direction."""
     x = x.detach().double().requires_grad_(True)

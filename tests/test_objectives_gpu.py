@@ -771,6 +771,28 @@ def test_lm_head_log_probs_one_logit_above_all():
     assert _err(dh, want) <= GRAD_TOL
 
 
+def test_rows_that_share_memory_and_an_empty_vocabulary():
+    """Broadcast and overlapping hidden states and heads are read as what they stand for; no vocabulary is refused."""
+    from parallel_b200.ops import objectives as O
+
+    h, w, ids, g = _head_inputs(33, 64, 300, ignored=0.1, seed=51)
+    flat = torch.randn(33 * 8 + 64, device="cuda").bfloat16()
+    for a, b in ((h[:1].expand(33, 64), w), (flat.as_strided((33, 64), (8, 1)), w), (h, w[:1].expand(300, 64))):
+        ref, rdh, rdw, top = _head_reference(a, b, ids, g, 1.0)
+        with torch.no_grad():
+            scored = O.lm_head_log_probs(a, b, ids)
+        ag, bg = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        logp = O.lm_head_log_probs(ag, bg, ids)
+        dh, dw = torch.autograd.grad(logp, (ag, bg), g)
+        _synced()
+        assert (scored.double() - ref).abs().max().item() <= (64 / 16 + 8) * 2.0 ** -23 * (top + 4)
+        assert torch.equal(scored, logp.detach())
+        assert _err(dh, rdh) <= GRAD_TOL or rdh.abs().max().item() < 1e-12
+        assert _err(dw, rdw) <= GRAD_TOL
+    with pytest.raises(ValueError):
+        O.lm_head_log_probs(h.requires_grad_(True), w[:0], ids.clamp_max(-1))
+
+
 # ----------------------------------------------------------------- offsets past 32 bits
 def test_more_than_2_to_the_31_logits():
     """15,000 rows of a 151,936 vocabulary: 2.28e9 exponentials, logits and gradients, checked where offsets are

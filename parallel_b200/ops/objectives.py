@@ -274,8 +274,10 @@ def _distillation_plain(x, top, ids, mask, tau):
     counts = have.any(1) if mask is None else have.any(1) & mask
     rows = counts.nonzero()[:, 0]
     have, ids = have[rows], ids[rows].clamp_min(0).long()
-    log_q = torch.log_softmax(top[rows].to(dt).div(tau).masked_fill(~have, -math.inf), dim=1)
-    log_p = torch.log_softmax(x[rows].to(dt) / tau, dim=1).gather(1, ids)
+    # differences to the maximum before the temperature: values at the end of their type's range stay finite
+    t, x = top[rows].to(dt).masked_fill(~have, -math.inf), x[rows].to(dt)
+    log_q = torch.log_softmax((t - t.amax(1, keepdim=True)) / tau, dim=1)
+    log_p = torch.log_softmax((x - x.detach().amax(1, keepdim=True)) / tau, dim=1).gather(1, ids)
     zero = torch.zeros((), dtype=dt, device=x.device)
     terms = torch.where(have, log_q.exp() * (torch.where(have, log_q, zero) - torch.where(have, log_p, zero)), zero)
     return tau * tau * terms.sum() / max(1, rows.numel())

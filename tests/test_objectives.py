@@ -118,6 +118,22 @@ def test_policy_and_preference_refusals():
         O.preference_loss(x, mask=x)
 
 
+def test_distillation_of_values_at_the_end_of_their_range():
+    """Masks of the type's lowest value, in the student's logits and in the teacher's, at a temperature below 1."""
+    low = torch.finfo(torch.float32).min
+    x, top = torch.randn(3, 6), torch.rand(3, 2)
+    x[0, 3:], x[1], top[2] = low, low, low
+    ids = torch.tensor([[0, 2]] * 3)
+    x.requires_grad_(True)
+    loss = O.distillation_loss(x, top, ids, temperature=0.5)
+    (grad,) = torch.autograd.grad(loss, x)
+    lp = torch.log_softmax(x.detach().double() / 0.5, 1).gather(1, ids)
+    lq = torch.log_softmax(top.double() / 0.5, 1)
+    want = 0.25 * (lq.exp() * (lq - lp)).sum(1).mean()
+    assert abs(loss.item() - want.item()) < 1e-6 and torch.isfinite(grad).all()
+    assert grad[0, 3:].abs().max() == 0 and grad[1].sum().abs() < 1e-6
+
+
 def test_distillation_loss_formula_and_gradient():
     torch.manual_seed(3)
     T, V, K, tau = 6, 11, 4, 1.7

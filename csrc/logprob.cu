@@ -10,8 +10,13 @@
 //                   base-2 log-sum-exp above its maximum.
 //   logprob_pack    (under a gradient) brings the rows that have a token to the
 //                   front; logprob_unpack takes their gradients back.
-//   logprob_bwd     in place over E: the gradient of the logits,
-//                   dl_v = c ([v = id] - 2^(x_v - lse2)), c = dlogp / temperature.
+//   logprob_bwd     in place over E: the gradient of the logits but the target,
+//                   dl_v = -c 2^(x_v - lse2), c = dlogp / temperature, and the
+//                   target's own c (1 - p), in fp32.
+//   logprob_unpack, logprob_own add the target's part of the gradients of h and
+//                   w, c (1 - p) w_id and c (1 - p) h, in fp32: it is most of
+//                   them, and as one more bf16 factor its rounding, the same in
+//                   a whole row of the product, would add up to 2^-9 of it.
 //
 // Maxima are kept as they come from the tensor core, unscaled, and only
 // differences of them are scaled, so no digit of an exponent is lost however
@@ -468,14 +473,14 @@ constexpr int kBwdThreads = 256;
 constexpr int kBwdUnroll = 4;
 
 // A warp takes a tile of a row at a time: one factor for its (256) consecutive
-// entries, 8 of them per lane and step.  The target's own entry is
-// c (1 - p) = -c expm1(logp), which E could not give where p is near 1.
+// entries, 8 of them per lane and step.  The target's entry, 0 in E, stays 0;
+// own[t] = c (1 - p) = -c expm1(logp).
 __global__ void __launch_bounds__(kBwdThreads)
     logprob_bwd_kernel(__nv_bfloat16* __restrict__ e, int64_t lde, const float2* __restrict__ stats, int tiles,
                        const float2* __restrict__ lse, float scale_mma, const float* __restrict__ logp,
                        const int64_t* __restrict__ ids, const int* __restrict__ perm,
                        const int* __restrict__ count, int row0, const float* __restrict__ g, float inv_tau, int V,
-                       const LogprobTiles geo) {
+                       float* __restrict__ own, const LogprobTiles geo) {
   pdl_prologue();
   const int64_t t = blockIdx.x;
   // behind the rows with a token: zeros up to the end of the last 64-deep step of
@@ -488,14 +493,14 @@ __global__ void __launch_bounds__(kBwdThreads)
   __nv_bfloat16* row = e + t * lde;
   const int lane = threadIdx.x & 31;
   const int warps = (int)gridDim.y * (kBwdThreads / 32);
-  const float own = id < 0 ? 0.f : -c * expm1f(logp[src]);
+  if (blockIdx.y == 0 && threadIdx.x == 0) own[t] = id < 0 ? 0.f : -c * expm1f(logp[src]);
   const float2* st = stats + t * tiles;
-  auto scaled = [&](uint4 u, float f, int col) {
+  auto scaled = [&](uint4 u, float f) {
     uint32_t* p = &u.x;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float2 x = unpack_e(p[q]);
-      p[q] = pack_bf16x2(col + 2 * q == id ? own : x.x * f, col + 2 * q + 1 == id ? own : x.y * f);
+      p[q] = pack_bf16x2(x.x * f, x.y * f);
     }
     return u;
   };
@@ -517,7 +522,7 @@ __global__ void __launch_bounds__(kBwdThreads)
       const int tj = tile + j * warps, col = tj * BN_MAX + lane * 8;
       if (tj < geo.n_full)
         *reinterpret_cast<uint4*>(row + col) =
-            id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(u[j], -c * ex2(fmaf(f[j] - top.x, scale_mma, -top.y)), col);
+            id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(u[j], -c * ex2(fmaf(f[j] - top.x, scale_mma, -top.y)));
     }
   }
   for (tile = geo.n_full + blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += warps) {
@@ -525,8 +530,19 @@ __global__ void __launch_bounds__(kBwdThreads)
     const int start = tile_start(geo, tile), end = min(V, start + geo.bn2);
     for (int col = start + lane * 8; col < end; col += 256) {
       uint4* p4 = reinterpret_cast<uint4*>(row + col);
-      *p4 = id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(*p4, f, col);
+      *p4 = id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(*p4, f);
     }
+  }
+}
+
+// v += f x, x eight bf16
+__device__ __forceinline__ void add_scaled(float* v, const uint4& x, float f) {
+  const uint32_t* w = &x.x;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float2 y = unpack_bf16x2(w[q]);
+    v[2 * q] = fmaf(f, y.x, v[2 * q]);
+    v[2 * q + 1] = fmaf(f, y.y, v[2 * q + 1]);
   }
 }
 
@@ -598,18 +614,23 @@ __global__ void __launch_bounds__(kPackThreads)
   }
 }
 
-// dst[perm[row0 + i]] = the sum over slices, in order, of row i of src - bf16
-// rows (one slice), or the fp32 slabs of a product that was split - for rows
-// with a token, 0 for the others; a block a row.
+// dst[perm[i]] = the sum over slices, in order, of row i of src - bf16 rows (one
+// slice), or fp32 slabs - and (own) own[i] w[ids[i]], for rows with a token, 0
+// for the others; a block a row.
 template <typename E>
 __global__ void __launch_bounds__(128)
     logprob_unpack_kernel(const E* __restrict__ src, int slices, const int* __restrict__ perm,
-                          const int* __restrict__ count, int row0, int T, int H, __nv_bfloat16* __restrict__ dst) {
+                          const int* __restrict__ count, int row0, int T, int H, const float* __restrict__ own,
+                          const int64_t* __restrict__ ids, const __nv_bfloat16* __restrict__ w, int64_t ldw, int V,
+                          __nv_bfloat16* __restrict__ dst) {
   pdl_prologue();
   const int i = blockIdx.x;
   const bool live = row0 + i < count[0];
   uint4* d = reinterpret_cast<uint4*>(dst + (int64_t)perm[i] * H);
   const int64_t slab = (int64_t)T * H;
+  const int64_t id = own && live ? ids[i] : 0;
+  const float f = own && live && id < V ? own[i] : 0.f;  // past the vocabulary: src is NaN already
+  const uint4* wr = own && live && id < V ? reinterpret_cast<const uint4*>(w + id * ldw) : nullptr;
   for (int k = threadIdx.x; k < H / 8; k += 128) {
     uint4 u = make_uint4(0u, 0u, 0u, 0u);
     if (live) {
@@ -617,6 +638,7 @@ __global__ void __launch_bounds__(128)
         u = reinterpret_cast<const uint4*>(src + (int64_t)i * H)[k];
       } else {
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const uint4 x = wr ? wr[k] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 4
         for (int s = 0; s < slices; ++s) {
           const float4* p = reinterpret_cast<const float4*>(src + s * slab + (int64_t)i * H) + 2 * k;
@@ -624,11 +646,80 @@ __global__ void __launch_bounds__(128)
           v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
           v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
         }
+        add_scaled(v, x, f);
         u = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
                        pack_bf16x2(v[6], v[7]));
       }
     }
     d[k] = u;
+  }
+}
+
+// dw[ids[t]] += own[t] h[t] over the rows that have a token: a block a row, in
+// which the first row of an id adds up all rows of that id (in the same order on
+// every run) and the others leave.  Each block looks through all ids, which stay
+// in L1: 6554 rows of 8192, H 1024: 38 us.
+constexpr int kOwnWarps = 4;
+constexpr int kOwnList = 512;
+template <typename E>
+__global__ void __launch_bounds__(32 * kOwnWarps)
+    logprob_own_kernel(const __nv_bfloat16* __restrict__ h, const int64_t* __restrict__ ids,
+                       const float* __restrict__ own, const int* __restrict__ count, int row0, int T, int V, int H,
+                       E* __restrict__ dw) {
+  pdl_prologue();
+  __shared__ int list[kOwnWarps][kOwnList], found[kOwnWarps];
+  const int n = min(T, count[0] - row0), t = blockIdx.x;
+  if (t >= n) return;
+  const int64_t id = ids[t];
+  if (id >= V) return;  // no row of the head; the gradient is NaN already
+  bool seen = false;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < t; i += 32 * kOwnWarps) seen = seen || ids[i] == id;
+  if (__syncthreads_or(seen)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // each warp looks through a quarter of the rows from t on, 256 at a time
+  const int per = (n - t + kOwnWarps - 1) / kOwnWarps;
+  int i = t + warp * per;
+  const int end = min(n, i + per);
+  for (;;) {
+    int m = 0;
+    while (i < end && m <= kOwnList - 256) {
+      int64_t v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = i + 32 * u + lane < end ? ids[i + 32 * u + lane] : -1;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const uint32_t hit = __ballot_sync(0xffffffffu, v[u] == id);
+        if (v[u] == id) list[warp][m + __popc(hit & ((1u << lane) - 1u))] = i + 32 * u + lane;
+        m += __popc(hit);
+      }
+      i += 256;
+    }
+    if (lane == 0) found[warp] = m;
+    const bool more = __syncthreads_or(i < end);
+    for (int col = threadIdx.x * 8; col < H; col += 32 * kOwnWarps * 8) {
+      float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < kOwnWarps; ++w) {
+        const int rows = found[w];
+#pragma unroll 4
+        for (int j = 0; j < rows; ++j) {
+          const int r = list[w][j];
+          add_scaled(a, *reinterpret_cast<const uint4*>(h + (int64_t)r * H + col), own[r]);
+        }
+      }
+      E* d = dw + id * H + col;
+      if constexpr (sizeof(E) == 2) {
+        uint4 u = *reinterpret_cast<uint4*>(d);
+        add_scaled(a, u, 1.f);
+        *reinterpret_cast<uint4*>(d) = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]),
+                                                  pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) d[q] += a[q];
+      }
+    }
+    if (!more) return;
+    __syncthreads();  // the list is free again
   }
 }
 
@@ -723,13 +814,14 @@ void logprob_fwd(const LogprobParams& p, cudaStream_t stream) {
 
 void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse, const float* logp, const int64_t* ids,
                  const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V, int H,
-                 const LogprobTiles& geo, cudaStream_t stream) {
+                 float* own, const LogprobTiles& geo, cudaStream_t stream) {
   if (T == 0) return;
   const int tiles = geo.n_full + geo.n_rest;
   // enough blocks for every SM when there are few rows
   const int segs = std::max(1, std::min((tiles + 7) / 8, (8 * num_sms() + T - 1) / T));
   launch_k(logprob_bwd_kernel, dim3(T, segs), kBwdThreads, 0, stream, (__nv_bfloat16*)e, lde, (const float2*)stats,
-           tiles, (const float2*)lse, mma_scale(inv_tau, H), logp, ids, perm, count, row0, g, inv_tau, V, geo);
+           tiles, (const float2*)lse, mma_scale(inv_tau, H), logp, ids, perm, count, row0, g, inv_tau, V, own,
+           geo);
 }
 
 void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, void* hp, int64_t* idp, int* perm,
@@ -744,13 +836,25 @@ void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, 
 }
 
 void logprob_unpack(const void* src, bool f32, int slices, const int* perm, const int* count, int row0, int T, int H,
-                    void* dst, cudaStream_t stream) {
+                    const float* own, const int64_t* ids, const void* w, int64_t ldw, int V, void* dst,
+                    cudaStream_t stream) {
+  PB_CHECK(f32 || !own, "logprob: the target's part is added to fp32 sums");
   if (f32)
-    launch_k(logprob_unpack_kernel<float>, T, 128, 0, stream, (const float*)src, slices, perm, count, row0, T,
-             H, (__nv_bfloat16*)dst);
+    launch_k(logprob_unpack_kernel<float>, T, 128, 0, stream, (const float*)src, slices, perm, count, row0, T, H, own,
+             ids, (const __nv_bfloat16*)w, ldw, V, (__nv_bfloat16*)dst);
   else
-    launch_k(logprob_unpack_kernel<__nv_bfloat16>, T, 128, 0, stream, (const __nv_bfloat16*)src, 1, perm,
-             count, row0, T, H, (__nv_bfloat16*)dst);
+    launch_k(logprob_unpack_kernel<__nv_bfloat16>, T, 128, 0, stream, (const __nv_bfloat16*)src, 1, perm, count, row0,
+             T, H, own, ids, (const __nv_bfloat16*)w, ldw, V, (__nv_bfloat16*)dst);
+}
+
+void logprob_own(const void* h, const int64_t* ids, const float* own, const int* count, int row0, int T, int V, int H,
+                 void* dw, bool f32, cudaStream_t stream) {
+  if (f32)
+    launch_k(logprob_own_kernel<float>, T, 32 * kOwnWarps, 0, stream, (const __nv_bfloat16*)h, ids, own, count, row0, T,
+             V, H, (float*)dw);
+  else
+    launch_k(logprob_own_kernel<__nv_bfloat16>, T, 32 * kOwnWarps, 0, stream, (const __nv_bfloat16*)h, ids, own, count,
+             row0, T, V, H, (__nv_bfloat16*)dw);
 }
 
 }  // namespace pb

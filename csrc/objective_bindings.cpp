@@ -67,9 +67,11 @@ std::vector<at::Tensor> logprob_pack(const at::Tensor& h, const at::Tensor& ids)
 }
 
 // logprob_unpack(src [slices * T, H] (bf16, one slice, or fp32 slabs), perm [T], count, row0, dst [T_all, H] bf16):
-// dst[perm[i]] = row i of src (its slices added) where packed row row0 + i has a token, else 0
+// dst[perm[i]] = row i of src (its slices added) where packed row row0 + i has a token, else 0; own [T] (with fp32
+// slabs, the rows' ids and the head w): own[i] w[ids[i]] is added to it
 void logprob_unpack(const at::Tensor& src, const at::Tensor& perm, const at::Tensor& count, int64_t row0,
-                    at::Tensor& dst) {
+                    at::Tensor& dst, const at::Tensor& own = {}, const at::Tensor& ids = {},
+                    const at::Tensor& w = {}) {
   const int64_t T = perm.numel(), H = dst.size(-1);
   const bool f32 = src.scalar_type() == at::kFloat;
   TORCH_CHECK(src.is_cuda() && src.is_contiguous() && (f32 || src.scalar_type() == at::kBFloat16) && src.dim() == 2 &&
@@ -80,10 +82,20 @@ void logprob_unpack(const at::Tensor& src, const at::Tensor& perm, const at::Ten
   CHECK_SAME_DEVICE(src, perm);
   CHECK_SAME_DEVICE(src, count);
   CHECK_SAME_DEVICE(src, dst);
+  const float* op = nullptr;
+  if (own.defined()) {
+    op = check_rows_f32(own, T, "logprob: own");
+    check_ids(ids, T, "logprob: ids");
+    check_rows_bf16(w, "logprob: w");
+    for (const at::Tensor* t : {&own, &ids, &w}) CHECK_SAME_DEVICE(src, *t);
+    TORCH_CHECK(w.size(1) == H && w.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) == 0,
+                "logprob: w must have 16-byte rows of dst's width");
+  }
   const c10::cuda::CUDAGuard g(src.device());
   pb::logprob_unpack(src.data_ptr(), f32, (int)(src.size(0) / T), check_rows_i32(perm, T, "logprob: perm"),
-                     check_rows_i32(count, 1, "logprob: count"), (int)row0, (int)T, (int)H, dst.data_ptr(),
-                     cur_stream());
+                     check_rows_i32(count, 1, "logprob: count"), (int)row0, (int)T, (int)H, op,
+                     op ? ids.data_ptr<int64_t>() : nullptr, op ? w.data_ptr() : nullptr, op ? w.stride(0) : 0,
+                     op ? (int)w.size(0) : 0, dst.data_ptr(), cur_stream());
 }
 
 // logprob_fwd(h [T, H], w [V, H], ids [T], inv_tau, logp [>= T], e [T, V] or None, perm [T] or None, count [1] or
@@ -142,9 +154,10 @@ std::vector<at::Tensor> logprob_fwd(const at::Tensor& h, const at::Tensor& w, co
   return {lse, stats};
 }
 
-// logprob_bwd(e [T, V], stats, lse [T, 2], ids [T], perm [T], count [1], row0, logp, g, inv_tau, H): e becomes the gradient
-// of h w^T; logp and g are in the caller's row order (row perm[t] for row t of e)
-void logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor& lse, const at::Tensor& ids,
+// logprob_bwd(e [T, V], stats, lse [T, 2], ids [T], perm [T], count [1], row0, logp, g, inv_tau, H) -> own [T]: e
+// becomes the gradient of h w^T but for the targets', which is own; logp and g are in the caller's row order (row
+// perm[t] for row t of e)
+at::Tensor logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor& lse, const at::Tensor& ids,
                  const at::Tensor& perm, const at::Tensor& count, int64_t row0, const at::Tensor& logp,
                  const at::Tensor& g, double inv_tau, int64_t H) {
   check_rows_bf16(e, "logprob: e");
@@ -159,10 +172,13 @@ void logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor& lse, 
   TORCH_CHECK(e.stride(0) % 8 == 0 && e.stride(0) >= (V + 7) / 8 * 8 &&
                   (reinterpret_cast<uintptr_t>(e.data_ptr()) & 15) == 0,
               "logprob: e must have 16-byte rows with room for whole 8-column groups");
+  at::Tensor own = at::empty({T}, lse.options());
   pb::logprob_bwd(e.data_ptr(), e.stride(0), stats.data_ptr<float>(), check_rows_f32(lse, T * 2, "logprob: lse"),
                   check_rows_f32(logp, logp.numel(), "logprob: logp"), ids.data_ptr<int64_t>(),
                   check_rows_i32(perm, T, "logprob: perm"), check_rows_i32(count, 1, "logprob: count"), (int)row0,
-                  check_rows_f32(g, g.numel(), "logprob: g"), (float)inv_tau, (int)T, (int)V, (int)H, tiles, cur_stream());
+                  check_rows_f32(g, g.numel(), "logprob: g"), (float)inv_tau, (int)T, (int)V, (int)H,
+                  own.data_ptr<float>(), tiles, cur_stream());
+  return own;
 }
 
 // ---------------------------------------------------------------- policy and preference losses
@@ -502,11 +518,11 @@ int grad_rows_slices(int64_t T, int64_t H, int64_t V) {
   return best;
 }
 
-// dl [T, V] @ w [V, H] for the rows that count: bf16 [T, H], or fp32 slabs [slices * T, H]
-at::Tensor grad_rows(const at::Tensor& dl, const at::Tensor& w, const at::Tensor& count, int64_t row0) {
+// dl [T, V] @ w [V, H] for the rows that count: bf16 [T, H], or (several slices, or f32) fp32 slabs [slices * T, H]
+at::Tensor grad_rows(const at::Tensor& dl, const at::Tensor& w, const at::Tensor& count, int64_t row0, bool f32) {
   const int64_t T = dl.size(0), V = w.size(0), H = w.size(1);
   const int slices = grad_rows_slices(T, H, V);
-  at::Tensor out = at::empty({slices * T, H}, dl.options().dtype(slices == 1 ? at::kBFloat16 : at::kFloat));
+  at::Tensor out = at::empty({slices * T, H}, dl.options().dtype(slices == 1 && !f32 ? at::kBFloat16 : at::kFloat));
   pb::GemmParams p{};
   p.A = dl.data_ptr();
   p.B = w.data_ptr();
@@ -519,7 +535,7 @@ at::Tensor grad_rows(const at::Tensor& dl, const at::Tensor& w, const at::Tensor
   p.K = (int)V;
   p.b_mn = true;
   p.alpha = 1.f;
-  p.epi = slices == 1 ? pb::kEpiStoreBf16 : pb::kEpiStoreF32;
+  p.epi = slices == 1 && !f32 ? pb::kEpiStoreBf16 : pb::kEpiStoreF32;
   p.splits = slices;
   p.live = count.data_ptr<int>();
   p.live_row0 = (int)row0;
@@ -605,9 +621,13 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
         at::Tensor again = at::empty_like(logp);  // the forward's logp stands
         stats = logprob_fwd(rows, w, ids, inv_tau, again, e, pm, count, r0)[1];
       }
-      logprob_bwd(e, stats, kept[i], ids, pm, count, r0, logp, g, inv_tau, H);
-      if (dh.defined()) logprob_unpack(grad_rows(e, w, count, r0), pm, count, r0, dh);
-      if (dw.defined()) grad_head(e, rows, dw, r0 > 0, count, r0);
+      const at::Tensor own = logprob_bwd(e, stats, kept[i], ids, pm, count, r0, logp, g, inv_tau, H);
+      if (dh.defined()) logprob_unpack(grad_rows(e, w, count, r0, true), pm, count, r0, dh, own, ids, w);
+      if (dw.defined()) {
+        grad_head(e, rows, dw, r0 > 0, count, r0);
+        pb::logprob_own(rows.data_ptr(), ids.data_ptr<int64_t>(), own.data_ptr<float>(), count.data_ptr<int>(), (int)r0,
+                        (int)n, (int)V, (int)H, dw.data_ptr(), dw.scalar_type() == at::kFloat, cur_stream());
+      }
     }
     return {dh, dw.defined() ? dw.to(w.scalar_type()) : dw, at::Tensor(), at::Tensor(), at::Tensor()};
   }
@@ -767,7 +787,7 @@ struct HeadDistillationNode : public torch::autograd::Function<HeadDistillationN
       pb::gemm_bf16(p, cur_stream());
       distill_rows(logits, prep, T, K, r0, tau, need_h || need_w ? c10::optional<at::Tensor>(logits) : c10::nullopt,
                    perm.data_ptr<int>());
-      if (need_h) logprob_unpack(grad_rows(logits, w, count, r0), pm, count, r0, dh);
+      if (need_h) logprob_unpack(grad_rows(logits, w, count, r0, false), pm, count, r0, dh);
       if (need_w) grad_head(logits, rows, dw, r0 > 0, count, r0);
     }
     if (ctx) {

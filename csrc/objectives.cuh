@@ -36,19 +36,24 @@ struct LogprobParams {
   float inv_tau;
 };
 void logprob_fwd(const LogprobParams& p, cudaStream_t stream);
-// e becomes the gradient (bf16) of the raw logits h w^T given g = d loss / d logp
-// (row t of e has its logp and g in row perm[t]; e starts at packed row row0)
+// e becomes the gradient (bf16) of the raw logits h w^T given g = d loss / d logp,
+// 0 at the target, whose gradient goes to own [T] in fp32 (row t of e has its
+// logp and g in row perm[t]; e starts at packed row row0)
 void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse, const float* logp, const int64_t* ids,
                  const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V, int H,
-                 const LogprobTiles& tiles, cudaStream_t stream);
+                 float* own, const LogprobTiles& tiles, cudaStream_t stream);
 // hp [T, H]: the rows of h with ids >= 0 in order, then zeros; idp the ids and
 // perm the rows in that order, count[0] the rows with a token
 void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, void* hp, int64_t* idp, int* perm,
                   int* count, cudaStream_t stream);
-// dst[perm[i]] = row i of src [T, H] (bf16, or f32: the sum of `slices` such slabs) for the packed rows
-// [row0, row0 + T) with a token, 0 for the others; perm starts at row0
+// dst[perm[i]] = row i of src [T, H] (bf16, or f32: the sum of `slices` such slabs, and of own[i] w[ids[i]] where own
+// is given) for the packed rows [row0, row0 + T) with a token, 0 for the others; perm, own and ids start at row0
 void logprob_unpack(const void* src, bool f32, int slices, const int* perm, const int* count, int row0, int T, int H,
-                    void* dst, cudaStream_t stream);
+                    const float* own, const int64_t* ids, const void* w, int64_t ldw, int V, void* dst,
+                    cudaStream_t stream);
+// dw [V, H] (fp32 or bf16, contiguous): dw[ids[t]] += own[t] h[t] over the packed rows [row0, row0 + T) with a token
+void logprob_own(const void* h, const int64_t* ids, const float* own, const int* count, int row0, int T, int V, int H,
+                 void* dw, bool f32, cudaStream_t stream);
 
 // ---- losses over token log-probabilities (objectives.cu); rows b have their
 // own strides, mask is bool bytes (optional).  chunk: objective_chunk(rows, S),

@@ -771,6 +771,53 @@ def test_lm_head_log_probs_one_logit_above_all():
     assert _err(dh, want) <= GRAD_TOL
 
 
+@pytest.mark.parametrize("T,H,V,blocks", [(1, 1024, 32003, 1), (8, 4096, 32003, 1), (130, 1536, 5001, 1),
+                                          (700, 64, 1003, 3)])
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_lm_head_log_probs_gradients_are_rounded_once_at_the_target(T, H, V, blocks, seed):
+    """The target's part of both gradients is fp32 until the result is rounded; the others' coefficients are rounded
+    to bf16, each on its own: the norms of what these add, sum of squares, at 2^-9 rms and three times that."""
+    from parallel_b200.ops import objectives as O
+
+    h, w, ids, g = _head_inputs(T, H, V, ignored=0.0, seed=100 + seed)
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    logp = O.lm_head_log_probs(h, w, ids, max_block_bytes=(6 << 30) if blocks == 1 else 2 * V * 256)
+    dh, dw = torch.autograd.grad(logp, (h, w), g)
+    _synced()
+    _, rdh, rdw, _ = _head_reference(h, w, ids, g, 1.0)
+    p = torch.softmax(h.detach().double() @ w.detach().double().t(), 1)
+    p[torch.arange(T, device="cuda"), ids] = 0
+    p2 = (p * g.double()[:, None]) ** 2
+    others_h = (p2 @ (w.detach().double() ** 2).sum(1)).sum().sqrt().item()
+    others_w = (p2.sum(1) @ (h.detach().double() ** 2).sum(1)).sqrt().item()
+    for got, want, others in ((dh, rdh, others_h), (dw, rdw, others_w)):
+        once = _err(want.bfloat16(), want)
+        assert _err(got, want) <= 1.05 * once + 3 * 2.0 ** -9 * others / want.norm().item()
+
+
+@pytest.mark.parametrize("blocks", [1, 3])
+def test_lm_head_log_probs_of_tokens_that_repeat(blocks):
+    """One id for all rows, few ids, and ids in runs: the head's gradient adds them up, in the same bits every time."""
+    from parallel_b200.ops import objectives as O
+
+    T, H, V = 3000, 136, 1003
+    h, w, _, g = _head_inputs(T, H, V, ignored=0.0, seed=61)
+    gen = torch.Generator(device="cuda").manual_seed(62)
+    for ids in (torch.full((T,), 7, device="cuda"), torch.randint(0, 3, (T,), device="cuda", generator=gen),
+                torch.arange(T, device="cuda") // 40):
+        ids = ids.masked_fill(torch.rand(T, device="cuda", generator=gen) < 0.1, -1)
+        out = []
+        for _ in range(2):
+            hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+            logp = O.lm_head_log_probs(hg, wg, ids, max_block_bytes=(6 << 30) if blocks == 1 else 2 * V * 1024)
+            out.append(torch.autograd.grad(logp, (hg, wg), g))
+        _synced()
+        _, rdh, rdw, _ = _head_reference(h, w, ids, g, 1.0)
+        assert _err(out[0][0], rdh) <= GRAD_TOL and _err(out[0][1], rdw) <= GRAD_TOL
+        assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
 def test_rows_that_share_memory_and_an_empty_vocabulary():
     """Broadcast and overlapping hidden states and heads are read as what they stand for; no vocabulary is refused."""
     from parallel_b200.ops import objectives as O

@@ -658,9 +658,12 @@ __global__ void __launch_bounds__(128)
 // dw[ids[t]] += own[t] h[t] over the rows that have a token: a block a row, in
 // which the first row of an id adds up all rows of that id (in the same order on
 // every run) and the others leave.  Each block looks through all ids, which stay
-// in L1: 6554 rows of 8192, H 1024: 38 us.
+// in L1, and the loads of a frequent id's rows go out eight at a time (8192 rows
+// of H 1024, 7500 ids: 55 us; one id for all rows, the worst: 708 us, 2065 one
+// at a time).
 constexpr int kOwnWarps = 4;
 constexpr int kOwnList = 512;
+constexpr int kOwnAhead = 8;  // rows in flight
 template <typename E>
 __global__ void __launch_bounds__(32 * kOwnWarps)
     logprob_own_kernel(const __nv_bfloat16* __restrict__ h, const int64_t* __restrict__ ids,
@@ -701,10 +704,23 @@ __global__ void __launch_bounds__(32 * kOwnWarps)
       float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       for (int w = 0; w < kOwnWarps; ++w) {
         const int rows = found[w];
-#pragma unroll 4
-        for (int j = 0; j < rows; ++j) {
-          const int r = list[w][j];
+        if (rows == 1) {  // mostly
+          const int r = list[w][0];
           add_scaled(a, *reinterpret_cast<const uint4*>(h + (int64_t)r * H + col), own[r]);
+          continue;
+        }
+        // the last rows again, times 0, where they do not fill a group
+        for (int j = 0; j < rows; j += kOwnAhead) {
+          uint4 x[kOwnAhead];
+          float f[kOwnAhead];
+#pragma unroll
+          for (int q = 0; q < kOwnAhead; ++q) {
+            const int r = list[w][min(j + q, rows - 1)];
+            x[q] = *reinterpret_cast<const uint4*>(h + (int64_t)r * H + col);
+            f[q] = j + q < rows ? own[r] : 0.f;
+          }
+#pragma unroll
+          for (int q = 0; q < kOwnAhead; ++q) add_scaled(a, x[q], f[q]);
         }
       }
       E* d = dw + id * H + col;

@@ -244,14 +244,14 @@ std::vector<c10::optional<at::Tensor>> policy_fwd(const at::Tensor& logp, const 
   p.S = (int)S;
   p.chunk = c.chunk;
   p.nchunk = c.n;
-  p.low = (float)low;
-  p.high = (float)high;
-  p.kl_coef = (float)kl_coef;
+  p.low = low;
+  p.high = high;
+  p.kl_coef = kl_coef;
   p.per_sequence = per_sequence;
   const auto f32 = logp.options();
   at::Tensor loss = at::empty({}, f32), clip = at::empty({}, f32), kl = at::empty({}, f32);
-  // scratch: 4 floats per chunk, then the ticket
-  at::Tensor scratch = at::empty({B * c.n * 4 + 1}, f32);
+  // scratch: a PolicyPart per chunk, then the ticket
+  at::Tensor scratch = at::empty({B * c.n * 8 + 1}, f32);
   at::Tensor inv = at::empty({1}, f32);
   c10::optional<at::Tensor> coef, inv_row;
   if (want_grad) coef = at::empty({B, S}, f32);
@@ -262,8 +262,9 @@ std::vector<c10::optional<at::Tensor>> policy_fwd(const at::Tensor& logp, const 
   p.loss = loss.data_ptr<float>();
   p.clip = clip.data_ptr<float>();
   p.kl = kl.data_ptr<float>();
-  p.parts = reinterpret_cast<float4*>(scratch.data_ptr<float>());
-  p.ticket = reinterpret_cast<int*>(scratch.data_ptr<float>() + B * c.n * 4);
+  static_assert(sizeof(pb::PolicyPart) == 32, "scratch of policy_fwd");
+  p.parts = reinterpret_cast<pb::PolicyPart*>(scratch.data_ptr<float>());
+  p.ticket = reinterpret_cast<int*>(scratch.data_ptr<float>() + B * c.n * 8);
   pb::policy_fwd(p, cur_stream());
   return {loss, clip, kl, coef, inv, inv_row};
 }
@@ -309,14 +310,14 @@ std::vector<at::Tensor> preference_fwd(const at::Tensor& logp, const c10::option
   p.S = (int)S;
   p.chunk = c.chunk;
   p.nchunk = c.n;
-  p.beta = (float)beta;
-  p.smoothing = (float)smoothing;
+  p.beta = beta;
+  p.smoothing = smoothing;
   p.average = average;
   const auto f32 = logp.options();
   at::Tensor loss = at::empty({}, f32), rewards = at::empty({B}, f32), coef = at::empty({B}, f32);
-  at::Tensor scratch = at::empty({B * c.n * 2 + 1}, f32);
-  p.parts = reinterpret_cast<float2*>(scratch.data_ptr<float>());
-  p.ticket = reinterpret_cast<int*>(scratch.data_ptr<float>() + B * c.n * 2);
+  at::Tensor scratch = at::empty({B * c.n * 4 + 1}, f32);
+  p.parts = reinterpret_cast<double2*>(scratch.data_ptr<float>());
+  p.ticket = reinterpret_cast<int*>(scratch.data_ptr<float>() + B * c.n * 4);
   p.loss = loss.data_ptr<float>();
   p.rewards = rewards.data_ptr<float>();
   p.coef = coef.data_ptr<float>();

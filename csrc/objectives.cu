@@ -1,14 +1,17 @@
 // Losses over token log-probabilities [B, S] (fp32): the clipped policy loss
 // with a KL term and the preference loss over pairs of sequences.
 //
-// Both are bound by latency up to some 100k tokens (one launch each way: 6 + 3
-// us on the GPU for 8 x 509 tokens, inside some 75 us of a call's host time) and
-// by memory far above (17 / 9 bytes read per token; 2M tokens: 21.5 + 3.6 us
-// for the policy loss, 16 + 3.4 for the preference loss).  A warp sums a chunk
+// Both are bound by latency up to some 100k tokens (one launch each way: 8.5 + 3
+// us on the GPU for 8 x 509 tokens, inside some 75 us of a call's host time), by
+// memory far above (17 / 9 bytes read per token; 2M tokens: 18 + 3.4 us for the
+// preference loss) and the policy loss there by its exponentials (32 + 3.6 us).  A warp sums a chunk
 // of one row and writes the chunk's partial sums, and the last block to finish
-// adds the partials in chunk order (fp64), so the results have the same bits on
-// every run.  What stands outside the mask is dropped by selection, never by a
-// product: it may be anything.
+// adds the partials in chunk order, so the results have the same bits on every
+// run.  Tokens are worked out and added in 64 bits: advantages of both signs
+// cancel, what is left is the loss, and in 32 bits it came out up to 14 times as
+// far off as a plain form's (4.9e-6 against 3.4e-7 of it).  Of 2M tokens that
+// takes 8 us on the GPU, which a call's host time covers.  What stands outside
+// the mask is dropped by selection, never by a product: it may be anything.
 #include <math.h>
 
 #include <algorithm>
@@ -24,7 +27,7 @@ constexpr int kWarps = 8;          // per block when there are many units
 constexpr int kAhead = 4;          // tokens a lane loads before it uses the first
 constexpr int kOneBlockUnits = 32;  // up to this many units one block does it all, without a ticket
 
-__device__ __forceinline__ float warp_add(float v) {
+__device__ __forceinline__ double warp_add(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -82,7 +85,8 @@ __global__ void __launch_bounds__(1024) policy_fwd_kernel(const PolicyParams p) 
     const float* ref = p.ref ? p.ref + b * p.ld_ref : nullptr;
     const float* adv = p.adv + b * p.adv_sb;
     const uint8_t* mask = p.mask ? p.mask + b * p.ld_mask : nullptr;
-    float loss = 0.f, n = 0.f, clip = 0.f, kl = 0.f;
+    double loss = 0.0, kl = 0.0;
+    int n = 0, clip = 0;
     // kAhead tokens a lane at a time: all their loads first, whatever the mask says
     // (what is outside it is dropped), then the arithmetic
     for (int64_t sb = s0 + lane; sb < s1; sb += 32 * kAhead) {
@@ -103,52 +107,57 @@ __global__ void __launch_bounds__(1024) policy_fwd_kernel(const PolicyParams p) 
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const float r = expf(l[j] - o[j]);
-        const float u = r * a[j];
-        const float c = fminf(fmaxf(r, p.low), p.high) * a[j];
+        const double r = exp((double)l[j] - (double)o[j]);
+        const double u = r * (double)a[j];
+        const double c = fmin(fmax(r, p.low), p.high) * (double)a[j];
         const bool clipped = u > c;  // false for NaN: u carries it on
-        float per = clipped ? -c : -u, coef = clipped ? 0.f : -u;
+        double per = clipped ? -c : -u, coef = clipped ? 0.0 : -u;
         if (ref) {
-          const float x = rl[j] - l[j];
-          const float e = expm1f(x), k = e - x;  // exp(x) - 1 - x without the cancellation at small x
+          const double x = (double)rl[j] - (double)l[j];
+          const double e = expm1(x), k = e - x;  // exp(x) - 1 - x without the cancellation at small x
           per += p.kl_coef * k;
           coef -= p.kl_coef * e;
-          kl += on[j] ? k : 0.f;
+          kl += on[j] ? k : 0.0;
         }
-        loss += on[j] ? per : 0.f;
-        n += on[j] ? 1.f : 0.f;
-        clip += on[j] && clipped ? 1.f : 0.f;
+        loss += on[j] ? per : 0.0;
+        n += on[j] ? 1 : 0;
+        clip += on[j] && clipped ? 1 : 0;
         const int64_t s = sb + 32 * j;
-        if (p.coef && s < s1) p.coef[b * p.S + s] = on[j] ? coef : 0.f;
+        if (p.coef && s < s1) p.coef[b * p.S + s] = on[j] ? (float)coef : 0.f;
       }
     }
     loss = warp_add(loss);
-    n = warp_add(n);
-    clip = warp_add(clip);
+    n = __reduce_add_sync(0xffffffffu, n);
+    clip = __reduce_add_sync(0xffffffffu, clip);
     kl = warp_add(kl);
-    if (lane == 0) p.parts[unit] = make_float4(loss, n, clip, kl);
+    if (lane == 0) {
+      p.parts[unit].sums = make_double2(loss, kl);
+      p.parts[unit].counts = make_int2(n, clip);
+    }
   }
   if (!last_block(p.ticket)) return;
   __shared__ double sh[32][5];
   double v[5] = {0.0, 0.0, 0.0, 0.0, 0.0};  // loss, tokens, clipped, kl, rows with a token
   if (!p.per_sequence) {
     for (int64_t i = threadIdx.x; i < units; i += blockDim.x) {
-      const float4 q = __ldcg(p.parts + i);
+      const double2 q = __ldcg(&p.parts[i].sums);
+      const int2 k = __ldcg(&p.parts[i].counts);
       v[0] += q.x;
-      v[1] += q.y;
-      v[2] += q.z;
-      v[3] += q.w;
+      v[1] += k.x;
+      v[2] += k.y;
+      v[3] += q.y;
     }
   } else {
     for (int64_t b = threadIdx.x; b < p.B; b += blockDim.x) {
       double row = 0.0, rn = 0.0;
 #pragma unroll 8
       for (int c = 0; c < p.nchunk; ++c) {
-        const float4 q = __ldcg(p.parts + b * p.nchunk + c);
+        const double2 q = __ldcg(&p.parts[b * p.nchunk + c].sums);
+        const int2 k = __ldcg(&p.parts[b * p.nchunk + c].counts);
         row += q.x;
-        rn += q.y;
-        v[2] += q.z;
-        v[3] += q.w;
+        rn += k.x;
+        v[2] += k.y;
+        v[3] += q.y;
       }
       if (rn > 0.0) {
         v[0] += row / rn;
@@ -200,7 +209,8 @@ __global__ void __launch_bounds__(1024) preference_fwd_kernel(const PreferencePa
     const float* lp = p.logp + b * p.ld_logp;
     const float* ref = p.ref ? p.ref + b * p.ld_ref : nullptr;
     const uint8_t* mask = p.mask ? p.mask + b * p.ld_mask : nullptr;
-    float d = 0.f, n = 0.f;
+    double d = 0.0;
+    int n = 0;
     for (int64_t sb = s0 + lane; sb < s1; sb += 32 * kAhead) {
       float l[kAhead], r[kAhead];
       bool on[kAhead];
@@ -217,13 +227,13 @@ __global__ void __launch_bounds__(1024) preference_fwd_kernel(const PreferencePa
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        d += on[j] ? l[j] - r[j] : 0.f;
-        n += on[j] ? 1.f : 0.f;
+        d += on[j] ? (double)l[j] - (double)r[j] : 0.0;
+        n += on[j] ? 1 : 0;
       }
     }
     d = warp_add(d);
-    n = warp_add(n);
-    if (lane == 0) p.parts[unit] = make_float2(d, n);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) p.parts[unit] = make_double2(d, (double)n);
   }
   if (!last_block(p.ticket)) return;
   __shared__ double sh[32][1];
@@ -236,26 +246,25 @@ __global__ void __launch_bounds__(1024) preference_fwd_kernel(const PreferencePa
       double d = 0.0, n = 0.0;
 #pragma unroll 8
       for (int c = 0; c < p.nchunk; ++c) {
-        const float2 v = __ldcg(p.parts + b * p.nchunk + c);
+        const double2 v = __ldcg(p.parts + b * p.nchunk + c);
         d += v.x;
         n += v.y;
       }
-      w[k] = (double)p.beta / (p.average ? fmax(n, 1.0) : 1.0);
+      w[k] = p.beta / (p.average ? fmax(n, 1.0) : 1.0);
       r[k] = w[k] * d;
       p.rewards[b] = (float)r[k];
     }
-    const float gap = (float)(r[0] - r[1]);
-    const float soft = log1pf(expf(-fabsf(gap)));  // -log sigmoid(x) = soft + max(-x, 0)
-    const float neg = gap < 0.f ? -gap : 0.f, pos = gap > 0.f ? gap : 0.f;
-    const float e = p.smoothing;
-    loss[0] += (double)((1.f - e) * (soft + neg) + e * (soft + pos));
+    const double gap = r[0] - r[1];
+    const double t = exp(-fabs(gap)), soft = log1p(t);  // -log sigmoid(x) = soft + max(-x, 0)
+    const double neg = gap < 0.0 ? -gap : 0.0, pos = gap > 0.0 ? gap : 0.0;
+    const double e = p.smoothing;
+    loss[0] += (1.0 - e) * (soft + neg) + e * (soft + pos);
     // sigmoid(-gap) and sigmoid(gap), each without cancellation
-    const float t = expf(-fabsf(gap));
-    const float small = t / (1.f + t), big = 1.f / (1.f + t);
-    const float s_neg = gap >= 0.f ? small : big, s_pos = gap >= 0.f ? big : small;
-    const float dgap = (e * s_pos - (1.f - e) * s_neg) / (float)p.P;
-    p.coef[i] = (float)(w[0] * (double)dgap);
-    p.coef[i + p.P] = (float)(-w[1] * (double)dgap);
+    const double small = t / (1.0 + t), big = 1.0 / (1.0 + t);
+    const double s_neg = gap >= 0.0 ? small : big, s_pos = gap >= 0.0 ? big : small;
+    const double dgap = (e * s_pos - (1.0 - e) * s_neg) / (double)p.P;
+    p.coef[i] = (float)(w[0] * dgap);
+    p.coef[i + p.P] = (float)(-w[1] * dgap);
   }
   block_add(loss, sh);
   if (threadIdx.x == 0) p.loss[0] = (float)(loss[0] / (double)p.P);
@@ -284,7 +293,8 @@ int unit_blocks(int64_t units) { return (int)((units + kWarps - 1) / kWarps); }
 // Tokens of a row that one warp sums: the longest that still gives each SM 16
 // warps, whose loads hide one another's latency, while the last block has few
 // partials to add (policy forward, 512 x 4096, inputs not in L2: 32.7 us with
-// 1024 tokens a warp, 21.5 with 512, 24.7 with 256).
+// 1024 tokens a warp, 21.5 with 512, 24.7 with 256, with the
+// arithmetic in 32 bits).
 int objective_chunk(int64_t rows, int64_t S) {
   int chunk = 1024;
   while (chunk > 128 && rows * ((S + chunk - 1) / chunk) < (int64_t)16 * num_sms()) chunk /= 2;

@@ -59,15 +59,20 @@ void logprob_own(const void* h, const int64_t* ids, const float* own, const int*
 // own strides, mask is bool bytes (optional).  chunk: objective_chunk(rows, S),
 // nchunk = max(1, ceil(S / chunk)); parts and ticket are scratch.
 int objective_chunk(int64_t rows, int64_t S);
+struct PolicyPart {
+  double2 sums;  // loss, kl
+  int2 counts;   // tokens, clipped tokens
+  int2 pad;      // to 32 bytes
+};
 struct PolicyParams {
   const float *logp, *old, *adv, *ref;  // ref optional
   const uint8_t* mask;
   int64_t ld_logp, ld_old, adv_sb, adv_ss, ld_ref, ld_mask;
   int B, S, chunk, nchunk;
-  float low, high, kl_coef;  // the clip range [low, high] of the ratio
+  double low, high, kl_coef;  // the clip range [low, high] of the ratio
   bool per_sequence;         // mean over rows of the row means, else mean over tokens
   float* coef;               // optional [B, S]: d (token loss) / d logp, 0 outside the mask
-  float4* parts;             // [B * nchunk]
+  PolicyPart* parts;         // [B * nchunk]
   int* ticket;
   float *loss, *clip, *kl;  // scalars
   float *inv, *inv_row;     // gradient = coef * inv (* inv_row [B] when per_sequence)
@@ -82,9 +87,9 @@ struct PreferenceParams {
   const uint8_t* mask;
   int64_t ld_logp, ld_ref, ld_mask;
   int P, S, chunk, nchunk;
-  float beta, smoothing;
+  double beta, smoothing;
   bool average;
-  float2* parts;  // [2P * nchunk]
+  double2* parts;  // [2P * nchunk]: sum, tokens
   int* ticket;
   float *loss, *rewards, *coef;  // scalar, [2P], [2P]: d loss / d (logp of a token of the row)
 };

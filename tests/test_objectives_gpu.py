@@ -265,7 +265,8 @@ def _policy_reference(logp, old, ref, adv, mask, per_sequence):
     lp, o, a = clean(logp), clean(old), clean(adv.expand_as(logp))
     r = (lp - o).exp()
     past = ((a > 0) & (r > 1 + HIGH)) | ((a < 0) & (r < 1 - LOW))
-    per = -torch.where(past, torch.where(a > 0, 1 + HIGH, 1 - LOW) * a, r * a)
+    edge = torch.where(a > 0, torch.full_like(a, 1 + HIGH), torch.full_like(a, 1 - LOW))
+    per = -torch.where(past, edge * a, r * a)
     grad, scale, kl = torch.where(past, 0.0, -r * a), (r * a).abs(), torch.zeros_like(lp)
     if ref is not None:
         x = clean(ref) - lp
@@ -459,6 +460,27 @@ def test_policy_and_preference_gradients_against_differences():
                     fd = (fn(logp + d).double() - fn(logp - d).double()).item() / (2 * eps)
                 # loss of order 1 in fp32 over 2 eps, and eps^2 / 6 times a third derivative of order 1
                 assert abs(fd - grad[b, s].item()) <= 8 * F32 / (2 * eps) * 8 + eps ** 2
+
+
+@pytest.mark.parametrize("B,S", [(2, 1), (8, 2), (4, 185), (30, 2000), (300, 333)])
+def test_policy_and_preference_losses_are_rounded_once(B, S):
+    """Losses, KL and rewards are sums that cancel, worked out in 64 bits and rounded to fp32 at the end."""
+    from parallel_b200.ops import objectives as O
+
+    for seed in range(4):
+        for masked in (False, True):
+            logp, old, ref, adv, mask = _token_inputs(B, S, seed=200 + seed, masked=masked)
+            for reduction in ("token", "sequence"):
+                out = O.policy_loss(logp, old, adv, mask=mask, ref_logp=ref, clip_low=LOW, clip_high=HIGH, kl_coef=KL,
+                                    reduction=reduction)
+                loss, _, kl, _, _, size = _policy_reference(logp, old, ref, adv, mask, reduction == "sequence")
+                assert abs(out.loss.item() - loss.item()) <= F32 * abs(loss.item()) + 1e-13 * size.item()
+                assert abs(out.kl.item() - kl.item()) <= F32 * kl.item() + 1e-13 * (1 + kl.item())
+            out = O.preference_loss(logp, ref_logp=ref, mask=mask, beta=0.1, label_smoothing=0.1)
+            loss, rewards, _, size = _preference_reference(logp, ref, mask, 0.1, 0.1, False)
+            assert ((out.rewards.double() - rewards).abs() <= F32 * rewards.abs() + 1e-13 * size).all()
+            assert abs(out.loss.item() - loss.item()) <= F32 * loss.item() + 1e-13 * (1 + size.max().item())
+    _synced()
 
 
 # ----------------------------------------------------------------- distillation

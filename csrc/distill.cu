@@ -260,6 +260,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const Dist
     if (tid == 0) p.row_loss[tg * C + rank] = 0.f;
     return;
   }
+  // A CTA's shared memory may be written by its peers once it has started: this
+  // barrier says that all have.  Its wait stands before the first such write,
+  // behind the first pass; the returns above are taken by whole clusters.
+  if (C > 1) cluster_arrive();
 
   // The teacher's entries in this CTA's columns (the others' ids become -1) and
   // the student's logits there, before a gradient may take their place.
@@ -329,6 +333,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const Dist
       if (lane == 0) stat[warp] = make_float2(mw, sw);
       __syncthreads();
     } else {
+      cluster_wait();
       if (lane < C) st_cluster_f2(&stat[rank * WARPS + warp], lane, make_float2(mw, sw));
       cluster_sync();
     }

@@ -1,9 +1,42 @@
 """Post-training objectives on CPU: the plain formulas and the refusals."""
+import os
+import re
+
 import pytest
 import torch
 
 from parallel_b200.ops import objectives as O
 
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc")
+
+
+def _kernels():
+    """(file, name, body without comments) of every kernel in csrc."""
+    for name in sorted(os.listdir(CSRC)):
+        if not name.endswith((".cu", ".cuh")):
+            continue
+        with open(os.path.join(CSRC, name)) as f:
+            src = re.sub(r"//[^\n]*", "", f.read())
+        for m in re.finditer(r"__global__ void\s+(?:__launch_bounds__\([^)]*\)\s*)?(\w+)\s*\([^;{]*\)\s*\{", src):
+            depth, end = 1, m.end()
+            while depth:
+                depth += {"{": 1, "}": -1}.get(src[end], 0)
+                end += 1
+            yield name, m.group(1), src[m.end():end]
+
+
+def test_peers_of_a_cluster_have_started_before_their_shared_memory_is_addressed():
+    """A CTA may write a peer's shared memory only once the peer has started, which a cluster barrier tells: its wait
+    stands before the first such access in every kernel."""
+    seen = 0
+    for file, kernel, body in _kernels():
+        remote = re.search(r"\b(st_cluster_\w+|mapa_shared)\(", body)
+        if remote is None:
+            continue
+        seen += 1
+        barrier = re.search(r"\b(cluster_sync|cluster_wait)\(\)", body)
+        assert barrier is not None and barrier.start() < remote.start(), f"{file}: {kernel}"
+    assert seen >= 3
 
 
 

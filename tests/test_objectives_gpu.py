@@ -578,6 +578,31 @@ def test_distillation_loss_row_strides_and_alignments(dtype):
     assert torch.equal(turned, first)
 
 
+@pytest.mark.parametrize("T,V", [(3, 262144), (17, 151936), (74, 65536), (148, 32768)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_of_few_rows_on_a_busy_gpu(T, V, dtype):
+    """Rows shared by a cluster of CTAs while another stream's kernels take and free the SMs, so that clusters start
+    at all times: the bits of a quiet GPU, every time."""
+    from parallel_b200.ops import objectives as O
+
+    logits, top, ids, mask = _teacher_inputs(T, V, 5, dtype, seed=T)
+    x = logits.requires_grad_(True)
+    first = O.distillation_loss(x, top, ids, mask=mask)
+    want = (first.detach(), torch.autograd.grad(first, x)[0])
+    other, busy = torch.cuda.Stream(), torch.randn(1 << 22, device="cuda")
+    other.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i in range(20):
+        with torch.cuda.stream(other):
+            for k in range(4):
+                busy = busy[: (1 << 22) - 4096 * ((i + k) % 7)].sin().repeat(2)[: 1 << 22]
+        loss = O.distillation_loss(x, top, ids, mask=mask)
+        got.append((loss.detach(), torch.autograd.grad(loss, x)[0]))
+    torch.cuda.current_stream().wait_stream(other)
+    _synced()
+    assert all(torch.equal(a, b) for pair in got for a, b in zip(pair, want))
+
+
 def test_distillation_loss_against_differences():
     from parallel_b200.ops import objectives as O
 

@@ -16,7 +16,9 @@
 //   logprob_unpack, logprob_own add the target's part of the gradients of h and
 //                   w, c (1 - p) w_id and c (1 - p) h, in fp32: it is most of
 //                   them, and as one more bf16 factor its rounding, the same in
-//                   a whole row of the product, would add up to 2^-9 of it.
+//                   a whole row of the product, would add up to 2^-9 of it.  Where
+//                   dw is bf16 a target's row was rounded once by the product (the
+//                   others' part, the smaller one) and is once more with its own.
 //
 // Maxima are kept as they come from the tensor core, unscaled, and only
 // differences of them are scaled, so no digit of an exponent is lost however
@@ -657,15 +659,42 @@ __global__ void __launch_bounds__(128)
 
 // dw[ids[t]] += own[t] h[t] over the rows that have a token: a block a row, in
 // which the first row of an id adds up all rows of that id (in the same order on
-// every run) and the others leave.  Each block looks through all ids, which stay
-// in L1, and the loads of a frequent id's rows go out eight at a time (8192 rows
-// of H 1024, 7500 ids: 55 us; one id for all rows, the worst: 708 us, 2065 one
-// at a time).
+// every run) and the others leave.  The sum of all of an id's rows is kept in fp32
+// and meets dw once.  Each block looks through all ids, so the time grows with
+// the square of the rows; up to 8192 rows the ids stay in L1 and the loads of a
+// frequent id's rows, which go out eight at a time, take longer (8192 rows of H
+// 1024, 7500 ids: 56 us; one id for all rows, the worst: 703 us, 2065 one at a
+// time).  64 registers: with more, fewer blocks look through the ids at a time (77:
+// 63 and 582 us).
 constexpr int kOwnWarps = 4;
 constexpr int kOwnList = 512;
 constexpr int kOwnAhead = 8;  // rows in flight
+// v += own[r] h[r] for the listed rows r, in order, eight columns of them
+__device__ __forceinline__ void add_rows(float* v, const __nv_bfloat16* __restrict__ h, int H,
+                                         const float* __restrict__ own, const int* list, int rows) {
+  if (rows == 1) {  // mostly
+    const int r = list[0];
+    add_scaled(v, *reinterpret_cast<const uint4*>(h + (int64_t)r * H), own[r]);
+    return;
+  }
+  // the last rows again, times 0, where they do not fill a group
+#pragma unroll 1
+  for (int j = 0; j < rows; j += kOwnAhead) {
+    uint4 x[kOwnAhead];
+    float f[kOwnAhead];
+#pragma unroll
+    for (int q = 0; q < kOwnAhead; ++q) {
+      const int r = list[min(j + q, rows - 1)];
+      x[q] = *reinterpret_cast<const uint4*>(h + (int64_t)r * H);
+      f[q] = j + q < rows ? own[r] : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < kOwnAhead; ++q) add_scaled(v, x[q], f[q]);
+  }
+}
+
 template <typename E>
-__global__ void __launch_bounds__(32 * kOwnWarps)
+__global__ void __launch_bounds__(32 * kOwnWarps, 8)
     logprob_own_kernel(const __nv_bfloat16* __restrict__ h, const int64_t* __restrict__ ids,
                        const float* __restrict__ own, const int* __restrict__ count, int row0, int T, int V, int H,
                        E* __restrict__ dw) {
@@ -682,9 +711,10 @@ __global__ void __launch_bounds__(32 * kOwnWarps)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // each warp looks through a quarter of the rows from t on, 256 at a time
   const int per = (n - t + kOwnWarps - 1) / kOwnWarps;
-  int i = t + warp * per;
-  const int end = min(n, i + per);
-  for (;;) {
+  const int first = t + warp * per, end = min(n, first + per);
+  int i = first;
+  // the next rows of the id, up to kOwnList a warp; true if there may be more
+  auto refill = [&] {
     int m = 0;
     while (i < end && m <= kOwnList - 256) {
       int64_t v[8];
@@ -699,30 +729,22 @@ __global__ void __launch_bounds__(32 * kOwnWarps)
       i += 256;
     }
     if (lane == 0) found[warp] = m;
-    const bool more = __syncthreads_or(i < end);
-    for (int col = threadIdx.x * 8; col < H; col += 32 * kOwnWarps * 8) {
-      float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int w = 0; w < kOwnWarps; ++w) {
-        const int rows = found[w];
-        if (rows == 1) {  // mostly
-          const int r = list[w][0];
-          add_scaled(a, *reinterpret_cast<const uint4*>(h + (int64_t)r * H + col), own[r]);
-          continue;
-        }
-        // the last rows again, times 0, where they do not fill a group
-        for (int j = 0; j < rows; j += kOwnAhead) {
-          uint4 x[kOwnAhead];
-          float f[kOwnAhead];
-#pragma unroll
-          for (int q = 0; q < kOwnAhead; ++q) {
-            const int r = list[w][min(j + q, rows - 1)];
-            x[q] = *reinterpret_cast<const uint4*>(h + (int64_t)r * H + col);
-            f[q] = j + q < rows ? own[r] : 0.f;
-          }
-#pragma unroll
-          for (int q = 0; q < kOwnAhead; ++q) add_scaled(a, x[q], f[q]);
-        }
+    return (bool)__syncthreads_or(i < end);
+  };
+  bool more = refill();
+  const bool one_list = !more;
+  for (int c0 = 0;;) {
+    const int col = c0 + threadIdx.x * 8;
+    float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (;;) {
+      if (col < H) {
+        for (int w = 0; w < kOwnWarps; ++w) add_rows(a, h + col, H, own, list[w], found[w]);
       }
+      if (!more) break;
+      __syncthreads();  // the list is free again
+      more = refill();
+    }
+    if (col < H) {
       E* d = dw + id * H + col;
       if constexpr (sizeof(E) == 2) {
         uint4 u = *reinterpret_cast<uint4*>(d);
@@ -734,8 +756,13 @@ __global__ void __launch_bounds__(32 * kOwnWarps)
         for (int q = 0; q < 8; ++q) d[q] += a[q];
       }
     }
-    if (!more) return;
-    __syncthreads();  // the list is free again
+    c0 += 32 * kOwnWarps * 8;
+    if (c0 >= H) return;
+    if (!one_list) {  // from the first rows again for the next columns
+      __syncthreads();
+      i = first;
+      more = refill();
+    }
   }
 }
 

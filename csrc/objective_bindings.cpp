@@ -611,7 +611,8 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
     const at::Tensor g = grads[0].contiguous();
     at::Tensor dh, dw;
     if (ctx->needs_input_grad(0)) dh = at::empty({T, H}, hp.options());
-    // one row block: the head's gradient is rounded once by its product; several add up in fp32 first
+    // one row block: the head's gradient is rounded by its product, and the rows of targets again with the target's
+    // part (an fp32 product would be twice the stores, and one more pass); several blocks add up in fp32 first
     if (ctx->needs_input_grad(1)) dw = at::empty({V, H}, block >= T ? w.options() : w.options().dtype(at::kFloat));
     at::Tensor e = kept[0], stats = kept[1];
     for (int64_t r0 = 0, i = 2; r0 < T; r0 += block, ++i) {

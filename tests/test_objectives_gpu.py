@@ -865,6 +865,22 @@ def test_lm_head_log_probs_of_tokens_that_repeat(blocks):
         assert all(torch.equal(a, b) for a, b in zip(*out))
 
 
+@pytest.mark.parametrize("T,H", [(16384, 64), (9000, 2056)])
+def test_lm_head_gradient_of_one_token_in_many_rows_is_rounded_once(T, H):
+    """All rows have one token and weights of both signs.  The product has nothing to add to that token's row of the
+    head's gradient, so the row is a sum in fp32 (off by about sqrt(T) 2^-24 of itself) and one rounding."""
+    from parallel_b200.ops import objectives as O
+
+    V = 300
+    h, w, _, g = _head_inputs(T, H, V, ignored=0.0, seed=71)
+    ids = torch.full((T,), 7, device="cuda")
+    wg = w.clone().requires_grad_(True)
+    (dw,) = torch.autograd.grad(O.lm_head_log_probs(h, wg, ids), wg, g)
+    _synced()
+    want = _head_reference(h, w, ids, g, 1.0)[2][7]
+    assert _err(dw[7], want) <= 1.05 * _err(want.bfloat16(), want)
+
+
 def test_rows_that_share_memory_and_an_empty_vocabulary():
     """Broadcast and overlapping hidden states and heads are read as what they stand for; no vocabulary is refused."""
     from parallel_b200.ops import objectives as O

@@ -9,6 +9,12 @@
 //                 two passes: running maximum and sum, then the gradient.
 //   distill_loss  the row losses, added in a fixed order.
 //
+// The gradient is written in the forward pass, for a loss that counts once.
+// Where the backward brings another weight, distill_rows runs again with it: a
+// bf16 gradient multiplied afterwards would be rounded twice, and reading it takes
+// as long as reading the logits (8192 x 151936 bf16: 935 us in the forward, 2 more
+// for a weight of 1, 1100 for another).
+//
 // What bounds it: one read and one write of each logit in HBM.  A row of
 // 151,936 bf16 logits is 304 KB, more than an SM's shared memory, so the second
 // pass reads it again, from L2: 2 CTAs on each of 148 SMs hold at most 90 MB of
@@ -164,9 +170,9 @@ struct Vec<__nv_bfloat16> {
       s[q] += ex2(exponent<NEAR>(__uint_as_float(w[q] & 0xffff0000u), ref, k2, c));
     }
   }
-  // f exp((l - ref) / tau), lf = log2(f) inside the exponent
+  // f exp((l - ref) / tau), lf = log2(|f|) inside the exponent, flip the signs of a pair where f < 0
   template <bool NEAR>
-  static __device__ __forceinline__ uint4 grad(const uint4& u, float ref, float k2, float, float lf) {
+  static __device__ __forceinline__ uint4 grad(const uint4& u, float ref, float k2, float, float lf, uint32_t flip) {
     const float c = NEAR ? fmaf(-ref, k2, lf) : lf;
     const uint32_t* w = &u.x;
     uint4 g;
@@ -174,7 +180,7 @@ struct Vec<__nv_bfloat16> {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       o[q] = pack_bf16x2(ex2(exponent<NEAR>(__uint_as_float(w[q] << 16), ref, k2, c)),
-                         ex2(exponent<NEAR>(__uint_as_float(w[q] & 0xffff0000u), ref, k2, c)));
+                         ex2(exponent<NEAR>(__uint_as_float(w[q] & 0xffff0000u), ref, k2, c))) ^ flip;
     return g;
   }
 };
@@ -196,7 +202,7 @@ struct Vec<float> {
     for (int q = 0; q < 4; ++q) s[q] += ex2((__uint_as_float(w[q]) - ref) * k2);
   }
   template <bool>
-  static __device__ __forceinline__ uint4 grad(const uint4& u, float ref, float k2, float f, float) {
+  static __device__ __forceinline__ uint4 grad(const uint4& u, float ref, float k2, float f, float, uint32_t) {
     const uint32_t* w = &u.x;
     uint4 g;
     uint32_t* o = &g.x;
@@ -209,12 +215,11 @@ struct Vec<float> {
 constexpr int kRowThreads = 512;
 constexpr int kUnroll = 4;  // vectors a thread has in flight
 
-// Grid: a cluster of p.cluster CTAs per row.  A row may start at any element:
-// up to 16 bytes in front of and behind its aligned vectors are taken one by
-// one by the first CTA.
-template <typename E>
-__global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const DistillParams p) {
-  pdl_prologue();
+// A cluster of p.cluster CTAs takes a row, t of this block of logits.  A row may
+// start at any element: up to 16 bytes in front of and behind its aligned vectors
+// are taken one by one by the first CTA.
+template <typename E, bool WEIGHTED>
+__device__ __forceinline__ void distill_row(const DistillParams& p, int64_t t, float weight) {
   using VE = Vec<E>;
   constexpr int WARPS = kRowThreads / 32;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -227,7 +232,6 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const Dist
 
   const int C = p.cluster;
   const int rank = C == 1 ? 0 : (int)cluster_ctarank();
-  const int64_t t = blockIdx.x / C;  // row of this block of logits
   // Packed rows: those behind the last 64-deep step of a sum over the rows that
   // count are neither read nor written.
   if (p.perm && p.row0 + t >= (max(p.counters[0], (int)p.row0 + 1) + 63) / 64 * 64) {
@@ -350,18 +354,20 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const Dist
     total = warp_sum(a);
     if (m == -INFINITY) total = NAN;  // no finite logit
   }
-  const float sc = p.tau / (float)max(1, p.counters[0]);
+  const float sc = weight * p.tau / (float)max(1, p.counters[0]);
   const float f = sc / total;
 
   if (out) {  // second pass: the gradient of the softmax
-    const float lf = log2f(f);
+    const float lf = log2f(WEIGHTED ? fabsf(f) : f);
+    const uint32_t flip = WEIGHTED && f < 0.f ? 0x80008000u : 0u;
     const bool near = VE::near(m, k2);
     auto store = [&](const uint4* u, int i0) {
 #pragma unroll
       for (int j = 0; j < kUnroll; ++j)
         if (i0 + j * kRowThreads < nv)
           __stcs(vout + i0 + j * kRowThreads,
-                 near ? VE::template grad<true>(u[j], m, k2, f, lf) : VE::template grad<false>(u[j], m, k2, f, lf));
+                 near ? VE::template grad<true>(u[j], m, k2, f, lf, flip)
+                      : VE::template grad<false>(u[j], m, k2, f, lf, flip));
     };
     for (int i0 = tid; i0 < nv; i0 += 2 * kStep) {
       again(ub, i0 + kStep);
@@ -406,6 +412,26 @@ __global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const Dist
   }
 }
 
+template <typename E>
+__global__ void __launch_bounds__(kRowThreads, 2) distill_rows_kernel(const DistillParams p) {
+  pdl_prologue();
+  distill_row<E, false>(p, blockIdx.x / p.cluster, 1.f);
+}
+
+// The gradient again where its weight is not 1.  The CTAs that fit at once take
+// the rows in turn: most weights are 1, and as many CTAs as rows take 30 us to
+// start and leave (8192 rows).
+template <typename E>
+__global__ void __launch_bounds__(kRowThreads, 2) distill_weighted_kernel(const DistillParams p) {
+  pdl_prologue();
+  const float weight = *p.weight;
+  if (weight == 1.f) return;
+  for (int64_t t = blockIdx.x / p.cluster; t < p.T; t += gridDim.x / p.cluster) {
+    distill_row<E, true>(p, t, weight);
+    __syncthreads();  // shared memory is free for the next row (clusters have one row each)
+  }
+}
+
 // The mean of the row losses, added in a fixed order by one block.
 constexpr int kLossThreads = 1024;
 __global__ void __launch_bounds__(kLossThreads) distill_loss_kernel(const DistillParams p) {
@@ -435,7 +461,7 @@ __global__ void __launch_bounds__(256) scale_kernel(E* __restrict__ x, int64_t n
 
 template <typename E>
 void launch_rows(const DistillParams& p, cudaStream_t stream) {
-  auto kern = distill_rows_kernel<E>;
+  auto kern = p.weight ? distill_weighted_kernel<E> : distill_rows_kernel<E>;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -449,7 +475,8 @@ void launch_rows(const DistillParams& p, cudaStream_t stream) {
   cfg.blockDim = dim3(kRowThreads, 1, 1);
   cfg.dynamicSmemBytes = (size_t)p.Kp * 12;
   cfg.stream = stream;
-  cfg.gridDim = dim3((unsigned)p.T * p.cluster, 1, 1);
+  const unsigned rows = p.weight && p.cluster == 1 ? std::min(p.T, 2 * num_sms()) : p.T;
+  cfg.gridDim = dim3(rows * p.cluster, 1, 1);
   PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
@@ -475,7 +502,7 @@ void distill_rows(const DistillParams& p0, bool bf16, cudaStream_t stream) {
     launch_rows<__nv_bfloat16>(p, stream);
   else
     launch_rows<float>(p, stream);
-  if (p.row0 + p.T == p.T_all) launch_k(distill_loss_kernel, 1, kLossThreads, 0, stream, p);
+  if (p.loss && p.row0 + p.T == p.T_all) launch_k(distill_loss_kernel, 1, kLossThreads, 0, stream, p);
 }
 
 void objective_scale(void* x, int64_t n, bool bf16, const float* g, cudaStream_t stream) {

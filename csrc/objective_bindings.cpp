@@ -409,9 +409,11 @@ std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& id
 
 // distill_rows(logits [T, V], prep ([scratch, loss] of all T_all rows), T_all, K, row0, tau, grad [T, V] or None):
 // the losses of rows [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss; with perm,
-// row i of the logits is row perm[i] of the teacher's
+// row i of the logits is row perm[i] of the teacher's; with weight (a scalar), the gradient alone, times it, if it
+// is not 1
 void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep, int64_t T_all, int64_t K, int64_t row0,
-                  double tau, const c10::optional<at::Tensor>& grad, const int* perm = nullptr) {
+                  double tau, const c10::optional<at::Tensor>& grad, const int* perm = nullptr,
+                  const c10::optional<at::Tensor>& weight = c10::nullopt) {
   TORCH_CHECK(logits.is_cuda() && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat) &&
                   logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) <= 1),
               "distill: logits must be CUDA bf16 or fp32 [T, V] with unit inner stride");
@@ -427,6 +429,11 @@ void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep,
   pb::DistillParams p{};
   sc.fill(p, prep[0]);
   p.loss = check_rows_f32(prep[1], 1, "distill: loss");
+  if (given(weight)) {
+    CHECK_SAME_DEVICE(logits, *weight);
+    p.weight = check_rows_f32(*weight, 1, "distill: weight");
+    p.loss = nullptr;  // it was handed out
+  }
   const int64_t es = logits.element_size();
   p.logits = logits.data_ptr();
   p.ld = logits.stride(0);
@@ -452,16 +459,15 @@ void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep,
   pb::distill_rows(p, bf16, cur_stream());
 }
 
-// grad_like(logits [T, V]) -> (grad [T, V], its flat storage): a tensor that is misaligned as logits is in every
-// row, so that both are read and written in the same 16-byte vectors
-std::vector<at::Tensor> grad_like(const at::Tensor& logits) {
+// grad_like(logits [T, V]) -> grad [T, V]: a tensor that is misaligned as logits is in every row, so that both are read
+// and written in the same 16-byte vectors
+at::Tensor grad_like(const at::Tensor& logits) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "grad_like: CUDA [T, V]");
   const c10::cuda::CUDAGuard g(logits.device());
   const int64_t T = logits.size(0), V = logits.size(1), unit = 16 / logits.element_size();
   const int64_t shift = (int64_t)(reinterpret_cast<uintptr_t>(logits.data_ptr()) & 15) / logits.element_size();
   const int64_t ld = V + ((logits.stride(0) - V) % unit + unit) % unit;
-  at::Tensor flat = at::empty({shift + T * ld}, logits.options());
-  return {flat.as_strided({T, V}, {ld, 1}, shift), flat};
+  return at::empty({shift + T * ld}, logits.options()).as_strided({T, V}, {ld, 1}, shift);
 }
 
 // objective_scale(x flat, g scalar): x *= g unless g is 1
@@ -715,25 +721,30 @@ std::vector<at::Tensor> preference_loss(const at::Tensor& logp, const c10::optio
 }
 
 // The gradient is written in the forward pass, from the one read of the
-// logits, and scaled by the incoming gradient in the backward.
+// logits; the backward writes it again if it comes with another weight than 1.
 struct DistillationNode : public torch::autograd::Function<DistillationNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& top,
                             const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau) {
     const auto prep = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau);
-    const std::vector<at::Tensor> grad = grad_like(logits);
-    distill_rows(logits, prep, top.size(0), top.size(1), 0, tau, grad[0]);
+    const at::Tensor grad = grad_like(logits);
+    distill_rows(logits, prep, top.size(0), top.size(1), 0, tau, grad);
     // not save_for_backward: the backward hands the gradient out, it does not keep it
     ctx->saved_data["grad"] = grad;
+    ctx->saved_data["scratch"] = prep[0];
+    ctx->saved_data["K"] = top.size(1);
+    ctx->saved_data["tau"] = tau;
+    ctx->save_for_backward({logits});
     return prep[1];
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     check_first_order("distillation_loss");
     TORCH_CHECK(ctx->saved_data.count("grad"), "distillation_loss supports one backward pass per forward");
-    std::vector<at::Tensor> grad = ctx->saved_data["grad"].toTensorVector();
+    const at::Tensor logits = ctx->get_saved_variables()[0], grad = ctx->saved_data["grad"].toTensor();
     ctx->saved_data.erase("grad");
-    objective_scale(grad[1], g[0]);
+    distill_rows(logits, {ctx->saved_data["scratch"].toTensor(), g[0]}, logits.size(0), ctx->saved_data["K"].toInt(), 0,
+                 ctx->saved_data["tau"].toDouble(), grad, nullptr, g[0]);
     variable_list grads(5);
-    grads[0] = grad[0];
+    grads[0] = grad;
     return grads;
   }
 };

@@ -102,8 +102,10 @@ void preference_bwd(const float* coef, const float* g, const uint8_t* mask, int6
 // negative = absent), mask (optional bool [T_all]).  distill_prep fills q, id,
 // live and counters[0] = rows that count; distill_rows then takes a block of
 // T rows of logits, [row0, row0 + T), in order; the block that ends at T_all
-// writes loss.  grad (optional) may be the logits themselves; the two must be
-// misaligned by the same number of bytes in every row.
+// writes loss (where given).  grad (optional) may be the logits themselves; the two
+// must be misaligned by the same number of bytes in every row.  weight (optional):
+// what the loss is multiplied with, on the device; the gradient is written again
+// with it, and nothing happens where it is 1.
 constexpr int kDistillMaxK = 1024;
 constexpr int kDistillMaxCluster = 8;
 struct DistillParams {
@@ -125,6 +127,7 @@ struct DistillParams {
   float* row_loss;  // [T_all * kDistillMaxCluster]: shares of a row's loss, cluster by cluster
   int* counters;   // [1]
   float* loss;
+  const float* weight;
 };
 void distill_prep(const DistillParams& p, cudaStream_t stream);  // T = T_all
 void distill_rows(const DistillParams& p, bool bf16, cudaStream_t stream);

@@ -241,7 +241,8 @@ def distillation_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_ids: t
     twice counts twice.  Rows outside mask (bool [...]) and rows without an
     entry do not count, and may hold anything; without any row the loss is 0.
     An id >= V makes the loss NaN (an ``IndexError`` on CPU).  The gradient
-    goes to logits alone; one backward pass per forward."""
+    goes to logits alone; one backward pass per forward, until which the logits
+    stay as they are."""
     top, ids, m = _check_teacher(logits.shape[:-1], top_logits, top_ids, mask, temperature)
     x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     tau = float(temperature)

@@ -603,6 +603,23 @@ def test_distillation_of_few_rows_on_a_busy_gpu(T, V, dtype):
     assert all(torch.equal(a, b) for pair in got for a, b in zip(pair, want))
 
 
+@pytest.mark.parametrize("weight", [1 / 3, -0.3, 1e-3, 0.0])
+@pytest.mark.parametrize("T,V", [(300, 5003), (17, 40000), (5, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_gradient_times_a_weight_is_rounded_once(T, V, dtype, weight):
+    """What the loss is multiplied with enters the gradient before it is rounded to the logits' type."""
+    from parallel_b200.ops import objectives as O
+
+    logits, top, ids, mask = _teacher_inputs(T, V, 6, dtype, seed=T)
+    x = logits.clone().requires_grad_(True)
+    (grad,) = torch.autograd.grad(weight * O.distillation_loss(x, top, ids, mask=mask, temperature=2.0), x)
+    _synced()
+    want = _distill_reference(logits, top, ids, mask, 2.0)[1] * torch.tensor(weight, dtype=torch.float32).item()
+    # the softmax in fp32, as without a weight: exponents of up to 40 units off by 2^-24 of themselves
+    assert _err(grad, want) <= 1.05 * _err(want.to(dtype), want) + 100 * F32
+    assert torch.equal(grad[~mask], torch.zeros_like(grad[~mask]))
+
+
 def test_distillation_loss_against_differences():
     from parallel_b200.ops import objectives as O
 

@@ -449,16 +449,6 @@ __global__ void __launch_bounds__(kLossThreads) distill_loss_kernel(const Distil
   }
 }
 
-// x[i] *= g[0] unless it is 1
-template <typename E>
-__global__ void __launch_bounds__(256) scale_kernel(E* __restrict__ x, int64_t n, const float* __restrict__ g) {
-  pdl_prologue();
-  const float s = g[0];
-  if (s == 1.f) return;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-    store1(x + i, load1(x + i) * s);
-}
-
 template <typename E>
 void launch_rows(const DistillParams& p, cudaStream_t stream) {
   auto kern = p.weight ? distill_weighted_kernel<E> : distill_rows_kernel<E>;
@@ -488,30 +478,30 @@ void distill_prep(const DistillParams& p, cudaStream_t stream) {
   launch_k(distill_prep_kernel, (p.T + kPrepWarps - 1) / kPrepWarps, 32 * kPrepWarps, 0, stream, p);
 }
 
+// a CTA per row, or a cluster while that leaves SMs idle and each CTA still has 2 vectors a thread; by all
+// rows, so that the blocks of one call write their shares of row_loss alike
+static int cluster_of(const DistillParams& p, bool bf16) {
+  const int nvec = p.V / (bf16 ? 8 : 4);
+  int cluster = 1;
+  while (cluster < kMaxCluster && 2 * cluster * (int64_t)p.T_all <= 2 * num_sms() && nvec / cluster >= 4 * kRowThreads)
+    cluster *= 2;
+  return cluster;
+}
+
 void distill_rows(const DistillParams& p0, bool bf16, cudaStream_t stream) {
   PB_CHECK(p0.K <= kDistillMaxK && (int64_t)p0.T * kMaxCluster < ((int64_t)1 << 31), "distill: too many rows or entries");
   DistillParams p = p0;
-  // a CTA per row, or a cluster while that leaves SMs idle and each CTA still has 2 vectors a thread; by all
-  // rows, so that the blocks of one call write their shares of row_loss alike
-  const int nvec = p.V / (bf16 ? 8 : 4);
-  p.cluster = 1;
-  while (p.cluster < kMaxCluster && 2 * p.cluster * (int64_t)p.T_all <= 2 * num_sms() &&
-         nvec / p.cluster >= 4 * kRowThreads)
-    p.cluster *= 2;
+  p.cluster = cluster_of(p, bf16);
   if (bf16)
     launch_rows<__nv_bfloat16>(p, stream);
   else
     launch_rows<float>(p, stream);
-  if (p.loss && p.row0 + p.T == p.T_all) launch_k(distill_loss_kernel, 1, kLossThreads, 0, stream, p);
 }
 
-void objective_scale(void* x, int64_t n, bool bf16, const float* g, cudaStream_t stream) {
-  if (n == 0) return;
-  const int blocks = (int)std::min<int64_t>((n + 255) / 256, (int64_t)8 * num_sms());
-  if (bf16)
-    launch_k(scale_kernel<__nv_bfloat16>, blocks, 256, 0, stream, (__nv_bfloat16*)x, n, g);
-  else
-    launch_k(scale_kernel<float>, blocks, 256, 0, stream, (float*)x, n, g);
+void distill_loss(const DistillParams& p0, bool bf16, cudaStream_t stream) {
+  DistillParams p = p0;
+  p.cluster = cluster_of(p, bf16);
+  launch_k(distill_loss_kernel, 1, kLossThreads, 0, stream, p);
 }
 
 }  // namespace pb

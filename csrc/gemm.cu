@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const int m = tm * BM + row;
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
-      gemm_detail::epilogue_row<BN, SWIGLU>(ep, t_row, m, M, N, tn * BN_OUT);
+      gemm_detail::epilogue_row<BN, SWIGLU>(ep, ep.alpha, t_row, m, M, N, tn * BN_OUT);
       tc_fence_before();
       mbar_arrive(&tempty_bar[acc]);
     }
@@ -244,7 +244,7 @@ void gemm_bf16(const GemmParams& p, cudaStream_t stream) {
   if (p.epi == kEpiSwiGLU) PB_CHECK(!p.a_mn && !p.b_mn, "gemm: SwiGLU epilogue needs K-major operands");
   // The CTA-pair kernel (256-row tiles) wins on every training shape measured
   // with M >= 256; smaller M keeps the one-CTA kernel.
-  if (p.kernel == 2 || p.gather || p.scatter || p.live || p.splits > 1 || p.epi == kEpiSplitOrdered ||
+  if (p.kernel == 2 || p.gather || p.scatter || p.live || p.alpha_dev || p.splits > 1 || p.epi == kEpiSplitOrdered ||
       (p.kernel == 0 && p.M >= 256))
     return gemm_bf16_pair(p, stream);
   if (p.epi == kEpiSwiGLU) {

@@ -85,6 +85,7 @@ struct GemmParams {
   const int* live = nullptr;
   int live_row0 = 0;
   bool live_k = false;
+  const float* alpha_dev = nullptr;      // on the device: alpha is multiplied with it (CTA-pair kernel, not SwiGLU or kEpiSplitOrdered)
   const ScatterArgs* scatter = nullptr;  // kEpiStoreBf16 rows to their sequence-parallel owners
   const GatherArgs* gather = nullptr;    // A assembled from sequence-parallel shards in-kernel
 };

@@ -25,6 +25,7 @@ struct EpiArgs {
   int* cnt;        // kEpiSplitOrdered: per (tile, CTA) count of published epilogue warps
   int out_f32;     // kEpiSplitOrdered: C is fp32
   int accum;       // kEpiSplitOrdered: C += result
+  const float* alpha_dev;  // CTA-pair kernel: alpha times this, where given
 };
 
 // TMA-store epilogue staging, per epilogue warp: three 32 x 32 bf16 boxes of
@@ -96,7 +97,7 @@ __device__ __forceinline__ void load_row_bf16(const __nv_bfloat16* src, float* v
 // accumulator column, m = output row, n_base = first output column of the
 // tile.  BN = accumulator columns (SwiGLU: [gate BN/2 | up BN/2]).
 template <int BN, bool SWIGLU>
-__device__ __forceinline__ void epilogue_row(const EpiArgs& ep, uint32_t t_row, int m, int M, int N, int n_base) {
+__device__ __forceinline__ void epilogue_row(const EpiArgs& ep, float alpha, uint32_t t_row, int m, int M, int N, int n_base) {
   constexpr int BN_OUT = SWIGLU ? BN / 2 : BN;
   if (SWIGLU) {
 #pragma unroll 1
@@ -135,7 +136,7 @@ __device__ __forceinline__ void epilogue_row(const EpiArgs& ep, uint32_t t_row, 
     const int n0 = n_base + c;
     if (m < M && n0 < N) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] *= ep.alpha;
+      for (int j = 0; j < 32; ++j) v[j] *= alpha;
       if (ep.epi == kEpiStoreBf16) {
         store_row_bf16(out_row_bf16(ep, m) + n0, v, n0, N);
       } else if (ep.epi == kEpiResidualBf16 || ep.epi == kEpiAccumBf16) {
@@ -185,7 +186,7 @@ __device__ __forceinline__ void epilogue_row(const EpiArgs& ep, uint32_t t_row, 
 // chunk follow one another, these do not (151936 x 4096 over 300 rows: 539 ->
 // 482 us).
 template <int BN, typename Release>
-__device__ __forceinline__ void epilogue_row_direct(const EpiArgs& ep, uint32_t t_row, int m, int M, int N, int n_base,
+__device__ __forceinline__ void epilogue_row_direct(const EpiArgs& ep, float alpha, uint32_t t_row, int m, int M, int N, int n_base,
                                                     Release release) {
   __nv_bfloat16* row = reinterpret_cast<__nv_bfloat16*>(ep.C) + (int64_t)m * ep.ldc + n_base;
 #pragma unroll 1
@@ -199,7 +200,7 @@ __device__ __forceinline__ void epilogue_row_direct(const EpiArgs& ep, uint32_t 
       for (int h = 0; h < 2; ++h) {
         uint32_t u[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) u[q] = pack_bf16x2(v[h * 16 + 2 * q] * ep.alpha, v[h * 16 + 2 * q + 1] * ep.alpha);
+        for (int q = 0; q < 8; ++q) u[q] = pack_bf16x2(v[h * 16 + 2 * q] * alpha, v[h * 16 + 2 * q + 1] * alpha);
         asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + c + h * 16), "r"(u[0]),
                      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                      : "memory");
@@ -229,7 +230,7 @@ __device__ __forceinline__ void stage_row_swz64(uint8_t* box, int r, const float
 // accumulator while the stores drain.  y0 = the warp's first output row,
 // n_base = the tile's first output column, N = output columns.
 template <int BN, bool SWIGLU, typename Release>
-__device__ __forceinline__ void epilogue_warp_tma(const EpiArgs& ep, const CUtensorMap* tmC, const CUtensorMap* tmR,
+__device__ __forceinline__ void epilogue_warp_tma(const EpiArgs& ep, float alpha, const CUtensorMap* tmC, const CUtensorMap* tmR,
                                                   uint32_t t_row, uint8_t* stage, int lane, int y0, int M, int N,
                                                   int n_base, Release release) {
   constexpr int BN_OUT = SWIGLU ? BN / 2 : BN;
@@ -265,7 +266,7 @@ __device__ __forceinline__ void epilogue_warp_tma(const EpiArgs& ep, const CUten
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) a[j] *= ep.alpha;
+      for (int j = 0; j < 32; ++j) a[j] *= alpha;
       // four boxes in turn: chunk c may be staged while chunks c - 3 .. c - 1 drain
       box0 = stage + ((c >> 5) & 3) * kEpiBoxBytes;
       if (lane == 0) bulk_wait_group_read<3>();
@@ -300,7 +301,7 @@ __device__ __forceinline__ void stage_row_swz128_f32(uint8_t* box, int r, const 
 // tensor map's per-slab row bound keeps the rows past M of a partial tile out
 // of the next slab.
 template <int BN, typename Release>
-__device__ __forceinline__ void epilogue_warp_tma_f32(const EpiArgs& ep, const CUtensorMap* tmC, uint32_t t_row,
+__device__ __forceinline__ void epilogue_warp_tma_f32(float alpha, const CUtensorMap* tmC, uint32_t t_row,
                                                       uint8_t* stage, int lane, int y0, int M, int N, int n_base,
                                                       int slab, Release release) {
   const bool rows_in = y0 < M;
@@ -313,7 +314,7 @@ __device__ __forceinline__ void epilogue_warp_tma_f32(const EpiArgs& ep, const C
     const int n0 = n_base + c;
     const bool store = rows_in && n0 < N;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) a[j] *= ep.alpha;
+    for (int j = 0; j < 32; ++j) a[j] *= alpha;
     uint8_t* box = stage + ((c >> 5) & 1) * kEpiBoxF32Bytes;
     if (lane == 0) bulk_wait_group_read<1>();
     __syncwarp();

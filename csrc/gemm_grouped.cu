@@ -211,9 +211,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // stacked output [E][M_group][N]; the caller routes only non-empty experts here
         const int m = e * M_group + tm * BM + row;
         const int bound = (tm * BM + row < M_group) ? M_total : 0;
-        gemm_detail::epilogue_row<BN, SWIGLU>(ep, t_row, m, bound, N, tn * BN_OUT);
+        gemm_detail::epilogue_row<BN, SWIGLU>(ep, ep.alpha, t_row, m, bound, N, tn * BN_OUT);
       } else {
-        gemm_detail::epilogue_row<BN, SWIGLU>(ep, t_row, tm * BM + row, M_total, N, tn * BN_OUT);
+        gemm_detail::epilogue_row<BN, SWIGLU>(ep, ep.alpha, t_row, tm * BM + row, M_total, N, tn * BN_OUT);
       }
       tc_fence_before();
       mbar_arrive(&tempty_bar[acc]);

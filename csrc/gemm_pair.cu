@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(GATHER ? kThreads + 64 : kThreads, 1)
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     uint8_t* stage = sEpi + quarter * gemm_detail::kEpiWarpBytes;
+    const float alpha = ep.alpha_dev ? ep.alpha * *ep.alpha_dev : ep.alpha;
     int local = 0;
     for (int w = cid; w < num_work; w += n_clusters, ++local) {
       const int tile = w % num_tiles;
@@ -396,24 +397,24 @@ __global__ void __launch_bounds__(GATHER ? kThreads + 64 : kThreads, 1)
         mbar_arrive_cluster(tempty);
         if (splits > 1) split_publish(cnt, sl, sl == splits - 1, lane);
       } else if (ep.tma == 2) {
-        gemm_detail::epilogue_warp_tma_f32<BN>(ep, &tmC, t_row, stage, lane, m - lane, M, N, tn * BN_OUT,
+        gemm_detail::epilogue_warp_tma_f32<BN>(alpha, &tmC, t_row, stage, lane, m - lane, M, N, tn * BN_OUT,
                                                w / num_tiles, [&] {
                                                  tc_fence_before();
                                                  mbar_arrive_cluster(tempty);
                                                });
       } else if (!SWIGLU && ep.tma == 3) {
-        gemm_detail::epilogue_row_direct<BN>(ep, t_row, m, M, N, tn * BN_OUT, [&] {
+        gemm_detail::epilogue_row_direct<BN>(ep, alpha, t_row, m, M, N, tn * BN_OUT, [&] {
           tc_fence_before();
           mbar_arrive_cluster_relaxed(tempty);
         });
       } else if (ep.tma) {
-        gemm_detail::epilogue_warp_tma<BN, SWIGLU>(ep, &tmC, &tmR, t_row, stage, lane, m - lane, M, N, tn * BN_OUT,
+        gemm_detail::epilogue_warp_tma<BN, SWIGLU>(ep, alpha, &tmC, &tmR, t_row, stage, lane, m - lane, M, N, tn * BN_OUT,
                                                    [&] {
                                                      tc_fence_before();
                                                      mbar_arrive_cluster(tempty);
                                                    });
       } else {
-        gemm_detail::epilogue_row<BN, SWIGLU>(ep, t_row, m, M, N, tn * BN_OUT);
+        gemm_detail::epilogue_row<BN, SWIGLU>(ep, alpha, t_row, m, M, N, tn * BN_OUT);
         tc_fence_before();
         mbar_arrive_cluster(tempty);
       }
@@ -491,6 +492,7 @@ void launch_pair(const GemmParams& p, cudaStream_t stream) {
     ep.out_f32 = p.out_f32 ? 1 : 0;
     ep.accum = p.accumulate ? 1 : 0;
   }
+  ep.alpha_dev = p.alpha_dev;
   if (p.scatter) ep.sc = *p.scatter;
   // TMA-store epilogue for the bf16 store and SwiGLU epilogues into local memory
   // (16-byte aligned bases and row strides; SwiGLU: whole 32-column chunks so a
@@ -543,7 +545,7 @@ void launch_pair(const GemmParams& p, cudaStream_t stream) {
 
 void gemm_bf16_pair(const GemmParams& p, cudaStream_t stream) {
   if (p.gather) {
-    PB_CHECK(!p.live, "gemm: the gather has no row count on the device");
+    PB_CHECK(!p.live && !p.alpha_dev, "gemm: the gather has no row count or factor on the device");
     // A (the gathered activations) is K-major by construction
     PB_CHECK(!p.a_mn, "gemm: the gathered A operand is K-major");
     PB_CHECK(p.gather->seq_local % 256 == 0 && p.gather->n_blocks == (p.M + 255) / 256 && p.M % 256 == 0 &&
@@ -553,6 +555,7 @@ void gemm_bf16_pair(const GemmParams& p, cudaStream_t stream) {
     if (!p.b_mn) return launch_pair<256, false, false, false, true>(p, stream);
     return launch_pair<256, false, true, false, true>(p, stream);
   }
+  PB_CHECK(!p.alpha_dev || (p.epi != kEpiSwiGLU && p.epi != kEpiSplitOrdered), "gemm: no device factor in this epilogue");
   PB_CHECK(!p.live || (!p.scatter && p.epi != kEpiSwiGLU && (!p.live_k || (p.a_mn && p.b_mn && p.splits <= 1))),
            "gemm: a row count on the device needs plain rows (or MN-major operands and one K slice)");
   if (p.scatter) PB_CHECK(p.epi == kEpiStoreBf16 && p.scatter->nranks <= 8, "gemm: scatter needs the bf16 store epilogue");

@@ -365,10 +365,9 @@ struct DistillScratch {
   }
 };
 
-// distill_prep(top [T, K], ids [T, K], mask [T] or None, V, inv_tau) -> [scratch, loss]
-std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& ids,
-                                     const c10::optional<at::Tensor>& mask, int64_t V, double inv_tau,
-                                     int64_t* key = nullptr) {
+// distill_prep(top [T, K], ids [T, K], mask [T] or None, V, inv_tau) -> scratch
+at::Tensor distill_prep(const at::Tensor& top, const at::Tensor& ids, const c10::optional<at::Tensor>& mask, int64_t V,
+                        double inv_tau, int64_t* key = nullptr) {
   TORCH_CHECK(top.is_cuda() && (top.scalar_type() == at::kBFloat16 || top.scalar_type() == at::kFloat) &&
                   top.dim() == 2 && (top.stride(1) == 1 || top.size(1) <= 1),
               "distill: teacher logits must be CUDA bf16 or fp32 [T, K] with unit inner stride");
@@ -390,7 +389,7 @@ std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& id
   const c10::cuda::CUDAGuard g(top.device());
   const auto f32 = top.options().dtype(at::kFloat);
   const DistillScratch sc(T, K);
-  at::Tensor scratch = at::empty({sc.words()}, f32), loss = T ? at::empty({}, f32) : at::zeros({}, f32);
+  at::Tensor scratch = at::empty({sc.words()}, f32);
   sc.fill(p, scratch);
   p.top = top.data_ptr();
   p.ids = ids.data_ptr();
@@ -404,15 +403,15 @@ std::vector<at::Tensor> distill_prep(const at::Tensor& top, const at::Tensor& id
   p.inv_tau = (float)inv_tau;
   p.key = key;
   pb::distill_prep(p, cur_stream());
-  return {scratch, loss};
+  return scratch;
 }
 
-// distill_rows(logits [T, V], prep ([scratch, loss] of all T_all rows), T_all, K, row0, tau, grad [T, V] or None):
-// the losses of rows [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss; with perm,
+// distill_rows(logits [T, V], scratch (distill_prep's of all T_all rows), T_all, K, row0, tau, grad [T, V] or None): the
+// losses of rows [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss; with perm,
 // row i of the logits is row perm[i] of the teacher's; with weight (a scalar), the gradient alone, times it, if it
 // is not 1
-void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep, int64_t T_all, int64_t K, int64_t row0,
-                  double tau, const c10::optional<at::Tensor>& grad, const int* perm = nullptr,
+void distill_rows(const at::Tensor& logits, const at::Tensor& scratch, int64_t T_all, int64_t K, int64_t row0, double tau,
+                  const c10::optional<at::Tensor>& grad, const int* perm = nullptr,
                   const c10::optional<at::Tensor>& weight = c10::nullopt) {
   TORCH_CHECK(logits.is_cuda() && (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat) &&
                   logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) <= 1),
@@ -422,17 +421,15 @@ void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep,
   TORCH_CHECK(V >= 1 && V <= kIntMax, "distill: vocabulary");
   TORCH_CHECK(row0 >= 0 && row0 + T <= T_all, "distill: rows outside the teacher's");
   const DistillScratch sc(T_all, K);
-  TORCH_CHECK(prep.size() == 2 && K >= 1 && K <= pb::kDistillMaxK, "distill: what distill_prep returned");
-  for (const at::Tensor& t : prep) CHECK_SAME_DEVICE(logits, t);
-  check_rows_f32(prep[0], sc.words(), "distill: scratch");
+  TORCH_CHECK(K >= 1 && K <= pb::kDistillMaxK, "distill: 1 to ", num(pb::kDistillMaxK), " teacher entries a row");
+  CHECK_SAME_DEVICE(logits, scratch);
+  check_rows_f32(scratch, sc.words(), "distill: scratch");
   if (T == 0) return;
   pb::DistillParams p{};
-  sc.fill(p, prep[0]);
-  p.loss = check_rows_f32(prep[1], 1, "distill: loss");
+  sc.fill(p, scratch);
   if (given(weight)) {
     CHECK_SAME_DEVICE(logits, *weight);
     p.weight = check_rows_f32(*weight, 1, "distill: weight");
-    p.loss = nullptr;  // it was handed out
   }
   const int64_t es = logits.element_size();
   p.logits = logits.data_ptr();
@@ -459,6 +456,19 @@ void distill_rows(const at::Tensor& logits, const std::vector<at::Tensor>& prep,
   pb::distill_rows(p, bf16, cur_stream());
 }
 
+// distill_loss(scratch (all rows of all blocks seen by distill_rows), T_all, K, V, bf16 logits) -> loss
+at::Tensor distill_loss(const at::Tensor& scratch, int64_t T_all, int64_t K, int64_t V, bool bf16) {
+  if (T_all == 0) return at::zeros({}, scratch.options());
+  const c10::cuda::CUDAGuard g(scratch.device());
+  at::Tensor loss = at::empty({}, scratch.options());
+  pb::DistillParams p{};
+  DistillScratch(T_all, K).fill(p, scratch);
+  p.V = (int)V;
+  p.loss = loss.data_ptr<float>();
+  pb::distill_loss(p, bf16, cur_stream());
+  return loss;
+}
+
 // grad_like(logits [T, V]) -> grad [T, V]: a tensor that is misaligned as logits is in every row, so that both are read
 // and written in the same 16-byte vectors
 at::Tensor grad_like(const at::Tensor& logits) {
@@ -468,16 +478,6 @@ at::Tensor grad_like(const at::Tensor& logits) {
   const int64_t shift = (int64_t)(reinterpret_cast<uintptr_t>(logits.data_ptr()) & 15) / logits.element_size();
   const int64_t ld = V + ((logits.stride(0) - V) % unit + unit) % unit;
   return at::empty({shift + T * ld}, logits.options()).as_strided({T, V}, {ld, 1}, shift);
-}
-
-// objective_scale(x flat, g scalar): x *= g unless g is 1
-void objective_scale(at::Tensor& x, const at::Tensor& g) {
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat),
-              "objective_scale: contiguous CUDA bf16 or fp32");
-  CHECK_SAME_DEVICE(x, g);
-  const c10::cuda::CUDAGuard guard(x.device());
-  pb::objective_scale(x.data_ptr(), x.numel(), x.scalar_type() == at::kBFloat16,
-                      check_rows_f32(g, 1, "objective_scale: g"), cur_stream());
 }
 
 // ---------------------------------------------------------------- differentiable entry points
@@ -525,8 +525,10 @@ int grad_rows_slices(int64_t T, int64_t H, int64_t V) {
   return best;
 }
 
-// dl [T, V] @ w [V, H] for the rows that count: bf16 [T, H], or (several slices, or f32) fp32 slabs [slices * T, H]
-at::Tensor grad_rows(const at::Tensor& dl, const at::Tensor& w, const at::Tensor& count, int64_t row0, bool f32) {
+// dl [T, V] @ w [V, H] (times factor[0]) for the rows that count: bf16 [T, H], or (several slices, or f32) fp32 slabs
+// [slices * T, H]
+at::Tensor grad_rows(const at::Tensor& dl, const at::Tensor& w, const at::Tensor& count, int64_t row0, bool f32,
+                     const float* factor = nullptr) {
   const int64_t T = dl.size(0), V = w.size(0), H = w.size(1);
   const int slices = grad_rows_slices(T, H, V);
   at::Tensor out = at::empty({slices * T, H}, dl.options().dtype(slices == 1 && !f32 ? at::kBFloat16 : at::kFloat));
@@ -544,15 +546,16 @@ at::Tensor grad_rows(const at::Tensor& dl, const at::Tensor& w, const at::Tensor
   p.alpha = 1.f;
   p.epi = slices == 1 && !f32 ? pb::kEpiStoreBf16 : pb::kEpiStoreF32;
   p.splits = slices;
+  p.alpha_dev = factor;
   p.live = count.data_ptr<int>();
   p.live_row0 = (int)row0;
   pb::gemm_bf16(p, cur_stream());
   return out;
 }
 
-// out (+)= dl^T h over the rows that count; out bf16, or fp32 where several row blocks add up
+// out (+)= dl^T h (times factor[0]) over the rows that count; out bf16, or fp32 where several row blocks add up
 void grad_head(const at::Tensor& dl, const at::Tensor& h, at::Tensor& out, bool accumulate, const at::Tensor& count,
-               int64_t row0) {
+               int64_t row0, const float* factor = nullptr) {
   pb::GemmParams p{};
   p.A = dl.data_ptr();
   p.B = h.data_ptr();
@@ -569,6 +572,7 @@ void grad_head(const at::Tensor& dl, const at::Tensor& h, at::Tensor& out, bool 
   p.live = count.data_ptr<int>();
   p.live_row0 = (int)row0;
   p.live_k = true;
+  p.alpha_dev = factor;
   pb::gemm_bf16(p, cur_stream());
 }
 
@@ -725,23 +729,22 @@ std::vector<at::Tensor> preference_loss(const at::Tensor& logp, const c10::optio
 struct DistillationNode : public torch::autograd::Function<DistillationNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& top,
                             const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau) {
-    const auto prep = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau);
-    const at::Tensor grad = grad_like(logits);
-    distill_rows(logits, prep, top.size(0), top.size(1), 0, tau, grad);
+    const at::Tensor scratch = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau), grad = grad_like(logits);
+    distill_rows(logits, scratch, top.size(0), top.size(1), 0, tau, grad);
     // not save_for_backward: the backward hands the gradient out, it does not keep it
     ctx->saved_data["grad"] = grad;
-    ctx->saved_data["scratch"] = prep[0];
+    ctx->saved_data["scratch"] = scratch;
     ctx->saved_data["K"] = top.size(1);
     ctx->saved_data["tau"] = tau;
     ctx->save_for_backward({logits});
-    return prep[1];
+    return distill_loss(scratch, top.size(0), top.size(1), logits.size(1), logits.scalar_type() == at::kBFloat16);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     check_first_order("distillation_loss");
     TORCH_CHECK(ctx->saved_data.count("grad"), "distillation_loss supports one backward pass per forward");
     const at::Tensor logits = ctx->get_saved_variables()[0], grad = ctx->saved_data["grad"].toTensor();
     ctx->saved_data.erase("grad");
-    distill_rows(logits, {ctx->saved_data["scratch"].toTensor(), g[0]}, logits.size(0), ctx->saved_data["K"].toInt(), 0,
+    distill_rows(logits, ctx->saved_data["scratch"].toTensor(), logits.size(0), ctx->saved_data["K"].toInt(), 0,
                  ctx->saved_data["tau"].toDouble(), grad, nullptr, g[0]);
     variable_list grads(5);
     grads[0] = grad;
@@ -752,81 +755,100 @@ struct DistillationNode : public torch::autograd::Function<DistillationNode> {
 at::Tensor distillation_loss(const at::Tensor& logits, const at::Tensor& top, const at::Tensor& ids,
                              const c10::optional<at::Tensor>& mask, double tau) {
   if (!wants_grad(logits)) {
-    const auto prep = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau);
-    distill_rows(logits, prep, top.size(0), top.size(1), 0, tau, c10::nullopt);
-    return prep[1];
+    const at::Tensor scratch = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau);
+    distill_rows(logits, scratch, top.size(0), top.size(1), 0, tau, c10::nullopt);
+    return distill_loss(scratch, top.size(0), top.size(1), logits.size(1), logits.scalar_type() == at::kBFloat16);
   }
   return DistillationNode::apply(logits, top, ids, mask, tau);
 }
 
 // Distillation through the LM head: blocks of bf16 logits of the packed rows
 // (those that count in front, zeros behind, as in LogProbsNode), overwritten by
-// their gradient, which the two products turn into those of h and w at once.
+// their gradient, which the backward's two products turn into those of h and w,
+// times the incoming gradient before they are rounded.  The first block's logit
+// gradient is kept for it (at most max_block_bytes); the logits of rows beyond are
+// computed again.  bf16 logits are what the model's own head returns and what its
+// cross-entropy works on (up to |logit| / 512 of a logit is lost); fp32 ones would
+// take twice the memory and could not become the products' operand in place.
 struct HeadDistillationNode : public torch::autograd::Function<HeadDistillationNode> {
+  // logits of packed rows [r0, r0 + n) in buf's first n rows
+  static at::Tensor block_logits(const at::Tensor& buf, const at::Tensor& rows, const at::Tensor& w,
+                                 const at::Tensor& count, int64_t r0) {
+    const at::Tensor logits = rows_of(buf, 0, rows.size(0));
+    pb::GemmParams p{};
+    p.A = rows.data_ptr();
+    p.B = w.data_ptr();
+    p.C = logits.data_ptr();
+    p.lda = rows.stride(0);
+    p.ldb = w.stride(0);
+    p.ldc = buf.stride(0);
+    p.M = (int)rows.size(0);
+    p.N = (int)w.size(0);
+    p.K = (int)w.size(1);
+    p.alpha = 1.f;
+    p.epi = pb::kEpiStoreBf16;
+    p.live = count.data_ptr<int>();
+    p.live_row0 = (int)r0;
+    pb::gemm_bf16(p, cur_stream());
+    return logits;
+  }
   static at::Tensor run(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& top,
-                        const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau, int64_t max_block_bytes,
-                        bool need_h, bool need_w) {
+                        const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau, int64_t max_block_bytes) {
     const c10::cuda::CUDAGuard guard(h.device());
     const int64_t T = h.size(0), V = w.size(0), H = w.size(1), K = top.size(1);
     TORCH_CHECK(H == h.size(1) && top.size(0) == T, "lm_head_distillation: shapes");
     CHECK_SAME_DEVICE(h, w);
     CHECK_SAME_DEVICE(h, top);
     at::Tensor key = at::empty({T}, h.options().dtype(at::kLong));
-    const auto prep = distill_prep(top, ids, mask, V, 1.0 / tau, key.data_ptr<int64_t>());
+    const at::Tensor scratch = distill_prep(top, ids, mask, V, 1.0 / tau, key.data_ptr<int64_t>());
     const auto packed = logprob_pack(h, key);  // rows, keys, perm, count
     const at::Tensor &hp = packed[0], &perm = packed[2], &count = packed[3];
     const int64_t block = block_rows(T, V, max_block_bytes);
     const at::Tensor buf = at::empty({block, (V + 63) / 64 * 64}, h.options()).narrow(1, 0, V);
-    at::Tensor dh, dw;
-    if (need_h) dh = at::empty({T, H}, h.options());
-    if (need_w) dw = at::empty({V, H}, block >= T ? w.options() : w.options().dtype(at::kFloat));
-    for (int64_t r0 = 0; r0 < T; r0 += block) {
-      const int64_t n = std::min(block, T - r0);
-      const at::Tensor logits = rows_of(buf, 0, n), rows = rows_of(hp, r0, n), pm = rows_of(perm, r0, n);
-      pb::GemmParams p{};
-      p.A = rows.data_ptr();
-      p.B = w.data_ptr();
-      p.C = logits.data_ptr();
-      p.lda = rows.stride(0);
-      p.ldb = w.stride(0);
-      p.ldc = buf.stride(0);
-      p.M = (int)n;
-      p.N = (int)V;
-      p.K = (int)H;
-      p.alpha = 1.f;
-      p.epi = pb::kEpiStoreBf16;
-      p.live = count.data_ptr<int>();
-      p.live_row0 = (int)r0;
-      pb::gemm_bf16(p, cur_stream());
-      distill_rows(logits, prep, T, K, r0, tau, need_h || need_w ? c10::optional<at::Tensor>(logits) : c10::nullopt,
+    for (int64_t r0 = (T - 1) / block * block; r0 >= 0; r0 -= block) {  // the first block last: it stays
+      const at::Tensor logits = block_logits(buf, rows_of(hp, r0, std::min(block, T - r0)), w, count, r0);
+      distill_rows(logits, scratch, T, K, r0, tau, ctx && r0 == 0 ? c10::optional<at::Tensor>(logits) : c10::nullopt,
                    perm.data_ptr<int>());
-      if (need_h) logprob_unpack(grad_rows(logits, w, count, r0, false), pm, count, r0, dh);
-      if (need_w) grad_head(logits, rows, dw, r0 > 0, count, r0);
     }
     if (ctx) {
-      // not save_for_backward: the backward hands the gradients out
-      ctx->saved_data["grads"] =
-          std::vector<at::Tensor>{need_h ? dh : at::empty({0}, h.options()),
-                                  need_w ? dw.to(w.scalar_type()) : at::empty({0}, h.options())};
-      ctx->saved_data["need_h"] = need_h;
-      ctx->saved_data["need_w"] = need_w;
+      ctx->save_for_backward({hp, w, perm, count});
+      ctx->saved_data["kept"] = std::vector<at::Tensor>{buf, scratch};
+      ctx->saved_data["K"] = K;
+      ctx->saved_data["tau"] = tau;
     }
-    return prep[1];
+    return distill_loss(scratch, T, K, V, true);
   }
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& top,
                             const at::Tensor& ids, const c10::optional<at::Tensor>& mask, double tau,
                             int64_t max_block_bytes) {
-    return run(ctx, h, w, top, ids, mask, tau, max_block_bytes, h.requires_grad(), w.requires_grad());
+    return run(ctx, h, w, top, ids, mask, tau, max_block_bytes);
   }
-  static variable_list backward(AutogradContext* ctx, variable_list g) {
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_first_order("lm_head_distillation");
-    TORCH_CHECK(ctx->saved_data.count("grads"), "lm_head_distillation supports one backward pass per forward");
-    std::vector<at::Tensor> grads = ctx->saved_data["grads"].toTensorVector();
-    ctx->saved_data.erase("grads");
+    TORCH_CHECK(ctx->saved_data.count("kept"), "lm_head_distillation supports one backward pass per forward");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &hp = saved[0], &w = saved[1], &perm = saved[2], &count = saved[3];
+    const std::vector<at::Tensor> kept = ctx->saved_data["kept"].toTensorVector();
+    ctx->saved_data.erase("kept");
+    const at::Tensor &buf = kept[0], &scratch = kept[1];
+    const double tau = ctx->saved_data["tau"].toDouble();
+    const int64_t K = ctx->saved_data["K"].toInt(), block = buf.size(0), T = hp.size(0), V = w.size(0), H = w.size(1);
+    const c10::cuda::CUDAGuard guard(hp.device());
+    CHECK_SAME_DEVICE(hp, grads[0]);
+    const float* factor = check_rows_f32(grads[0], 1, "lm_head_distillation: gradient");
+    at::Tensor dh, dw;
+    if (ctx->needs_input_grad(0)) dh = at::empty({T, H}, hp.options());
+    if (ctx->needs_input_grad(1)) dw = at::empty({V, H}, block >= T ? w.options() : w.options().dtype(at::kFloat));
+    for (int64_t r0 = 0; r0 < T; r0 += block) {
+      const int64_t n = std::min(block, T - r0);
+      const at::Tensor rows = rows_of(hp, r0, n), dl = r0 ? block_logits(buf, rows, w, count, r0) : buf;
+      if (r0) distill_rows(dl, scratch, T, K, r0, tau, dl, perm.data_ptr<int>());
+      if (dh.defined()) logprob_unpack(grad_rows(dl, w, count, r0, false, factor), rows_of(perm, r0, n), count, r0, dh);
+      if (dw.defined()) grad_head(dl, rows, dw, r0 > 0, count, r0, factor);
+    }
     variable_list out(7);
-    if (ctx->saved_data["need_h"].toBool()) out[0] = grads[0];
-    if (ctx->saved_data["need_w"].toBool()) out[1] = grads[1];
-    for (at::Tensor& t : grads) objective_scale(t, g[0]);
+    out[0] = dh;
+    if (dw.defined()) out[1] = dw.to(w.scalar_type());
     return out;
   }
 };
@@ -836,7 +858,7 @@ at::Tensor lm_head_distillation(const at::Tensor& h, const at::Tensor& w, const 
   check_rows_bf16(h, "lm_head_distillation: h");
   check_rows_bf16(w, "lm_head_distillation: w");
   if (wants_grad(h) || wants_grad(w)) return HeadDistillationNode::apply(h, w, top, ids, mask, tau, max_block_bytes);
-  return HeadDistillationNode::run(nullptr, h, w, top, ids, mask, tau, max_block_bytes, false, false);
+  return HeadDistillationNode::run(nullptr, h, w, top, ids, mask, tau, max_block_bytes);
 }
 
 }  // namespace

@@ -101,11 +101,11 @@ void preference_bwd(const float* coef, const float* g, const uint8_t* mask, int6
 // Teacher entries [T_all, K]: values (bf16 or fp32) and ids (int32 or int64,
 // negative = absent), mask (optional bool [T_all]).  distill_prep fills q, id,
 // live and counters[0] = rows that count; distill_rows then takes a block of
-// T rows of logits, [row0, row0 + T), in order; the block that ends at T_all
-// writes loss (where given).  grad (optional) may be the logits themselves; the two
-// must be misaligned by the same number of bytes in every row.  weight (optional):
-// what the loss is multiplied with, on the device; the gradient is written again
-// with it, and nothing happens where it is 1.
+// T rows of logits, [row0, row0 + T), and distill_loss writes the loss of all
+// blocks.  grad (optional) may be the logits themselves; the two must be
+// misaligned by the same number of bytes in every row.  weight (optional): what
+// the loss is multiplied with, on the device; the gradient is written again with
+// it, and nothing happens where it is 1.
 constexpr int kDistillMaxK = 1024;
 constexpr int kDistillMaxCluster = 8;
 struct DistillParams {
@@ -131,8 +131,6 @@ struct DistillParams {
 };
 void distill_prep(const DistillParams& p, cudaStream_t stream);  // T = T_all
 void distill_rows(const DistillParams& p, bool bf16, cudaStream_t stream);
-
-// x[i] *= g[0] unless it is 1
-void objective_scale(void* x, int64_t n, bool bf16, const float* g, cudaStream_t stream);
+void distill_loss(const DistillParams& p, bool bf16, cudaStream_t stream);  // bf16: the logits' type
 
 }  // namespace pb

@@ -254,8 +254,9 @@ def distillation_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_ids: t
 def lm_head_distillation(h: torch.Tensor, w: torch.Tensor, top_logits: torch.Tensor, top_ids: torch.Tensor,
                          mask: torch.Tensor | None = None, temperature: float = 1.0,
                          max_block_bytes: int = 6 << 30) -> torch.Tensor:
-    """``distillation_loss(h @ w.T, ...)`` for hidden states h [..., H] and the LM head w [V, H], with at most
-    ``max_block_bytes`` of bf16 logits held at a time; the gradient goes to h and w."""
+    """``distillation_loss(h @ w.T, ...)`` for hidden states h [..., H] and the LM head w [V, H], with bf16 logits.  At
+    most ``max_block_bytes`` of them are held at a time, the first block's until the backward pass; logits of rows
+    beyond it are computed twice.  The gradient goes to h and w; one backward pass per forward."""
     _check_head(h, w)
     top, ids, m = _check_teacher(h.shape[:-1], top_logits, top_ids, mask, temperature)
     h2, tau = h.reshape(-1, h.shape[-1]), float(temperature)

@@ -717,6 +717,37 @@ def test_lm_head_distillation(T, V, blocks):
     assert torch.equal(dh[~mask], torch.zeros_like(dh[~mask]))
 
 
+@pytest.mark.parametrize("weight", [1.0, 1 / 3, -0.3, 1e-3])
+@pytest.mark.parametrize("blocks", [1, 3])
+def test_lm_head_distillation_gradients_times_a_weight_are_rounded_once(blocks, weight):
+    """Logits that bf16 holds exactly, so that the logits' gradient is known to its rounding (one in 10^4 entries may
+    fall to the other side): its products with the head and the hidden states, times the weight, are rounded once."""
+    from parallel_b200.ops import objectives as O
+
+    T, H, V, K, tau = 700, 64, 1003, 6, 2.0
+    gen = torch.Generator(device="cuda").manual_seed(81)
+    h = torch.zeros(T, H, device="cuda")
+    h.scatter_(1, torch.rand(T, H, device="cuda", generator=gen).topk(8, 1).indices, 1.0)
+    h *= torch.randint(0, 2, (T, H), device="cuda", generator=gen) * 2 - 1
+    w = torch.randint(-8, 9, (V, H), device="cuda", generator=gen) / 4  # logits: quarters up to 16
+    logits = h.double() @ w.double().t()
+    assert torch.equal(logits.bfloat16().double(), logits)
+    ids = torch.randint(0, V, (T, K), device="cuda", generator=gen)
+    top = 6 * torch.rand(T, K, device="cuda", generator=gen)
+    mask = torch.rand(T, device="cuda", generator=gen) >= 0.3
+    hg, wg = h.bfloat16().requires_grad_(True), w.bfloat16().requires_grad_(True)
+    loss = O.lm_head_distillation(hg, wg, top, ids, mask=mask, temperature=tau,
+                                  max_block_bytes=(6 << 30) if blocks == 1 else 2 * V * 256)
+    dh, dw = torch.autograd.grad(weight * loss, (hg, wg))
+    _synced()
+    ref, dl = _distill_reference(logits, top, ids, mask, tau)
+    assert abs(loss.item() - ref.item()) <= 100 * F32 * tau ** 2 * (ref.item() + 40)
+    dl = dl.bfloat16().double() * torch.tensor(weight, dtype=torch.float32).item()
+    for got, want in ((dh, dl @ w.double()), (dw, dl.t() @ h.double())):
+        assert _err(got, want) <= 1.05 * _err(want.bfloat16(), want)
+    assert torch.equal(dh[~mask], torch.zeros_like(dh[~mask]))
+
+
 # ----------------------------------------------------------------- values at the ends of the types
 @pytest.mark.parametrize("V", [40, 1003, 40000])
 @pytest.mark.parametrize("tau", [0.5, 1.0, 4.0])

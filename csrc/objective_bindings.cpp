@@ -489,6 +489,17 @@ using torch::autograd::variable_list;
 
 bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
+// A dual tensor without requires_grad would pass the nodes by and lose its tangent.
+void check_no_tangent(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, ": forward-mode derivatives are not implemented");
+}
+
+// What takes no gradient takes no tangent either.
+at::Tensor constant(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined() ? t.detach() : t; }
+c10::optional<at::Tensor> constant(const c10::optional<at::Tensor>& t) {
+  return given(t) ? c10::optional<at::Tensor>(constant(*t)) : c10::nullopt;
+}
+
 at::Tensor or_undefined(const c10::optional<at::Tensor>& t) { return given(t) ? *t : at::Tensor(); }
 c10::optional<at::Tensor> or_none(const at::Tensor& t) {
   return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt;
@@ -652,6 +663,8 @@ at::Tensor lm_head_log_probs(const at::Tensor& h, const at::Tensor& w, const at:
                              int64_t max_block_bytes) {
   check_rows_bf16(h, "lm_head_log_probs: h");
   check_rows_bf16(w, "lm_head_log_probs: w");
+  check_no_tangent(h, "lm_head_log_probs");
+  check_no_tangent(w, "lm_head_log_probs");
   TORCH_CHECK(w.size(0) >= 1, "lm_head_log_probs: an empty vocabulary");
   if (wants_grad(h) || wants_grad(w)) return LogProbsNode::apply(h, w, ids, inv_tau, max_block_bytes);
   const c10::cuda::CUDAGuard guard(h.device());
@@ -688,11 +701,12 @@ struct PolicyLossNode : public torch::autograd::Function<PolicyLossNode> {
 std::vector<at::Tensor> policy_loss(const at::Tensor& logp, const at::Tensor& old, const at::Tensor& adv,
                                     const c10::optional<at::Tensor>& mask, const c10::optional<at::Tensor>& ref,
                                     double low, double high, double kl_coef, bool per_sequence) {
+  check_no_tangent(logp, "policy_loss");
   if (!wants_grad(logp)) {
     const auto out = policy_fwd(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence, false);
     return {*out[0], *out[1], *out[2]};
   }
-  return PolicyLossNode::apply(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence);
+  return PolicyLossNode::apply(logp, constant(old), constant(adv), mask, constant(ref), low, high, kl_coef, per_sequence);
 }
 
 struct PreferenceLossNode : public torch::autograd::Function<PreferenceLossNode> {
@@ -717,11 +731,12 @@ struct PreferenceLossNode : public torch::autograd::Function<PreferenceLossNode>
 std::vector<at::Tensor> preference_loss(const at::Tensor& logp, const c10::optional<at::Tensor>& ref,
                                         const c10::optional<at::Tensor>& mask, double beta, double smoothing,
                                         bool average) {
+  check_no_tangent(logp, "preference_loss");
   if (!wants_grad(logp)) {
     const auto out = preference_fwd(logp, ref, mask, beta, smoothing, average);
     return {out[0], out[1]};
   }
-  return PreferenceLossNode::apply(logp, ref, mask, beta, smoothing, average);
+  return PreferenceLossNode::apply(logp, constant(ref), mask, beta, smoothing, average);
 }
 
 // The gradient is written in the forward pass, from the one read of the
@@ -754,6 +769,7 @@ struct DistillationNode : public torch::autograd::Function<DistillationNode> {
 
 at::Tensor distillation_loss(const at::Tensor& logits, const at::Tensor& top, const at::Tensor& ids,
                              const c10::optional<at::Tensor>& mask, double tau) {
+  check_no_tangent(logits, "distillation_loss");
   if (!wants_grad(logits)) {
     const at::Tensor scratch = distill_prep(top, ids, mask, logits.size(1), 1.0 / tau);
     distill_rows(logits, scratch, top.size(0), top.size(1), 0, tau, c10::nullopt);
@@ -857,6 +873,8 @@ at::Tensor lm_head_distillation(const at::Tensor& h, const at::Tensor& w, const 
                                 const c10::optional<at::Tensor>& mask, double tau, int64_t max_block_bytes) {
   check_rows_bf16(h, "lm_head_distillation: h");
   check_rows_bf16(w, "lm_head_distillation: w");
+  check_no_tangent(h, "lm_head_distillation");
+  check_no_tangent(w, "lm_head_distillation");
   if (wants_grad(h) || wants_grad(w)) return HeadDistillationNode::apply(h, w, top, ids, mask, tau, max_block_bytes);
   return HeadDistillationNode::run(nullptr, h, w, top, ids, mask, tau, max_block_bytes);
 }

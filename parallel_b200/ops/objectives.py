@@ -10,7 +10,8 @@
   logits, and ``lm_head_distillation``, the same through the LM head.
 
 As in ``functional``, CUDA tensors run the sm_100a kernels and CPU tensors run
-the plain PyTorch statement of the same formula.
+the plain PyTorch statement of the same formula.  The kernels have first-order
+gradients; forward-mode derivatives are refused.
 """
 from __future__ import annotations
 

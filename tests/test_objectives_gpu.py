@@ -1103,3 +1103,32 @@ def test_only_the_first_argument_gets_a_gradient():
         assert leaf.grad is not None and other.grad is None
         assert not fn(leaf.detach()).requires_grad
     _synced()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(grad):
+    """The kernels have no tangents: a dual tensor is refused, with or without a gradient, instead of losing its."""
+    import torch.autograd.forward_ad as fwd
+
+    from parallel_b200.ops import objectives as O
+
+    def leaf(*shape):
+        return torch.randn(*shape, device="cuda").requires_grad_(grad)
+
+    h, w, lp, x = leaf(4, 64).bfloat16(), leaf(30, 64).bfloat16(), leaf(4, 5), leaf(4, 30)
+    ids, top, tid = torch.arange(4, device="cuda"), torch.rand(4, 3, device="cuda"), torch.arange(12, device="cuda").view(4, 3)
+    with fwd.dual_level():
+        def dual(t):
+            return fwd.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: O.lm_head_log_probs(dual(h), w, ids), lambda: O.lm_head_log_probs(h, dual(w), ids),
+                     lambda: O.policy_loss(dual(lp), lp, lp), lambda: O.preference_loss(dual(lp)),
+                     lambda: O.distillation_loss(dual(x), top, tid), lambda: O.lm_head_distillation(dual(h), w, top, tid),
+                     lambda: O.lm_head_distillation(h, dual(w), top, tid)):
+            with pytest.raises(RuntimeError):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                call()
+        # what takes no gradient takes no tangent either
+        O.policy_loss(lp, dual(lp), dual(lp), ref_logp=dual(lp))
+    _synced()

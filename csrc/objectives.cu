@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(1024) preference_fwd_kernel(const PreferencePa
     const double t = exp(-fabs(gap)), soft = log1p(t);  // -log sigmoid(x) = soft + max(-x, 0)
     const double neg = gap < 0.0 ? -gap : 0.0, pos = gap > 0.0 ? gap : 0.0;
     const double e = p.smoothing;
-    loss[0] += (1.0 - e) * (soft + neg) + e * (soft + pos);
+    // a side that does not count enters neither: its loss may be infinite
+    loss[0] += (e < 1.0 ? (1.0 - e) * (soft + neg) : 0.0) + (e > 0.0 ? e * (soft + pos) : 0.0);
     // sigmoid(-gap) and sigmoid(gap), each without cancellation
     const double small = t / (1.0 + t), big = 1.0 / (1.0 + t);
     const double s_neg = gap >= 0.0 ? small : big, s_pos = gap >= 0.0 ? big : small;

@@ -201,8 +201,9 @@ def _preference_plain(logp, ref, mask, beta, smoothing, average):
     rewards = beta * (sums / m.sum(1).clamp_min(1).to(logp.dtype) if average else sums)
     P = logp.shape[0] // 2
     gap = rewards[:P] - rewards[P:]
-    loss = -((1.0 - smoothing) * F.logsigmoid(gap) + smoothing * F.logsigmoid(-gap)).mean()
-    return PreferenceLoss(loss, rewards.detach())
+    # a side that does not count enters neither: its loss may be infinite
+    sides = [share * F.logsigmoid(side) for share, side in ((1.0 - smoothing, gap), (smoothing, -gap)) if share]
+    return PreferenceLoss(-sum(sides).mean(), rewards.detach())
 
 
 # ----------------------------------------------------------------- distillation from a teacher's top logits

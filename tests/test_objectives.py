@@ -138,6 +138,22 @@ def test_preference_loss_formula_and_gradient():
         _differences(fn, logp)
 
 
+def test_preference_loss_of_impossible_tokens():
+    """A rejected token of probability zero: an infinite gap, and a loss of 0 with unsmoothed labels.  A chosen one:
+    an infinite loss with the gradient of a certain error."""
+    inf = float("inf")
+    for side, smoothing, want, grads in ((2, 0.0, 0.0, (0.0, 0.0)), (0, 0.0, inf, (-0.5, 0.5)), (2, 0.25, inf, (0.125, -0.125)),
+                                         (0, 0.25, inf, (-0.375, 0.375)), (0, 1.0, 0.0, (0.0, 0.0)), (2, 1.0, inf, (0.5, -0.5))):
+        lp = torch.zeros(4, 6)
+        lp[side, 3] = -inf  # pair 0; pair 1 has a gap of 0
+        lp.requires_grad_(True)
+        out = O.preference_loss(lp, beta=1.0, label_smoothing=smoothing)
+        (grad,) = torch.autograd.grad(out.loss, lp)
+        assert out.loss.item() == want if want else abs(out.loss.item() - 0.5 * 0.6931471805599453) < 1e-6
+        assert grad[0].tolist() == [grads[0]] * 6 and grad[2].tolist() == [grads[1]] * 6
+        assert torch.isfinite(grad).all()
+
+
 def test_policy_and_preference_refusals():
     x = torch.zeros(4, 5)
     with pytest.raises(ValueError):

@@ -115,8 +115,10 @@ __global__ void __launch_bounds__(1024) policy_fwd_kernel(const PolicyParams p) 
         if (ref) {
           const double x = (double)rl[j] - (double)l[j];
           const double e = expm1(x), k = e - x;  // exp(x) - 1 - x without the cancellation at small x
-          per += p.kl_coef * k;
-          coef -= p.kl_coef * e;
+          if (p.kl_coef != 0.0) {  // without the term the estimate may be infinite
+            per += p.kl_coef * k;
+            coef -= p.kl_coef * e;
+          }
           kl += on[j] ? k : 0.0;
         }
         loss += on[j] ? per : 0.0;

@@ -160,7 +160,8 @@ def _policy_plain(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence):
     if ref is not None:
         d = ref[at] - x
         kl = torch.expm1(d) - d
-        per = per + kl_coef * kl
+        if kl_coef:  # without the term the estimate may be infinite
+            per = per + kl_coef * kl
     n = max(1, x.numel())
     if per_sequence:
         rows = m.sum(1)

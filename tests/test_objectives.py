@@ -119,6 +119,22 @@ def test_policy_loss_formula_and_gradient():
         _differences(fn, logp)
 
 
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_policy_loss_without_a_kl_term_takes_any_reference(reduction):
+    """kl_coef 0: the reference is reported on and nothing else, where the estimate is infinite too."""
+    lp = -torch.rand(3, 7)
+    ref = lp.clone()
+    ref[1, 2], ref[2, 3] = -float("inf"), 3e38
+    adv = torch.randn(3, 7)
+    outs = []
+    for r in (None, ref):
+        x = lp.clone().requires_grad_(True)
+        out = O.policy_loss(x, lp - 0.1, adv, ref_logp=r, reduction=reduction)
+        outs.append((out.loss.detach(), out.clip_fraction, torch.autograd.grad(out.loss, x)[0]))
+    assert out.kl.item() == float("inf")
+    assert torch.isfinite(outs[0][0]) and all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 def test_preference_loss_formula_and_gradient():
     torch.manual_seed(2)
     P, S = 3, 8

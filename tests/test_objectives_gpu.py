@@ -340,6 +340,25 @@ def test_policy_loss_strided_inputs_streams_and_same_bits():
     assert all(torch.equal(a.detach(), b) for a, b in zip(got, want)) and torch.equal(g1, g2)
 
 
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_policy_loss_without_a_kl_term_takes_any_reference(reduction):
+    """kl_coef 0: the reference is reported on and nothing else, where the estimate is infinite too."""
+    from parallel_b200.ops import objectives as O
+
+    lp = -torch.rand(3, 7, device="cuda")
+    ref = lp.clone()
+    ref[1, 2], ref[2, 3] = -float("inf"), 3e38
+    adv = torch.randn(3, 7, device="cuda")
+    outs = []
+    for r in (None, ref):
+        x = lp.clone().requires_grad_(True)
+        out = O.policy_loss(x, lp - 0.1, adv, ref_logp=r, reduction=reduction)
+        outs.append((out.loss.detach(), out.clip_fraction, torch.autograd.grad(out.loss, x)[0]))
+    _synced()
+    assert out.kl.item() == float("inf")
+    assert torch.isfinite(outs[0][0]) and all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 def test_policy_loss_without_tokens_and_refusals():
     from parallel_b200.ops import objectives as O
 

@@ -117,7 +117,7 @@ def _unit_inner(t: torch.Tensor | None) -> torch.Tensor | None:
 def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor,
                 mask: torch.Tensor | None = None, ref_logp: torch.Tensor | None = None, clip_low: float = 0.2,
                 clip_high: float = 0.2, kl_coef: float = 0.0, reduction: str = "token") -> PolicyLoss:
-    """Clipped policy loss of token log-probabilities, logp fp32 [B, S].
+    """Clipped policy loss of token log-probabilities, logp fp32 [B, S], in 64 bits and rounded once.
 
     With r = exp(logp - old_logp) and advantage A, a token's loss is
     ``-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef k`` with
@@ -151,11 +151,14 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Te
 def _policy_plain(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence):
     m = torch.ones_like(logp, dtype=torch.bool) if mask is None else mask
     at = m.nonzero(as_tuple=True)  # the tokens that count; the others never enter
-    x = logp[at]
-    ratio = torch.exp(x - old[at])
-    u, c = ratio * adv[at], ratio.detach().clamp(low, high) * adv[at]
-    clipped = u.detach() > c
-    per = -torch.where(clipped, c, u)
+    x, a = logp[at].double(), adv[at].double()
+    gap = x - old[at]
+    with torch.no_grad():
+        ratio = torch.exp(gap)
+        c = ratio.clamp(low, high) * a
+        clipped = ratio * a > c
+    # the ratio of a clipped token stays out of the graph: it may be infinite
+    per = -torch.where(clipped, c, torch.exp(gap.masked_fill(clipped, 0.0)) * a)
     kl = torch.zeros_like(x)
     if ref is not None:
         d = ref[at] - x
@@ -168,7 +171,8 @@ def _policy_plain(logp, old, adv, mask, ref, low, high, kl_coef, per_sequence):
         weight = (1.0 / rows.clamp_min(1).to(x.dtype) / max(1, int((rows > 0).sum())))[at[0]]
     else:
         weight = 1.0 / n
-    return PolicyLoss((per * weight).sum(), clipped.to(x.dtype).sum() / n, kl.detach().sum() / n)
+    out = (per * weight).sum(), clipped.double().sum() / n, kl.detach().sum() / n
+    return PolicyLoss(*(t.to(logp.dtype) for t in out))
 
 
 def preference_loss(logp: torch.Tensor, ref_logp: torch.Tensor | None = None, mask: torch.Tensor | None = None,

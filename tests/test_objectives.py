@@ -135,6 +135,17 @@ def test_policy_loss_without_a_kl_term_takes_any_reference(reduction):
     assert torch.isfinite(outs[0][0]) and all(torch.equal(a, b) for a, b in zip(*outs))
 
 
+def test_policy_loss_of_ratios_past_the_range_of_fp32():
+    """A clipped ratio sends no gradient however large it is, and an advantage of 0 no loss."""
+    for gap, adv, want in ((200.0, 1.0, -1.28), (1000.0, 1.0, -1.28), (200.0, 0.0, 0.0), (-200.0, -1.0, 0.8)):
+        lp = torch.tensor([[gap, -0.5]], requires_grad=True)
+        old = torch.tensor([[0.0, -0.5]])
+        out = O.policy_loss(lp, old, torch.tensor([[adv, 2.0]]), clip_low=0.2, clip_high=0.28)
+        (grad,) = torch.autograd.grad(out.loss, lp)
+        assert abs(out.loss.item() - (want - 2.0) / 2) < 1e-6 and out.clip_fraction.item() == (0.5 if adv else 0.0)
+        assert grad.tolist() == [[0.0, -1.0]]
+
+
 def test_preference_loss_formula_and_gradient():
     torch.manual_seed(2)
     P, S = 3, 8

@@ -4,9 +4,9 @@
 //   logprob_gemm    CTA-pair tcgen05 GEMM h w^T whose epilogue turns each row
 //                   of an output tile into (max, sum of 2^(x - max)), x the
 //                   logit in base 2, the target column left out; under a
-//                   gradient it also stores E = 2^(x - tile max) in 16 bits.
+//                   gradient it also stores E = 2^(x - group max) in 16 bits.
 //   logprob_finish  per row: the target logit as its own dot product, the
-//                   merge of the row's tile statistics, logp and the row's
+//                   merge of the row's statistics, logp and the row's
 //                   base-2 log-sum-exp above its maximum.
 //   logprob_pack    (under a gradient) brings the rows that have a token to the
 //                   front; logprob_unpack takes their gradients back.
@@ -31,10 +31,10 @@
 // on that logit.  The other logits enter as a sum of many, where only the mean
 // of that loss shows; it is added back (kTruncation).
 //
-// E is relative to the tile's own maximum, which is known when the tile is
+// E is relative to its group's own maximum, which is known when the tile is
 // stored, while the row's log-sum-exp is not: an entry keeps 10 bits of its
 // probability whatever its size (pack_e), and the backward is one multiplication
-// per entry (the factor 2^(tile max - lse2), shared by a tile's row) in a pass
+// per entry (the factor 2^(group max - lse2), shared by a group) in a pass
 // bound by memory.  bf16 logits would lose |l| / 256 of the exponent instead.
 #include <cuda_bf16.h>
 #include <math.h>
@@ -72,15 +72,21 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Column tiles: the first n_full are BN_MAX wide, the others bn2.  Whole waves of
-// wide tiles over the CTA pairs, and what is left over in tiles narrow enough
-// for one more wave: 151,936 columns are 8 waves of 256 on 74 pairs and 384
-// columns, which as two wide tiles cost a ninth wave (64 rows, H 1024: 62.2 ->
-// 60.1 us; 8 rows of V 10000: 12.6 -> 11.6; 333 rows, H 4096: 435 -> 439).
-__device__ __forceinline__ int tile_start(const LogprobTiles& g, int tn) {
-  return tn < g.n_full ? tn * BN_MAX : g.n_full * BN_MAX + (tn - g.n_full) * g.bn2;
+// Column groups and tiles.  A group is what one pair of statistics covers, a tile
+// what one accumulator holds.  The first n_full of either are BN_MAX wide; behind
+// them come narrower groups, and tiles of bn2 columns, one or more of these groups.
+// For few rows that makes whole waves of wide tiles over the CTA pairs and one of
+// tiles narrow enough for what is left over: 151,936 columns are 8 waves of 256 on
+// 74 pairs and 384 columns, which as two wide tiles cost a ninth wave (64 rows, H
+// 1024: 62.2 -> 60.1 us; 8 rows of V 10000: 12.6 -> 11.6).  The groups go by the
+// vocabulary alone and the tiles by the rows too, so a row's sums are added in the
+// same order, and its log-probability has the same bits, in whatever batch it comes.
+__device__ __forceinline__ int tile_start(const LogprobGroups& g, int bn2, int tn) {
+  return tn < g.n_full ? tn * BN_MAX : g.n_full * BN_MAX + (tn - g.n_full) * bn2;
 }
-__device__ __forceinline__ int tile_width(const LogprobTiles& g, int tn) { return tn < g.n_full ? BN_MAX : g.bn2; }
+__device__ __forceinline__ int tile_width(const LogprobGroups& g, int bn2, int tn) {
+  return tn < g.n_full ? BN_MAX : bn2;
+}
 
 // Wait for this thread's TMEM loads; the registers are operands, so no use of
 // them can move above the wait.
@@ -142,18 +148,18 @@ __device__ __forceinline__ void scaled_diff(float& a, float& b, float m, float s
   b = d.y;
 }
 
-// Statistics of one accumulator row (one thread) of `bn` columns from TMEM: the
-// maximum first (E needs one reference for the whole tile), then the sum of the
+// Statistics of one accumulator row (one thread) of `bn` columns from TMEM, a group:
+// the maximum first (E needs one reference for the whole group), then the sum of the
 // exponentials, which under a gradient (STORE) also go to E, straight from
 // registers.  Staging them in shared memory for tile stores put 128 KB more per
 // tile on a shared memory that the MMAs already read at its rate (8192 rows,
 // 6554 with a token: 1605 us; like this 1463).  Scoring takes the same two
 // passes, although a running maximum would do: the log-probabilities then are
 // the same bits as in training, and a policy's ratio to itself is exactly 1.
-// `release` runs after the last TMEM read.
+// `release` runs after the last TMEM read of the tile's `last` group.
 template <bool STORE, typename Release>
 __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, int V, int64_t id, float scale,
-                                            __nv_bfloat16* e_row, bool row_in, Release release) {
+                                            __nv_bfloat16* e_row, bool row_in, bool last, Release release) {
   float m = -INFINITY;
 #pragma unroll 1
   for (int c = 0; c < bn; c += 32) {
@@ -170,7 +176,7 @@ __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, 
     float v[32];
     tmem_ld32(t_row + c, v);
     wait_ld(v);
-    if (c + 32 >= bn) release();
+    if (last && c + 32 >= bn) release();
     const int n0 = n_base + c;
     mask_cols(v, n0, V, id);
 #pragma unroll
@@ -202,8 +208,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     logprob_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmB2, __nv_bfloat16* __restrict__ e, int64_t lde,
                         const int64_t* __restrict__ ids, const int* __restrict__ count, int row0,
-                        float2* __restrict__ stats, int T_all, int V, int H, int a_rows, const LogprobTiles geo,
-                        float scale, int* err) {
+                        float2* __restrict__ stats, int T_all, int V, int H, int a_rows, const LogprobGroups geo,
+                        int bn2, int tiles2, float scale, int* err) {
   pdl_prologue();
   const int T = count ? min(T_all, max(0, *count - row0)) : T_all;  // the rows in front that have a token
   extern __shared__ uint8_t smem_raw[];
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
 
   const int tiles_m = (T + 2 * BM_CTA - 1) / (2 * BM_CTA);
-  const int tiles_n = geo.n_full + geo.n_rest;
+  const int tiles_n = geo.n_full + tiles2;
   const int64_t num_tiles = (int64_t)tiles_m * tiles_n;
   const int num_kb = (H + BK - 1) / BK;
   const int n_clusters = gridDim.x >> 1;
@@ -274,8 +280,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int64_t w = cid; w < num_tiles && ok; w += n_clusters) {
         const int tm = (int)(w % tiles_m), tn = (int)(w / tiles_m);
         const int a_row = tm * 2 * BM_CTA + (int)rank * BM_CTA;
-        const int bn = tile_width(geo, tn);
-        const int b_row = tile_start(geo, tn) + (int)rank * (bn / 2);
+        const int bn = tile_width(geo, bn2, tn);
+        const int b_row = tile_start(geo, bn2, tn) + (int)rank * (bn / 2);
         const CUtensorMap* map_b = tn < geo.n_full ? &tmB : &tmB2;
         const uint32_t stage_bytes = a_bytes + (uint32_t)bn * BK * 2;
         for (int kb = 0; kb < num_kb; ++kb) {
@@ -306,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int local = 0;
       bool ok = true;
       for (int64_t w = cid; w < num_tiles && ok; w += n_clusters, ++local) {
-        const uint32_t idesc = idesc_bf16(2 * BM_CTA, tile_width(geo, (int)(w / tiles_m)), false, false);
+        const uint32_t idesc = idesc_bf16(2 * BM_CTA, tile_width(geo, bn2, (int)(w / tiles_m)), false, false);
         const int acc = local & 1;
         const uint32_t acc_phase = (local >> 1) & 1;
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1, err)) break;
@@ -349,9 +355,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         continue;
       }
       const int64_t id = t < T ? ids[t] : -1;
-      const int bn = tile_width(geo, tn), n0 = tile_start(geo, tn);
-      const float2 st = row_stats<STORE>(t_row, bn, n0, V, id, scale, e + (int64_t)t * lde, t < T, release);
-      if (t < T) stats[(int64_t)t * tiles_n + tn] = st;
+      const int n0 = tile_start(geo, bn2, tn);
+      int width = BN_MAX, group = tn, groups = 1;
+      if (tn >= geo.n_full) {
+        width = 1 << geo.shift;
+        group = geo.n_full + ((tn - geo.n_full) * bn2 >> geo.shift);
+        groups = min(bn2 >> geo.shift, geo.n_full + geo.n_rest - group);
+      }
+      float2* out = stats + (int64_t)t * (geo.n_full + geo.n_rest) + group;
+      for (int i = 0; i < groups; ++i) {
+        const float2 st = row_stats<STORE>(t_row + i * width, width, n0 + i * width, V, id, scale, e + (int64_t)t * lde,
+                                           t < T, i + 1 == groups, release);
+        if (t < T) out[i] = st;
+      }
     }
   }
 
@@ -377,13 +393,13 @@ constexpr int kFinThreads = 128;
 
 // One block per row of h; its log-probability goes to row perm[t] (t without
 // perm).  dot in 64 bits (bf16 products are exact in fp32; eight of them are
-// added in fp32, the rest in double), then the tile statistics: with d = m -
+// added in fp32, the rest in double), then the groups' statistics: with d = m -
 // x_id (base 2), logp = -log(1 + s 2^d), written so that neither a large nor a
 // small d loses digits.  lse: the row's maximum m, unscaled, and lse2 - m.
 __global__ void __launch_bounds__(kFinThreads)
     logprob_finish_kernel(const __nv_bfloat16* __restrict__ h, int64_t ldh, const __nv_bfloat16* __restrict__ w,
                           int64_t ldw, const int64_t* __restrict__ ids, const int* __restrict__ perm,
-                          const float2* __restrict__ stats, int tiles, int V, int H, float scale, float scale_mma,
+                          const float2* __restrict__ stats, int groups, int V, int H, float scale, float scale_mma,
                           float* __restrict__ logp, float2* __restrict__ lse) {
   pdl_prologue();
   const int64_t t = blockIdx.x;
@@ -414,8 +430,8 @@ __global__ void __launch_bounds__(kFinThreads)
     dot += (double)p;
   }
   float m = -INFINITY, s = 0.f;
-  const float2* sr = stats + t * tiles;
-  for (int i = threadIdx.x; i < tiles; i += kFinThreads) {
+  const float2* sr = stats + t * groups;
+  for (int i = threadIdx.x; i < groups; i += kFinThreads) {
     const float2 v = sr[i];
     const float mn = fmaxf(m, v.x);
     if (mn == -INFINITY) {
@@ -474,15 +490,15 @@ __global__ void __launch_bounds__(kFinThreads)
 constexpr int kBwdThreads = 256;
 constexpr int kBwdUnroll = 4;
 
-// A warp takes a tile of a row at a time: one factor for its (256) consecutive
-// entries, 8 of them per lane and step.  The target's entry, 0 in E, stays 0;
+// A warp takes 256 columns of a row at a time, 8 of them per lane, which are of one
+// group and have one factor.  The target's entry, 0 in E, stays 0;
 // own[t] = c (1 - p) = -c expm1(logp).
 __global__ void __launch_bounds__(kBwdThreads)
-    logprob_bwd_kernel(__nv_bfloat16* __restrict__ e, int64_t lde, const float2* __restrict__ stats, int tiles,
+    logprob_bwd_kernel(__nv_bfloat16* __restrict__ e, int64_t lde, const float2* __restrict__ stats,
                        const float2* __restrict__ lse, float scale_mma, const float* __restrict__ logp,
                        const int64_t* __restrict__ ids, const int* __restrict__ perm,
                        const int* __restrict__ count, int row0, const float* __restrict__ g, float inv_tau, int V,
-                       float* __restrict__ own, const LogprobTiles geo) {
+                       float* __restrict__ own, const LogprobGroups geo) {
   pdl_prologue();
   const int64_t t = blockIdx.x;
   // behind the rows with a token: zeros up to the end of the last 64-deep step of
@@ -496,7 +512,7 @@ __global__ void __launch_bounds__(kBwdThreads)
   const int lane = threadIdx.x & 31;
   const int warps = (int)gridDim.y * (kBwdThreads / 32);
   if (blockIdx.y == 0 && threadIdx.x == 0) own[t] = id < 0 ? 0.f : -c * expm1f(logp[src]);
-  const float2* st = stats + t * tiles;
+  const float2* st = stats + t * (geo.n_full + geo.n_rest);
   auto scaled = [&](uint4 u, float f) {
     uint32_t* p = &u.x;
 #pragma unroll
@@ -506,33 +522,25 @@ __global__ void __launch_bounds__(kBwdThreads)
     }
     return u;
   };
-  int tile = blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5);
-  // wide tiles, kBwdUnroll of them in flight: a tile is one vector a lane
-  for (; tile < geo.n_full; tile += kBwdUnroll * warps) {
+  // kBwdUnroll vectors a lane in flight
+  const int windows = (V + BN_MAX - 1) / BN_MAX;
+  for (int i = blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5); i < windows; i += kBwdUnroll * warps) {
     uint4 u[kBwdUnroll];
     float f[kBwdUnroll];
 #pragma unroll
     for (int j = 0; j < kBwdUnroll; ++j) {
-      const int tj = tile + j * warps;
-      if (id >= 0 && tj < geo.n_full) {
-        u[j] = __ldcs(reinterpret_cast<const uint4*>(row + tj * BN_MAX + lane * 8));
-        f[j] = st[tj].x;
+      const int wi = i + j * warps, col = wi * BN_MAX + lane * 8;
+      if (id >= 0 && col < V) {
+        u[j] = __ldcs(reinterpret_cast<const uint4*>(row + col));
+        f[j] = st[wi < geo.n_full ? wi : geo.n_full + ((col - geo.n_full * BN_MAX) >> geo.shift)].x;
       }
     }
 #pragma unroll
     for (int j = 0; j < kBwdUnroll; ++j) {
-      const int tj = tile + j * warps, col = tj * BN_MAX + lane * 8;
-      if (tj < geo.n_full)
+      const int col = (i + j * warps) * BN_MAX + lane * 8;
+      if (col < V)
         *reinterpret_cast<uint4*>(row + col) =
             id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(u[j], -c * ex2(fmaf(f[j] - top.x, scale_mma, -top.y)));
-    }
-  }
-  for (tile = geo.n_full + blockIdx.y * (kBwdThreads / 32) + (threadIdx.x >> 5); tile < tiles; tile += warps) {
-    const float f = id < 0 ? 0.f : -c * ex2(fmaf(st[tile].x - top.x, scale_mma, -top.y));
-    const int start = tile_start(geo, tile), end = min(V, start + geo.bn2);
-    for (int col = start + lane * 8; col < end; col += 256) {
-      uint4* p4 = reinterpret_cast<uint4*>(row + col);
-      *p4 = id < 0 ? make_uint4(0u, 0u, 0u, 0u) : scaled(*p4, f);
     }
   }
 }
@@ -768,7 +776,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 8)
 
 template <bool STORE>
 void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const LogprobParams& p,
-                 int a_rows, float scale, cudaStream_t stream) {
+                 int a_rows, int bn2, float scale, cudaStream_t stream) {
   auto kern = logprob_gemm_kernel<STORE>;
   static std::mutex mu;
   static int max_clusters[64] = {0};
@@ -800,12 +808,13 @@ void launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap
     }
     clusters = max_clusters[dev & 63];
   }
-  const int64_t tiles = (int64_t)((p.T + 2 * BM_CTA - 1) / (2 * BM_CTA)) * (p.tiles.n_full + p.tiles.n_rest);
+  const int tiles2 = (p.V - p.groups.n_full * BN_MAX + bn2 - 1) / bn2;
+  const int64_t tiles = (int64_t)((p.T + 2 * BM_CTA - 1) / (2 * BM_CTA)) * (p.groups.n_full + tiles2);
   clusters = (int)std::max<int64_t>(1, std::min<int64_t>(clusters, tiles));
   cfg.gridDim = dim3(2 * clusters, 1, 1);
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   PB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, ta, tb, tb2, (__nv_bfloat16*)p.e, p.lde, p.ids, p.count, p.row0, reinterpret_cast<float2*>(p.stats),
-                                   p.T, p.V, p.H, a_rows, p.tiles, scale, error_word(dev)));
+                                   p.T, p.V, p.H, a_rows, p.groups, bn2, tiles2, scale, error_word(dev)));
 }
 
 // Base-2 logit per unit of the tensor core's dot product: what its truncation
@@ -816,19 +825,31 @@ float mma_scale(float inv_tau, int H) {
 
 }  // namespace
 
-LogprobTiles logprob_tiles(int T, int V) {
-  const int64_t tiles_m = (T + 2 * BM_CTA - 1) / (2 * BM_CTA), pairs = std::max(1, num_sms() / 2);
-  const int wide = V / BN_MAX;  // whole wide tiles
-  const int64_t waves = tiles_m * wide / pairs;
-  LogprobTiles g;
-  g.n_full = (int)std::min<int64_t>(wide, waves * pairs / tiles_m);
+LogprobGroups logprob_groups(int V) {
+  const int pairs = std::max(1, num_sms() / 2);
+  LogprobGroups g;
+  g.n_full = V / BN_MAX / pairs * pairs;
   const int rest = V - g.n_full * BN_MAX;
-  // the narrowest multiple of 32 whose tiles fit one wave
-  g.bn2 = BN_MAX;
-  for (int bn = BN_MAX - 32; bn >= 32; bn -= 32)
-    if (tiles_m * ((rest + bn - 1) / bn) <= pairs) g.bn2 = bn;
-  g.n_rest = (rest + g.bn2 - 1) / g.bn2;
+  // the narrowest tiles, in steps of 32, of which a row tile's fit one wave; groups of the power of two in that
+  int bn = 32;
+  while (bn < BN_MAX && (rest + bn - 1) / bn > pairs) bn += 32;
+  g.shift = 5;
+  while (bn % (2 << g.shift) == 0) ++g.shift;
+  g.n_rest = (rest + (1 << g.shift) - 1) >> g.shift;
   return g;
+}
+
+// Width of the tiles behind the first n_full, for T rows: the waves that they take
+// times a tile's time, which goes by the operand rows that it loads (1237 rows of V
+// 32003, H 2048: 120 us in tiles of 192, 92 in 256).
+static int rest_width(const LogprobGroups& g, int T, int V) {
+  const int64_t tiles_m = (T + 2 * BM_CTA - 1) / (2 * BM_CTA), pairs = std::max(1, num_sms() / 2);
+  const int rest = V - g.n_full * BN_MAX;
+  auto cost = [&](int bn) { return (tiles_m * ((rest + bn - 1) / bn) + pairs - 1) / pairs * (bn + std::min(T, 2 * BM_CTA)); };
+  int best = BN_MAX;
+  for (int bn = 1 << g.shift; bn < BN_MAX; bn += 1 << g.shift)
+    if (cost(bn) < cost(best)) best = bn;
+  return best;
 }
 
 void logprob_fwd(const LogprobParams& p, cudaStream_t stream) {
@@ -842,28 +863,27 @@ void logprob_fwd(const LogprobParams& p, cudaStream_t stream) {
   const int a_rows = p.T < BM_CTA ? (p.T + 7) / 8 * 8 : BM_CTA;
   const CUtensorMap ta = make_tmap_2d_bf16(p.h, p.H, p.T, p.ldh, BK, a_rows);
   const CUtensorMap tb = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, BN_MAX / 2);
-  const CUtensorMap tb2 = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, p.tiles.bn2 / 2);
+  const int bn2 = rest_width(p.groups, p.T, p.V);
+  const CUtensorMap tb2 = make_tmap_2d_bf16(p.w, p.H, p.V, p.ldw, BK, bn2 / 2);
   if (p.e) {
     PB_CHECK(p.lde % 32 == 0 && (reinterpret_cast<uintptr_t>(p.e) & 63) == 0, "logprob: E must have 64-byte rows");
-    launch_gemm<true>(ta, tb, tb2, p, a_rows, scale_mma, stream);
+    launch_gemm<true>(ta, tb, tb2, p, a_rows, bn2, scale_mma, stream);
   } else {
-    launch_gemm<false>(ta, tb, tb2, p, a_rows, scale_mma, stream);
+    launch_gemm<false>(ta, tb, tb2, p, a_rows, bn2, scale_mma, stream);
   }
-  const int tiles = p.tiles.n_full + p.tiles.n_rest;
   launch_k(logprob_finish_kernel, p.T, kFinThreads, 0, stream, (const __nv_bfloat16*)p.h, p.ldh,
-           (const __nv_bfloat16*)p.w, p.ldw, p.ids, p.perm, (const float2*)p.stats, tiles, p.V, p.H, scale,
+           (const __nv_bfloat16*)p.w, p.ldw, p.ids, p.perm, (const float2*)p.stats, p.groups.n(), p.V, p.H, scale,
            scale_mma, p.logp, reinterpret_cast<float2*>(p.lse));
 }
 
 void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse, const float* logp, const int64_t* ids,
                  const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V, int H,
-                 float* own, const LogprobTiles& geo, cudaStream_t stream) {
+                 float* own, const LogprobGroups& geo, cudaStream_t stream) {
   if (T == 0) return;
-  const int tiles = geo.n_full + geo.n_rest;
   // enough blocks for every SM when there are few rows
-  const int segs = std::max(1, std::min((tiles + 7) / 8, (8 * num_sms() + T - 1) / T));
+  const int segs = std::max(1, std::min((V + 8 * BN_MAX - 1) / (8 * BN_MAX), (8 * num_sms() + T - 1) / T));
   launch_k(logprob_bwd_kernel, dim3(T, segs), kBwdThreads, 0, stream, (__nv_bfloat16*)e, lde, (const float2*)stats,
-           tiles, (const float2*)lse, mma_scale(inv_tau, H), logp, ids, perm, count, row0, g, inv_tau, V, own,
+           (const float2*)lse, mma_scale(inv_tau, H), logp, ids, perm, count, row0, g, inv_tau, V, own,
            geo);
 }
 

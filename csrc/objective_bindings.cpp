@@ -99,7 +99,7 @@ void logprob_unpack(const at::Tensor& src, const at::Tensor& perm, const at::Ten
 }
 
 // logprob_fwd(h [T, H], w [V, H], ids [T], inv_tau, logp [>= T], e [T, V] or None, perm [T] or None, count [1] or
-// None, row0) -> (lse [T, 2], stats [T, tiles, 2]); logp of row t goes to logp[perm[t]] (logp[t] without perm).  With
+// None, row0) -> (lse [T, 2], stats [T, groups, 2]); logp of row t goes to logp[perm[t]] (logp[t] without perm).  With
 // count, h holds packed rows from row row0 on, of which the first count[0] have a token.
 std::vector<at::Tensor> logprob_fwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, double inv_tau,
                                     at::Tensor& logp, const c10::optional<at::Tensor>& e,
@@ -118,9 +118,9 @@ std::vector<at::Tensor> logprob_fwd(const at::Tensor& h, const at::Tensor& w, co
   CHECK_SAME_DEVICE(h, logp);
   const c10::cuda::CUDAGuard g(h.device());
   pb::LogprobParams p{};
-  p.tiles = pb::logprob_tiles((int)T, (int)V);
+  p.groups = pb::logprob_groups((int)V);
   const auto f32 = h.options().dtype(at::kFloat);
-  at::Tensor lse = at::empty({T, 2}, f32), stats = at::empty({T, p.tiles.n_full + p.tiles.n_rest, 2}, f32);
+  at::Tensor lse = at::empty({T, 2}, f32), stats = at::empty({T, p.groups.n(), 2}, f32);
   p.h = h.data_ptr();
   p.w = w.data_ptr();
   p.ids = ids.data_ptr<int64_t>();
@@ -167,8 +167,8 @@ at::Tensor logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor&
   for (const at::Tensor* t : {&stats, &lse, &ids, &perm, &count, &logp, &g}) CHECK_SAME_DEVICE(e, *t);
   TORCH_CHECK(logp.numel() == g.numel() && g.numel() >= T, "logprob: logp and g must have one entry per row");
   const c10::cuda::CUDAGuard guard(e.device());
-  const pb::LogprobTiles tiles = pb::logprob_tiles((int)T, (int)V);
-  check_rows_f32(stats, T * (tiles.n_full + tiles.n_rest) * 2, "logprob: stats");
+  const pb::LogprobGroups groups = pb::logprob_groups((int)V);
+  check_rows_f32(stats, T * groups.n() * 2, "logprob: stats");
   TORCH_CHECK(e.stride(0) % 8 == 0 && e.stride(0) >= (V + 7) / 8 * 8 &&
                   (reinterpret_cast<uintptr_t>(e.data_ptr()) & 15) == 0,
               "logprob: e must have 16-byte rows with room for whole 8-column groups");
@@ -177,7 +177,7 @@ at::Tensor logprob_bwd(at::Tensor& e, const at::Tensor& stats, const at::Tensor&
                   check_rows_f32(logp, logp.numel(), "logprob: logp"), ids.data_ptr<int64_t>(),
                   check_rows_i32(perm, T, "logprob: perm"), check_rows_i32(count, 1, "logprob: count"), (int)row0,
                   check_rows_f32(g, g.numel(), "logprob: g"), (float)inv_tau, (int)T, (int)V, (int)H,
-                  own.data_ptr<float>(), tiles, cur_stream());
+                  own.data_ptr<float>(), groups, cur_stream());
   return own;
 }
 

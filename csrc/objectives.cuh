@@ -11,14 +11,15 @@ namespace pb {
 
 // ---- log-probabilities of given tokens (logprob.cu)
 // h [T, H] and w [V, H] bf16; ids [T] (negative: no token, logp 0).
-// stats [T, tiles, 2] fp32: per row and tile of vocabulary columns the maximum
+// stats [T, groups, 2] fp32: per row and group of vocabulary columns the maximum
 // of h . w and the sum of 2^(x - x at the maximum), x the logit in base 2, target
 // left out.
-// e (optional, 16-bit [T, lde >= V]): 2^(x - tile max), in a format of logprob.cu.
-struct LogprobTiles {
-  int n_full, n_rest, bn2;  // n_full tiles of 256 columns, then n_rest of bn2
+// e (optional, 16-bit [T, lde >= V]): 2^(x - group max), in a format of logprob.cu.
+struct LogprobGroups {
+  int n_full, n_rest, shift;  // n_full groups of 256 columns, then n_rest of 1 << shift
+  int n() const { return n_full + n_rest; }
 };
-LogprobTiles logprob_tiles(int T, int V);
+LogprobGroups logprob_groups(int V);
 struct LogprobParams {
   const void* h;
   const void* w;
@@ -28,11 +29,11 @@ struct LogprobParams {
   int row0;
   float* stats;
   float* logp;
-  float* lse;  // [T, 2]: the maximum of h . w over row t's tiles, the row's base-2 log-sum-exp above it
+  float* lse;  // [T, 2]: the maximum of h . w over row t's groups, the row's base-2 log-sum-exp above it
   void* e;
   int64_t ldh, ldw, lde;
   int T, V, H;
-  LogprobTiles tiles;
+  LogprobGroups groups;
   float inv_tau;
 };
 void logprob_fwd(const LogprobParams& p, cudaStream_t stream);
@@ -41,7 +42,7 @@ void logprob_fwd(const LogprobParams& p, cudaStream_t stream);
 // logp and g in row perm[t]; e starts at packed row row0)
 void logprob_bwd(void* e, int64_t lde, const float* stats, const float* lse, const float* logp, const int64_t* ids,
                  const int* perm, const int* count, int row0, const float* g, float inv_tau, int T, int V, int H,
-                 float* own, const LogprobTiles& tiles, cudaStream_t stream);
+                 float* own, const LogprobGroups& groups, cudaStream_t stream);
 // hp [T, H]: the rows of h with ids >= 0 in order, then zeros; idp the ids and
 // perm the rows in that order, count[0] the rows with a token
 void logprob_pack(const void* h, int64_t ldh, const int64_t* ids, int T, int H, void* hp, int64_t* idp, int* perm,

@@ -78,6 +78,26 @@ def test_lm_head_log_probs_scored_and_trained_are_the_same_bits(T, H, V):
     assert torch.equal(scored, trained.detach())
 
 
+@pytest.mark.parametrize("H,V", [(64, 32003), (192, 5001), (64, 151936)])
+def test_lm_head_log_probs_do_not_depend_on_the_batch(H, V):
+    """A rollout scored in one batch and trained on in others, split by `max_block_bytes` or not: the same bits, so the
+    first update's ratios are exactly 1."""
+    from parallel_b200.ops import objectives as O
+
+    T = 4096
+    h, w, ids, _ = _head_inputs(T, H, V, ignored=0.2, seed=91)
+    with torch.no_grad():
+        scored = O.lm_head_log_probs(h, w, ids)
+        parts = [O.lm_head_log_probs(h[a:b], w, ids[a:b]) for a, b in ((0, 1), (1, 9), (9, 300), (300, 1500), (1500, T))]
+    hg = h.clone().requires_grad_(True)
+    whole = O.lm_head_log_probs(hg, w, ids)
+    micro = torch.cat([O.lm_head_log_probs(hg[a:a + 1024], w, ids[a:a + 1024]) for a in range(0, T, 1024)])
+    split = O.lm_head_log_probs(hg, w, ids, max_block_bytes=2 * V * 512)
+    _synced()
+    for other in (torch.cat(parts), whole.detach(), micro.detach(), split.detach()):
+        assert torch.equal(scored, other)
+
+
 @pytest.mark.parametrize("T,H,V,tau", [(1, 64, 8, 1.0), (1, 1024, 32003, 1.0), (5, 72, 1, 1.0), (2, 8, 2, 0.5),
                                        (33, 128, 257, 1.3), (255, 200, 1000, 1.0), (256, 64, 4096, 2.0),
                                        (257, 512, 5001, 0.7), (1000, 1024, 32003, 1.0), (130, 4096, 20011, 1.0)])

@@ -406,6 +406,13 @@ at::Tensor distill_prep(const at::Tensor& top, const at::Tensor& ids, const c10:
   return scratch;
 }
 
+// Whether two [T, V] tensors of one type are misaligned by the same number of bytes in every row.
+bool same_alignment(const at::Tensor& a, const at::Tensor& b) {
+  auto off = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) & 15; };
+  return (a.size(1) <= 1 || (a.stride(1) == 1 && b.stride(1) == 1)) && off(a) == off(b) &&
+         (a.size(0) <= 1 || (a.stride(0) - b.stride(0)) * a.element_size() % 16 == 0);
+}
+
 // distill_rows(logits [T, V], scratch (distill_prep's of all T_all rows), T_all, K, row0, tau, grad [T, V] or None): the
 // losses of rows [row0, row0 + T) and, with grad (may be logits itself), the gradient of the loss; with perm,
 // row i of the logits is row perm[i] of the teacher's; with weight (a scalar), the gradient alone, times it, if it
@@ -431,15 +438,11 @@ void distill_rows(const at::Tensor& logits, const at::Tensor& scratch, int64_t T
     CHECK_SAME_DEVICE(logits, *weight);
     p.weight = check_rows_f32(*weight, 1, "distill: weight");
   }
-  const int64_t es = logits.element_size();
   p.logits = logits.data_ptr();
   p.ld = logits.stride(0);
   if (given(grad)) {
-    TORCH_CHECK(grad->scalar_type() == logits.scalar_type() && grad->dim() == 2 && grad->size(0) == T &&
-                    grad->size(1) == V && (grad->stride(1) == 1 || V <= 1) &&
-                    (reinterpret_cast<uintptr_t>(grad->data_ptr()) & 15) ==
-                        (reinterpret_cast<uintptr_t>(logits.data_ptr()) & 15) &&
-                    (T <= 1 || (grad->stride(0) - logits.stride(0)) * es % 16 == 0),
+    TORCH_CHECK(grad->scalar_type() == logits.scalar_type() && grad->sizes() == logits.sizes() &&
+                    same_alignment(logits, *grad),
                 "distill: grad must have logits' type, shape and alignment");
     CHECK_SAME_DEVICE(logits, *grad);
     p.grad = grad->data_ptr();
@@ -757,8 +760,10 @@ struct DistillationNode : public torch::autograd::Function<DistillationNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     check_first_order("distillation_loss");
     TORCH_CHECK(ctx->saved_data.count("grad"), "distillation_loss supports one backward pass per forward");
-    const at::Tensor logits = ctx->get_saved_variables()[0], grad = ctx->saved_data["grad"].toTensor();
+    at::Tensor logits = ctx->get_saved_variables()[0];
+    const at::Tensor grad = ctx->saved_data["grad"].toTensor();
     ctx->saved_data.erase("grad");
+    if (!same_alignment(logits, grad)) logits = grad_like(grad).copy_(logits);  // saved-tensor hooks may lay it out anew
     distill_rows(logits, ctx->saved_data["scratch"].toTensor(), logits.size(0), ctx->saved_data["K"].toInt(), 0,
                  ctx->saved_data["tau"].toDouble(), grad, nullptr, g[0]);
     variable_list grads(5);

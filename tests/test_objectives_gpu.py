@@ -678,6 +678,30 @@ def test_distillation_gradient_times_a_weight_is_rounded_once(T, V, dtype, weigh
     assert torch.equal(grad[~mask], torch.zeros_like(grad[~mask]))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_of_saved_logits_that_come_back_elsewhere(dtype):
+    """Saved-tensor hooks (offloading, checkpointing) may return the logits in another layout than they had."""
+    from parallel_b200.ops import objectives as O
+
+    T, V = 21, 1003
+    logits, top, ids, mask = _teacher_inputs(T, V, 6, dtype, seed=3)
+    wide = torch.zeros(T, V + 4, device="cuda", dtype=dtype)
+    wide[:, 1:V + 1] = logits
+    x = wide[:, 1:V + 1].requires_grad_(True)
+    grads = []
+    for hooks in (False, True):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu() if hooks else t,
+                                                      lambda t: t.cuda().contiguous() if hooks else t):
+            loss = O.distillation_loss(x, top, ids, mask=mask)
+        grads.append([torch.autograd.grad(loss / 3, x)[0]])
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu() if hooks else t,
+                                                      lambda t: t.cuda().contiguous() if hooks else t):
+            loss = O.distillation_loss(x, top, ids, mask=mask)
+        grads[-1].append(torch.autograd.grad(loss, x)[0])
+    _synced()
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
 def test_distillation_loss_against_differences():
     from parallel_b200.ops import objectives as O
 

@@ -23,8 +23,7 @@ cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 //   out: [M, N] bf16 or fp32 depending on epi
 void gemm(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, bool b_mn, int64_t epi,
           double alpha, const c10::optional<at::Tensor>& r, int64_t b_up_offset, int64_t n_out, int64_t kernel,
-          int64_t splits, const c10::optional<at::Tensor>& ws, bool accumulate,
-          const c10::optional<at::Tensor>& live, int64_t live_row0, bool live_k) {
+          int64_t splits, const c10::optional<at::Tensor>& ws, bool accumulate) {
   CHECK_CUDA_BF16(a);
   CHECK_CUDA_BF16(b);
   TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && out.dim() == 2, "gemm: 2-D operands expected");
@@ -84,14 +83,6 @@ void gemm(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, 
     TORCH_CHECK(epi != pb::kEpiResidualBf16, "gemm: residual epilogue needs r");
     p.R = nullptr;
     p.ldr = 0;
-  }
-  if (live.has_value() && live->defined()) {
-    // rows that count, known on the device: of out's rows, or (live_k) of the operands'
-    TORCH_CHECK(live->is_cuda() && live->device() == a.device() && live->scalar_type() == at::kInt && live->numel() == 1,
-                "gemm: live must be CUDA int32 [1]");
-    p.live = live->data_ptr<int>();
-    p.live_row0 = (int)live_row0;
-    p.live_k = live_k;
   }
   pb::gemm_bf16(p, cur_stream());
 }
@@ -291,8 +282,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("b"), pybind11::arg("out"), pybind11::arg("a_mn"), pybind11::arg("b_mn"),
         pybind11::arg("epi"), pybind11::arg("alpha"), pybind11::arg("r") = pybind11::none(),
         pybind11::arg("b_up_offset") = 0, pybind11::arg("n_out") = 0, pybind11::arg("kernel") = 0,
-        pybind11::arg("splits") = 1, pybind11::arg("ws") = pybind11::none(), pybind11::arg("accumulate") = false,
-        pybind11::arg("live") = pybind11::none(), pybind11::arg("live_row0") = 0, pybind11::arg("live_k") = false);
+        pybind11::arg("splits") = 1, pybind11::arg("ws") = pybind11::none(), pybind11::arg("accumulate") = false);
   m.def("gemm_ag", &gemm_ag, "GEMM with the sequence-parallel all-gather of A in the same kernel",
         pybind11::arg("dst"), pybind11::arg("src_ptrs"), pybind11::arg("src_ld"), pybind11::arg("flags"),
         pybind11::arg("target"), pybind11::arg("seq"), pybind11::arg("seq_local"), pybind11::arg("batch"),

@@ -184,7 +184,7 @@ __device__ __forceinline__ void epilogue_row(const EpiArgs& ep, float alpha, uin
 // lane, for whole 32-column chunks.  For sums over few rows, where a tile's
 // store takes longer than its products: staging, fence and tile store of a
 // chunk follow one another, these do not (151936 x 4096 over 300 rows: 539 ->
-// 482 us).
+// 482 us, and 383 with the accumulator handed back before the stores are done).
 template <int BN, typename Release>
 __device__ __forceinline__ void epilogue_row_direct(const EpiArgs& ep, float alpha, uint32_t t_row, int m, int M, int N, int n_base,
                                                     Release release) {
@@ -193,7 +193,7 @@ __device__ __forceinline__ void epilogue_row_direct(const EpiArgs& ep, float alp
   for (int c = 0; c < BN; c += 32) {
     float v[32];
     tmem_ld32(t_row + c, v);
-    tmem_wait_ld();
+    tmem_wait_ld32(v);
     if (c + 32 >= BN) release();
     if (m < M && n_base + c < N) {
 #pragma unroll

@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(GATHER ? kThreads + 64 : kThreads, 1)
     for (int w = cid; w < num_work; w += n_clusters, ++local) {
       const int tile = w % num_tiles;
       const int tm = GATHER ? ga.m_order[tile % tiles_m] : n_first ? tile / tiles_n : tile % tiles_m;
-        const int tn = !GATHER && n_first ? tile % tiles_n : tile / tiles_m;
+      const int tn = !GATHER && n_first ? tile % tiles_n : tile / tiles_m;
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
       if (!mbar_wait(&tfull_bar[acc], acc_phase, err)) break;

@@ -88,17 +88,6 @@ __device__ __forceinline__ int tile_width(const LogprobGroups& g, int bn2, int t
   return tn < g.n_full ? BN_MAX : bn2;
 }
 
-// Wait for this thread's TMEM loads; the registers are operands, so no use of
-// them can move above the wait.
-__device__ __forceinline__ void wait_ld(float* v) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
-                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
-                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
-                 "+f"(v[30]), "+f"(v[31])::"memory");
-}
-
 // Accumulators of columns [n0, n0 + 32): -inf past the vocabulary and at the
 // row's target, so neither enters the maximum or the sum.
 __device__ __forceinline__ void mask_cols(float* v, int n0, int V, int64_t id) {
@@ -165,7 +154,7 @@ __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, 
   for (int c = 0; c < bn; c += 32) {
     float v[32];
     tmem_ld32(t_row + c, v);
-    wait_ld(v);
+    tmem_wait_ld32(v);
     mask_cols(v, n_base + c, V, id);
     m = fmaxf(m, max32(v));
   }
@@ -175,7 +164,7 @@ __device__ __forceinline__ float2 row_stats(uint32_t t_row, int bn, int n_base, 
   for (int c = 0; c < bn; c += 32) {
     float v[32];
     tmem_ld32(t_row + c, v);
-    wait_ld(v);
+    tmem_wait_ld32(v);
     if (last && c + 32 >= bn) release();
     const int n0 = n_base + c;
     mask_cols(v, n0, V, id);

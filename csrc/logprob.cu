@@ -8,8 +8,9 @@
 //   logprob_finish  per row: the target logit as its own dot product, the
 //                   merge of the row's statistics, logp and the row's
 //                   base-2 log-sum-exp above its maximum.
-//   logprob_pack    (under a gradient) brings the rows that have a token to the
-//                   front; logprob_unpack takes their gradients back.
+//   logprob_pack    (under a gradient, and from 768 rows on) brings the rows that
+//                   have a token to the front; logprob_unpack takes their
+//                   gradients back.
 //   logprob_bwd     in place over E: the gradient of the logits but the target,
 //                   dl_v = -c 2^(x_v - lse2), c = dlogp / temperature, and the
 //                   target's own c (1 - p), in fp32.
@@ -28,8 +29,8 @@
 // and logp = -log1p(sum of the others / target): the tensor core truncates as
 // it accumulates (measured on a target logit of 13: 1.6e-5 low at H = 1024,
 // 5e-5 at H = 4096), and where the target is nearly certain all of logp hangs
-// on that logit.  The other logits enter as a sum of many, where only the mean
-// of that loss shows; it is added back (kTruncation).
+// on that logit.  The other logits enter as a sum of many, where the mean of that
+// loss shows; an estimate of it is added back (kTruncation).
 //
 // E is relative to its group's own maximum, which is known when the tile is
 // stored, while the row's log-sum-exp is not: an entry keeps 10 bits of its
@@ -59,11 +60,16 @@ constexpr int STAGES = 7;
 constexpr int SMEM_BYTES = STAGES * (A_BYTES + B_BYTES) + 1024 + 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// Mean relative loss of an accumulated dot product per 16-deep step: each step
-// truncates the running sum towards zero in its 24th bit.  For a sum that grows
-// evenly to its end that is about half a unit of half the final value a step,
-// 0.36 x 2^-24; measured, 0.25 to 0.28 for logits of 4 to 32 at H = 512 to 4096,
-// the spread around it a tenth to a third of it.
+// Estimate of the mean relative loss of an accumulated dot product per 16-deep
+// step.  Each step truncates the running sum towards zero in its 24th bit, so a
+// step loses less than 2^-23 of the sum it leaves; for one that grows evenly to
+// its end half a unit a step would be 0.36 x 2^-24 of the end.  The constant is not
+// derived but fitted: 0.25 to 0.28 was measured for normally distributed
+// components, logits of 4 to 32, H = 512 to 4096, the spread around it a tenth to a
+// third of it.  Where one early component makes the logit more is lost; where a
+// late one does nothing is, and what is given back is the error: 4e-6 of the logit
+// at H = 4096, as much as is lost without it in the even case.  There it takes
+// logp's error against 64 bits from 2.9e-6 to 8e-8 of its norm.
 constexpr double kTruncation = 0.26 / (1 << 24);
 
 __device__ __forceinline__ float ex2(float x) {
@@ -111,7 +117,9 @@ __device__ __forceinline__ float max32(const float* v) {
 
 // Two values of [0, 2) in 16 bits each: a float's sign and upper exponent bit
 // are 0 there, so 7 bits of exponent and 9 of mantissa remain (bf16 has 7 of
-// mantissa); rounded to nearest.  NaN does not survive, nor need it: the row's
+// mantissa); rounded to nearest.  Half the memory and time of fp32 between forward
+// and backward, for a quarter of the error that the logits' gradient takes next, as
+// the bf16 operand of both products.  NaN does not survive, nor need it: the row's
 // sum has it, and with that every gradient of the row.
 __device__ __forceinline__ uint32_t pack_e(float a, float b) {
   // bits 29..14, moved to the upper half with the rounding's half added
@@ -480,7 +488,8 @@ constexpr int kBwdThreads = 256;
 constexpr int kBwdUnroll = 4;
 
 // A warp takes 256 columns of a row at a time, 8 of them per lane, which are of one
-// group and have one factor.  The target's entry, 0 in E, stays 0;
+// group and have one factor.  The result is rounded to bf16, each entry on its own:
+// the tensor cores multiply nothing wider at their full rate.  The target's entry, 0 in E, stays 0;
 // own[t] = c (1 - p) = -c expm1(logp).
 __global__ void __launch_bounds__(kBwdThreads)
     logprob_bwd_kernel(__nv_bfloat16* __restrict__ e, int64_t lde, const float2* __restrict__ stats,

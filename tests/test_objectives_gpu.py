@@ -136,6 +136,26 @@ def test_lm_head_log_probs_nearly_certain_tokens_keep_their_digits():
     assert ((logp.double() - ref) / ref).abs().max().item() <= (512 / 16 + 8) * 2.0 ** -23 * 40
 
 
+@pytest.mark.parametrize("at", [0, 4095])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_lm_head_log_probs_of_hidden_states_with_one_large_component(at, sign):
+    """The whole of a logit in one component, the first or the last: the sum has its full size in every step or in
+    none.  Either way a step loses less than a unit in the 24th bit, and what is given back is a quarter of that."""
+    from parallel_b200.ops import objectives as O
+
+    T, H, V = 64, 4096, 5001
+    g = torch.Generator(device="cuda").manual_seed(95)
+    h = (0.01 * torch.randn(T, H, device="cuda", generator=g))
+    w = (torch.randn(V, H, device="cuda", generator=g) / math.sqrt(H))
+    h[:, at], w[:, at] = 40.0, sign * (0.75 + 0.05 * torch.rand(V, device="cuda", generator=g))
+    h, w = h.bfloat16(), w.bfloat16()
+    ids = torch.randint(0, V, (T,), device="cuda", generator=g)
+    logp = O.lm_head_log_probs(h, w, ids)
+    _synced()
+    ref, _, _, top = _head_reference(h, w, ids, torch.ones(T, device="cuda"), 1.0)
+    assert (logp.double() - ref).abs().max().item() <= (H / 16 + 8) * 2.0 ** -23 * top
+
+
 @pytest.mark.parametrize("ignored", [0.0, 0.5, 1.0])
 def test_lm_head_log_probs_row_blocks_and_garbage_in_ignored_rows(ignored):
     """Rows beyond the block are scored twice and the head's gradient adds up over blocks; ignored rows may hold

@@ -17,7 +17,7 @@
 //
 // What bounds it: one read and one write of each logit in HBM.  A row of
 // 151,936 bf16 logits is 304 KB, more than an SM's shared memory, so the second
-// pass reads it again, from L2: 2 CTAs on each of 148 SMs hold at most 90 MB of
+// pass reads it again, from L2 for two thirds and more: 2 CTAs on each of 148 SMs hold at most 90 MB of
 // rows there, of which a CTA in its first pass has not read all and one in its
 // second does not need all (it reads and writes with evict-first).
 // Sharing a row between the 8 CTAs of a cluster, which keeps it in registers
@@ -26,7 +26,7 @@
 // prefetch and the exponentials kept): each row then waits for an exchange
 // between 8 SMs, with too few warps beside it to fill the time.  Measured: 8192
 // x 151936 bf16, 64 entries: 877 us, 0.88 of the measured copy rate (of one
-// read and one write); 1021 x 32003 fp32: 57 us.
+// read and one write; 935 on GPUs with less clock); 1021 x 32003 fp32: 58 us.
 #include <cuda_bf16.h>
 #include <math.h>
 

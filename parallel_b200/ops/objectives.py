@@ -56,7 +56,8 @@ def lm_head_log_probs(h: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, tempe
     token: its log-probability is 0 and it sends back no gradient.  An id >= V
     gives NaN (an ``IndexError`` on CPU).  The gradient goes to h and w; one
     backward pass per forward.  ``max_block_bytes`` bounds the [rows, V] block
-    held between forward and backward; rows beyond it are computed twice."""
+    held between forward and backward; rows beyond it are computed twice.  On
+    CUDA a row's log-probability has the same bits in whatever batch it comes."""
     _check_temperature(temperature)
     _check_head(h, w)
     if ids.dtype != torch.int64 or ids.numel() * h.shape[-1] != h.numel():

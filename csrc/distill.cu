@@ -17,9 +17,10 @@
 //
 // What bounds it: one read and one write of each logit in HBM.  A row of
 // 151,936 bf16 logits is 304 KB, more than an SM's shared memory, so the second
-// pass reads it again, from L2 for two thirds and more: 2 CTAs on each of 148 SMs hold at most 90 MB of
-// rows there, of which a CTA in its first pass has not read all and one in its
-// second does not need all (it reads and writes with evict-first).
+// pass reads it again, from L2 for two thirds and more: 2 CTAs on each of 148 SMs
+// hold at most 90 MB of rows there, of which a CTA in its first pass has not read
+// all and one in its second does not need all (it reads and writes with
+// evict-first).
 // Sharing a row between the 8 CTAs of a cluster, which keeps it in registers
 // and needs no second read, was slower in every form that was tried (8192 x
 // 151936 bf16: 1211 us as short-lived CTAs, 1229 us persistent with bulk-copy
